@@ -19,6 +19,9 @@
  *                       and csrc/rmsnorm.cu:19-57        (the hand-written CUDA baseline)
  *   kf_query_gemm_config  tuning/search.py:299-394      shared-memory / feasibility model
  *   kf_gemv_noalloc     as kf_gemv, for callers that cannot hand over a workspace
+ *   kf_prefill_attention, kf_tree_attention, kf_rotary, kf_build_slots
+ *                       a decoder block served from a paged key/value cache (the
+ *                       reference leaves attention to PyTorch: no counterpart)
  *   kf_linear_bias_act_allgather, kf_peer_barrier(_counted), kf_ipc_handle / _open / _close
  *                       the column-sharded fused linear over several GPUs (the
  *                       reference is single-GPU: no counterpart)
@@ -287,6 +290,97 @@ KF_API int32_t kf_softmax_rows(int32_t dtype, const void* x, int64_t sx_row, voi
 KF_API int32_t kf_rmsnorm_rows(int32_t dtype, const void* x, int64_t sx_row, const void* gamma,
                         void* y, int64_t sy_row, int64_t rows, int64_t cols, float eps,
                         const kf_rows_config* cfg, void* stream);
+
+/* ---- attention for serving --------------------------------------------------- *
+ * o = softmax(scale q k^T) v per head, query head h reading key head
+ * h / (heads / kv_heads); scores, statistics and sums in fp32 (matrix products on
+ * tensor cores read the weights p rounded to the operands' 16-bit type). Strides
+ * in elements; the last dimension of every operand is contiguous; dim <= 256.
+ * Offsets and lengths are read on the device only, and clamped to the arrays
+ * they index. A row that sees no key gets zeros and a log-sum-exp of -infinity,
+ * and so do rows of q past the last offset. What a row does not see does not
+ * reach it, whatever it holds (stale pages, infinities, NaN).
+ *
+ * kf_prefill_attention: prompts of any lengths packed without padding. q and out
+ * are [rows, heads, dim], k and v [keys, kv_heads, dim]; request r has the rows
+ * [cu_q[r], cu_q[r+1]) of q and [cu_k[r], cu_k[r+1]) of k and v (int32, seqs + 1
+ * of them, from 0). causal != 0: the last row of a request sees all of its keys,
+ * each row before it one less. lse (or null): [rows, heads] natural-log sums. */
+KF_API int32_t kf_prefill_attention(int32_t dtype, const void* q, int64_t sq_row, int64_t sq_head,
+                                    const void* k, int64_t sk_row, int64_t sk_head, const void* v,
+                                    int64_t sv_row, int64_t sv_head, void* out, int64_t so_row,
+                                    int64_t so_head, float* lse, const int32_t* cu_q, const int32_t* cu_k,
+                                    int64_t seqs, int64_t rows, int64_t keys, int64_t heads,
+                                    int64_t kv_heads, int64_t dim, float scale, int32_t causal,
+                                    void* stream);
+
+/* kf_tree_attention: new tokens over a paged cache. Pages are
+ * [pages, kv_heads, block_size, dim] (any strides); position i of request r is
+ * slot i % block_size of page block_table[r][i / block_size] (int32, -1: none).
+ * Request r has context[r] cached tokens, which its rows
+ * [cu_q[r], cu_q[r+1]) of q all see (cu_q null: one row per request), and row j
+ * of the request is the token at position context[r] + j, whose key and value
+ * are in the cache already. Bit b of a row's tree_mask words [rows, mask_words]
+ * says whether it sees row b of its request (itself included); without a mask
+ * (mask_words 0) the rows are a chain, each seeing those before it and itself.
+ * The workspace (kf_tree_attention_workspace_bytes, 256-byte aligned, zeroed
+ * before its first use and left so that it serves the next call) holds the
+ * partial results of a cache split over CTAs. */
+KF_API int32_t kf_tree_attention(int32_t dtype, const void* q, int64_t sq_row, int64_t sq_head,
+                                 const void* k_cache, int64_t sk_page, int64_t sk_head, int64_t sk_slot,
+                                 const void* v_cache, int64_t sv_page, int64_t sv_head, int64_t sv_slot,
+                                 void* out, int64_t so_row, int64_t so_head, float* lse,
+                                 const int32_t* block_table, int64_t table_stride, int64_t table_cols,
+                                 int64_t pages, int64_t block_size, const int32_t* context,
+                                 const int32_t* cu_q, const int64_t* tree_mask, int64_t mask_words,
+                                 int64_t seqs, int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim,
+                                 float scale, void* workspace, int64_t workspace_bytes, void* stream);
+KF_API int64_t kf_tree_attention_workspace_bytes(int32_t device, int32_t dtype, int64_t seqs, int64_t rows,
+                                                 int64_t heads, int64_t kv_heads, int64_t dim);
+
+/* ---- rotary positions --------------------------------------------------------- *
+ * Where kf_rotary also writes a paged cache: v [tokens, kv_heads, dim] and the
+ * turned k go to slot slots[t] % block_size of page slots[t] / block_size
+ * (nowhere if slots[t] is negative or past the pages). */
+typedef struct kf_rotary_cache {
+  const void* v;
+  int64_t sv_row, sv_head;
+  void* k_cache;
+  int64_t sk_page, sk_head, sk_slot;
+  void* v_cache;
+  int64_t sv_page, svc_head, sv_slot;
+  int64_t pages, block_size;
+  const int64_t* slots;
+} kf_rotary_cache;
+
+/* q [tokens, heads, dim] and k [tokens, kv_heads, dim], the first rot elements of
+ * each head turned by the angles of positions[t]: pairs (i, i + rot/2), or
+ * (2i, 2i + 1) if interleaved. table: [table_rows, rot] fp32, rot/2 cosines then
+ * rot/2 sines of each position; a position outside it gives NaN. inverse != 0
+ * turns back (the gradient of the forward turn). q_out may be q and k_out k.
+ * cache (or null): also the cache write; k_out may then be null. */
+KF_API int32_t kf_rotary(int32_t dtype, const void* q, int64_t sq_row, int64_t sq_head, void* q_out,
+                         int64_t sqo_row, int64_t sqo_head, const void* k, int64_t sk_row, int64_t sk_head,
+                         void* k_out, int64_t sko_row, int64_t sko_head, const int32_t* positions,
+                         const float* table, int64_t table_rows, int64_t rot, int64_t tokens,
+                         int64_t heads, int64_t kv_heads, int64_t dim, int32_t interleaved, int32_t inverse,
+                         const kf_rotary_cache* cache, void* stream);
+
+/* ---- block tables and slot maps ------------------------------------------------ *
+ * One serving step's plan from request lengths. Request r holds context[r] tokens
+ * in the first ceil(context[r] / block_size) pages of its row of block_table
+ * [seqs, table_cols] and adds added[r]; the pages it still needs are taken from
+ * free_blocks in order, request after request, and written into its row (-1 where
+ * the list ends). Writes cu_new[seqs + 1], the offsets of the added tokens;
+ * positions and slots [max_tokens] of each (slot: page x block_size + offset in
+ * it; -1 without a page; position 0 and slot -1 past the last token);
+ * counts[0]: pages needed, counts[1]: added tokens that got no slot. The same
+ * call on the same lengths writes the same values again. */
+KF_API int32_t kf_build_slots(const int32_t* context, const int32_t* added, int64_t seqs,
+                              int32_t* block_table, int64_t table_stride, int64_t table_cols,
+                              const int32_t* free_blocks, int64_t n_free, int64_t block_size,
+                              int64_t max_tokens, int32_t* cu_new, int32_t* positions, int64_t* slots,
+                              int32_t* counts, void* stream);
 
 /* ---- fused linear + all-gather over NVLink ---------------------------------- *
  * kf_linear_bias_act, and every output tile is also stored into the n_peers

@@ -228,6 +228,86 @@ int stream_default_warps(int64_t cols, int elem);
 int launch_rows_stream(const RowsArgs& args, const kf_rows_config& cfg, const DeviceInfo& dev,
                        cudaStream_t stream);
 
+// One attention problem as the C ABI received it (element strides; the last
+// dimension of every operand is contiguous). Packed prompts: k and v are rows
+// [keys, kv_heads, dim] and cu_k gives each request's; a cache: `paged`,
+// k and v are pages [pages, kv_heads, block_size, dim] with sk_t the stride
+// between slots, and request r's keys are its `context` cached tokens and then
+// one key per row of q.
+struct AttnArgs {
+  int dtype = KF_FP16;
+  const void* q = nullptr;
+  int64_t sq_t = 0, sq_h = 0;
+  const void* k = nullptr;
+  int64_t sk_t = 0, sk_h = 0, sk_p = 0;
+  const void* v = nullptr;
+  int64_t sv_t = 0, sv_h = 0, sv_p = 0;
+  void* out = nullptr;
+  int64_t so_t = 0, so_h = 0;
+  float* lse = nullptr;  // [rows, heads], or null
+  const int32_t* cu_q = nullptr;  // [seqs + 1]; null: one row per request
+  const int32_t* cu_k = nullptr;
+  int paged = 0;
+  const int32_t* table = nullptr;
+  int64_t table_stride = 0, table_cols = 0, pages = 0, block_size = 1;
+  const int32_t* context = nullptr;
+  const unsigned long long* mask = nullptr;  // [rows, mask_words]; null: rows are a chain
+  int64_t mask_words = 0;
+  int64_t seqs = 0, rows = 0, keys = 0, heads = 0, kv_heads = 0, dim = 0;
+  float scale_log2 = 0.0f;  // scale * log2(e)
+  int causal = 1;
+  void* workspace = nullptr;
+  int64_t workspace_bytes = 0;
+};
+constexpr int64_t ATTN_MAX_DIM = 256;
+// A warp per row and head, key by key: every type, stride and mask.
+int launch_attention_rows(const AttnArgs& args, cudaStream_t stream);
+
+// Rotary positions (rotary.cu): q and k turned by their positions' angles; with
+// a cache, k and v also go to the slots of their pages.
+struct RotaryArgs {
+  int dtype = KF_FP16;
+  const void* q = nullptr;
+  int64_t sq_t = 0, sq_h = 0;
+  void* q_out = nullptr;
+  int64_t sqo_t = 0, sqo_h = 0;
+  const void* k = nullptr;
+  int64_t sk_t = 0, sk_h = 0;
+  void* k_out = nullptr;  // or null
+  int64_t sko_t = 0, sko_h = 0;
+  const void* v = nullptr;
+  int64_t sv_t = 0, sv_h = 0;
+  const int32_t* positions = nullptr;
+  const float* table = nullptr;  // [table_rows, rot]: cosines, then sines
+  int64_t table_rows = 0, rot = 0;
+  void* k_cache = nullptr;
+  int64_t skc_p = 0, skc_h = 0, skc_s = 0;
+  void* v_cache = nullptr;
+  int64_t svc_p = 0, svc_h = 0, svc_s = 0;
+  int64_t pages = 0, block_size = 1;
+  const int64_t* slots = nullptr;
+  int64_t tokens = 0, heads = 0, kv_heads = 0, dim = 0;
+  int interleaved = 0, inverse = 0;
+};
+int launch_rotary(const RotaryArgs& args, const DeviceInfo& dev, cudaStream_t stream);
+
+// Block tables and slot maps from request lengths (slots.cu).
+struct SlotsArgs {
+  const int32_t* context = nullptr;
+  const int32_t* added = nullptr;
+  int64_t seqs = 0;
+  int32_t* table = nullptr;
+  int64_t table_stride = 0, table_cols = 0;
+  const int32_t* free_blocks = nullptr;
+  int64_t n_free = 0;
+  int64_t block_size = 1, max_tokens = 0;
+  int32_t* cu_new = nullptr;
+  int32_t* positions = nullptr;
+  int64_t* slots = nullptr;
+  int32_t* counts = nullptr;  // [2]: blocks taken, tokens dropped
+};
+int launch_slots(const SlotsArgs& args, const DeviceInfo& dev, cudaStream_t stream);
+
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 }  // namespace kf

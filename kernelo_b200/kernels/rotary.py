@@ -1,0 +1,177 @@
+"""Rotary positions on sm_100a, with the paged cache's write fused in.
+
+The first ``rot`` elements of each head are turned pair by pair by the angle of
+the token's position: pairs ``(i, i + rot/2)``, or ``(2i, 2i + 1)`` with
+``interleaved=True``; the rest of the head is left as it is. The angles come
+from a table that :func:`rotary_table` makes once, in 64 bits, plain or scaled
+for contexts longer than a model was trained on. The rotation is orthogonal, so
+its gradient is the turn back: ``inverse=True``.
+"""
+
+from __future__ import annotations
+
+import math
+
+import torch
+
+from kernelo_b200.kernels.attention import _check_index
+from kernelo_b200.runtime import native
+
+SCALINGS = ("linear", "base", "parts")
+
+
+def rotary_table(
+    max_positions: int,
+    rotary_dim: int,
+    *,
+    base: float = 10000.0,
+    scaling: str | None = None,
+    factor: float = 1.0,
+    original_positions: int | None = None,
+    low_turns: float = 1.0,
+    high_turns: float = 32.0,
+    device: torch.device | str = "cuda",
+) -> torch.Tensor:
+    """cos and sin of every position: fp32 ``(max_positions, rotary_dim)``, cosines first.
+
+    Pair ``i`` turns by ``position * base ** (-2 i / rotary_dim)``. ``scaling``
+    stretches the table to ``factor`` times the trained context:
+
+    * ``"linear"`` -- positions divided by ``factor``;
+    * ``"base"`` -- ``base`` raised by ``factor ** (rotary_dim / (rotary_dim - 2))``,
+      which divides the slowest pair's frequency by ``factor`` and leaves the fastest;
+    * ``"parts"`` -- pairs that turn at least ``high_turns`` times within
+      ``original_positions`` keep their frequency, those that turn at most
+      ``low_turns`` times have it divided by ``factor``, the ones between are
+      blended linearly in their number of turns.
+    """
+    if rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError(f"rotary_dim must be even and positive, got {rotary_dim}")
+    if max_positions < 0:
+        raise ValueError(f"max_positions must not be negative, got {max_positions}")
+    if scaling is not None and scaling not in SCALINGS:
+        raise ValueError(f"scaling must be None or one of {SCALINGS}, got {scaling!r}")
+    if scaling is not None and not factor >= 1.0:
+        raise ValueError(f"factor must be at least 1, got {factor}")
+    if scaling == "base":
+        if rotary_dim == 2:
+            raise ValueError("scaling 'base' needs at least two pairs")
+        base = base * factor ** (rotary_dim / (rotary_dim - 2))
+    frequency = base ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64, device=device) / rotary_dim)
+    if scaling == "linear":
+        frequency = frequency / factor
+    elif scaling == "parts":
+        if original_positions is None or not high_turns > low_turns:
+            raise ValueError("scaling 'parts' needs original_positions and high_turns > low_turns")
+        turns = original_positions * frequency / (2 * math.pi)
+        keep = ((turns - low_turns) / (high_turns - low_turns)).clamp(0.0, 1.0)
+        frequency = frequency * (keep + (1.0 - keep) / factor)
+    angle = torch.arange(max_positions, dtype=torch.float64, device=device)[:, None] * frequency
+    return torch.cat([angle.cos(), angle.sin()], dim=1).float()
+
+
+def _check(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, table: torch.Tensor) -> None:
+    if q.ndim != 3 or k.ndim != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
+        raise ValueError("expected q (tokens, heads, dim) and k (tokens, kv_heads, dim), got "
+                         f"{tuple(q.shape)} and {tuple(k.shape)}")
+    if q.device.type != "cuda":
+        raise ValueError(f"q must be a CUDA tensor, got {q.device}")
+    _check_operand("q", q, q)
+    _check_operand("k", k, q)
+    _check_index("positions", positions, q.device)
+    if positions.shape != q.shape[:1]:
+        raise ValueError(f"positions must have shape ({q.shape[0]},), got {tuple(positions.shape)}")
+    _check_index("table", table, q.device, torch.float32)
+    if table.ndim != 2 or table.shape[1] % 2 or table.shape[1] > q.shape[2]:
+        raise ValueError(f"table must be (positions, rotary_dim) with an even rotary_dim of at most {q.shape[2]}, "
+                         f"got {tuple(table.shape)}")
+
+
+def _check_operand(name: str, t: torch.Tensor, like: torch.Tensor) -> None:
+    if t.dtype != like.dtype:
+        raise ValueError(f"dtype mismatch: {like.dtype} vs {name} {t.dtype}")
+    if t.device != like.device:
+        raise ValueError(f"{name} must be on {like.device}, got {t.device}")
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
+        raise ValueError(f"{name} must have a contiguous last dimension. Pass {name}.contiguous() explicitly.")
+
+
+def _output(name: str, out: torch.Tensor | None, like: torch.Tensor) -> torch.Tensor:
+    if out is None:
+        return torch.empty(like.shape, device=like.device, dtype=like.dtype)
+    if out is not like:
+        if out.shape != like.shape:
+            raise ValueError(f"{name} must have shape {tuple(like.shape)}, got {tuple(out.shape)}")
+        _check_operand(name, out, like)
+    return out
+
+
+def rotary(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    positions: torch.Tensor,
+    table: torch.Tensor,
+    *,
+    interleaved: bool = False,
+    inverse: bool = False,
+    q_out: torch.Tensor | None = None,
+    k_out: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """q ``(tokens, heads, dim)`` and k ``(tokens, kv_heads, dim)`` turned by ``positions`` (int32).
+
+    ``q_out`` / ``k_out`` may be q and k themselves. A position outside the
+    table gives NaN. ``inverse=True`` turns back: the gradient of the outputs
+    goes in, that of the inputs comes out.
+    """
+    _check(q, k, positions, table)
+    q_out, k_out = _output("q_out", q_out, q), _output("k_out", k_out, k)
+    if q.numel() or k.numel():
+        native.rotary(q, k, q_out, k_out, positions, table, interleaved=interleaved, inverse=inverse)
+    return q_out, k_out
+
+
+def rotary_to_cache(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    positions: torch.Tensor,
+    table: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    slots: torch.Tensor,
+    *,
+    interleaved: bool = False,
+    q_out: torch.Tensor | None = None,
+    k_out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """:func:`rotary`, with the turned k and v written to their cache slots.
+
+    ``slots`` (int64 ``(tokens,)``) are ``page * block + offset`` into caches
+    ``(pages, kv_heads, block, dim)``; a negative one is not written. Returns
+    the turned q; the turned k is also written to ``k_out`` when given (a
+    prompt's attention reads it packed). Two tokens with one slot: either may
+    end up in it.
+    """
+    _check(q, k, positions, table)
+    if v.shape != k.shape:
+        raise ValueError(f"v must have k's shape {tuple(k.shape)}, got {tuple(v.shape)}")
+    _check_operand("v", v, q)
+    if k_cache.ndim != 4 or k_cache.shape != v_cache.shape or k_cache.shape[1] != k.shape[1] \
+            or k_cache.shape[3] != k.shape[2] or k_cache.shape[2] < 1:
+        raise ValueError(f"expected caches (pages, {k.shape[1]}, block, {k.shape[2]}), got {tuple(k_cache.shape)} "
+                         f"and {tuple(v_cache.shape)}")
+    _check_operand("k_cache", k_cache, q)
+    _check_operand("v_cache", v_cache, q)
+    _check_index("slots", slots, q.device, torch.int64)
+    if slots.shape != q.shape[:1]:
+        raise ValueError(f"slots must have shape ({q.shape[0]},), got {tuple(slots.shape)}")
+    q_out = _output("q_out", q_out, q)
+    if k_out is not None:
+        k_out = _output("k_out", k_out, k)
+    if q.numel() or k.numel():
+        sv, skc, svc = v.stride(), k_cache.stride(), v_cache.stride()
+        cache = native.KfRotaryCache(v.data_ptr(), sv[0], sv[1], k_cache.data_ptr(), skc[0], skc[1], skc[2],
+                                     v_cache.data_ptr(), svc[0], svc[1], svc[2], k_cache.shape[0], k_cache.shape[2],
+                                     slots.data_ptr())
+        native.rotary(q, k, q_out, k_out, positions, table, interleaved=interleaved, inverse=False, cache=cache)
+    return q_out
