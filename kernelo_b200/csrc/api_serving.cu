@@ -69,6 +69,7 @@ int32_t kf_prefill_attention(int32_t dtype, const void* q, int64_t sq_row, int64
   a.seqs = seqs, a.rows = rows, a.keys = keys, a.heads = heads, a.kv_heads = kv_heads, a.dim = dim;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.causal = causal != 0;
+  if (attention_prefill_supported(a)) return launch_attention_prefill(a, *dev, static_cast<cudaStream_t>(stream));
   return launch_attention_rows(a, static_cast<cudaStream_t>(stream));
 }
 

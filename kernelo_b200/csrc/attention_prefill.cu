@@ -1,0 +1,497 @@
+// Prompt attention on the 5th-generation tensor cores: causal or not, grouped
+// heads, requests of any lengths packed without padding.
+//
+// A CTA takes 256 rows of one request and head as two tiles of 128 and walks
+// the keys 128 at a time, with the softmax's running maximum and sum:
+//
+//   S = Q K^T                      tcgen05, fp32 in TMEM, 128 x 128 per tile
+//   m' = max(m, max S),  P = 2^(c S - c m'),  l = l 2^(c m - c m') + sum P
+//   O = O 2^(c m - c m') + P V     tcgen05, P read from TMEM        (c = scale log2 e)
+//
+//   warps 0-3, 4-7   softmax of tile 0 and 1, a thread per row: S from TMEM into
+//                    registers, P (16 bit) back over the same columns.
+//   warp 8           TMA: Q once, then K and V blocks through a ring.
+//   warp 9           issues the MMAs. While one tile's warps compute their
+//                    weights the tensor cores work for the other tile.
+//
+// m is raised, and O (in TMEM) rescaled, only when a row's maximum grew by more
+// than 2^8: until then the weights are at most 256, which 16 bits and the fp32 sums
+// hold as well. P is rounded to the operands' type for the second product; l sums
+// the unrounded weights.
+//
+// Keys of the next request in a request's last block have weight zero, and
+// their V rows are zeroed in shared memory (0 x inf is NaN); a row that still
+// comes out non-finite (its own later tokens hold infinities) is recomputed key
+// by key.
+#include <cudaTypedefs.h>
+
+#include <mutex>
+
+#include "attention.cuh"
+
+namespace kf {
+namespace {
+
+constexpr int BLK = 128;       // rows of a tile, keys of a block
+constexpr int PAIR = 2 * BLK;  // rows of a CTA
+constexpr int SOFTMAX_WARPS = 8;
+constexpr int TMA_WARP = 8, MMA_WARP = 9;
+constexpr int THREADS = 10 * 32;
+constexpr uint32_t TMEM_COLS = 512;  // S0 | S1 | O0 | O1, 128 each
+constexpr float RAISE_LOG2 = 8.0f;
+constexpr uint64_t DRAIN_NS = 100000000ull;
+
+template <int DH>
+struct Shape {
+  static constexpr int HALVES = DH / 64;            // 128-byte swizzle atoms of a row
+  static constexpr int TILE = BLK * DH * 2;         // bytes of a Q, K or V tile
+  static constexpr int STAGES = DH == 128 ? 5 : 8;  // K and V tiles in flight
+  static constexpr int SMEM = 1024 + 2 * TILE + STAGES * TILE + 256;
+};
+
+struct Item {
+  int row0;       // first row of q
+  int rows;       // of the request from row0 on, at most PAIR
+  int node0;      // row0's place in its request
+  int first_key;  // first row of k and v
+  int keys;
+  int shift;      // keys - rows of the request: row i sees i + 1 + shift keys
+};
+
+// The tile pair with number `g`, counted through the requests, the last rows of
+// a request (which see the most keys) first. Called by a whole warp.
+__device__ __forceinline__ bool find_item(const AttnArgs& p, int g, int lane, Item* out) {
+  for (int r0 = 0; r0 <= p.seqs; r0 += 32) {
+    const int r = r0 + lane;
+    int begin = 0, end = 0;
+    if (r <= p.seqs) request_rows(p, r, &begin, &end);
+    const int tiles = (end - begin + PAIR - 1) / PAIR;
+    int upto = tiles;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
+    }
+    const int total = __shfl_sync(0xffffffffu, upto, 31);
+    if (g < total) {
+      if (upto > g && upto - tiles <= g) {
+        const int tile = upto - 1 - g;
+        long long first, length;
+        request_keys(p, r, end - begin, &first, &length);
+        out->node0 = tile * PAIR;
+        out->row0 = begin + out->node0;
+        out->rows = min(PAIR, end - out->row0);
+        out->first_key = static_cast<int>(first);
+        out->keys = static_cast<int>(length);
+        out->shift = static_cast<int>(length) - (end - begin);
+      }
+      return true;
+    }
+    g -= total;
+  }
+  return false;
+}
+
+// Keys that row i (of the item) sees.
+__device__ __forceinline__ int visible(const AttnArgs& p, const Item& it, int i) {
+  if (!p.causal) return it.keys;
+  return min(it.keys, max(0, it.node0 + i + 1 + it.shift));
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack_pair(float a, float b) {
+  uint32_t r;
+  if constexpr (DType<T>::code == KF_BF16) {
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  } else {
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  }
+  return r;
+}
+
+template <typename T, int DH>
+__device__ __noinline__ void redo_row(const AttnArgs& p, int t, int head, int lane) {
+  float acc[DH / 32], m, l;
+  attend_row<T, DH / 32>(p, t, head, lane, acc, &m, &l);
+  write_row<T, DH / 32>(p, t, head, lane, acc, m, l);
+}
+
+template <typename T, int DH>
+__global__ void __launch_bounds__(THREADS, 1)
+    prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                   const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ AttnArgs p, int vector_out, int* status) {
+  using S = Shape<DH>;
+  constexpr int STAGES = S::STAGES;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  uint8_t* q_tiles = smem;
+  uint8_t* ring = smem + 2 * S::TILE;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(ring + STAGES * S::TILE);
+  // bars: q[2] | full[STAGES] | empty[STAGES] | s_full[2] | p_full[2] | o_full[2]
+  __shared__ Item item;
+  __shared__ int has_item;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_word;
+  volatile int* abort_flag = &abort_word;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t q_bar = smem_u32(bars), full = q_bar + 16, empty = full + 8 * STAGES, s_full = empty + 8 * STAGES,
+                 p_full = s_full + 16, o_full = p_full + 16;
+  const int heads = static_cast<int>(p.heads);
+  const int head = static_cast<int>(blockIdx.x % heads);
+
+  if (warp == 0) {
+    const bool found = find_item(p, static_cast<int>(blockIdx.x / heads), lane, &item);
+    if (lane == 0) has_item = found;
+  } else if (warp == TMA_WARP && lane == 0) {
+    for (int i = 0; i < 2 + 2 * STAGES + 2; ++i) mbar_init(q_bar + 8 * i, 1);
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(p_full + 8 * t, SOFTMAX_WARPS / 2);
+      mbar_init(o_full + 8 * t, 1);
+    }
+    abort_word = 0;
+    mbar_init_fence();
+    tma_prefetch_desc(&tm_q);
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+  } else if (warp == MMA_WARP) {
+    tmem_alloc(smem_u32(&tmem_slot), TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  const Item it = item;
+  // key blocks of each tile: those that its last row sees some of
+  int blocks[2] = {0, 0};
+  if (has_item) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+      if (it.rows > t * BLK) blocks[t] = (visible(p, it, min(it.rows, (t + 1) * BLK) - 1) + BLK - 1) / BLK;
+  }
+  const int most = max(blocks[0], blocks[1]);
+
+  if (!has_item) {
+    // nothing of this number; only the TMEM to give back
+  } else if (warp == TMA_WARP) {
+    if (lane == 0 && most > 0) {
+      const int kv_head = head / static_cast<int>(p.heads / p.kv_heads);
+      bool ok = true;
+      int issued = 0;
+      auto load = [&](uint32_t dst, const CUtensorMap* map, uint32_t bar, int h, int row) {
+        mbar_arrive_expect_tx(bar, S::TILE);
+#pragma unroll
+        for (int x = 0; x < S::HALVES; ++x) tma_load_3d(dst + x * BLK * 128, map, bar, 64 * x, h, row);
+      };
+      auto next = [&](const CUtensorMap* map, int block) {
+        const int slot = issued % STAGES;
+        if (!mbar_wait(empty + 8 * slot, ((issued / STAGES) & 1) ^ 1, abort_flag, status, SITE_ATTN_LOAD)) return false;
+        load(smem_u32(ring + slot * S::TILE), map, full + 8 * slot, kv_head, it.first_key + block * BLK);
+        ++issued;
+        return true;
+      };
+      load(smem_u32(q_tiles), &tm_q, q_bar, head, it.row0);
+      ok = next(&tm_k, 0);
+      load(smem_u32(q_tiles + S::TILE), &tm_q, q_bar + 8, head, it.row0 + BLK);
+      for (int j = 0; ok && j < most; ++j) {
+        ok = next(&tm_v, j);
+        if (ok && j + 1 < most) ok = next(&tm_k, j + 1);
+      }
+      if (!ok) {  // let the copies in flight land before the shared memory goes away
+        for (int t = 0; t < 2; ++t) mbar_wait(q_bar + 8 * t, 0, nullptr, status, SITE_DRAIN, DRAIN_NS);
+        for (int s = 0; s < STAGES && s < issued; ++s)
+          mbar_wait(full + 8 * s, ((issued - 1 - s) / STAGES) & 1, nullptr, status, SITE_DRAIN, DRAIN_NS);
+      }
+    }
+  } else if (warp == MMA_WARP) {
+    if (most > 0) {
+      const uint32_t fmt = DType<T>::code == KF_BF16 ? 1u : 0u;
+      const uint32_t idesc_s = instr_desc_f16(fmt, 0, 0, BLK, BLK);
+      const uint32_t idesc_o = instr_desc_f16(fmt, 0, 1, BLK, DH);
+      const uint64_t q_desc = smem_desc_sw128(smem_u32(q_tiles), 16, 1024);
+      int taken = 0;  // ring tiles waited for
+      bool ok = true;
+      auto wait = [&](uint32_t bar, int parity) {  // the lanes stay together, also when a wait gives up
+        ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, SITE_ATTN_MMA));
+        tc_fence_after();
+      };
+      auto wait_tile = [&]() {
+        const int slot = taken % STAGES;
+        wait(full + 8 * slot, (taken / STAGES) & 1);
+        ++taken;
+        return slot;
+      };
+      auto scores = [&](int t, int slot) {  // S_t = Q_t K^T
+        const uint64_t a = q_desc + static_cast<uint64_t>(t * S::TILE / 16);
+        const uint64_t b = smem_desc_sw128(smem_u32(ring + slot * S::TILE), 16, 1024);
+#pragma unroll
+        for (int k = 0; k < DH / 16; ++k) {
+          const uint64_t step = static_cast<uint64_t>((k / 4) * (BLK * 128 / 16) + (k % 4) * 2);
+          tc_mma_f16(tmem + t * BLK, a + step, b + step, idesc_s, k > 0);
+        }
+        tc_commit(s_full + 8 * t);
+      };
+      auto products = [&](int t, int slot, bool accumulate) {  // O_t += P_t V
+        const uint64_t b = smem_desc_sw128(smem_u32(ring + slot * S::TILE), BLK * 128, 1024);
+#pragma unroll
+        for (int k = 0; k < BLK / 16; ++k)
+          tc_mma_f16_ta(tmem + 2 * BLK + t * BLK, tmem + t * BLK + 8 * k, b + static_cast<uint64_t>(k * 128), idesc_o,
+                        accumulate || k > 0);
+        tc_commit(o_full + 8 * t);
+      };
+      int k_slot = wait_tile();
+      for (int t = 0; ok && t < 2; ++t) {
+        wait(q_bar + 8 * t, 0);
+        if (ok && blocks[t] > 0 && lane == 0) scores(t, k_slot);
+      }
+      if (ok && lane == 0) tc_commit(empty + 8 * k_slot);
+      for (int j = 0; ok && j < most; ++j) {
+        const int v_slot = wait_tile();
+        if (!ok) break;
+        const int held = it.keys - j * BLK;  // of the request's keys in this block
+        if (held < BLK) {
+          for (int i = lane; i < (BLK - held) * S::HALVES * 8; i += 32) {
+            const int h = i / ((BLK - held) * 8), rest = i - h * (BLK - held) * 8;
+            *reinterpret_cast<uint4*>(ring + v_slot * S::TILE + h * BLK * 128 + held * 128 + rest * 16) =
+                make_uint4(0u, 0u, 0u, 0u);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+        bool k_ready = false;
+        for (int t = 0; ok && t < 2; ++t) {
+          if (j >= blocks[t]) continue;
+          wait(p_full + 8 * t, j & 1);
+          if (!ok) break;
+          if (lane == 0) products(t, v_slot, j > 0);
+          if (j + 1 < blocks[t]) {
+            if (!k_ready) {
+              k_slot = wait_tile();
+              if (!ok) break;
+              k_ready = true;
+            }
+            if (lane == 0) scores(t, k_slot);
+          }
+        }
+        if (ok && lane == 0) {
+          tc_commit(empty + 8 * v_slot);
+          if (k_ready) tc_commit(empty + 8 * k_slot);
+        }
+        __syncwarp();
+      }
+    }
+  } else {
+    const int t = warp >> 2;
+    const int row = (warp & 3) * 32 + lane;  // of the tile
+    const int i = t * BLK + row;             // of the item
+    const bool valid = i < it.rows;
+    const int limit = valid ? visible(p, it, i) : 0;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const uint32_t s_addr = lanes + t * BLK, o_addr = lanes + 2 * BLK + t * BLK;
+    const float c = p.scale_log2;
+    float m = -INFINITY, l = 0.0f;
+    bool ok = true;
+    for (int j = 0; j < blocks[t]; ++j) {
+      ok = mbar_wait(s_full + 8 * t, j & 1, abort_flag, status, SITE_ATTN_SOFTMAX);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      float s[BLK];
+#pragma unroll
+      for (int x = 0; x < BLK; x += 32) tmem_ld_32(s_addr + x, reinterpret_cast<uint32_t*>(s + x));
+      tmem_ld_wait();
+      const int left = limit - j * BLK;
+      if (left < BLK) {
+#pragma unroll
+        for (int x = 0; x < BLK; ++x)
+          if (x >= left) s[x] = -INFINITY;
+      }
+      __syncwarp();
+      float top[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+      for (int x = 4; x < BLK; x += 8) {
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+          top[y] = x + 4 + y < BLK ? fmaxf(fmaxf(top[y], s[x + y]), s[x + 4 + y]) : fmaxf(top[y], s[x + y]);
+      }
+      const float m_new = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
+      if (j == 0) {
+        m = m_new;
+      } else if (__any_sync(0xffffffffu, (m_new - m) * c > RAISE_LOG2)) {
+        ok = mbar_wait(o_full + 8 * t, (j - 1) & 1, abort_flag, status, SITE_ATTN_SOFTMAX);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        const float fix = m_new > m ? ex2_ftz((m - m_new) * c) : 1.0f;
+        l *= fix;
+        m = m_new;
+#pragma unroll 1
+        for (int x = 0; x < DH; x += 32) {
+          uint32_t o[32];
+          tmem_ld_32(o_addr + x, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * fix);
+          tmem_st_32(o_addr + x, o);
+        }
+      }
+      const float cm = m == -INFINITY ? 0.0f : m * c;
+      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int x = 0; x < BLK; x += 64) {
+        uint32_t w[32];
+#pragma unroll
+        for (int y = 0; y < 64; y += 2) {
+          const float a = ex2_ftz(fmaf(s[x + y], c, -cm)), b = ex2_ftz(fmaf(s[x + y + 1], c, -cm));
+          sum[(y / 2) & 3] += a + b;
+          w[y / 2] = pack_pair<T>(a, b);
+        }
+        tmem_st_32(s_addr + x / 2, w);
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_full + 8 * t);
+    }
+    if (ok && blocks[t] > 0) {
+      ok = mbar_wait(o_full + 8 * t, (blocks[t] - 1) & 1, abort_flag, status, SITE_ATTN_SOFTMAX);
+      ok = __all_sync(0xffffffffu, ok);
+      tc_fence_after();
+    }
+    if (ok && it.rows > t * BLK) {
+      const int q_row = it.row0 + i;
+      T* out = static_cast<T*>(p.out) + static_cast<long long>(q_row) * p.so_t + head * p.so_h;
+      const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+      float bad = 0.0f;  // NaN if anything in the row is not finite
+#pragma unroll 1
+      for (int x = 0; x < DH; x += 32) {
+        uint32_t o[32];
+        if (blocks[t] > 0) {
+          tmem_ld_32(o_addr + x, o);
+          tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int y = 0; y < 32; ++y) o[y] = 0u;
+        }
+        uint32_t w[16];
+#pragma unroll
+        for (int y = 0; y < 32; y += 2) {
+          // a row that sees nothing may hold anything in O: its result is zero
+          const float a = l > 0.0f ? __uint_as_float(o[y]) * inv : 0.0f;
+          const float b = l > 0.0f ? __uint_as_float(o[y + 1]) * inv : 0.0f;
+          bad = fmaf(a, 0.0f, fmaf(b, 0.0f, bad));
+          w[y / 2] = pack_pair<T>(a, b);
+        }
+        if (valid) {
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            if (x + 8 * y >= p.dim) break;
+            if (vector_out) {
+              *reinterpret_cast<uint4*>(out + x + 8 * y) = make_uint4(w[4 * y], w[4 * y + 1], w[4 * y + 2], w[4 * y + 3]);
+            } else {
+              const T* e = reinterpret_cast<const T*>(w + 4 * y);
+#pragma unroll
+              for (int z = 0; z < 8; ++z) out[x + 8 * y + z] = e[z];
+            }
+          }
+        }
+        __syncwarp();
+      }
+      if (p.lse != nullptr && valid)
+        p.lse[static_cast<long long>(q_row) * heads + head] =
+            l > 0.0f ? m * c * 0.69314718055994530942f + logf(l) : -INFINITY;
+      // l that is NaN (a score is) has left zeros: those rows too
+      uint32_t again = __ballot_sync(0xffffffffu, valid && (!(bad == 0.0f) || !(l >= 0.0f && l < INFINITY)));
+      while (again != 0) {
+        const int src = __ffs(again) - 1;
+        again &= again - 1;
+        redo_row<T, DH>(p, __shfl_sync(0xffffffffu, q_row, src), head, lane);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == MMA_WARP) tmem_dealloc(tmem, TMEM_COLS);
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encoder() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* sym = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(sym);
+  });
+  return fn;
+}
+
+// [rows, heads, dim] as boxes of 128 rows x 64 elements of one head; elements
+// past the head and rows past the last are filled with zeros.
+int encode_heads(CUtensorMap* map, int dtype, const void* ptr, int64_t rows, int64_t heads, int64_t dim, int64_t s_row,
+                 int64_t s_head) {
+  auto enc = encoder();
+  if (enc == nullptr) return set_error(KF_ERR_LAUNCH, "cuTensorMapEncodeTiled unavailable");
+  const int64_t whole = ceil_div(dim, 8) * 8;
+  // a dimension of one has no stride to speak of
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(dim), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(2 * (heads > 1 ? s_head : whole)),
+                                 static_cast<cuuint64_t>(2 * (rows > 1 ? s_row : whole))};
+  const cuuint32_t box[3] = {64, 1, BLK}, unit[3] = {1, 1, 1};
+  const CUresult r = enc(map, dtype == KF_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                         const_cast<void*>(ptr), dims, strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return set_error(KF_ERR_UNALIGNED, "prompt attention: cuTensorMapEncodeTiled rejected an operand (error " +
+                                           std::to_string(r) + ")");
+  return KF_OK;
+}
+
+bool on_grid(const void* ptr, int64_t s_row, int64_t rows, int64_t s_head, int64_t heads) {
+  const auto fits = [](int64_t s, int64_t n) { return n <= 1 || (s > 0 && s % 8 == 0 && s < (1ll << 38)); };
+  return reinterpret_cast<uintptr_t>(ptr) % 16 == 0 && fits(s_row, rows) && fits(s_head, heads);
+}
+
+template <typename T, int DH>
+int launch_typed(const AttnArgs& a, const DeviceInfo& dev, cudaStream_t stream) {
+  CUtensorMap q, k, v;
+  int rc = encode_heads(&q, a.dtype, a.q, a.rows, a.heads, a.dim, a.sq_t, a.sq_h);
+  if (rc == KF_OK) rc = encode_heads(&k, a.dtype, a.k, a.keys, a.kv_heads, a.dim, a.sk_t, a.sk_h);
+  if (rc == KF_OK) rc = encode_heads(&v, a.dtype, a.v, a.keys, a.kv_heads, a.dim, a.sv_t, a.sv_h);
+  if (rc != KF_OK) return rc;
+  static std::once_flag once;
+  static cudaError_t attr = cudaSuccess;
+  std::call_once(once, [] {
+    attr = cudaFuncSetAttribute(prefill_kernel<T, DH>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<DH>::SMEM);
+  });
+  if (attr != cudaSuccess) return cuda_error(attr, "prefill attributes");
+  const int64_t blocks = (a.rows / PAIR + a.seqs + 1) * a.heads;
+  const int vector_out = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.so_t % 8 == 0 && a.so_h % 8 == 0;
+  prefill_kernel<T, DH><<<static_cast<unsigned>(blocks), THREADS, Shape<DH>::SMEM, stream>>>(q, k, v, a, vector_out,
+                                                                                            dev.status);
+  const cudaError_t err = cudaGetLastError();
+  return err == cudaSuccess ? KF_OK : cuda_error(err, "launch(prompt attention)");
+}
+
+}  // namespace
+
+bool attention_prefill_supported(const AttnArgs& a) {
+  return (a.dtype == KF_FP16 || a.dtype == KF_BF16) && a.dim <= 128 && a.dim % 8 == 0 && a.keys > 0 &&
+         a.scale_log2 > 0.0f && on_grid(a.q, a.sq_t, a.rows, a.sq_h, a.heads) &&
+         on_grid(a.k, a.sk_t, a.keys, a.sk_h, a.kv_heads) && on_grid(a.v, a.sv_t, a.keys, a.sv_h, a.kv_heads) &&
+         (a.rows / PAIR + a.seqs + 1) * a.heads <= 0x7fffffffll;
+}
+
+int launch_attention_prefill(const AttnArgs& a, const DeviceInfo& dev, cudaStream_t stream) {
+  if (a.dtype == KF_FP16)
+    return a.dim <= 64 ? launch_typed<__half, 64>(a, dev, stream) : launch_typed<__half, 128>(a, dev, stream);
+  return a.dim <= 64 ? launch_typed<__nv_bfloat16, 64>(a, dev, stream) : launch_typed<__nv_bfloat16, 128>(a, dev, stream);
+}
+
+}  // namespace kf

@@ -262,6 +262,10 @@ struct AttnArgs {
 constexpr int64_t ATTN_MAX_DIM = 256;
 // A warp per row and head, key by key: every type, stride and mask.
 int launch_attention_rows(const AttnArgs& args, cudaStream_t stream);
+// Packed prompts on tcgen05 tiles (attention_prefill.cu): fp16/bf16, heads of up
+// to 128 elements on the 16-byte grid, a positive scale.
+bool attention_prefill_supported(const AttnArgs& args);
+int launch_attention_prefill(const AttnArgs& args, const DeviceInfo& dev, cudaStream_t stream);
 
 // Rotary positions (rotary.cu): q and k turned by their positions' angles; with
 // a cache, k and v also go to the slots of their pages.
