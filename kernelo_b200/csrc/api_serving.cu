@@ -83,7 +83,7 @@ int32_t kf_tree_attention(int32_t dtype, const void* q, int64_t sq_row, int64_t 
   int rc = check_heads(dtype, rows, seqs, heads, kv_heads, dim);
   if (rc != KF_OK) return rc;
   if (table_cols < 0 || pages < 0 || mask_words < 0) return invalid("negative size");
-  if (block_size < 1) return invalid("block_size must be positive");
+  if (block_size < 1 || block_size > INT32_LIMIT) return invalid("block_size must be positive and fit 32 bits");
   if (!std::isfinite(scale)) return invalid("scale must be finite");
   if (rows == 0 || heads == 0 || dim == 0) return KF_OK;
   if (q == nullptr || out == nullptr || (seqs > 0 && context == nullptr) ||
@@ -110,15 +110,22 @@ int32_t kf_tree_attention(int32_t dtype, const void* q, int64_t sq_row, int64_t 
   a.seqs = seqs, a.rows = rows, a.heads = heads, a.kv_heads = kv_heads, a.dim = dim;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.workspace = workspace, a.workspace_bytes = workspace_bytes;
+  if (attention_tree_supported(a)) return launch_attention_tree(a, *dev, static_cast<cudaStream_t>(stream));
   return launch_attention_rows(a, static_cast<cudaStream_t>(stream));
 }
 
 int64_t kf_tree_attention_workspace_bytes(int32_t device, int32_t dtype, int64_t seqs, int64_t rows, int64_t heads,
                                           int64_t kv_heads, int64_t dim) {
-  const int rc = check_heads(dtype, rows, seqs, heads, kv_heads, dim);
+  int rc = check_heads(dtype, rows, seqs, heads, kv_heads, dim);
   if (rc != KF_OK) return -rc;
-  (void)device;
-  return 0;
+  if (heads == 0 || dtype == KF_FP32) return 0;
+  DeviceInfo* dev = nullptr;
+  rc = device_info(device, &dev);
+  if (rc != KF_OK) return -rc;
+  AttnArgs a;
+  a.dtype = dtype;
+  a.seqs = seqs, a.rows = rows, a.heads = heads, a.kv_heads = kv_heads, a.dim = dim;
+  return attention_tree_workspace_bytes(a, *dev);
 }
 
 int32_t kf_rotary(int32_t dtype, const void* q, int64_t sq_row, int64_t sq_head, void* q_out, int64_t sqo_row,

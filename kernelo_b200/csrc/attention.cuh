@@ -35,7 +35,8 @@ __device__ __forceinline__ void request_keys(const AttnArgs& p, int r, int nodes
   if (p.paged) {
     const long long room = p.table_cols * p.block_size;
     const long long n = static_cast<long long>(max(__ldg(p.context + r), 0)) + nodes;
-    *length = n < room ? n : room;
+    // positions are counted in 31 bits
+    *length = min(min(n, room), 0x7fffff00ll);
     return;
   }
   const int keys = static_cast<int>(p.keys);

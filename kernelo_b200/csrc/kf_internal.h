@@ -266,6 +266,11 @@ int launch_attention_rows(const AttnArgs& args, cudaStream_t stream);
 // to 128 elements on the 16-byte grid, a positive scale.
 bool attention_prefill_supported(const AttnArgs& args);
 int launch_attention_prefill(const AttnArgs& args, const DeviceInfo& dev, cudaStream_t stream);
+// New tokens over a paged cache on mma.sync tiles (attention_tree.cu): fp16/bf16,
+// heads of up to 128 elements on the 16-byte grid.
+bool attention_tree_supported(const AttnArgs& args);
+int64_t attention_tree_workspace_bytes(const AttnArgs& args, const DeviceInfo& dev);
+int launch_attention_tree(const AttnArgs& args, const DeviceInfo& dev, cudaStream_t stream);
 
 // Rotary positions (rotary.cu): q and k turned by their positions' angles; with
 // a cache, k and v also go to the slots of their pages.
