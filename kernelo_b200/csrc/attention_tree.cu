@@ -17,18 +17,22 @@
 //   s = scale log2(e) q k^T,  m' = max(m, max s),  p = 2^(s - m'),
 //   l = l 2^(m - m') + sum p,  O = O 2^(m - m') + p v       (mma.sync, fp32 sums)
 //
-// K and V blocks arrive by 16-byte cp.async into a ring of stages, each row at
-// the page its block table names; rows past the request's end or without a page
-// are zeros, and weights of keys a row does not see are zero. A row that comes
-// out non-finite (a node it does not see holds infinities) is recomputed key by key.
+// One more warp loads: it reads the block table ahead and fills a ring of K and
+// V blocks, with one TMA box per run of keys that is whole in any page (gcd of
+// page and block, 8 keys at least), or where pages are not multiples of 8 keys
+// with 16-byte cp.async. Pages a table does not name are read as zeros (a box
+// past the last page); V rows past the request's end are zeroed in shared memory
+// (0 x NaN is NaN); weights of keys that a row does not see are zero. A row that
+// comes out non-finite (a node it does not see holds infinities) is recomputed key by key.
 //
 // With one new token and G heads to a key head, G of the 16 rows are real: the
 // products are free beside the cache's bytes, which bound the call until
 // nodes x G passes about 64.
-#include <cuda.h>
+#include <cudaTypedefs.h>
 
 #include <initializer_list>
 #include <mutex>
+#include <numeric>
 #include <string>
 
 #include "attention.cuh"
@@ -42,16 +46,19 @@ constexpr int MIN_BLOCKS = 4; // a CTA's run: fewer blocks cost more to join tha
 template <int DP_, int R_, int C_, int STAGES_>
 struct Shape {
   static constexpr int DP = DP_, R = R_, C = C_, STAGES = STAGES_;
-  static constexpr int M = 16 * R, WARPS = R * C, THREADS = 32 * WARPS;
-  static constexpr int ROW = DP * 2;             // bytes of a K or V row in the ring
-  static constexpr int TILE = KEYS * ROW;
-  static constexpr int PITCH = DP + 8;           // floats of a row of the joined result
-  static constexpr int SMEM = STAGES * 2 * TILE + M * PITCH * 4 + 2 * M * C * 4 + STAGES * KEYS + 64;
+  // With 8 warps of products the loading warp gets a warpgroup of its own, whose
+  // registers go to them: 3 x 168 a thread become 2 x 224 and 56.
+  static constexpr int M = 16 * R, WARPS = R * C, LOADERS = WARPS == 8 ? 4 : 1, THREADS = 32 * (WARPS + LOADERS);
+  static constexpr int HALVES = DP == 128 ? 2 : 1;  // boxes of at most 128 bytes a row
+  static constexpr int TILE = KEYS * DP * 2;        // bytes of a K or V block in the ring
+  static constexpr int PITCH = DP + 8;              // floats of a row of the joined result
+  static constexpr int SMEM = 1024 + STAGES * 2 * TILE + M * PITCH * 4 + 2 * M * C * 4 + STAGES * 24;
   static constexpr int64_t PARTIAL = M * DP + 2 * M;  // floats of a partial result
 };
 
 // Workspace: arrival counters of items cut between CTAs, one per CTA, at a fixed
 // place and zero between calls; then two partial results per CTA.
+constexpr uint64_t DRAIN_NS = 100000000ull;
 constexpr int64_t COUNTER_BYTES = 64 * 1024;
 
 struct Run {
@@ -60,29 +67,29 @@ struct Run {
 
 // The block that a CTA works on: request, key head, row tile, block of keys.
 struct Cursor {
-  long long unit, item;  // number of this unit, and of the item's first
+  int left;  // units of the CTA's run from this one on
   int r, head, tile, blk;
   int row0, nodes, tiles, blocks;
-  long long context, length;
+  int context, length;
 };
 
 __device__ __forceinline__ void load_request(const AttnArgs& p, Cursor& c, int group, int m) {
   int begin, end;
   request_rows(p, c.r, &begin, &end);
-  long long first;
-  request_keys(p, c.r, end - begin, &first, &c.length);
+  long long first, length;
+  request_keys(p, c.r, end - begin, &first, &length);
+  c.length = static_cast<int>(length);
   c.row0 = begin;
   c.nodes = end - begin;
   c.context = c.r < p.seqs ? max(__ldg(p.context + c.r), 0) : 0;
   c.tiles = static_cast<int>((static_cast<long long>(c.nodes) * group + m - 1) / m);
-  c.blocks = max(1, static_cast<int>((c.length + KEYS - 1) / KEYS));
+  c.blocks = max(1, (c.length + KEYS - 1) / KEYS);
 }
 
 __device__ __forceinline__ void advance(const AttnArgs& p, Cursor& c, int group, int m) {
-  ++c.unit;
+  --c.left;
   if (++c.blk < c.blocks) return;
   c.blk = 0;
-  c.item = c.unit;
   if (++c.tile < c.tiles) return;
   c.tile = 0;
   if (++c.head < p.kv_heads) return;
@@ -96,11 +103,6 @@ __device__ __forceinline__ void advance(const AttnArgs& p, Cursor& c, int group,
 __device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, bool present) {
   // nothing is read where the row is absent: 16 bytes of zeros
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(present ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 __device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
@@ -116,14 +118,15 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t add
                : "memory");
 }
 
-// Byte offset of 16-byte chunk `chunk` of row `row` in a tile: chunks are XORed
-// with the row so that eight rows of one column meet eight bank groups.
+// Byte offset of 16-byte chunk `chunk` of row `row` in a tile, as TMA's swizzles
+// place it: rows of 128 bytes (64 elements, a second half behind the first) or of
+// 64 bytes, chunks XORed so that eight rows of one column meet eight bank groups.
 template <int DP>
 __device__ __forceinline__ uint32_t chunk_at(int row, int chunk) {
   if constexpr (DP >= 64) {
-    return static_cast<uint32_t>(row * (DP * 2) + ((chunk ^ (row & 7)) << 4));
-  } else {  // two rows to 128 bytes
-    return static_cast<uint32_t>(row * (DP * 2) + ((chunk ^ ((row >> 1) & 3)) << 4));
+    return static_cast<uint32_t>((chunk >> 3) * (KEYS * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
+  } else {
+    return static_cast<uint32_t>(row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4));
   }
 }
 
@@ -180,32 +183,43 @@ struct Divisor {
   int shift;
 };
 
-template <typename T, typename S>
+template <typename T, typename S, bool BULK>
 __global__ void __launch_bounds__(S::THREADS, S::WARPS == 4 ? 2 : 1)
-    tree_kernel(const __grid_constant__ AttnArgs p, const Divisor by_page, int vector_out) {
+    tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                const __grid_constant__ AttnArgs p, const Divisor by_page, int box_rows, int vector_out, int* status) {
   constexpr int DP = S::DP, C = S::C, M = S::M, STAGES = S::STAGES, THREADS = S::THREADS;
-  constexpr int KW = KEYS / C;            // keys of a warp
-  constexpr int CHUNKS = DP / 8;          // 16-byte chunks of a row
-  constexpr int ROWS = THREADS / CHUNKS;  // rows a pass of all threads loads
-  constexpr int PASSES = KEYS / ROWS;
-  extern __shared__ __align__(128) uint8_t smem[];
+  constexpr int KW = KEYS / C;  // keys of a warp
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  // ring | joined | maxima and sums (16-byte vectors up to here) | barriers | present
   float* joined = reinterpret_cast<float*>(smem + STAGES * 2 * S::TILE);
   float* part_m = joined + M * S::PITCH;
   float* part_l = part_m + M * C;
-  uint8_t* present = reinterpret_cast<uint8_t*>(part_l + M * C);
-  __shared__ long long scan[S::WARPS];
+  uint64_t* bars = reinterpret_cast<uint64_t*>(part_l + M * C);
+  volatile uint32_t* present = reinterpret_cast<volatile uint32_t*>(bars + 2 * STAGES);  // a bit per key of each stage
+  static_assert(S::TILE % 1024 == 0 && (M * S::PITCH) % 4 == 0 && S::PITCH % 4 == 0 && (M * C) % 2 == 0 && S::PARTIAL % 4 == 0,
+                "vectors of 16 bytes and barriers of 8");
+  __shared__ long long scan[S::WARPS + S::LOADERS];
   __shared__ long long found_rest;
-  __shared__ int found_r, last_one;
+  __shared__ int found_r, last_one, abort_word;
+  volatile int* abort_flag = &abort_word;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int wr = warp / C, wc = warp % C;  // row group, key group
   const int group = static_cast<int>(p.heads / p.kv_heads);
-  const int chunks = static_cast<int>(p.dim) / 8;
-  const uint32_t ring = smem_u32(smem);
+  const uint32_t ring = smem_u32(smem), full = smem_u32(bars), empty = full + 8 * STAGES;
   float* partials = reinterpret_cast<float*>(static_cast<uint8_t*>(p.workspace) + COUNTER_BYTES);
   int* counters = static_cast<int*>(p.workspace);
 
-  if (chunks < CHUNKS)  // columns past the head stay zero
+  if (tid == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(full + 8 * s, BULK ? 1 : 33);
+      mbar_init(empty + 8 * s, S::WARPS);
+    }
+    abort_word = 0;
+    mbar_init_fence();
+  }
+  if (!BULK && p.dim < DP)  // columns past the head stay zero
     for (int i = tid; i < STAGES * 2 * S::TILE / 16; i += THREADS)
       reinterpret_cast<uint4*>(smem)[i] = make_uint4(0u, 0u, 0u, 0u);
 
@@ -233,7 +247,7 @@ __global__ void __launch_bounds__(S::THREADS, S::WARPS == 4 ? 2 : 1)
     long long before = 0;
     run.total = 0;
 #pragma unroll
-    for (int w = 0; w < S::WARPS; ++w) {
+    for (int w = 0; w < S::WARPS + S::LOADERS; ++w) {
       if (w < warp) before += scan[w];
       run.total += scan[w];
     }
@@ -255,6 +269,7 @@ __global__ void __launch_bounds__(S::THREADS, S::WARPS == 4 ? 2 : 1)
   }
   const long long first = run.per * blockIdx.x, stop = min(first + run.per, run.total);
   if (first >= stop) return;
+  const int units = static_cast<int>(stop - first);
   Cursor at;
   at.r = found_r;
   load_request(p, at, group, M);
@@ -264,56 +279,114 @@ __global__ void __launch_bounds__(S::THREADS, S::WARPS == 4 ? 2 : 1)
     at.blk = static_cast<int>(rest - static_cast<long long>(tile) * at.blocks);
     at.head = tile / at.tiles;
     at.tile = tile - at.head * at.tiles;
-    at.unit = first;
-    at.item = first - at.blk;
+    at.left = units;
   }
-  Cursor ahead = at;  // the next block to load
 
-  const int load_chunk = tid % CHUNKS, load_row = tid / CHUNKS;
-  auto load = [&](int stage) {
-    if (ahead.unit < stop) {
-      const T* k = static_cast<const T*>(p.k) + ahead.head * p.sk_h + load_chunk * 8;
-      const T* v = static_cast<const T*>(p.v) + ahead.head * p.sv_h + load_chunk * 8;
-      int page[PASSES], slot[PASSES];
-#pragma unroll
-      for (int i = 0; i < PASSES; ++i) {
-        const long long pos = static_cast<long long>(ahead.blk) * KEYS + i * ROWS + load_row;
-        page[i] = -1;
-        slot[i] = 0;
-        if (pos < ahead.length) {
+  if (warp >= S::WARPS) {
+    // ------------------------------------------------------------ loads
+    if constexpr (S::LOADERS == 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp > S::WARPS) return;
+    constexpr int OPS = 2 * S::HALVES;  // boxes of one run of keys
+    int slot = 0, phase = 1;
+    for (; at.left > 0; advance(p, at, group, M)) {
+      const int pos0 = at.blk * KEYS;
+      uint32_t bits[2] = {0u, 0u};
+      if constexpr (BULK) {
+        const int part = lane / OPS, op = lane % OPS;
+        const bool mine = part * box_rows < KEYS;
+        const int pos = pos0 + part * box_rows;
+        int page = -1, in_page = 0;
+        if (mine && pos < at.length) {
           const uint32_t n = static_cast<uint32_t>(pos);
           const uint32_t col = static_cast<uint32_t>(static_cast<uint64_t>(n) * by_page.mul >> by_page.shift);
-          slot[i] = static_cast<int>(n - col * static_cast<uint32_t>(p.block_size));
-          page[i] = __ldg(p.table + ahead.r * p.table_stride + col);
+          in_page = static_cast<int>(n - col * static_cast<uint32_t>(p.block_size));
+          page = __ldg(p.table + at.r * p.table_stride + col);
+          if (page < 0 || page >= p.pages) page = -1;
         }
-      }
+        if (page >= 0) {
+          const int rows = min(box_rows, at.length - pos);
+          const unsigned long long b = (~0ull >> (64 - rows)) << (part * box_rows);
+          bits[0] = static_cast<uint32_t>(b);
+          bits[1] = static_cast<uint32_t>(b >> 32);
+        }
+        bits[0] = __reduce_or_sync(0xffffffffu, bits[0]);
+        bits[1] = __reduce_or_sync(0xffffffffu, bits[1]);
+        mbar_wait(empty + 8 * slot, phase, abort_flag, status, SITE_ATTN_LOAD);
+        __syncwarp();
+        if (lane == 0) {
+          present[2 * slot] = bits[0];
+          present[2 * slot + 1] = bits[1];
+          mbar_arrive_expect_tx(full + 8 * slot, 2 * S::TILE);
+        }
+        __syncwarp();
+        if (mine) {
+          const int half = op >> 1;
+          const uint32_t dst = ring + (2 * slot + (op & 1)) * S::TILE + half * (KEYS * 128) + part * box_rows * (DP >= 64 ? 128 : 64);
+          tma_load_4d(dst, (op & 1) ? &tm_v : &tm_k, full + 8 * slot, 64 * half, in_page, at.head,
+                      page >= 0 ? page : static_cast<int>(p.pages));
+        }
+        __syncwarp();
+      } else {
+        // a lane copies two rows of keys
+        const int chunks = static_cast<int>(p.dim) / 8;
+        int page[2], in_page[2];
 #pragma unroll
-      for (int i = 0; i < PASSES; ++i) {
-        const int row = i * ROWS + load_row;
-        const bool here = page[i] >= 0 && page[i] < p.pages;
-        const long long pg = here ? page[i] : 0, sl = here ? slot[i] : 0;
-        const uint32_t dst = ring + stage * 2 * S::TILE + chunk_at<DP>(row, load_chunk);
-        if (load_chunk < chunks) {
-          cp_async_16(dst, k + (pg * p.sk_p + sl * p.sk_t), here);
-          cp_async_16(dst + S::TILE, v + (pg * p.sv_p + sl * p.sv_t), here);
+        for (int i = 0; i < 2; ++i) {
+          const int pos = pos0 + lane + 32 * i;
+          page[i] = -1;
+          in_page[i] = 0;
+          if (pos < at.length) {
+            const uint32_t n = static_cast<uint32_t>(pos);
+            const uint32_t col = static_cast<uint32_t>(static_cast<uint64_t>(n) * by_page.mul >> by_page.shift);
+            in_page[i] = static_cast<int>(n - col * static_cast<uint32_t>(p.block_size));
+            page[i] = __ldg(p.table + at.r * p.table_stride + col);
+            if (page[i] < 0 || page[i] >= p.pages) page[i] = -1;
+          }
+          bits[i] = __ballot_sync(0xffffffffu, page[i] >= 0);
         }
-        if (load_chunk == 0) present[stage * KEYS + row] = here;
+        mbar_wait(empty + 8 * slot, phase, abort_flag, status, SITE_ATTN_LOAD);
+        __syncwarp();
+        if (lane < 2) present[2 * slot + lane] = bits[lane];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const long long pg = max(page[i], 0);
+          const T* k = static_cast<const T*>(p.k) + at.head * p.sk_h + pg * p.sk_p + in_page[i] * p.sk_t;
+          const T* v = static_cast<const T*>(p.v) + at.head * p.sv_h + pg * p.sv_p + in_page[i] * p.sv_t;
+          const uint32_t dst = ring + 2 * slot * S::TILE;
+          for (int c = 0; c < chunks; ++c) {
+            cp_async_16(dst + chunk_at<DP>(lane + 32 * i, c), k + 8 * c, page[i] >= 0);
+            cp_async_16(dst + S::TILE + chunk_at<DP>(lane + 32 * i, c), v + 8 * c, page[i] >= 0);
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(full + 8 * slot);  // for `present`; and each lane once its copies have landed
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(full + 8 * slot) : "memory");
       }
-      advance(p, ahead, group, M);
+      if (++slot == STAGES) {
+        slot = 0;
+        phase ^= 1;
+      }
     }
-    cp_async_commit();  // an empty group keeps the count
-  };
+    if (*abort_flag) {
+      // a wait gave up: let the copies in flight land before the shared memory goes away
+      for (int s = 0; s < STAGES && s < units; ++s)
+        mbar_wait(full + 8 * s, ((units - 1 - s) / STAGES) & 1, nullptr, status, SITE_DRAIN, DRAIN_NS);
+    }
+    return;
+  }
 
-  if (chunks < CHUNKS) __syncthreads();  // the zeros, before any copy lands
-#pragma unroll
-  for (int s = 0; s < STAGES - 1; ++s) load(s);
-
+  // -------------------------------------------------------------- products
+  if constexpr (S::LOADERS == 4) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+  // A wait that gives up records its status and the warps go on together (the
+  // results are lost, the barriers between them are not).
+  const int wr = warp / C, wc = warp % C;  // row group, key group
+  const auto join = [] { asm volatile("bar.sync 1, %0;" ::"n"(32 * S::WARPS) : "memory"); };
   uint32_t qf[DP / 16][4];
   float o[DP / 8][4];
   float m[2], l[2];
-  int stage = 0;
+  int stage = 0, phase = 0;
   bool fresh = true;
-  while (at.unit < stop) {
+  while (at.left > 0) {
     const int tile_row = at.tile * M + wr * 16 + (lane >> 2);  // of this lane's first row, over nodes x group
     const int real = at.nodes * group;                         // rows of the item
     if (fresh) {
@@ -337,10 +410,8 @@ __global__ void __launch_bounds__(S::THREADS, S::WARPS == 4 ? 2 : 1)
 #pragma unroll
       for (int n = 0; n < DP / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
     }
-    cp_async_wait<STAGES - 2>();
-    __syncthreads();  // the block has landed, and everyone is done with the one before
-    load(stage == 0 ? STAGES - 1 : stage - 1);
-
+    mbar_wait(full + 8 * stage, phase, abort_flag, status, SITE_ATTN_SOFTMAX);
+    __syncwarp();
     const uint32_t k_tile = ring + stage * 2 * S::TILE, v_tile = k_tile + S::TILE;
     float s[KW / 8][4];
 #pragma unroll
@@ -357,29 +428,43 @@ __global__ void __launch_bounds__(S::THREADS, S::WARPS == 4 ? 2 : 1)
       }
     }
     // base-2 scores, -inf where a row sees nothing
-    const long long key0 = static_cast<long long>(at.blk) * KEYS + wc * KW;
+    const int key0 = at.blk * KEYS + wc * KW;
     const int node_of[2] = {tile_row / group, (tile_row + 8) / group};
     const bool drafts = key0 + KW > at.context;  // some of these keys are nodes of the request
+    const uint32_t mine = present[2 * stage + wc * KW / 32] >> (wc * KW % 32);  // this warp's keys, from bit 0
+    if (!drafts && (KW == 32 ? mine == 0xffffffffu : (mine & 0xffffu) == 0xffffu)) {
 #pragma unroll
-    for (int n = 0; n < KW / 8; ++n) {
-      const int col = n * 8 + 2 * (lane & 3);
-      const uint32_t pair = *reinterpret_cast<const uint16_t*>(present + stage * KEYS + wc * KW + col);
+      for (int n = 0; n < KW / 8; ++n) {
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        bool seen = (pair >> (8 * (x & 1))) & 1u;
-        if (drafts) {
-          const long long j = key0 + col + (x & 1) - at.context;
-          const int node = node_of[x >> 1];
+        for (int x = 0; x < 4; ++x) s[n][x] *= p.scale_log2;
+      }
+    } else {
+#pragma unroll
+      for (int n = 0; n < KW / 8; ++n) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int col = n * 8 + 2 * (lane & 3) + (x & 1);
+          bool seen = (mine >> col) & 1u;
+          const int j = key0 + col - at.context;
           if (j >= 0) {
+            const int node = node_of[x >> 1];
             if (p.mask == nullptr) {
               seen = seen && j <= node;
             } else {
-              seen = seen && node < at.nodes && j < 64 * p.mask_words &&
+              seen = seen && node < at.nodes && (j >> 6) < p.mask_words &&
                      ((__ldg(p.mask + (at.row0 + node) * p.mask_words + (j >> 6)) >> (j & 63)) & 1ull);
             }
           }
+          s[n][x] = seen ? s[n][x] * p.scale_log2 : -INFINITY;
         }
-        s[n][x] = seen ? s[n][x] * p.scale_log2 : -INFINITY;
+      }
+      if (BULK && key0 + KW > at.length) {  // rows past the request's end hold anything
+        const int from = max(at.length - key0, 0);
+        for (int i = from * (DP / 8) + lane; i < KW * (DP / 8); i += 32)
+          *reinterpret_cast<uint4*>(smem + (2 * stage + 1) * S::TILE + chunk_at<DP>(wc * KW + i / (DP / 8), i % (DP / 8))) =
+              make_uint4(0u, 0u, 0u, 0u);
+        fence_proxy_async_smem();  // before the next box lands here
+        __syncwarp();
       }
     }
 #pragma unroll
@@ -420,11 +505,17 @@ __global__ void __launch_bounds__(S::THREADS, S::WARPS == 4 ? 2 : 1)
         mma16816<T>(o[2 * n + 1], a0, a1, a2, a3, b[2], b[3]);
       }
     }
-    if (++stage == STAGES) stage = 0;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(empty + 8 * stage);
+    if (++stage == STAGES) {
+      stage = 0;
+      phase ^= 1;
+    }
 
-    const Cursor done = at;
-    advance(p, at, group, M);
-    if (at.unit < stop && at.item != at.unit) continue;
+    if (at.left > 1 && at.blk + 1 < at.blocks) {
+      advance(p, at, group, M);
+      continue;
+    }
 
     // The item's last block of this run: join the key groups' sums.
     fresh = true;
@@ -438,7 +529,7 @@ __global__ void __launch_bounds__(S::THREADS, S::WARPS == 4 ? 2 : 1)
         part_l[row * C + wc] = l[h];
       }
     }
-    __syncthreads();
+    join();
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int row = wr * 16 + (lane >> 2) + 8 * h;
@@ -470,12 +561,12 @@ __global__ void __launch_bounds__(S::THREADS, S::WARPS == 4 ? 2 : 1)
           }
         }
       }
-      __syncthreads();
+      join();
     }
-    const int rows_here = min(M, done.nodes * group - done.tile * M);
-    const long long item_end = done.item + done.blocks;
-    const bool whole = done.item >= first && item_end <= stop;
-    float* slot = partials + (2ll * blockIdx.x + (done.item >= first)) * S::PARTIAL;
+    const int rows_here = min(M, at.nodes * group - at.tile * M);
+    const int item = units - at.left - at.blk;  // the item's first unit, counted from the run's
+    const bool whole = item >= 0 && at.blk + 1 == at.blocks;
+    float* slot = partials + (2ll * blockIdx.x + (item >= 0)) * S::PARTIAL;
     for (int row = warp; row < rows_here; row += S::WARPS) {
       float top = -INFINITY, sum = 0.0f;
 #pragma unroll
@@ -488,8 +579,8 @@ __global__ void __launch_bounds__(S::THREADS, S::WARPS == 4 ? 2 : 1)
       const float4 v = 4 * lane < DP ? *reinterpret_cast<const float4*>(joined + row * S::PITCH + 4 * lane)
                                      : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       if (whole) {
-        const int at_row = done.tile * M + row;
-        store_row<T, DP>(p, done.row0 + at_row / group, done.head * group + at_row % group, lane, v, top, sum, vector_out);
+        const int at_row = at.tile * M + row;
+        store_row<T, DP>(p, at.row0 + at_row / group, at.head * group + at_row % group, lane, v, top, sum, vector_out);
       } else {
         if (4 * lane < DP) __stcg(reinterpret_cast<float4*>(slot + row * DP + 4 * lane), v);
         if (lane == 0) {
@@ -499,11 +590,12 @@ __global__ void __launch_bounds__(S::THREADS, S::WARPS == 4 ? 2 : 1)
       }
     }
     if (!whole) {
-      const int owner = static_cast<int>(done.item / run.per), last = static_cast<int>((item_end - 1) / run.per);
+      const int owner = static_cast<int>((first + item) / run.per);
+      const int last = static_cast<int>((first + item + at.blocks - 1) / run.per);
       __threadfence();
-      __syncthreads();
+      join();
       if (tid == 0) last_one = atomicAdd(counters + owner, 1) == last - owner;
-      __syncthreads();
+      join();
       if (last_one) {
         __threadfence();
         for (int row = warp; row < rows_here; row += S::WARPS) {
@@ -528,31 +620,82 @@ __global__ void __launch_bounds__(S::THREADS, S::WARPS == 4 ? 2 : 1)
             v.z = fmaf(w.z, fix, v.z);
             v.w = fmaf(w.w, fix, v.w);
           }
-          const int at_row = done.tile * M + row;
-          store_row<T, DP>(p, done.row0 + at_row / group, done.head * group + at_row % group, lane, v, top, sum, vector_out);
+          const int at_row = at.tile * M + row;
+          store_row<T, DP>(p, at.row0 + at_row / group, at.head * group + at_row % group, lane, v, top, sum, vector_out);
         }
         if (tid == 0) counters[owner] = 0;
       }
     }
-    __syncthreads();  // `joined` and the maxima may be written again
+    join();  // `joined` and the maxima may be written again
+    advance(p, at, group, M);
   }
-  cp_async_wait<0>();
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encoder() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* sym = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(sym);
+  });
+  return fn;
+}
+
+// Pages [pages, kv_heads, block_size, dim] as boxes of `box_rows` slots x 64 (32)
+// elements; what lies past the head or past the last page is filled with zeros.
+bool encode_pages(CUtensorMap* map, const AttnArgs& a, const void* ptr, int64_t s_page, int64_t s_head, int64_t s_slot,
+                  int box_rows, int width) {
+  auto enc = encoder();
+  if (enc == nullptr) return false;
+  const auto bytes = [](int64_t s, int64_t n) { return static_cast<cuuint64_t>(n > 1 ? 2 * s : 16); };
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(a.dim), static_cast<cuuint64_t>(a.block_size),
+                              static_cast<cuuint64_t>(a.kv_heads), static_cast<cuuint64_t>(a.pages)};
+  const cuuint64_t strides[3] = {bytes(s_slot, a.block_size), bytes(s_head, a.kv_heads), bytes(s_page, a.pages)};
+  const cuuint32_t box[4] = {static_cast<cuuint32_t>(width), static_cast<cuuint32_t>(box_rows), 1, 1};
+  const cuuint32_t unit[4] = {1, 1, 1, 1};
+  return enc(map, a.dtype == KF_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+             const_cast<void*>(ptr), dims, strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             width == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <typename T, typename S>
-int launch_shape(const AttnArgs& a, int ctas, cudaStream_t stream) {
+int launch_shape(const AttnArgs& a, const DeviceInfo& dev, int ctas, cudaStream_t stream) {
   static std::once_flag once;
   static cudaError_t attr = cudaSuccess;
+  static bool registers_suffice = true;
   std::call_once(once, [] {
-    attr = cudaFuncSetAttribute(tree_kernel<T, S>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+    attr = cudaFuncSetAttribute(tree_kernel<T, S, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+    if (attr == cudaSuccess)
+      attr = cudaFuncSetAttribute(tree_kernel<T, S, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+    // the warpgroups' shares must not exceed what the block is launched with
+    for (const bool bulk : {true, false}) {
+      cudaFuncAttributes f{};
+      if (attr == cudaSuccess)
+        attr = bulk ? cudaFuncGetAttributes(&f, tree_kernel<T, S, true>) : cudaFuncGetAttributes(&f, tree_kernel<T, S, false>);
+      if (S::LOADERS == 4 && attr == cudaSuccess && 3 * f.numRegs < 2 * 224 + 56) registers_suffice = false;
+    }
   });
   if (attr != cudaSuccess) return cuda_error(attr, "tree attention attributes");
+  if (!registers_suffice) return set_error(KF_ERR_UNSUPPORTED, "tree attention: built with too few registers to split");
   const uint64_t d = static_cast<uint64_t>(a.block_size);
   int s = 0;
   while ((1ull << s) < d) ++s;
   const Divisor by{static_cast<uint32_t>(((1ull << (31 + s)) + d - 1) / d), 31 + s};
   const int vector_out = reinterpret_cast<uintptr_t>(a.out) % 8 == 0 && a.so_t % 4 == 0 && a.so_h % 4 == 0;
-  tree_kernel<T, S><<<static_cast<unsigned>(ctas), S::THREADS, S::SMEM, stream>>>(a, by, vector_out);
+  // Keys that lie in one page wherever a block starts; boxes of 8 or more keep
+  // whole swizzle patterns. A cache that no tensor map describes (a stride of
+  // zero or beyond its range) is copied row by row.
+  CUtensorMap k{}, v{};
+  const int box_rows = static_cast<int>(std::gcd(a.block_size, static_cast<int64_t>(KEYS)));
+  const int width = S::DP < 64 ? 32 : 64;
+  const bool bulk = box_rows >= 8 && encode_pages(&k, a, a.k, a.sk_p, a.sk_h, a.sk_t, box_rows, width) &&
+                    encode_pages(&v, a, a.v, a.sv_p, a.sv_h, a.sv_t, box_rows, width);
+  const auto kernel = bulk ? tree_kernel<T, S, true> : tree_kernel<T, S, false>;
+  kernel<<<static_cast<unsigned>(ctas), S::THREADS, S::SMEM, stream>>>(k, v, a, by, box_rows, vector_out, dev.status);
   const cudaError_t err = cudaGetLastError();
   return err == cudaSuccess ? KF_OK : cuda_error(err, "launch(tree attention)");
 }
@@ -566,14 +709,14 @@ struct Plan {
 Plan plan_for(const AttnArgs& a, int sm_count) {
   Plan plan;
   const int64_t each = ceil_div(a.rows, a.seqs > 0 ? a.seqs : 1) * (a.heads / a.kv_heads);
-  plan.m = each <= 16 ? 16 : each <= 32 ? 32 : 64;
+  plan.m = each <= 16 ? 16 : 64;
   plan.ctas = plan.m == 16 ? 2 * sm_count : sm_count;
   plan.dp = a.dim <= 32 ? 32 : a.dim <= 64 ? 64 : 128;
   return plan;
 }
 
 template <typename T>
-int launch_typed(const AttnArgs& a, const Plan& plan, cudaStream_t stream) {
+int launch_typed(const AttnArgs& a, const Plan& plan, const DeviceInfo& dev, cudaStream_t stream) {
   // no more CTAs than a table of full rows could give work
   const int64_t group = a.heads / a.kv_heads;
   const int64_t tiles = (a.rows * group / plan.m + a.seqs + 1) * a.kv_heads;
@@ -581,19 +724,17 @@ int launch_typed(const AttnArgs& a, const Plan& plan, cudaStream_t stream) {
   int ctas = plan.ctas;
   if (tiles < ctas && blocks < ctas && ceil_div(tiles * blocks, MIN_BLOCKS) < ctas)
     ctas = static_cast<int>(ceil_div(tiles * blocks, MIN_BLOCKS));
+  const bool few = plan.m == 16;
   switch (plan.dp) {
     case 32:
-      return plan.m == 16   ? launch_shape<T, Shape<32, 1, 4, 8>>(a, ctas, stream)
-             : plan.m == 32 ? launch_shape<T, Shape<32, 2, 4, 8>>(a, ctas, stream)
-                            : launch_shape<T, Shape<32, 4, 2, 8>>(a, ctas, stream);
+      return few ? launch_shape<T, Shape<32, 1, 4, 8>>(a, dev, ctas, stream)
+                 : launch_shape<T, Shape<32, 4, 2, 8>>(a, dev, ctas, stream);
     case 64:
-      return plan.m == 16   ? launch_shape<T, Shape<64, 1, 4, 6>>(a, ctas, stream)
-             : plan.m == 32 ? launch_shape<T, Shape<64, 2, 4, 8>>(a, ctas, stream)
-                            : launch_shape<T, Shape<64, 4, 2, 8>>(a, ctas, stream);
+      return few ? launch_shape<T, Shape<64, 1, 4, 6>>(a, dev, ctas, stream)
+                 : launch_shape<T, Shape<64, 4, 2, 8>>(a, dev, ctas, stream);
     default:
-      return plan.m == 16   ? launch_shape<T, Shape<128, 1, 4, 3>>(a, ctas, stream)
-             : plan.m == 32 ? launch_shape<T, Shape<128, 2, 4, 6>>(a, ctas, stream)
-                            : launch_shape<T, Shape<128, 4, 2, 5>>(a, ctas, stream);
+      return few ? launch_shape<T, Shape<128, 1, 4, 3>>(a, dev, ctas, stream)
+                 : launch_shape<T, Shape<128, 4, 2, 5>>(a, dev, ctas, stream);
   }
 }
 
@@ -624,7 +765,7 @@ int launch_attention_tree(const AttnArgs& a, const DeviceInfo& dev, cudaStream_t
                                            std::to_string(a.workspace == nullptr ? 0 : a.workspace_bytes));
   const Plan plan = plan_for(a, dev.sm_count);
   if (plan.ctas > COUNTER_BYTES / 4) return set_error(KF_ERR_UNSUPPORTED, "tree attention: too many SMs");
-  return a.dtype == KF_FP16 ? launch_typed<__half>(a, plan, stream) : launch_typed<__nv_bfloat16>(a, plan, stream);
+  return a.dtype == KF_FP16 ? launch_typed<__half>(a, plan, dev, stream) : launch_typed<__nv_bfloat16>(a, plan, dev, stream);
 }
 
 }  // namespace kf
