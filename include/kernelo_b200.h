@@ -291,6 +291,8 @@ KF_API int32_t kf_rmsnorm_rows(int32_t dtype, const void* x, int64_t sx_row, con
                         void* y, int64_t sy_row, int64_t rows, int64_t cols, float eps,
                         const kf_rows_config* cfg, void* stream);
 
+/* The serving operators take their arguments as one struct of 8-byte fields. */
+
 /* ---- attention for serving --------------------------------------------------- *
  * o = softmax(scale q k^T) v per head, query head h reading key head
  * h / (heads / kv_heads); scores, statistics and sums in fp32 (matrix products on
@@ -306,13 +308,24 @@ KF_API int32_t kf_rmsnorm_rows(int32_t dtype, const void* x, int64_t sx_row, con
  * [cu_q[r], cu_q[r+1]) of q and [cu_k[r], cu_k[r+1]) of k and v (int32, seqs + 1
  * of them, from 0). causal != 0: the last row of a request sees all of its keys,
  * each row before it one less. lse (or null): [rows, heads] natural-log sums. */
-KF_API int32_t kf_prefill_attention(int32_t dtype, const void* q, int64_t sq_row, int64_t sq_head,
-                                    const void* k, int64_t sk_row, int64_t sk_head, const void* v,
-                                    int64_t sv_row, int64_t sv_head, void* out, int64_t so_row,
-                                    int64_t so_head, float* lse, const int32_t* cu_q, const int32_t* cu_k,
-                                    int64_t seqs, int64_t rows, int64_t keys, int64_t heads,
-                                    int64_t kv_heads, int64_t dim, float scale, int32_t causal,
-                                    void* stream);
+typedef struct kf_prefill_args {
+  int64_t dtype;
+  const void* q;
+  int64_t sq_row, sq_head;
+  const void* k;
+  int64_t sk_row, sk_head;
+  const void* v;
+  int64_t sv_row, sv_head;
+  void* out;
+  int64_t so_row, so_head;
+  float* lse;
+  const int32_t* cu_q;
+  const int32_t* cu_k;
+  int64_t seqs, rows, keys, heads, kv_heads, dim;
+  double scale;
+  int64_t causal;
+} kf_prefill_args;
+KF_API int32_t kf_prefill_attention(const kf_prefill_args* args, void* stream);
 
 /* kf_tree_attention: new tokens over a paged cache. Pages are
  * [pages, kv_heads, block_size, dim] (any strides); position i of request r is
@@ -326,45 +339,68 @@ KF_API int32_t kf_prefill_attention(int32_t dtype, const void* q, int64_t sq_row
  * The workspace (kf_tree_attention_workspace_bytes, 256-byte aligned, zeroed
  * before its first use and left so that it serves the next call) holds the
  * partial results of a cache split over CTAs. */
-KF_API int32_t kf_tree_attention(int32_t dtype, const void* q, int64_t sq_row, int64_t sq_head,
-                                 const void* k_cache, int64_t sk_page, int64_t sk_head, int64_t sk_slot,
-                                 const void* v_cache, int64_t sv_page, int64_t sv_head, int64_t sv_slot,
-                                 void* out, int64_t so_row, int64_t so_head, float* lse,
-                                 const int32_t* block_table, int64_t table_stride, int64_t table_cols,
-                                 int64_t pages, int64_t block_size, const int32_t* context,
-                                 const int32_t* cu_q, const int64_t* tree_mask, int64_t mask_words,
-                                 int64_t seqs, int64_t rows, int64_t heads, int64_t kv_heads, int64_t dim,
-                                 float scale, void* workspace, int64_t workspace_bytes, void* stream);
+typedef struct kf_tree_args {
+  int64_t dtype;
+  const void* q;
+  int64_t sq_row, sq_head;
+  const void* k_cache;
+  int64_t sk_page, sk_head, sk_slot;
+  const void* v_cache;
+  int64_t sv_page, sv_head, sv_slot;
+  void* out;
+  int64_t so_row, so_head;
+  float* lse;
+  const int32_t* block_table;
+  int64_t table_stride, table_cols;
+  int64_t pages, block_size;
+  const int32_t* context;
+  const int32_t* cu_q;
+  const int64_t* tree_mask;
+  int64_t mask_words;
+  int64_t seqs, rows, heads, kv_heads, dim;
+  double scale;
+  void* workspace;
+  int64_t workspace_bytes;
+} kf_tree_args;
+KF_API int32_t kf_tree_attention(const kf_tree_args* args, void* stream);
 KF_API int64_t kf_tree_attention_workspace_bytes(int32_t device, int32_t dtype, int64_t seqs, int64_t rows,
                                                  int64_t heads, int64_t kv_heads, int64_t dim);
 
 /* ---- rotary positions --------------------------------------------------------- *
- * Where kf_rotary also writes a paged cache: v [tokens, kv_heads, dim] and the
- * turned k go to slot slots[t] % block_size of page slots[t] / block_size
- * (nowhere if slots[t] is negative or past the pages). */
-typedef struct kf_rotary_cache {
-  const void* v;
-  int64_t sv_row, sv_head;
-  void* k_cache;
-  int64_t sk_page, sk_head, sk_slot;
-  void* v_cache;
-  int64_t sv_page, svc_head, sv_slot;
-  int64_t pages, block_size;
-  const int64_t* slots;
-} kf_rotary_cache;
-
-/* q [tokens, heads, dim] and k [tokens, kv_heads, dim], the first rot elements of
+ * q [tokens, heads, dim] and k [tokens, kv_heads, dim], the first rot elements of
  * each head turned by the angles of positions[t]: pairs (i, i + rot/2), or
  * (2i, 2i + 1) if interleaved. table: [table_rows, rot] fp32, rot/2 cosines then
  * rot/2 sines of each position; a position outside it gives NaN. inverse != 0
  * turns back (the gradient of the forward turn). q_out may be q and k_out k.
- * cache (or null): also the cache write; k_out may then be null. */
-KF_API int32_t kf_rotary(int32_t dtype, const void* q, int64_t sq_row, int64_t sq_head, void* q_out,
-                         int64_t sqo_row, int64_t sqo_head, const void* k, int64_t sk_row, int64_t sk_head,
-                         void* k_out, int64_t sko_row, int64_t sko_head, const int32_t* positions,
-                         const float* table, int64_t table_rows, int64_t rot, int64_t tokens,
-                         int64_t heads, int64_t kv_heads, int64_t dim, int32_t interleaved, int32_t inverse,
-                         const kf_rotary_cache* cache, void* stream);
+ * slots not null: v [tokens, kv_heads, dim] and the turned k also go to slot
+ * slots[t] % block_size of page slots[t] / block_size of caches
+ * [pages, kv_heads, block_size, dim] (nowhere if slots[t] is negative or past the
+ * pages); k_out may then be null. */
+typedef struct kf_rotary_args {
+  int64_t dtype;
+  const void* q;
+  int64_t sq_row, sq_head;
+  void* q_out;
+  int64_t sqo_row, sqo_head;
+  const void* k;
+  int64_t sk_row, sk_head;
+  void* k_out;
+  int64_t sko_row, sko_head;
+  const int32_t* positions;
+  const float* table;
+  int64_t table_rows, rot;
+  int64_t tokens, heads, kv_heads, dim;
+  int64_t interleaved, inverse;
+  const void* v;
+  int64_t sv_row, sv_head;
+  void* k_cache;
+  int64_t skc_page, skc_head, skc_slot;
+  void* v_cache;
+  int64_t svc_page, svc_head, svc_slot;
+  int64_t pages, block_size;
+  const int64_t* slots;
+} kf_rotary_args;
+KF_API int32_t kf_rotary(const kf_rotary_args* args, void* stream);
 
 /* ---- block tables and slot maps ------------------------------------------------ *
  * One serving step's plan from request lengths. Request r holds context[r] tokens
@@ -376,11 +412,20 @@ KF_API int32_t kf_rotary(int32_t dtype, const void* q, int64_t sq_row, int64_t s
  * it; -1 without a page; position 0 and slot -1 past the last token);
  * counts[0]: pages needed, counts[1]: added tokens that got no slot. The same
  * call on the same lengths writes the same values again. */
-KF_API int32_t kf_build_slots(const int32_t* context, const int32_t* added, int64_t seqs,
-                              int32_t* block_table, int64_t table_stride, int64_t table_cols,
-                              const int32_t* free_blocks, int64_t n_free, int64_t block_size,
-                              int64_t max_tokens, int32_t* cu_new, int32_t* positions, int64_t* slots,
-                              int32_t* counts, void* stream);
+typedef struct kf_slots_args {
+  const int32_t* context;
+  const int32_t* added;
+  int64_t seqs;
+  int32_t* block_table;
+  int64_t table_stride, table_cols;
+  const int32_t* free_blocks;
+  int64_t n_free, block_size, max_tokens;
+  int32_t* cu_new;
+  int32_t* positions;
+  int64_t* slots;
+  int32_t* counts;
+} kf_slots_args;
+KF_API int32_t kf_build_slots(const kf_slots_args* args, void* stream);
 
 /* ---- fused linear + all-gather over NVLink ---------------------------------- *
  * kf_linear_bias_act, and every output tile is also stored into the n_peers

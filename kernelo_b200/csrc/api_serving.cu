@@ -12,7 +12,7 @@ namespace {
 
 int invalid(const std::string& message) { return set_error(KF_ERR_INVALID_ARGUMENT, message); }
 
-bool known_dtype(int d) { return d == KF_FP16 || d == KF_BF16 || d == KF_FP32; }
+bool known_dtype(int64_t d) { return d == KF_FP16 || d == KF_BF16 || d == KF_FP32; }
 
 int this_device(DeviceInfo** dev) {
   int device = 0;
@@ -20,9 +20,10 @@ int this_device(DeviceInfo** dev) {
   return rc != KF_OK ? rc : device_info(device, dev);
 }
 
+constexpr double LOG2_E = 1.4426950408889634;
 constexpr int64_t INT32_LIMIT = 0x7fffffffll;
 
-int check_heads(int dtype, int64_t rows, int64_t seqs, int64_t heads, int64_t kv_heads, int64_t dim) {
+int check_heads(int64_t dtype, int64_t rows, int64_t seqs, int64_t heads, int64_t kv_heads, int64_t dim) {
   if (!known_dtype(dtype)) return invalid("unknown dtype code");
   if (rows < 0 || seqs < 0 || heads < 0 || kv_heads < 0 || dim < 0) return invalid("negative size");
   if (rows > INT32_LIMIT || seqs > INT32_LIMIT) return invalid("rows and requests are counted in 32 bits");
@@ -42,74 +43,69 @@ using namespace kf;
 
 extern "C" {
 
-int32_t kf_prefill_attention(int32_t dtype, const void* q, int64_t sq_row, int64_t sq_head, const void* k,
-                             int64_t sk_row, int64_t sk_head, const void* v, int64_t sv_row, int64_t sv_head,
-                             void* out, int64_t so_row, int64_t so_head, float* lse, const int32_t* cu_q,
-                             const int32_t* cu_k, int64_t seqs, int64_t rows, int64_t keys, int64_t heads,
-                             int64_t kv_heads, int64_t dim, float scale, int32_t causal, void* stream) {
-  int rc = check_heads(dtype, rows, seqs, heads, kv_heads, dim);
+int32_t kf_prefill_attention(const kf_prefill_args* args, void* stream) {
+  if (args == nullptr) return invalid("null arguments");
+  const kf_prefill_args& g = *args;
+  int rc = check_heads(g.dtype, g.rows, g.seqs, g.heads, g.kv_heads, g.dim);
   if (rc != KF_OK) return rc;
-  if (keys < 0 || keys > INT32_LIMIT) return invalid("keys are counted in 32 bits");
-  if (!std::isfinite(scale)) return invalid("scale must be finite");
-  if (rows == 0 || heads == 0 || dim == 0) return KF_OK;
-  if (q == nullptr || out == nullptr || cu_q == nullptr || cu_k == nullptr ||
-      (keys > 0 && (k == nullptr || v == nullptr)))
+  if (g.keys < 0 || g.keys > INT32_LIMIT) return invalid("keys are counted in 32 bits");
+  if (!std::isfinite(g.scale)) return invalid("scale must be finite");
+  if (g.rows == 0 || g.heads == 0 || g.dim == 0) return KF_OK;
+  if (g.q == nullptr || g.out == nullptr || g.cu_q == nullptr || g.cu_k == nullptr ||
+      (g.keys > 0 && (g.k == nullptr || g.v == nullptr)))
     return invalid("null pointer");
   DeviceInfo* dev = nullptr;
   rc = this_device(&dev);
   if (rc != KF_OK) return rc;
   AttnArgs a;
-  a.dtype = dtype;
-  a.q = q, a.sq_t = sq_row, a.sq_h = sq_head;
-  a.k = k, a.sk_t = sk_row, a.sk_h = sk_head;
-  a.v = v, a.sv_t = sv_row, a.sv_h = sv_head;
-  a.out = out, a.so_t = so_row, a.so_h = so_head;
-  a.lse = lse;
-  a.cu_q = cu_q, a.cu_k = cu_k;
-  a.seqs = seqs, a.rows = rows, a.keys = keys, a.heads = heads, a.kv_heads = kv_heads, a.dim = dim;
-  a.scale_log2 = scale * 1.4426950408889634f;
-  a.causal = causal != 0;
+  a.dtype = static_cast<int>(g.dtype);
+  a.q = g.q, a.sq_t = g.sq_row, a.sq_h = g.sq_head;
+  a.k = g.k, a.sk_t = g.sk_row, a.sk_h = g.sk_head;
+  a.v = g.v, a.sv_t = g.sv_row, a.sv_h = g.sv_head;
+  a.out = g.out, a.so_t = g.so_row, a.so_h = g.so_head;
+  a.lse = g.lse;
+  a.cu_q = g.cu_q, a.cu_k = g.cu_k;
+  a.seqs = g.seqs, a.rows = g.rows, a.keys = g.keys, a.heads = g.heads, a.kv_heads = g.kv_heads, a.dim = g.dim;
+  a.scale_log2 = static_cast<float>(g.scale * LOG2_E);
+  a.causal = g.causal != 0;
   if (attention_prefill_supported(a)) return launch_attention_prefill(a, *dev, static_cast<cudaStream_t>(stream));
   return launch_attention_rows(a, static_cast<cudaStream_t>(stream));
 }
 
-int32_t kf_tree_attention(int32_t dtype, const void* q, int64_t sq_row, int64_t sq_head, const void* k_cache,
-                          int64_t sk_page, int64_t sk_head, int64_t sk_slot, const void* v_cache, int64_t sv_page,
-                          int64_t sv_head, int64_t sv_slot, void* out, int64_t so_row, int64_t so_head, float* lse,
-                          const int32_t* block_table, int64_t table_stride, int64_t table_cols, int64_t pages,
-                          int64_t block_size, const int32_t* context, const int32_t* cu_q, const int64_t* tree_mask,
-                          int64_t mask_words, int64_t seqs, int64_t rows, int64_t heads, int64_t kv_heads,
-                          int64_t dim, float scale, void* workspace, int64_t workspace_bytes, void* stream) {
-  int rc = check_heads(dtype, rows, seqs, heads, kv_heads, dim);
+int32_t kf_tree_attention(const kf_tree_args* args, void* stream) {
+  if (args == nullptr) return invalid("null arguments");
+  const kf_tree_args& g = *args;
+  int rc = check_heads(g.dtype, g.rows, g.seqs, g.heads, g.kv_heads, g.dim);
   if (rc != KF_OK) return rc;
-  if (table_cols < 0 || pages < 0 || mask_words < 0) return invalid("negative size");
-  if (block_size < 1 || block_size > INT32_LIMIT) return invalid("block_size must be positive and fit 32 bits");
-  if (!std::isfinite(scale)) return invalid("scale must be finite");
-  if (rows == 0 || heads == 0 || dim == 0) return KF_OK;
-  if (q == nullptr || out == nullptr || (seqs > 0 && context == nullptr) ||
-      (seqs > 0 && table_cols > 0 && block_table == nullptr) ||
-      (pages > 0 && (k_cache == nullptr || v_cache == nullptr)) || (mask_words > 0 && tree_mask == nullptr))
+  if (g.table_cols < 0 || g.pages < 0 || g.mask_words < 0) return invalid("negative size");
+  if (g.pages > INT32_LIMIT || g.mask_words > INT32_LIMIT) return invalid("pages and mask words are counted in 32 bits");
+  if (g.block_size < 1 || g.block_size > INT32_LIMIT) return invalid("block_size must be positive and fit 32 bits");
+  if (!std::isfinite(g.scale)) return invalid("scale must be finite");
+  if (g.rows == 0 || g.heads == 0 || g.dim == 0) return KF_OK;
+  if (g.q == nullptr || g.out == nullptr || (g.seqs > 0 && g.context == nullptr) ||
+      (g.seqs > 0 && g.table_cols > 0 && g.block_table == nullptr) ||
+      (g.pages > 0 && (g.k_cache == nullptr || g.v_cache == nullptr)) || (g.mask_words > 0 && g.tree_mask == nullptr))
     return invalid("null pointer");
   DeviceInfo* dev = nullptr;
   rc = this_device(&dev);
   if (rc != KF_OK) return rc;
   AttnArgs a;
-  a.dtype = dtype;
-  a.q = q, a.sq_t = sq_row, a.sq_h = sq_head;
-  a.k = k_cache, a.sk_p = sk_page, a.sk_h = sk_head, a.sk_t = sk_slot;
-  a.v = v_cache, a.sv_p = sv_page, a.sv_h = sv_head, a.sv_t = sv_slot;
-  a.out = out, a.so_t = so_row, a.so_h = so_head;
-  a.lse = lse;
-  a.cu_q = cu_q;
+  a.dtype = static_cast<int>(g.dtype);
+  a.q = g.q, a.sq_t = g.sq_row, a.sq_h = g.sq_head;
+  a.k = g.k_cache, a.sk_p = g.sk_page, a.sk_h = g.sk_head, a.sk_t = g.sk_slot;
+  a.v = g.v_cache, a.sv_p = g.sv_page, a.sv_h = g.sv_head, a.sv_t = g.sv_slot;
+  a.out = g.out, a.so_t = g.so_row, a.so_h = g.so_head;
+  a.lse = g.lse;
+  a.cu_q = g.cu_q;
   a.paged = 1;
-  a.table = block_table, a.table_stride = table_stride, a.table_cols = table_cols;
-  a.pages = pages, a.block_size = block_size;
-  a.context = context;
-  a.mask = mask_words > 0 ? reinterpret_cast<const unsigned long long*>(tree_mask) : nullptr;
-  a.mask_words = mask_words;
-  a.seqs = seqs, a.rows = rows, a.heads = heads, a.kv_heads = kv_heads, a.dim = dim;
-  a.scale_log2 = scale * 1.4426950408889634f;
-  a.workspace = workspace, a.workspace_bytes = workspace_bytes;
+  a.table = g.block_table, a.table_stride = g.table_stride, a.table_cols = g.table_cols;
+  a.pages = g.pages, a.block_size = g.block_size;
+  a.context = g.context;
+  a.mask = g.mask_words > 0 ? reinterpret_cast<const unsigned long long*>(g.tree_mask) : nullptr;
+  a.mask_words = g.mask_words;
+  a.seqs = g.seqs, a.rows = g.rows, a.heads = g.heads, a.kv_heads = g.kv_heads, a.dim = g.dim;
+  a.scale_log2 = static_cast<float>(g.scale * LOG2_E);
+  a.workspace = g.workspace, a.workspace_bytes = g.workspace_bytes;
   if (attention_tree_supported(a)) return launch_attention_tree(a, *dev, static_cast<cudaStream_t>(stream));
   return launch_attention_rows(a, static_cast<cudaStream_t>(stream));
 }
@@ -128,71 +124,62 @@ int64_t kf_tree_attention_workspace_bytes(int32_t device, int32_t dtype, int64_t
   return attention_tree_workspace_bytes(a, *dev);
 }
 
-int32_t kf_rotary(int32_t dtype, const void* q, int64_t sq_row, int64_t sq_head, void* q_out, int64_t sqo_row,
-                  int64_t sqo_head, const void* k, int64_t sk_row, int64_t sk_head, void* k_out, int64_t sko_row,
-                  int64_t sko_head, const int32_t* positions, const float* table, int64_t table_rows, int64_t rot,
-                  int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int32_t interleaved, int32_t inverse,
-                  const kf_rotary_cache* cache, void* stream) {
-  if (!known_dtype(dtype)) return invalid("unknown dtype code");
-  if (tokens < 0 || heads < 0 || kv_heads < 0 || dim < 0 || table_rows < 0 || rot < 0) return invalid("negative size");
-  if (rot % 2 != 0 || rot > dim)
-    return invalid("the turned part must be even and at most the head; got " + std::to_string(rot) + " of " +
-                   std::to_string(dim));
-  if (tokens == 0 || dim == 0 || heads + kv_heads == 0) return KF_OK;
-  if ((heads > 0 && (q == nullptr || q_out == nullptr)) || (kv_heads > 0 && k == nullptr) ||
-      (rot > 0 && (positions == nullptr || (table_rows > 0 && table == nullptr))))
-    return invalid("null pointer");
-  if (kv_heads > 0 && k_out == nullptr && cache == nullptr) return invalid("k needs an output or a cache");
-  if (heads > INT32_LIMIT || kv_heads > INT32_LIMIT / 2 || dim > INT32_LIMIT / 4)
+int32_t kf_rotary(const kf_rotary_args* args, void* stream) {
+  if (args == nullptr) return invalid("null arguments");
+  const kf_rotary_args& g = *args;
+  if (!known_dtype(g.dtype)) return invalid("unknown dtype code");
+  if (g.tokens < 0 || g.heads < 0 || g.kv_heads < 0 || g.dim < 0 || g.table_rows < 0 || g.rot < 0 || g.pages < 0)
+    return invalid("negative size");
+  if (g.rot % 2 != 0 || g.rot > g.dim)
+    return invalid("the turned part must be even and at most the head; got " + std::to_string(g.rot) + " of " +
+                   std::to_string(g.dim));
+  if (g.heads > INT32_LIMIT / 4 || g.kv_heads > INT32_LIMIT / 4 || g.dim > INT32_LIMIT / 4)
     return invalid("heads and their elements are counted in 32 bits");
+  if (g.tokens == 0 || g.dim == 0 || g.heads + g.kv_heads == 0) return KF_OK;
+  if ((g.heads > 0 && (g.q == nullptr || g.q_out == nullptr)) || (g.kv_heads > 0 && g.k == nullptr) ||
+      (g.rot > 0 && (g.positions == nullptr || (g.table_rows > 0 && g.table == nullptr))))
+    return invalid("null pointer");
+  const bool cached = g.slots != nullptr && g.kv_heads > 0;
+  if (g.kv_heads > 0 && g.k_out == nullptr && !cached) return invalid("k needs an output or a cache");
+  if (cached && g.block_size < 1) return invalid("block_size must be positive");
+  if (cached && (g.v == nullptr || (g.pages > 0 && (g.k_cache == nullptr || g.v_cache == nullptr))))
+    return invalid("null pointer");
   RotaryArgs a;
-  a.dtype = dtype;
-  a.q = q, a.sq_t = sq_row, a.sq_h = sq_head;
-  a.q_out = q_out, a.sqo_t = sqo_row, a.sqo_h = sqo_head;
-  a.k = k, a.sk_t = sk_row, a.sk_h = sk_head;
-  a.k_out = k_out, a.sko_t = sko_row, a.sko_h = sko_head;
-  a.positions = positions, a.table = table, a.table_rows = table_rows, a.rot = rot;
-  if (cache != nullptr && kv_heads > 0) {
-    if (cache->block_size < 1) return invalid("block_size must be positive");
-    if (cache->pages < 0) return invalid("negative size");
-    if (cache->v == nullptr || cache->slots == nullptr ||
-        (cache->pages > 0 && (cache->k_cache == nullptr || cache->v_cache == nullptr)))
-      return invalid("null pointer");
-    a.v = cache->v, a.sv_t = cache->sv_row, a.sv_h = cache->sv_head;
-    a.k_cache = cache->k_cache, a.skc_p = cache->sk_page, a.skc_h = cache->sk_head, a.skc_s = cache->sk_slot;
-    a.v_cache = cache->v_cache, a.svc_p = cache->sv_page, a.svc_h = cache->svc_head, a.svc_s = cache->sv_slot;
-    a.pages = cache->pages, a.block_size = cache->block_size;
-    a.slots = cache->slots;
+  a.dtype = static_cast<int>(g.dtype);
+  a.q = g.q, a.sq_t = g.sq_row, a.sq_h = g.sq_head;
+  a.q_out = g.q_out, a.sqo_t = g.sqo_row, a.sqo_h = g.sqo_head;
+  a.k = g.k, a.sk_t = g.sk_row, a.sk_h = g.sk_head;
+  a.k_out = g.k_out, a.sko_t = g.sko_row, a.sko_h = g.sko_head;
+  a.positions = g.positions, a.table = g.table, a.table_rows = g.table_rows, a.rot = g.rot;
+  if (cached) {
+    a.v = g.v, a.sv_t = g.sv_row, a.sv_h = g.sv_head;
+    a.k_cache = g.k_cache, a.skc_p = g.skc_page, a.skc_h = g.skc_head, a.skc_s = g.skc_slot;
+    a.v_cache = g.v_cache, a.svc_p = g.svc_page, a.svc_h = g.svc_head, a.svc_s = g.svc_slot;
+    a.pages = g.pages, a.block_size = g.block_size;
+    a.slots = g.slots;
   }
-  a.tokens = tokens, a.heads = heads, a.kv_heads = kv_heads, a.dim = dim;
-  a.interleaved = interleaved != 0, a.inverse = inverse != 0;
+  a.tokens = g.tokens, a.heads = g.heads, a.kv_heads = g.kv_heads, a.dim = g.dim;
+  a.interleaved = g.interleaved != 0, a.inverse = g.inverse != 0;
   DeviceInfo* dev = nullptr;
   const int rc = this_device(&dev);
   if (rc != KF_OK) return rc;
   return launch_rotary(a, *dev, static_cast<cudaStream_t>(stream));
 }
 
-int32_t kf_build_slots(const int32_t* context, const int32_t* added, int64_t seqs, int32_t* block_table,
-                       int64_t table_stride, int64_t table_cols, const int32_t* free_blocks, int64_t n_free,
-                       int64_t block_size, int64_t max_tokens, int32_t* cu_new, int32_t* positions, int64_t* slots,
-                       int32_t* counts, void* stream) {
-  if (seqs < 0 || table_cols < 0 || n_free < 0 || max_tokens < 0) return invalid("negative size");
-  if (max_tokens > INT32_LIMIT) return invalid("tokens are counted in 32 bits");
-  if (block_size < 1) return invalid("block_size must be positive");
-  if (cu_new == nullptr || counts == nullptr || (seqs > 0 && (context == nullptr || added == nullptr)) ||
-      (seqs > 0 && table_cols > 0 && block_table == nullptr) || (n_free > 0 && free_blocks == nullptr) ||
-      (max_tokens > 0 && (positions == nullptr || slots == nullptr)))
+int32_t kf_build_slots(const kf_slots_args* args, void* stream) {
+  if (args == nullptr) return invalid("null arguments");
+  const kf_slots_args& g = *args;
+  if (g.seqs < 0 || g.table_cols < 0 || g.n_free < 0 || g.max_tokens < 0) return invalid("negative size");
+  if (g.max_tokens > INT32_LIMIT) return invalid("tokens are counted in 32 bits");
+  if (g.block_size < 1) return invalid("block_size must be positive");
+  if (g.cu_new == nullptr || g.counts == nullptr || (g.seqs > 0 && (g.context == nullptr || g.added == nullptr)) ||
+      (g.seqs > 0 && g.table_cols > 0 && g.block_table == nullptr) || (g.n_free > 0 && g.free_blocks == nullptr) ||
+      (g.max_tokens > 0 && (g.positions == nullptr || g.slots == nullptr)))
     return invalid("null pointer");
   DeviceInfo* dev = nullptr;
   const int rc = this_device(&dev);
   if (rc != KF_OK) return rc;
-  SlotsArgs a;
-  a.context = context, a.added = added, a.seqs = seqs;
-  a.table = block_table, a.table_stride = table_stride, a.table_cols = table_cols;
-  a.free_blocks = free_blocks, a.n_free = n_free;
-  a.block_size = block_size, a.max_tokens = max_tokens;
-  a.cu_new = cu_new, a.positions = positions, a.slots = slots, a.counts = counts;
-  return launch_slots(a, *dev, static_cast<cudaStream_t>(stream));
+  return launch_slots(g, *dev, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -301,21 +301,7 @@ struct RotaryArgs {
 int launch_rotary(const RotaryArgs& args, const DeviceInfo& dev, cudaStream_t stream);
 
 // Block tables and slot maps from request lengths (slots.cu).
-struct SlotsArgs {
-  const int32_t* context = nullptr;
-  const int32_t* added = nullptr;
-  int64_t seqs = 0;
-  int32_t* table = nullptr;
-  int64_t table_stride = 0, table_cols = 0;
-  const int32_t* free_blocks = nullptr;
-  int64_t n_free = 0;
-  int64_t block_size = 1, max_tokens = 0;
-  int32_t* cu_new = nullptr;
-  int32_t* positions = nullptr;
-  int64_t* slots = nullptr;
-  int32_t* counts = nullptr;  // [2]: blocks taken, tokens dropped
-};
-int launch_slots(const SlotsArgs& args, const DeviceInfo& dev, cudaStream_t stream);
+int launch_slots(const kf_slots_args& args, const DeviceInfo& dev, cudaStream_t stream);
 
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 

@@ -63,7 +63,7 @@ __device__ __forceinline__ Sums block_exclusive(Sums v, Sums* total, Sums* scrat
   return before;
 }
 
-__global__ void __launch_bounds__(SLOTS_THREADS) slots_kernel(const SlotsArgs p) {
+__global__ void __launch_bounds__(SLOTS_THREADS) slots_kernel(const kf_slots_args p) {
   __shared__ Sums scratch[SLOTS_WARPS];
   __shared__ long long first_token[SLOTS_THREADS + 1];  // of the chunk's requests
   __shared__ long long first_page[SLOTS_THREADS + 1];   // index into the free list
@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(SLOTS_THREADS) slots_kernel(const SlotsArgs p)
       const long long room = p.max_tokens - my_token;  // outputs left for this request
       const long long stop = have + min(add, max(room, 0ll));
       long long good = 0;
-      if (have < held * block && held <= p.table_cols && p.table[r * p.table_stride + held - 1] >= 0)
+      if (have < held * block && held <= p.table_cols && p.block_table[r * p.table_stride + held - 1] >= 0)
         good += min(stop, held * block) - min(stop, have);
       const long long cols = min(min(after, static_cast<long long>(p.table_cols)),
                                  held + max(p.n_free - my_page, 0ll));
@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(SLOTS_THREADS) slots_kernel(const SlotsArgs p)
       int page = -1;
       if (col < p.table_cols) {
         if (col < mine) {
-          page = p.table[(r0 + a) * p.table_stride + col];
+          page = p.block_table[(r0 + a) * p.table_stride + col];
         } else {
           const long long f = first_page[a] + col - mine;
           if (f < p.n_free) page = __ldg(p.free_blocks + f);
@@ -146,7 +146,7 @@ __global__ void __launch_bounds__(SLOTS_THREADS) slots_kernel(const SlotsArgs p)
         if (first_page[mid] <= f) a = mid; else b = mid - 1;
       }
       const long long col = (cached[a] + block - 1) / block + (f - first_page[a]);
-      if (col < p.table_cols) p.table[(r0 + a) * p.table_stride + col] = f < p.n_free ? __ldg(p.free_blocks + f) : -1;
+      if (col < p.table_cols) p.block_table[(r0 + a) * p.table_stride + col] = f < p.n_free ? __ldg(p.free_blocks + f) : -1;
     }
     carry.tokens += total.tokens;
     carry.pages += total.pages;
@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(SLOTS_THREADS) slots_kernel(const SlotsArgs p)
 
 }  // namespace
 
-int launch_slots(const SlotsArgs& a, const DeviceInfo& dev, cudaStream_t stream) {
+int launch_slots(const kf_slots_args& a, const DeviceInfo& dev, cudaStream_t stream) {
   const int64_t want = ceil_div(a.max_tokens, SLOTS_THREADS * 4);
   const int64_t grid = want < 1 ? 1 : want > dev.sm_count ? dev.sm_count : want;
   slots_kernel<<<static_cast<unsigned>(grid), SLOTS_THREADS, 0, stream>>>(a);

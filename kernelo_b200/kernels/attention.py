@@ -35,27 +35,34 @@ def _check_heads(q: torch.Tensor, kv_heads: int, dim: int) -> None:
 
 
 def _check_operand(name: str, t: torch.Tensor, q: torch.Tensor) -> None:
-    if t.dtype != q.dtype:
-        raise ValueError(f"dtype mismatch: q {q.dtype} vs {name} {t.dtype}")
-    if t.device != q.device:
-        raise ValueError(f"q and {name} must be on one device")
+    if t.dtype is not q.dtype:
+        raise ValueError(f"dtype mismatch: {q.dtype} vs {name} {t.dtype}")
+    if t.get_device() != q.get_device():
+        raise ValueError(f"{name} must be on one device with the first operand, got {t.device} and {q.device}")
     if t.stride(-1) != 1 and t.shape[-1] > 1:
         raise ValueError(f"{name} must have a contiguous last dimension. Pass {name}.contiguous() explicitly.")
 
 
-def _check_index(name: str, t: torch.Tensor, device: torch.device, dtype: torch.dtype = torch.int32) -> None:
-    if t.dtype != dtype:
+def _check_index(name: str, t: torch.Tensor, q: torch.Tensor, dtype: torch.dtype = torch.int32) -> None:
+    if t.dtype is not dtype:
         raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
-    if t.device != device:
-        raise ValueError(f"{name} must be on {device}, got {t.device}")
+    if t.get_device() != q.get_device():
+        raise ValueError(f"{name} must be on {q.device}, got {t.device}")
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
+
+
+def _empty_like(t: torch.Tensor) -> torch.Tensor:
+    """A contiguous tensor of t's shape (empty_like is the cheaper call, but keeps a view's order)."""
+    if t.is_contiguous():
+        return torch.empty_like(t)
+    return torch.empty(t.shape, device=t.device, dtype=t.dtype)
 
 
 def _check_query(q: torch.Tensor) -> None:
     if q.ndim != 3:
         raise ValueError(f"expected q as (rows, heads, dim), got shape {tuple(q.shape)}")
-    if q.device.type != "cuda":
+    if not q.is_cuda:
         raise ValueError(f"q must be a CUDA tensor, got {q.device}")
     if q.stride(2) != 1 and q.shape[2] > 1:
         raise ValueError("q must have a contiguous last dimension. Pass q.contiguous() explicitly.")
@@ -63,12 +70,12 @@ def _check_query(q: torch.Tensor) -> None:
 
 def _outputs(q: torch.Tensor, out: torch.Tensor | None, return_lse: bool):
     if out is None:
-        out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+        out = _empty_like(q)
     else:
         if out.shape != q.shape:
             raise ValueError(f"out must have shape {tuple(q.shape)}, got {tuple(out.shape)}")
         _check_operand("out", out, q)
-    lse = torch.empty(q.shape[:2], device=q.device, dtype=torch.float32) if return_lse else None
+    lse = torch.empty(q.shape[0], q.shape[1], device=q.device, dtype=torch.float32) if return_lse else None
     return out, lse
 
 
@@ -99,7 +106,7 @@ def prefill_attention(
     _check_heads(q, k.shape[1], k.shape[2])
     _check_operand("k", k, q)
     _check_operand("v", v, q)
-    _check_index("cu_q", cu_q, q.device)
+    _check_index("cu_q", cu_q, q)
     if cu_q.ndim != 1 or cu_q.shape[0] < 1:
         raise ValueError(f"cu_q must have shape (requests + 1,), got {tuple(cu_q.shape)}")
     if cu_k is None:
@@ -107,7 +114,7 @@ def prefill_attention(
             raise ValueError(f"{k.shape[0]} keys for {q.shape[0]} rows: pass cu_k")
         cu_k = cu_q
     elif cu_k is not cu_q:
-        _check_index("cu_k", cu_k, q.device)
+        _check_index("cu_k", cu_k, q)
         if cu_k.shape != cu_q.shape:
             raise ValueError(f"cu_q and cu_k must have one shape, got {tuple(cu_q.shape)} and {tuple(cu_k.shape)}")
     out, lse = _outputs(q, out, return_lse)
@@ -152,22 +159,22 @@ def tree_attention(
     if block_table.ndim != 2 or block_table.dtype != torch.int32:
         raise ValueError(f"block_table must be int32 (requests, blocks), got {block_table.dtype} "
                          f"{tuple(block_table.shape)}")
-    if block_table.device != q.device:
+    if block_table.get_device() != q.get_device():
         raise ValueError(f"block_table must be on {q.device}, got {block_table.device}")
     if block_table.stride(1) != 1 and block_table.shape[1] > 1:
         raise ValueError("block_table must have contiguous rows")
     seqs = block_table.shape[0]
-    _check_index("context_lens", context_lens, q.device)
-    if context_lens.shape != (seqs,):
+    _check_index("context_lens", context_lens, q)
+    if context_lens.ndim != 1 or context_lens.shape[0] != seqs:
         raise ValueError(f"context_lens must have shape ({seqs},), got {tuple(context_lens.shape)}")
     if cu_q is not None:
-        _check_index("cu_q", cu_q, q.device)
-        if cu_q.shape != (seqs + 1,):
+        _check_index("cu_q", cu_q, q)
+        if cu_q.ndim != 1 or cu_q.shape[0] != seqs + 1:
             raise ValueError(f"cu_q must have shape ({seqs + 1},), got {tuple(cu_q.shape)}")
     elif q.shape[0] != seqs:
         raise ValueError(f"{q.shape[0]} rows for {seqs} requests: pass cu_q")
     if tree_mask is not None:
-        _check_index("tree_mask", tree_mask, q.device, torch.int64)
+        _check_index("tree_mask", tree_mask, q, torch.int64)
         if tree_mask.ndim != 2 or tree_mask.shape[0] != q.shape[0] or tree_mask.shape[1] < 1:
             raise ValueError(f"tree_mask must have shape ({q.shape[0]}, words), got {tuple(tree_mask.shape)}")
     out, lse = _outputs(q, out, return_lse)

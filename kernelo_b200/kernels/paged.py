@@ -53,21 +53,21 @@ def build_slots(
     if block_table.ndim != 2 or block_table.dtype != torch.int32:
         raise ValueError(f"block_table must be int32 (requests, blocks), got {block_table.dtype} "
                          f"{tuple(block_table.shape)}")
-    if device.type != "cuda":
+    if not block_table.is_cuda:
         raise ValueError(f"block_table must be a CUDA tensor, got {device}")
     if block_table.stride(1) != 1 and block_table.shape[1] > 1:
         raise ValueError("block_table must have contiguous rows")
     seqs = block_table.shape[0]
     for name, t in (("context_lens", context_lens), ("new_lens", new_lens)):
-        _check_index(name, t, device)
-        if t.shape != (seqs,):
+        _check_index(name, t, block_table)
+        if t.ndim != 1 or t.shape[0] != seqs:
             raise ValueError(f"{name} must have shape ({seqs},), got {tuple(t.shape)}")
-    _check_index("free_blocks", free_blocks, device)
+    _check_index("free_blocks", free_blocks, block_table)
     if free_blocks.ndim != 1:
         raise ValueError(f"free_blocks must have one dimension, got shape {tuple(free_blocks.shape)}")
     slots = torch.empty(max_tokens, device=device, dtype=torch.int64)
-    # one buffer for the 32-bit outputs: an allocation costs more than the kernel's writes
-    words = torch.empty(max_tokens + seqs + 3, device=device, dtype=torch.int32)
-    positions, cu_new, counts = words[:max_tokens], words[max_tokens:max_tokens + seqs + 1], words[-2:]
-    native.build_slots(context_lens, new_lens, block_table, free_blocks, block_size, cu_new, positions, slots, counts)
-    return StepSlots(cu_new, positions, slots, counts[:1], counts[1:])
+    # one buffer for the 32-bit outputs: an allocation or a view costs the host more than the kernel's writes the GPU
+    positions, cu_new, taken, dropped = torch.empty(max_tokens + seqs + 3, device=device, dtype=torch.int32) \
+        .split_with_sizes((max_tokens, seqs + 1, 1, 1))
+    native.build_slots(context_lens, new_lens, block_table, free_blocks, block_size, cu_new, positions, slots, taken)
+    return StepSlots(cu_new, positions, slots, taken, dropped)

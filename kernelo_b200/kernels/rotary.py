@@ -14,7 +14,7 @@ import math
 
 import torch
 
-from kernelo_b200.kernels.attention import _check_index
+from kernelo_b200.kernels.attention import _check_index, _check_operand, _empty_like
 from kernelo_b200.runtime import native
 
 SCALINGS = ("linear", "base", "parts")
@@ -74,31 +74,22 @@ def _check(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, table: tor
     if q.ndim != 3 or k.ndim != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
         raise ValueError("expected q (tokens, heads, dim) and k (tokens, kv_heads, dim), got "
                          f"{tuple(q.shape)} and {tuple(k.shape)}")
-    if q.device.type != "cuda":
+    if not q.is_cuda:
         raise ValueError(f"q must be a CUDA tensor, got {q.device}")
     _check_operand("q", q, q)
     _check_operand("k", k, q)
-    _check_index("positions", positions, q.device)
-    if positions.shape != q.shape[:1]:
+    _check_index("positions", positions, q)
+    if positions.ndim != 1 or positions.shape[0] != q.shape[0]:
         raise ValueError(f"positions must have shape ({q.shape[0]},), got {tuple(positions.shape)}")
-    _check_index("table", table, q.device, torch.float32)
+    _check_index("table", table, q, torch.float32)
     if table.ndim != 2 or table.shape[1] % 2 or table.shape[1] > q.shape[2]:
         raise ValueError(f"table must be (positions, rotary_dim) with an even rotary_dim of at most {q.shape[2]}, "
                          f"got {tuple(table.shape)}")
 
 
-def _check_operand(name: str, t: torch.Tensor, like: torch.Tensor) -> None:
-    if t.dtype != like.dtype:
-        raise ValueError(f"dtype mismatch: {like.dtype} vs {name} {t.dtype}")
-    if t.device != like.device:
-        raise ValueError(f"{name} must be on {like.device}, got {t.device}")
-    if t.stride(-1) != 1 and t.shape[-1] > 1:
-        raise ValueError(f"{name} must have a contiguous last dimension. Pass {name}.contiguous() explicitly.")
-
-
 def _output(name: str, out: torch.Tensor | None, like: torch.Tensor) -> torch.Tensor:
     if out is None:
-        return torch.empty(like.shape, device=like.device, dtype=like.dtype)
+        return _empty_like(like)
     if out is not like:
         if out.shape != like.shape:
             raise ValueError(f"{name} must have shape {tuple(like.shape)}, got {tuple(out.shape)}")
@@ -162,16 +153,13 @@ def rotary_to_cache(
                          f"and {tuple(v_cache.shape)}")
     _check_operand("k_cache", k_cache, q)
     _check_operand("v_cache", v_cache, q)
-    _check_index("slots", slots, q.device, torch.int64)
-    if slots.shape != q.shape[:1]:
+    _check_index("slots", slots, q, torch.int64)
+    if slots.ndim != 1 or slots.shape[0] != q.shape[0]:
         raise ValueError(f"slots must have shape ({q.shape[0]},), got {tuple(slots.shape)}")
     q_out = _output("q_out", q_out, q)
     if k_out is not None:
         k_out = _output("k_out", k_out, k)
     if q.numel() or k.numel():
-        sv, skc, svc = v.stride(), k_cache.stride(), v_cache.stride()
-        cache = native.KfRotaryCache(v.data_ptr(), sv[0], sv[1], k_cache.data_ptr(), skc[0], skc[1], skc[2],
-                                     v_cache.data_ptr(), svc[0], svc[1], svc[2], k_cache.shape[0], k_cache.shape[2],
-                                     slots.data_ptr())
-        native.rotary(q, k, q_out, k_out, positions, table, interleaved=interleaved, inverse=False, cache=cache)
+        native.rotary(q, k, q_out, k_out, positions, table, interleaved=interleaved, inverse=False, v=v,
+                      k_cache=k_cache, v_cache=v_cache, slots=slots)
     return q_out

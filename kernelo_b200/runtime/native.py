@@ -22,6 +22,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import os
+import struct
 import threading
 from dataclasses import dataclass
 
@@ -158,28 +159,16 @@ class KfPeerSync(ctypes.Structure):
     ]
 
 
-class KfRotaryCache(ctypes.Structure):
-    _fields_ = [
-        ("v", ctypes.c_void_p),
-        ("sv_row", ctypes.c_int64),
-        ("sv_head", ctypes.c_int64),
-        ("k_cache", ctypes.c_void_p),
-        ("sk_page", ctypes.c_int64),
-        ("sk_head", ctypes.c_int64),
-        ("sk_slot", ctypes.c_int64),
-        ("v_cache", ctypes.c_void_p),
-        ("sv_page", ctypes.c_int64),
-        ("svc_head", ctypes.c_int64),
-        ("sv_slot", ctypes.c_int64),
-        ("pages", ctypes.c_int64),
-        ("block_size", ctypes.c_int64),
-        ("slots", ctypes.c_void_p),
-    ]
-
-
 _i32, _i64, _vp, _f32 = ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p, ctypes.c_float
 _GP = ctypes.POINTER(KfGemmConfig)
 _RP = ctypes.POINTER(KfRowsConfig)
+# The serving operators' argument structs: 8-byte fields in the header's order,
+# packed in one call (33 separate ctypes arguments cost 3 us a call, this 0.5 us).
+_packed = ctypes.c_char_p
+PREFILL_ARGS = struct.Struct("22qdq")
+TREE_ARGS = struct.Struct("30qd2q")
+ROTARY_ARGS = struct.Struct("37q")
+SLOTS_ARGS = struct.Struct("14q")
 
 _SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "kf_abi_version": (_i32, []),
@@ -214,15 +203,11 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "kf_ipc_handle": (_i32, [_vp, _vp, ctypes.POINTER(_i64)]),
     "kf_ipc_open": (_i32, [_vp, ctypes.POINTER(_vp)]),
     "kf_ipc_close": (_i32, [_vp]),
-    "kf_prefill_attention": (_i32, [_i32, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp,
-                                    _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _i32, _vp]),
-    "kf_tree_attention": (_i32, [_i32, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64,
-                                 _i64, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64,
-                                 _i64, _i64, _f32, _vp, _i64, _vp]),
+    "kf_prefill_attention": (_i32, [_packed, _vp]),
+    "kf_tree_attention": (_i32, [_packed, _vp]),
     "kf_tree_attention_workspace_bytes": (_i64, [_i32, _i32, _i64, _i64, _i64, _i64, _i64]),
-    "kf_rotary": (_i32, [_i32, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64,
-                         _i64, _i64, _i64, _i64, _i64, _i32, _i32, ctypes.POINTER(KfRotaryCache), _vp]),
-    "kf_build_slots": (_i32, [_vp, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp]),
+    "kf_rotary": (_i32, [_packed, _vp]),
+    "kf_build_slots": (_i32, [_packed, _vp]),
 }
 
 _lock = threading.Lock()
@@ -644,13 +629,35 @@ def prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: to
                       causal: bool) -> None:
     lib = _lib or load()
     rows, heads, dim = q.shape
-    sq, sk, sv, so = q.stride(), k.stride(), v.stride(), out.stride()
-    status = lib.kf_prefill_attention(native_code(q.dtype), q.data_ptr(), sq[0], sq[1], k.data_ptr(), sk[0], sk[1],
-                                      v.data_ptr(), sv[0], sv[1], out.data_ptr(), so[0], so[1], _ptr(lse),
-                                      cu_q.data_ptr(), cu_k.data_ptr(), cu_q.shape[0] - 1, rows, k.shape[0], heads,
-                                      k.shape[1], dim, scale, causal, current_stream_handle(q.device))
+    sq_row, sq_head, _ = q.stride()
+    sk_row, sk_head, _ = k.stride()
+    sv_row, sv_head, _ = v.stride()
+    so_row, so_head, _ = out.stride()
+    keys, kv_heads, _ = k.shape
+    status = lib.kf_prefill_attention(
+        PREFILL_ARGS.pack(native_code(q.dtype), q.data_ptr(), sq_row, sq_head, k.data_ptr(), sk_row, sk_head,
+                          v.data_ptr(), sv_row, sv_head, out.data_ptr(), so_row, so_head,
+                          0 if lse is None else lse.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), cu_q.shape[0] - 1,
+                          rows, keys, heads, kv_heads, dim, scale, causal),
+        current_stream_handle(q.device))
     if status:
         check(status, "kf_prefill_attention")
+
+
+def _tree_workspace(dev: torch.device, stream: int, code: int, seqs: int, rows: int, heads: int, kv_heads: int,
+                    dim: int) -> tuple[int, int]:
+    """(address, bytes) of the stream's workspace for a call of these sizes."""
+    key = ("tree_attention", dev.index, code, seqs, rows, heads, kv_heads, dim)
+    ws_bytes = _workspace_sizes.get(key)
+    if ws_bytes is None:
+        ws_bytes = load().kf_tree_attention_workspace_bytes(dev.index or 0, code, seqs, rows, heads, kv_heads, dim)
+        if ws_bytes < 0:
+            check(int(-ws_bytes), "kf_tree_attention_workspace_bytes")
+        if len(_workspace_sizes) > 4096:
+            _workspace_sizes.clear()
+        _workspace_sizes[key] = ws_bytes
+    ws = workspaces.get(dev, stream, ws_bytes)
+    return (0 if ws is None else ws.data_ptr()), ws_bytes
 
 
 def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, out: torch.Tensor,
@@ -663,52 +670,68 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     rows, heads, dim = q.shape
     pages, kv_heads, block_size, _ = k_cache.shape
     seqs, table_cols = block_table.shape
-    key = ("tree_attention", dev.index, code, seqs, rows, heads, kv_heads, dim)
-    ws_bytes = _workspace_sizes.get(key)
-    if ws_bytes is None:
-        ws_bytes = lib.kf_tree_attention_workspace_bytes(dev.index or 0, code, seqs, rows, heads, kv_heads, dim)
-        if ws_bytes < 0:
-            check(int(-ws_bytes), "kf_tree_attention_workspace_bytes")
-        if len(_workspace_sizes) > 4096:
-            _workspace_sizes.clear()
-        _workspace_sizes[key] = ws_bytes
-    ws = workspaces.get(dev, stream, ws_bytes)
-    sq, sk, sv, so = q.stride(), k_cache.stride(), v_cache.stride(), out.stride()
-    status = lib.kf_tree_attention(code, q.data_ptr(), sq[0], sq[1], k_cache.data_ptr(), sk[0], sk[1], sk[2],
-                                   v_cache.data_ptr(), sv[0], sv[1], sv[2], out.data_ptr(), so[0], so[1], _ptr(lse),
-                                   block_table.data_ptr(), block_table.stride(0), table_cols, pages, block_size,
-                                   context.data_ptr(), _ptr(cu_q), _ptr(tree_mask),
-                                   0 if tree_mask is None else tree_mask.shape[1], seqs, rows, heads, kv_heads, dim,
-                                   scale, _ptr(ws), ws_bytes, stream)
+    ws_ptr, ws_bytes = _tree_workspace(dev, stream, code, seqs, rows, heads, kv_heads, dim)
+    sq_row, sq_head, _ = q.stride()
+    sk_page, sk_head, sk_slot, _ = k_cache.stride()
+    sv_page, sv_head, sv_slot, _ = v_cache.stride()
+    so_row, so_head, _ = out.stride()
+    status = lib.kf_tree_attention(
+        TREE_ARGS.pack(code, q.data_ptr(), sq_row, sq_head, k_cache.data_ptr(), sk_page, sk_head, sk_slot,
+                       v_cache.data_ptr(), sv_page, sv_head, sv_slot, out.data_ptr(), so_row, so_head,
+                       0 if lse is None else lse.data_ptr(), block_table.data_ptr(), block_table.stride(0), table_cols,
+                       pages, block_size, context.data_ptr(), 0 if cu_q is None else cu_q.data_ptr(),
+                       0 if tree_mask is None else tree_mask.data_ptr(),
+                       0 if tree_mask is None else tree_mask.shape[1], seqs, rows, heads, kv_heads, dim, scale,
+                       ws_ptr, ws_bytes),
+        stream)
     if status:
         check(status, "kf_tree_attention")
 
 
 def rotary(q: torch.Tensor, k: torch.Tensor, q_out: torch.Tensor, k_out: torch.Tensor | None,
            positions: torch.Tensor, table: torch.Tensor, *, interleaved: bool, inverse: bool,
-           cache: KfRotaryCache | None = None) -> None:
-    """Turn q and k by their positions' angles (and, with ``cache``, write it)."""
+           v: torch.Tensor | None = None, k_cache: torch.Tensor | None = None, v_cache: torch.Tensor | None = None,
+           slots: torch.Tensor | None = None) -> None:
+    """Turn q and k by their positions' angles (and, with ``slots``, write the cache)."""
     lib = _lib or load()
     tokens, heads, dim = q.shape
-    sq, sk, sqo = q.stride(), k.stride(), q_out.stride()
-    sko = (0, 0) if k_out is None else k_out.stride()
-    status = lib.kf_rotary(native_code(q.dtype), q.data_ptr(), sq[0], sq[1], q_out.data_ptr(), sqo[0], sqo[1],
-                           k.data_ptr(), sk[0], sk[1], _ptr(k_out), sko[0], sko[1], positions.data_ptr(),
-                           table.data_ptr(), table.shape[0], table.shape[1], tokens, heads, k.shape[1], dim,
-                           interleaved, inverse, cache, current_stream_handle(q.device))
+    sq_row, sq_head, _ = q.stride()
+    sqo_row, sqo_head, _ = q_out.stride()
+    sk_row, sk_head, _ = k.stride()
+    sko_row, sko_head, _ = (0, 0, 0) if k_out is None else k_out.stride()
+    table_rows, rot = table.shape
+    if slots is None:
+        cached = _NO_CACHE
+    else:
+        sv_row, sv_head, _ = v.stride()
+        skc_page, skc_head, skc_slot, _ = k_cache.stride()
+        svc_page, svc_head, svc_slot, _ = v_cache.stride()
+        cached = (v.data_ptr(), sv_row, sv_head, k_cache.data_ptr(), skc_page, skc_head, skc_slot, v_cache.data_ptr(),
+                  svc_page, svc_head, svc_slot, k_cache.shape[0], k_cache.shape[2], slots.data_ptr())
+    status = lib.kf_rotary(
+        ROTARY_ARGS.pack(native_code(q.dtype), q.data_ptr(), sq_row, sq_head, q_out.data_ptr(), sqo_row, sqo_head,
+                         k.data_ptr(), sk_row, sk_head, 0 if k_out is None else k_out.data_ptr(), sko_row, sko_head,
+                         positions.data_ptr(), table.data_ptr(), table_rows, rot, tokens, heads, k.shape[1], dim,
+                         interleaved, inverse, *cached),
+        current_stream_handle(q.device))
     if status:
         check(status, "kf_rotary")
+
+
+_NO_CACHE = (0,) * 14
 
 
 def build_slots(context: torch.Tensor, added: torch.Tensor, block_table: torch.Tensor, free_blocks: torch.Tensor,
                 block_size: int, cu_new: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor,
                 counts: torch.Tensor) -> None:
+    """``counts``: the first of two int32 words."""
     lib = _lib or load()
-    status = lib.kf_build_slots(context.data_ptr(), added.data_ptr(), context.shape[0], block_table.data_ptr(),
-                                block_table.stride(0), block_table.shape[1], free_blocks.data_ptr(),
-                                free_blocks.shape[0], block_size, slots.shape[0], cu_new.data_ptr(),
-                                positions.data_ptr(), slots.data_ptr(), counts.data_ptr(),
-                                current_stream_handle(block_table.device))
+    seqs, table_cols = block_table.shape
+    status = lib.kf_build_slots(
+        SLOTS_ARGS.pack(context.data_ptr(), added.data_ptr(), seqs, block_table.data_ptr(), block_table.stride(0),
+                        table_cols, free_blocks.data_ptr(), free_blocks.shape[0], block_size, slots.shape[0],
+                        cu_new.data_ptr(), positions.data_ptr(), slots.data_ptr(), counts.data_ptr()),
+        current_stream_handle(block_table.device))
     if status:
         check(status, "kf_build_slots")
 
