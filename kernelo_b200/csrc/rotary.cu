@@ -10,7 +10,10 @@
 // The inverse is the gradient, since the rotation is orthogonal. With a cache,
 // the turned k and the v of each token also go to its slot (none if negative).
 //
-// Bound by bytes: every element is read once and written once to each place.
+// Bound by bytes: every element is read once and written once to each place. A
+// thread turns the two vectors (16 bytes each where layout and alignment allow)
+// that hold its pairs for several heads: its cosines and sines are loaded once for
+// all of them.
 #include <cuda.h>
 
 #include <initializer_list>
@@ -22,6 +25,8 @@ namespace kf {
 namespace {
 
 constexpr int ROTARY_THREADS = 256;
+constexpr int BATCH = 2;       // heads whose loads are in flight together
+constexpr int HEADS_EACH = 6;  // that a thread turns with one load of its angles
 
 // A thread turns one unit of a token's heads: the two vectors of VE elements
 // that hold VE pairs, or two plain vectors of the rest of the head.
@@ -30,11 +35,10 @@ struct alignas(sizeof(T) * VE) Vec {
   T e[VE];
 };
 
+// Threads of a block: units of a head (turned ones first, then plain ones) x
+// heads side by side x tokens.
 struct RotaryPlan {
-  int units;         // per head: turned ones first, then plain ones
-  int turned;
-  int head_lanes;    // threads that share a token's heads, each taking every head_lanes-th
-  int per_token;     // units * head_lanes
+  int units, turned, lanes, tokens;
 };
 
 template <typename T, int VE>
@@ -61,13 +65,11 @@ __device__ __forceinline__ void turn(Vec<T, VE>& x, Vec<T, VE>& y, const float (
 }
 
 template <typename T, int VE>
-__global__ void __launch_bounds__(ROTARY_THREADS) rotary_kernel(const RotaryArgs p, const RotaryPlan plan) {
+__global__ void __launch_bounds__(ROTARY_THREADS, 4) rotary_kernel(const __grid_constant__ RotaryArgs p, const RotaryPlan plan) {
   using V = Vec<T, VE>;
-  const long long at = static_cast<long long>(blockIdx.x) * ROTARY_THREADS + threadIdx.x;
-  const long long t = at / plan.per_token;
+  const long long t = static_cast<long long>(blockIdx.x) * plan.tokens + threadIdx.z;
   if (t >= p.tokens) return;
-  const int rest = static_cast<int>(at - t * plan.per_token);
-  const int unit = rest % plan.units, lane = rest / plan.units;
+  const int unit = threadIdx.x;
   const int rot = static_cast<int>(p.rot), half = rot / 2;
 
   // The unit's two vectors by their first element; `pairs` its table column.
@@ -88,54 +90,96 @@ __global__ void __launch_bounds__(ROTARY_THREADS) rotary_kernel(const RotaryArgs
     const int pos = __ldg(p.positions + t);
     const bool known = pos >= 0 && pos < p.table_rows;
     const float* row = p.table + static_cast<long long>(known ? pos : 0) * rot + pairs;
+    if (known) {
+      if constexpr (VE >= 4) {
 #pragma unroll
-    for (int i = 0; i < VE; ++i) {
-      c[i] = known ? __ldg(row + i) : __int_as_float(0x7fc00000);
-      s[i] = known ? __ldg(row + half + i) : __int_as_float(0x7fc00000);
-      if (p.inverse) s[i] = -s[i];
+        for (int i = 0; i < VE; i += 4) {
+          const float4 a = __ldg(reinterpret_cast<const float4*>(row + i));
+          const float4 b = __ldg(reinterpret_cast<const float4*>(row + half + i));
+          c[i] = a.x, c[i + 1] = a.y, c[i + 2] = a.z, c[i + 3] = a.w;
+          s[i] = b.x, s[i + 1] = b.y, s[i + 2] = b.z, s[i + 3] = b.w;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < VE; ++i) {
+          c[i] = __ldg(row + i);
+          s[i] = __ldg(row + half + i);
+        }
+      }
+      if (p.inverse) {
+#pragma unroll
+        for (int i = 0; i < VE; ++i) s[i] = -s[i];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < VE; ++i) c[i] = s[i] = __int_as_float(0x7fc00000);
     }
+  }
+  const int hq = static_cast<int>(p.heads), hk = static_cast<int>(p.kv_heads), lanes = plan.lanes;
+  int h = threadIdx.y;
+  {
+    const T* q = static_cast<const T*>(p.q) + t * p.sq_t;
+    T* q_out = static_cast<T*>(p.q_out) + t * p.sqo_t;
+    for (; h < hq; h += BATCH * lanes) {
+      V x[BATCH], y[BATCH];
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        if (h + i * lanes < hq) {
+          const T* from = q + (h + i * lanes) * p.sq_h;
+          x[i] = *reinterpret_cast<const V*>(from + e0);
+          if (second) y[i] = *reinterpret_cast<const V*>(from + e1);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        if (h + i * lanes < hq) {
+          if (turned) turn<T, VE>(x[i], y[i], c, s, p.interleaved);
+          T* to = q_out + (h + i * lanes) * p.sqo_h;
+          *reinterpret_cast<V*>(to + e0) = x[i];
+          if (second) *reinterpret_cast<V*>(to + e1) = y[i];
+        }
+      }
+    }
+    // on with the heads of k where this thread's stride left q
+    while (h - lanes >= hq) h -= lanes;
   }
   long long page = -1, slot = 0;
   if (p.slots != nullptr) {
     const long long n = __ldg(reinterpret_cast<const long long*>(p.slots) + t);
     if (n >= 0 && n < p.pages * p.block_size) {
-      page = n / p.block_size;
+      if (((n | p.block_size) >> 32) == 0) {
+        page = static_cast<uint32_t>(n) / static_cast<uint32_t>(p.block_size);
+      } else {
+        page = n / p.block_size;
+      }
       slot = n - page * p.block_size;
     }
   }
-  const int hq = static_cast<int>(p.heads), hk = static_cast<int>(p.kv_heads);
-  const int all = hq + hk + (p.slots != nullptr ? hk : 0);
-  for (int h = lane; h < all; h += plan.head_lanes) {
-    const T* src;
-    T *to, *cached = nullptr;
-    bool turn_it = turned;
-    if (h < hq) {
-      src = static_cast<const T*>(p.q) + t * p.sq_t + h * p.sq_h;
-      to = static_cast<T*>(p.q_out) + t * p.sqo_t + h * p.sqo_h;
-    } else if (h < hq + hk) {
-      const int g = h - hq;
-      src = static_cast<const T*>(p.k) + t * p.sk_t + g * p.sk_h;
-      to = p.k_out != nullptr ? static_cast<T*>(p.k_out) + t * p.sko_t + g * p.sko_h : nullptr;
-      if (page >= 0) cached = static_cast<T*>(p.k_cache) + page * p.skc_p + g * p.skc_h + slot * p.skc_s;
-    } else {
-      const int g = h - hq - hk;
-      src = static_cast<const T*>(p.v) + t * p.sv_t + g * p.sv_h;
-      to = nullptr;
-      if (page >= 0) cached = static_cast<T*>(p.v_cache) + page * p.svc_p + g * p.svc_h + slot * p.svc_s;
-      turn_it = false;
-    }
-    if (to == nullptr && cached == nullptr) continue;
-    V x = *reinterpret_cast<const V*>(src + e0), y{};
-    if (second) y = *reinterpret_cast<const V*>(src + e1);
-    if (turn_it) turn<T, VE>(x, y, c, s, p.interleaved);
-    if (to != nullptr) {
+  if (page < 0 && p.k_out == nullptr) return;
+  for (; h < hq + hk; h += lanes) {
+    const int g = h - hq;
+    const T* from = static_cast<const T*>(p.k) + t * p.sk_t + g * p.sk_h;
+    V x = *reinterpret_cast<const V*>(from + e0), y;
+    if (second) y = *reinterpret_cast<const V*>(from + e1);
+    if (turned) turn<T, VE>(x, y, c, s, p.interleaved);
+    if (p.k_out != nullptr) {
+      T* to = static_cast<T*>(p.k_out) + t * p.sko_t + g * p.sko_h;
       *reinterpret_cast<V*>(to + e0) = x;
       if (second) *reinterpret_cast<V*>(to + e1) = y;
     }
-    if (cached != nullptr) {
-      *reinterpret_cast<V*>(cached + e0) = x;
-      if (second) *reinterpret_cast<V*>(cached + e1) = y;
+    if (page >= 0) {
+      T* to = static_cast<T*>(p.k_cache) + page * p.skc_p + g * p.skc_h + slot * p.skc_s;
+      *reinterpret_cast<V*>(to + e0) = x;
+      if (second) *reinterpret_cast<V*>(to + e1) = y;
     }
+  }
+  if (page < 0) return;
+  for (; h < hq + 2 * hk; h += lanes) {
+    const int g = h - hq - hk;
+    const T* from = static_cast<const T*>(p.v) + t * p.sv_t + g * p.sv_h;
+    T* to = static_cast<T*>(p.v_cache) + page * p.svc_p + g * p.svc_h + slot * p.svc_s;
+    *reinterpret_cast<V*>(to + e0) = *reinterpret_cast<const V*>(from + e0);
+    if (second) *reinterpret_cast<V*>(to + e1) = *reinterpret_cast<const V*>(from + e1);
   }
 }
 
@@ -147,41 +191,57 @@ bool on_grid(const void* ptr, int64_t vec, int elem, std::initializer_list<int64
   return true;
 }
 
+// Whether heads, halves, table rows and strides hold whole vectors of VE elements.
 template <typename T, int VE>
-int launch_typed(const RotaryArgs& a, cudaStream_t stream) {
+bool whole_vectors(const RotaryArgs& a) {
+  const int elem = static_cast<int>(sizeof(T));
+  return a.dim % VE == 0 && a.rot % (2 * VE) == 0 &&
+         (VE < 4 || reinterpret_cast<uintptr_t>(a.table) % 16 == 0) && on_grid(a.q, VE, elem, {a.sq_t, a.sq_h}) &&
+         on_grid(a.q_out, VE, elem, {a.sqo_t, a.sqo_h}) && on_grid(a.k, VE, elem, {a.sk_t, a.sk_h}) &&
+         on_grid(a.k_out, VE, elem, {a.sko_t, a.sko_h}) && on_grid(a.v, VE, elem, {a.sv_t, a.sv_h}) &&
+         on_grid(a.k_cache, VE, elem, {a.skc_p, a.skc_h, a.skc_s}) &&
+         on_grid(a.v_cache, VE, elem, {a.svc_p, a.svc_h, a.svc_s});
+}
+
+template <typename T, int VE>
+int launch_typed(const RotaryArgs& a, const DeviceInfo& dev, cudaStream_t stream) {
+  const int64_t turned = a.rot / 2 / VE, units = turned + ceil_div(a.dim - a.rot, 2 * VE);
+  if (units > ROTARY_THREADS) return set_error(KF_ERR_UNSUPPORTED, "rotary: heads too wide for their alignment");
+  // Heads side by side: HEADS_EACH heads a thread, or one where that leaves the
+  // GPU without threads to cover its latency (a decoding step).
+  const int64_t all = a.heads + a.kv_heads * (a.slots != nullptr ? 2 : 1);
+  const bool few = a.tokens * units * ceil_div(all, HEADS_EACH) < static_cast<int64_t>(dev.sm_count) * 1024;
   RotaryPlan plan;
-  plan.turned = static_cast<int>(a.rot / 2 / VE);
-  plan.units = plan.turned + static_cast<int>(ceil_div(a.dim - a.rot, 2 * VE));
-  plan.head_lanes = 1;
-  plan.per_token = plan.units * plan.head_lanes;
-  const int64_t blocks = ceil_div(a.tokens * plan.per_token, ROTARY_THREADS);
+  plan.units = static_cast<int>(units);
+  plan.turned = static_cast<int>(turned);
+  const int64_t most = ROTARY_THREADS / units;
+  const int64_t lanes = few ? all : ceil_div(all, HEADS_EACH);
+  plan.lanes = static_cast<int>(lanes < most ? lanes : most);
+  plan.tokens = ROTARY_THREADS / (plan.units * plan.lanes);
+  if (plan.tokens > 64) plan.tokens = 64;  // the limit of a block's third extent
+  const int64_t blocks = ceil_div(a.tokens, plan.tokens);
   if (blocks > 0x7fffffffll) return set_error(KF_ERR_UNSUPPORTED, "rotary: tokens beyond the grid");
-  rotary_kernel<T, VE><<<static_cast<unsigned>(blocks), ROTARY_THREADS, 0, stream>>>(a, plan);
+  rotary_kernel<T, VE><<<static_cast<unsigned>(blocks), dim3(plan.units, plan.lanes, plan.tokens), 0, stream>>>(a, plan);
   const cudaError_t err = cudaGetLastError();
   return err == cudaSuccess ? KF_OK : cuda_error(err, "launch(rotary)");
 }
 
 template <typename T>
-int pick(const RotaryArgs& a, cudaStream_t stream) {
-  constexpr int VE = 16 / static_cast<int>(sizeof(T));
-  const int elem = static_cast<int>(sizeof(T));
-  // 16-byte vectors where heads, halves and strides hold whole ones; the turned
-  // part is VE pairs a unit in both layouts
-  const bool whole = a.dim % VE == 0 && a.rot % (2 * VE) == 0 && on_grid(a.q, VE, elem, {a.sq_t, a.sq_h}) &&
-                     on_grid(a.q_out, VE, elem, {a.sqo_t, a.sqo_h}) && on_grid(a.k, VE, elem, {a.sk_t, a.sk_h}) &&
-                     on_grid(a.k_out, VE, elem, {a.sko_t, a.sko_h}) && on_grid(a.v, VE, elem, {a.sv_t, a.sv_h}) &&
-                     on_grid(a.k_cache, VE, elem, {a.skc_p, a.skc_h, a.skc_s}) &&
-                     on_grid(a.v_cache, VE, elem, {a.svc_p, a.svc_h, a.svc_s});
-  return whole ? launch_typed<T, VE>(a, stream) : launch_typed<T, 1>(a, stream);
+int pick(const RotaryArgs& a, const DeviceInfo& dev, cudaStream_t stream) {
+  if constexpr (sizeof(T) == 2)
+    if (whole_vectors<T, 8>(a)) return launch_typed<T, 8>(a, dev, stream);
+  if (whole_vectors<T, 4>(a)) return launch_typed<T, 4>(a, dev, stream);
+  if (whole_vectors<T, 2>(a)) return launch_typed<T, 2>(a, dev, stream);
+  return launch_typed<T, 1>(a, dev, stream);
 }
 
 }  // namespace
 
-int launch_rotary(const RotaryArgs& a, const DeviceInfo&, cudaStream_t stream) {
+int launch_rotary(const RotaryArgs& a, const DeviceInfo& dev, cudaStream_t stream) {
   switch (a.dtype) {
-    case KF_FP16: return pick<__half>(a, stream);
-    case KF_BF16: return pick<__nv_bfloat16>(a, stream);
-    default: return pick<float>(a, stream);
+    case KF_FP16: return pick<__half>(a, dev, stream);
+    case KF_BF16: return pick<__nv_bfloat16>(a, dev, stream);
+    default: return pick<float>(a, dev, stream);
   }
 }
 
