@@ -23,7 +23,7 @@
 // their V rows are zeroed in shared memory (0 x inf is NaN); a row that still
 // comes out non-finite (its own later tokens hold infinities) is recomputed key
 // by key.
-#include <cudaTypedefs.h>
+#include <cuda.h>
 
 #include <mutex>
 
@@ -418,41 +418,6 @@ __global__ void __launch_bounds__(THREADS, 1)
   if (warp == MMA_WARP) tmem_dealloc(tmem, TMEM_COLS);
 }
 
-PFN_cuTensorMapEncodeTiled_v12000 encoder() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* sym = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(sym);
-  });
-  return fn;
-}
-
-// [rows, heads, dim] as boxes of 128 rows x 64 elements of one head; elements
-// past the head and rows past the last are filled with zeros.
-int encode_heads(CUtensorMap* map, int dtype, const void* ptr, int64_t rows, int64_t heads, int64_t dim, int64_t s_row,
-                 int64_t s_head) {
-  auto enc = encoder();
-  if (enc == nullptr) return set_error(KF_ERR_LAUNCH, "cuTensorMapEncodeTiled unavailable");
-  const int64_t whole = ceil_div(dim, 8) * 8;
-  // a dimension of one has no stride to speak of
-  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(dim), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(rows)};
-  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(2 * (heads > 1 ? s_head : whole)),
-                                 static_cast<cuuint64_t>(2 * (rows > 1 ? s_row : whole))};
-  const cuuint32_t box[3] = {64, 1, BLK}, unit[3] = {1, 1, 1};
-  const CUresult r = enc(map, dtype == KF_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
-                         const_cast<void*>(ptr), dims, strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS)
-    return set_error(KF_ERR_UNALIGNED, "prompt attention: cuTensorMapEncodeTiled rejected an operand (error " +
-                                           std::to_string(r) + ")");
-  return KF_OK;
-}
-
 bool on_grid(const void* ptr, int64_t s_row, int64_t rows, int64_t s_head, int64_t heads) {
   const auto fits = [](int64_t s, int64_t n) { return n <= 1 || (s > 0 && s % 8 == 0 && s < (1ll << 38)); };
   return reinterpret_cast<uintptr_t>(ptr) % 16 == 0 && fits(s_row, rows) && fits(s_head, heads);
@@ -461,9 +426,9 @@ bool on_grid(const void* ptr, int64_t s_row, int64_t rows, int64_t s_head, int64
 template <typename T, int DH>
 int launch_typed(const AttnArgs& a, const DeviceInfo& dev, cudaStream_t stream) {
   CUtensorMap q, k, v;
-  int rc = encode_heads(&q, a.dtype, a.q, a.rows, a.heads, a.dim, a.sq_t, a.sq_h);
-  if (rc == KF_OK) rc = encode_heads(&k, a.dtype, a.k, a.keys, a.kv_heads, a.dim, a.sk_t, a.sk_h);
-  if (rc == KF_OK) rc = encode_heads(&v, a.dtype, a.v, a.keys, a.kv_heads, a.dim, a.sv_t, a.sv_h);
+  int rc = encode_heads(&q, a.dtype, a.q, a.rows, a.heads, a.dim, a.sq_t, a.sq_h, 1, BLK);
+  if (rc == KF_OK) rc = encode_heads(&k, a.dtype, a.k, a.keys, a.kv_heads, a.dim, a.sk_t, a.sk_h, 1, BLK);
+  if (rc == KF_OK) rc = encode_heads(&v, a.dtype, a.v, a.keys, a.kv_heads, a.dim, a.sv_t, a.sv_h, 1, BLK);
   if (rc != KF_OK) return rc;
   static std::once_flag once;
   static cudaError_t attr = cudaSuccess;

@@ -27,7 +27,7 @@
 //
 // With one new token and G heads to a key head, G of the 16 rows are real: the
 // products are free beside the cache's bytes, which bound the call.
-#include <cudaTypedefs.h>
+#include <cuda.h>
 
 #include <initializer_list>
 #include <mutex>
@@ -448,37 +448,6 @@ __global__ void __launch_bounds__(THREADS, 2)
   }
 }
 
-PFN_cuTensorMapEncodeTiled_v12000 encoder() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* sym = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(sym);
-  });
-  return fn;
-}
-
-// Pages [pages, kv_heads, block_size, dim] as boxes of `box_rows` slots x 64 (32)
-// elements; what lies past the head or past the last page is filled with zeros.
-bool encode_pages(CUtensorMap* map, const AttnArgs& a, const void* ptr, int64_t s_page, int64_t s_head, int64_t s_slot,
-                  int box_rows, int width) {
-  auto enc = encoder();
-  if (enc == nullptr) return false;
-  const auto bytes = [](int64_t s, int64_t n) { return static_cast<cuuint64_t>(n > 1 ? 2 * s : 16); };
-  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(a.dim), static_cast<cuuint64_t>(a.block_size),
-                              static_cast<cuuint64_t>(a.kv_heads), static_cast<cuuint64_t>(a.pages)};
-  const cuuint64_t strides[3] = {bytes(s_slot, a.block_size), bytes(s_head, a.kv_heads), bytes(s_page, a.pages)};
-  const cuuint32_t box[4] = {static_cast<cuuint32_t>(width), static_cast<cuuint32_t>(box_rows), 1, 1};
-  const cuuint32_t unit[4] = {1, 1, 1, 1};
-  return enc(map, a.dtype == KF_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
-             const_cast<void*>(ptr), dims, strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE,
-             width == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <typename T, typename S>
 int launch_shape(const AttnArgs& a, const DeviceInfo& dev, int ctas, cudaStream_t stream) {
   static std::once_flag once;
@@ -538,8 +507,16 @@ bool attention_tree_supported(const AttnArgs& a) {
          on_grid(a.q, 8, {a.sq_t, a.sq_h});
 }
 
+// Rows that a request has for a key head on average: above 16 the products of
+// mma.sync tiles take longer than the cache's bytes.
+static bool many_rows(const AttnArgs& a) {
+  return ceil_div(a.rows, a.seqs > 0 ? a.seqs : 1) * (a.heads / a.kv_heads) > M;
+}
+
 int64_t attention_tree_workspace_bytes(const AttnArgs& a, const DeviceInfo& dev) {
-  return TREE_COUNTER_BYTES + 4ll * 2 * (2 * dev.sm_count) * M * (padded_dim(a) + 2);
+  const int64_t narrow = TREE_COUNTER_BYTES + 4ll * 2 * (2 * dev.sm_count) * M * (padded_dim(a) + 2);
+  const int64_t wide = many_rows(a) ? attention_tree_wide_workspace_bytes(a, dev) : 0;
+  return narrow > wide ? narrow : wide;
 }
 
 int launch_attention_tree(const AttnArgs& a, const DeviceInfo& dev, cudaStream_t stream) {
@@ -548,6 +525,7 @@ int launch_attention_tree(const AttnArgs& a, const DeviceInfo& dev, cudaStream_t
     return set_error(KF_ERR_WORKSPACE, "tree attention needs " + std::to_string(need) + " bytes of workspace; got " +
                                            std::to_string(a.workspace == nullptr ? 0 : a.workspace_bytes));
   if (2 * dev.sm_count > TREE_COUNTER_BYTES / 4) return set_error(KF_ERR_UNSUPPORTED, "tree attention: too many SMs");
+  if (many_rows(a) && attention_tree_wide_supported(a)) return launch_attention_tree_wide(a, dev, stream);
   return a.dtype == KF_FP16 ? launch_typed<__half>(a, dev, stream) : launch_typed<__nv_bfloat16>(a, dev, stream);
 }
 

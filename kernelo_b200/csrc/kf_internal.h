@@ -1,6 +1,7 @@
 // Host-side declarations shared by the translation units of libkernelo_b200.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -260,14 +261,31 @@ struct AttnArgs {
   int64_t workspace_bytes = 0;
 };
 constexpr int64_t ATTN_MAX_DIM = 256;
+// Tensor maps (attention_maps.cu), 16-bit types. [rows, heads, dim] as boxes of
+// box_rows x box_heads x 64 elements in the 128-byte swizzle; elements past the
+// head and rows past the last are filled with zeros.
+int encode_heads(CUtensorMap* map, int dtype, const void* ptr, int64_t rows, int64_t heads, int64_t dim, int64_t s_row,
+                 int64_t s_head, int box_heads, int box_rows);
+// Pages [pages, kv_heads, block_size, dim] as boxes of box_rows slots x `width`
+// elements (64, or 32 in the 64-byte swizzle); what lies past the head or past the
+// last page is filled with zeros. False where no tensor map describes the cache.
+bool encode_pages(CUtensorMap* map, const AttnArgs& args, const void* ptr, int64_t s_page, int64_t s_head, int64_t s_slot,
+                  int box_rows, int width);
 // A warp per row and head, key by key: every type, stride and mask.
 int launch_attention_rows(const AttnArgs& args, cudaStream_t stream);
 // Packed prompts on tcgen05 tiles (attention_prefill.cu): fp16/bf16, heads of up
 // to 128 elements on the 16-byte grid, a positive scale.
 bool attention_prefill_supported(const AttnArgs& args);
 int launch_attention_prefill(const AttnArgs& args, const DeviceInfo& dev, cudaStream_t stream);
+// Many rows to a key head (attention_tree_wide.cu): tcgen05 tiles of 128 rows,
+// pages of whole runs of 8 keys or more.
+bool attention_tree_wide_supported(const AttnArgs& args);
+int64_t attention_tree_wide_workspace_bytes(const AttnArgs& args, const DeviceInfo& dev);
+int launch_attention_tree_wide(const AttnArgs& args, const DeviceInfo& dev, cudaStream_t stream);
+
 // New tokens over a paged cache on mma.sync tiles (attention_tree.cu): fp16/bf16,
-// heads of up to 128 elements on the 16-byte grid.
+// heads of up to 128 elements on the 16-byte grid. Takes the wide form where a
+// request has more than 16 rows to a key head on average.
 bool attention_tree_supported(const AttnArgs& args);
 int64_t attention_tree_workspace_bytes(const AttnArgs& args, const DeviceInfo& dev);
 int launch_attention_tree(const AttnArgs& args, const DeviceInfo& dev, cudaStream_t stream);
