@@ -10,6 +10,7 @@
 #pragma once
 
 #include "attention.cuh"
+#include "attention_softmax.cuh"
 
 namespace kf {
 
@@ -219,17 +220,6 @@ __device__ __forceinline__ uint32_t nodes_seen(const AttnArgs& p, const Cursor& 
   unsigned long long v = w < p.mask_words ? __ldg(words + w) >> b : 0ull;
   if (b > 32 && w + 1 < p.mask_words) v |= __ldg(words + w + 1) << (64 - b);
   return static_cast<uint32_t>(v);
-}
-
-template <typename T>
-__device__ __forceinline__ uint32_t pack_pair(float a, float b) {
-  uint32_t r;
-  if constexpr (DType<T>::code == KF_BF16) {
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
-  } else {
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
-  }
-  return r;
 }
 
 template <typename T, int NE>

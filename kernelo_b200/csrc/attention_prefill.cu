@@ -11,8 +11,9 @@
 //   warps 0-3, 4-7   softmax of tile 0 and 1, a thread per row: S from TMEM into
 //                    registers, P (16 bit) back over the same columns.
 //   warp 8           TMA: Q once, then K and V blocks through a ring.
-//   warp 9           issues the MMAs. While one tile's warps compute their
-//                    weights the tensor cores work for the other tile.
+//   warp 9           one thread issues the MMAs. While one tile's warps compute
+//                    their weights the tensor cores work for the other tile.
+//   warp 10          zeroes what the last V block holds of the next request.
 //
 // m is raised, and O (in TMEM) rescaled, only when a row's maximum grew by more
 // than 2^8: until then the weights are at most 256, which 16 bits and the fp32 sums
@@ -28,6 +29,7 @@
 #include <mutex>
 
 #include "attention.cuh"
+#include "attention_softmax.cuh"
 
 namespace kf {
 namespace {
@@ -35,8 +37,11 @@ namespace {
 constexpr int BLK = 128;       // rows of a tile, keys of a block
 constexpr int PAIR = 2 * BLK;  // rows of a CTA
 constexpr int SOFTMAX_WARPS = 8;
-constexpr int TMA_WARP = 8, MMA_WARP = 9;
-constexpr int THREADS = 10 * 32;
+constexpr int TMA_WARP = 8, MMA_WARP = 9, CLEAN_WARP = 10;
+// Three warpgroups; the last (loads, products) hands registers to the softmax:
+// 3 x 168 a thread become 2 x 216 and 72.
+constexpr int THREADS = 3 * 128;
+constexpr int LAUNCH_REGISTERS = 168;
 constexpr uint32_t TMEM_COLS = 512;  // S0 | S1 | O0 | O1, 128 each
 constexpr float RAISE_LOG2 = 8.0f;
 constexpr uint64_t DRAIN_NS = 100000000ull;
@@ -98,17 +103,6 @@ __device__ __forceinline__ int visible(const AttnArgs& p, const Item& it, int i)
   return min(it.keys, max(0, it.node0 + i + 1 + it.shift));
 }
 
-template <typename T>
-__device__ __forceinline__ uint32_t pack_pair(float a, float b) {
-  uint32_t r;
-  if constexpr (DType<T>::code == KF_BF16) {
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
-  } else {
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
-  }
-  return r;
-}
-
 template <typename T, int DH>
 __device__ __noinline__ void redo_row(const AttnArgs& p, int t, int head, int lane) {
   float acc[DH / 32], m, l;
@@ -128,7 +122,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint8_t* q_tiles = smem;
   uint8_t* ring = smem + 2 * S::TILE;
   uint64_t* bars = reinterpret_cast<uint64_t*>(ring + STAGES * S::TILE);
-  // bars: q[2] | full[STAGES] | empty[STAGES] | s_full[2] | p_full[2] | o_full[2]
+  // bars: q[2] | full[STAGES] | empty[STAGES] | s_full[2] | p_full[2] | o_full[2] | dirty | clean
   __shared__ Item item;
   __shared__ int has_item;
   __shared__ uint32_t tmem_slot;
@@ -137,7 +131,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t q_bar = smem_u32(bars), full = q_bar + 16, empty = full + 8 * STAGES, s_full = empty + 8 * STAGES,
-                 p_full = s_full + 16, o_full = p_full + 16;
+                 p_full = s_full + 16, o_full = p_full + 16, dirty = o_full + 16, clean = dirty + 8;
   const int heads = static_cast<int>(p.heads);
   const int head = static_cast<int>(blockIdx.x % heads);
 
@@ -150,6 +144,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       mbar_init(p_full + 8 * t, SOFTMAX_WARPS / 2);
       mbar_init(o_full + 8 * t, 1);
     }
+    mbar_init(dirty, 1);
+    mbar_init(clean, 1);
     abort_word = 0;
     mbar_init_fence();
     tma_prefetch_desc(&tm_q);
@@ -173,9 +169,9 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
   const int most = max(blocks[0], blocks[1]);
 
-  if (!has_item) {
-    // nothing of this number; only the TMEM to give back
-  } else if (warp == TMA_WARP) {
+  if (warp >= SOFTMAX_WARPS) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (has_item && warp == TMA_WARP) {
     if (lane == 0 && most > 0) {
       const int kv_head = head / static_cast<int>(p.heads / p.kv_heads);
       bool ok = true;
@@ -205,84 +201,95 @@ __global__ void __launch_bounds__(THREADS, 1)
           mbar_wait(full + 8 * s, ((issued - 1 - s) / STAGES) & 1, nullptr, status, SITE_DRAIN, DRAIN_NS);
       }
     }
-  } else if (warp == MMA_WARP) {
-    if (most > 0) {
-      const uint32_t fmt = DType<T>::code == KF_BF16 ? 1u : 0u;
-      const uint32_t idesc_s = instr_desc_f16(fmt, 0, 0, BLK, BLK);
-      const uint32_t idesc_o = instr_desc_f16(fmt, 0, 1, BLK, DH);
+    } else if (has_item && warp == CLEAN_WARP) {
+      // The last block of a request: its V rows past the request's keys, when the
+      // thread of the products has seen them land
+      const int held = it.keys - (most - 1) * BLK;
+      if (most > 0 && held < BLK) {
+        const int slot = (2 * most - 1) % STAGES;  // of the ring: K V K V ...
+        mbar_wait(dirty, 0, abort_flag, status, SITE_ATTN_LOAD);
+        __syncwarp();
+        for (int i = lane; i < (BLK - held) * S::HALVES * 8; i += 32) {
+          const int h = i / ((BLK - held) * 8), rest = i - h * (BLK - held) * 8;
+          *reinterpret_cast<uint4*>(ring + slot * S::TILE + h * BLK * 128 + held * 128 + rest * 16) =
+              make_uint4(0u, 0u, 0u, 0u);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(clean);
+      }
+    } else if (has_item && warp == MMA_WARP && lane == 0 && most > 0) {
+      // One thread, and as few instructions as can be between one product and the
+      // next: the tensor cores run dry behind every one of them.
+      constexpr uint32_t fmt = DType<T>::code == KF_BF16 ? 1u : 0u;
+      constexpr uint32_t idesc_s = instr_desc_f16(fmt, 0, 0, BLK, BLK), idesc_o = instr_desc_f16(fmt, 0, 1, BLK, DH);
       const uint64_t q_desc = smem_desc_sw128(smem_u32(q_tiles), 16, 1024);
-      int taken = 0;  // ring tiles waited for
+      const uint64_t k_desc = smem_desc_sw128(smem_u32(ring), 16, 1024), v_desc = smem_desc_sw128(smem_u32(ring), BLK * 128, 1024);
+      int slot = 0, phase = 0;  // of the ring's next tile
       bool ok = true;
-      auto wait = [&](uint32_t bar, int parity) {  // the lanes stay together, also when a wait gives up
-        ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, SITE_ATTN_MMA));
+      auto wait = [&](uint32_t bar, int parity) {
+        if (!mbar_try_wait(bar, parity)) ok = mbar_wait(bar, parity, abort_flag, status, SITE_ATTN_MMA) && ok;
         tc_fence_after();
       };
       auto wait_tile = [&]() {
-        const int slot = taken % STAGES;
-        wait(full + 8 * slot, (taken / STAGES) & 1);
-        ++taken;
-        return slot;
+        const int at = slot;
+        wait(full + 8 * at, phase);
+        if (++slot == STAGES) {
+          slot = 0;
+          phase ^= 1;
+        }
+        return at;
       };
-      auto scores = [&](int t, int slot) {  // S_t = Q_t K^T
-        const uint64_t a = q_desc + static_cast<uint64_t>(t * S::TILE / 16);
-        const uint64_t b = smem_desc_sw128(smem_u32(ring + slot * S::TILE), 16, 1024);
+      auto scores = [&](int t, int at) {  // S_t = Q_t K^T
+        const uint64_t a = q_desc + static_cast<uint64_t>(t * S::TILE / 16), b = k_desc + static_cast<uint64_t>(at * (S::TILE / 16));
 #pragma unroll
         for (int k = 0; k < DH / 16; ++k) {
           const uint64_t step = static_cast<uint64_t>((k / 4) * (BLK * 128 / 16) + (k % 4) * 2);
           tc_mma_f16(tmem + t * BLK, a + step, b + step, idesc_s, k > 0);
         }
-        tc_commit(s_full + 8 * t);
+        tc_commit(s_full + 8 * t);  // with it all products before are done, O_t's too
       };
-      auto products = [&](int t, int slot, bool accumulate) {  // O_t += P_t V
-        const uint64_t b = smem_desc_sw128(smem_u32(ring + slot * S::TILE), BLK * 128, 1024);
+      auto products = [&](int t, int at, bool accumulate) {  // O_t += P_t V
+        const uint64_t b = v_desc + static_cast<uint64_t>(at * (S::TILE / 16));
 #pragma unroll
         for (int k = 0; k < BLK / 16; ++k)
           tc_mma_f16_ta(tmem + 2 * BLK + t * BLK, tmem + t * BLK + 8 * k, b + static_cast<uint64_t>(k * 128), idesc_o,
                         accumulate || k > 0);
-        tc_commit(o_full + 8 * t);
       };
-      int k_slot = wait_tile();
-      for (int t = 0; ok && t < 2; ++t) {
+      int k_at = wait_tile();
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
         wait(q_bar + 8 * t, 0);
-        if (ok && blocks[t] > 0 && lane == 0) scores(t, k_slot);
+        if (ok && blocks[t] > 0) scores(t, k_at);
       }
-      if (ok && lane == 0) tc_commit(empty + 8 * k_slot);
+      tc_commit(empty + 8 * k_at);
       for (int j = 0; ok && j < most; ++j) {
-        const int v_slot = wait_tile();
-        if (!ok) break;
-        const int held = it.keys - j * BLK;  // of the request's keys in this block
-        if (held < BLK) {
-          for (int i = lane; i < (BLK - held) * S::HALVES * 8; i += 32) {
-            const int h = i / ((BLK - held) * 8), rest = i - h * (BLK - held) * 8;
-            *reinterpret_cast<uint4*>(ring + v_slot * S::TILE + h * BLK * 128 + held * 128 + rest * 16) =
-                make_uint4(0u, 0u, 0u, 0u);
-          }
-          fence_proxy_async_smem();
-          __syncwarp();
+        const int v_at = wait_tile();
+        if (j + 1 < most) {
+          k_at = wait_tile();
+        } else if (it.keys - j * BLK < BLK) {
+          mbar_arrive(dirty);
+          wait(clean, 0);
         }
-        bool k_ready = false;
-        for (int t = 0; ok && t < 2; ++t) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
           if (j >= blocks[t]) continue;
           wait(p_full + 8 * t, j & 1);
           if (!ok) break;
-          if (lane == 0) products(t, v_slot, j > 0);
+          products(t, v_at, j > 0);
           if (j + 1 < blocks[t]) {
-            if (!k_ready) {
-              k_slot = wait_tile();
-              if (!ok) break;
-              k_ready = true;
-            }
-            if (lane == 0) scores(t, k_slot);
+            scores(t, k_at);
+          } else {
+            tc_commit(o_full + 8 * t);
           }
         }
-        if (ok && lane == 0) {
-          tc_commit(empty + 8 * v_slot);
-          if (k_ready) tc_commit(empty + 8 * k_slot);
-        }
-        __syncwarp();
+        tc_commit(empty + 8 * v_at);
+        if (j + 1 < most) tc_commit(empty + 8 * k_at);
       }
     }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    if (has_item) {
     const int t = warp >> 2;
     const int row = (warp & 3) * 32 + lane;  // of the tile
     const int i = t * BLK + row;             // of the item
@@ -309,21 +316,11 @@ __global__ void __launch_bounds__(THREADS, 1)
           if (x >= left) s[x] = -INFINITY;
       }
       __syncwarp();
-      float top[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-      for (int x = 4; x < BLK; x += 8) {
-#pragma unroll
-        for (int y = 0; y < 4; ++y)
-          top[y] = x + 4 + y < BLK ? fmaxf(fmaxf(top[y], s[x + y]), s[x + 4 + y]) : fmaxf(top[y], s[x + y]);
-      }
-      const float m_new = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
+      const float m_new = row_max(s, m);
       if (j == 0) {
         m = m_new;
       } else if (__any_sync(0xffffffffu, (m_new - m) * c > RAISE_LOG2)) {
-        ok = mbar_wait(o_full + 8 * t, (j - 1) & 1, abort_flag, status, SITE_ATTN_SOFTMAX);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        tc_fence_after();
+        // S of this block came with the end of all products before it: O rests
         const float fix = m_new > m ? ex2_ftz((m - m_new) * c) : 1.0f;
         l *= fix;
         m = m_new;
@@ -338,26 +335,10 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
       }
       const float cm = m == -INFINITY ? 0.0f : m * c;
-      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int x = 0; x < BLK; x += 64) {
-        uint32_t w[32];
-#pragma unroll
-        for (int y = 0; y < 64; y += 2) {
-          const float a = ex2_ftz(fmaf(s[x + y], c, -cm)), b = ex2_ftz(fmaf(s[x + y + 1], c, -cm));
-          sum[(y / 2) & 3] += a + b;
-          w[y / 2] = pack_pair<T>(a, b);
-        }
-        tmem_st_32(s_addr + x / 2, w);
-      }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(p_full + 8 * t);
+      l += row_weights<T>(s, c, cm, s_addr, p_full + 8 * t, lane);
     }
     if (ok && blocks[t] > 0) {
-      ok = mbar_wait(o_full + 8 * t, (blocks[t] - 1) & 1, abort_flag, status, SITE_ATTN_SOFTMAX);
+      ok = mbar_wait(o_full + 8 * t, 0, abort_flag, status, SITE_ATTN_SOFTMAX);
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
     }
@@ -411,6 +392,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         redo_row<T, DH>(p, __shfl_sync(0xffffffffu, q_row, src), head, lane);
       }
     }
+    }
   }
   tc_fence_before();
   __syncthreads();
@@ -432,10 +414,16 @@ int launch_typed(const AttnArgs& a, const DeviceInfo& dev, cudaStream_t stream) 
   if (rc != KF_OK) return rc;
   static std::once_flag once;
   static cudaError_t attr = cudaSuccess;
+  static int registers = 0;
   std::call_once(once, [] {
     attr = cudaFuncSetAttribute(prefill_kernel<T, DH>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<DH>::SMEM);
+    cudaFuncAttributes f{};
+    if (attr == cudaSuccess) attr = cudaFuncGetAttributes(&f, prefill_kernel<T, DH>);
+    registers = f.numRegs;
   });
   if (attr != cudaSuccess) return cuda_error(attr, "prefill attributes");
+  if (registers < LAUNCH_REGISTERS)  // the warpgroups' shares must not exceed what the block is launched with
+    return set_error(KF_ERR_UNSUPPORTED, "prompt attention: built with too few registers to split");
   const int64_t blocks = (a.rows / PAIR + a.seqs + 1) * a.heads;
   const int vector_out = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.so_t % 8 == 0 && a.so_h % 8 == 0;
   prefill_kernel<T, DH><<<static_cast<unsigned>(blocks), THREADS, Shape<DH>::SMEM, stream>>>(q, k, v, a, vector_out,

@@ -237,13 +237,16 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       const int buf = done_items & 1;
       if (first) wait(o_free + 8 * buf, ((done_items >> 1) & 1) ^ 1);
-      wait(p_full + 8 * (unit & 1), (unit >> 1) & 1);
-      if (lane == 0) {
-        const uint64_t b = smem_desc_sw128(smem_u32(ring + slot * S::TILE), KEYS * 128, 1024);
+      const uint64_t b = smem_desc_sw128(smem_u32(ring + slot * S::TILE), KEYS * 128, 1024);
+      auto products = [&](int k0, int k1) {
 #pragma unroll
-        for (int k = 0; k < KEYS / 16; ++k)
+        for (int k = k0; k < k1; ++k)
           tc_mma_f16_ta(tmem + 2 * KEYS + buf * 128, tmem + (unit & 1) * KEYS + 8 * k, b + static_cast<uint64_t>(k * 128),
                         idesc_o, !first || k > 0);
+      };
+      wait(p_full + 8 * (unit & 1), (unit >> 1) & 1);
+      if (lane == 0) {
+        products(0, KEYS / 16);
         tc_commit(o_done + 8 * (unit & 1));
         tc_commit(empty + 8 * slot);
       }
@@ -285,24 +288,22 @@ __global__ void __launch_bounds__(THREADS, 1)
       for (int x = 0; x < KEYS; x += 32) tmem_ld_32(s_addr + x, reinterpret_cast<uint32_t*>(s + x));
       tmem_ld_wait();
       const int key0 = at.blk * KEYS;
+      uint32_t seen[4], both = 0xffffffffu;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        uint32_t seen = present[4 * (unit % INFO) + w];
-        if (key0 + 32 * w + 32 > at.context) seen &= nodes_seen(p, at, node, key0 + 32 * w - at.context);
-        if (seen != 0xffffffffu) {
+      for (int w = 0; w < 4; ++w) both &= seen[w] = present[4 * (unit % INFO) + w];
+      // a block of cached tokens, all there, needs no look at its keys
+      const bool all_seen = key0 + KEYS <= at.context && both == 0xffffffffu;
+      if (!all_seen) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          seen[w] &= nodes_seen(p, at, node, key0 + 32 * w - at.context);
 #pragma unroll
           for (int x = 0; x < 32; ++x)
-            if (!((seen >> x) & 1u)) s[32 * w + x] = -INFINITY;
+            if (!((seen[w] >> x) & 1u)) s[32 * w + x] = -INFINITY;
         }
       }
       __syncwarp();
-      float top[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-      for (int x = 4; x < KEYS; x += 4) {
-#pragma unroll
-        for (int y = 0; y < 4; ++y) top[y] = fmaxf(top[y], s[x + y]);
-      }
-      const float m_new = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
+      const float m_new = row_max(s, m);
       if (first) {
         m = m_new;
       } else if (__any_sync(0xffffffffu, (m_new - m) * c > RAISE_LOG2)) {
@@ -323,23 +324,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
       }
       const float cm = m == -INFINITY ? 0.0f : m * c;
-      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int x = 0; x < KEYS; x += 64) {
-        uint32_t w[32];
-#pragma unroll
-        for (int y = 0; y < 64; y += 2) {
-          const float a = ex2_ftz(fmaf(s[x + y], c, -cm)), b = ex2_ftz(fmaf(s[x + y + 1], c, -cm));
-          sum[(y / 2) & 3] += a + b;
-          w[y / 2] = pack_pair<T>(a, b);
-        }
-        tmem_st_32(s_addr + x / 2, w);
-      }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(p_full + 8 * (unit & 1));
+      l += row_weights<T>(s, c, cm, s_addr, p_full + 8 * (unit & 1), lane);
       first = walk.item_ends(at);
       if (!first) {
         walk.advance(p, at);
