@@ -11,8 +11,9 @@
 //   warps 0-3, 4-7   softmax of tile 0 and 1, a thread per row: S from TMEM into
 //                    registers, P (16 bit) back over the same columns.
 //   warp 8           TMA: Q once, then K and V blocks through a ring.
-//   warp 9           one thread issues the MMAs. While one tile's warps compute
-//                    their weights the tensor cores work for the other tile.
+//   warp 9           issues the MMAs. While one tile's warps compute their
+//                    weights the tensor cores work for the other tile; the second
+//                    product starts when half of a block's weights are there.
 //   warp 10          zeroes what the last V block holds of the next request.
 //
 // m is raised, and O (in TMEM) rescaled, only when a row's maximum grew by more
@@ -39,7 +40,7 @@ constexpr int PAIR = 2 * BLK;  // rows of a CTA
 constexpr int SOFTMAX_WARPS = 8;
 constexpr int TMA_WARP = 8, MMA_WARP = 9, CLEAN_WARP = 10;
 // Three warpgroups; the last (loads, products) hands registers to the softmax:
-// 3 x 168 a thread become 2 x 216 and 72.
+// 3 x 168 a thread become 2 x 208 and 88.
 constexpr int THREADS = 3 * 128;
 constexpr int LAUNCH_REGISTERS = 168;
 constexpr uint32_t TMEM_COLS = 512;  // S0 | S1 | O0 | O1, 128 each
@@ -122,7 +123,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint8_t* q_tiles = smem;
   uint8_t* ring = smem + 2 * S::TILE;
   uint64_t* bars = reinterpret_cast<uint64_t*>(ring + STAGES * S::TILE);
-  // bars: q[2] | full[STAGES] | empty[STAGES] | s_full[2] | p_full[2] | o_full[2] | dirty | clean
+  // bars: q[2] | full[STAGES] | empty[STAGES] | s_full[2] | p_half[2] | p_full[2] | o_full[2] | dirty | clean
   __shared__ Item item;
   __shared__ int has_item;
   __shared__ uint32_t tmem_slot;
@@ -131,7 +132,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t q_bar = smem_u32(bars), full = q_bar + 16, empty = full + 8 * STAGES, s_full = empty + 8 * STAGES,
-                 p_full = s_full + 16, o_full = p_full + 16, dirty = o_full + 16, clean = dirty + 8;
+                 p_half = s_full + 16, p_full = p_half + 16, o_full = p_full + 16, dirty = o_full + 16, clean = dirty + 8;
   const int heads = static_cast<int>(p.heads);
   const int head = static_cast<int>(blockIdx.x % heads);
 
@@ -141,6 +142,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   } else if (warp == TMA_WARP && lane == 0) {
     for (int i = 0; i < 2 + 2 * STAGES + 2; ++i) mbar_init(q_bar + 8 * i, 1);
     for (int t = 0; t < 2; ++t) {
+      mbar_init(p_half + 8 * t, SOFTMAX_WARPS / 2);
       mbar_init(p_full + 8 * t, SOFTMAX_WARPS / 2);
       mbar_init(o_full + 8 * t, 1);
     }
@@ -170,7 +172,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   const int most = max(blocks[0], blocks[1]);
 
   if (warp >= SOFTMAX_WARPS) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (has_item && warp == TMA_WARP) {
     if (lane == 0 && most > 0) {
       const int kv_head = head / static_cast<int>(p.heads / p.kv_heads);
@@ -218,17 +220,26 @@ __global__ void __launch_bounds__(THREADS, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(clean);
       }
-    } else if (has_item && warp == MMA_WARP && lane == 0 && most > 0) {
-      // One thread, and as few instructions as can be between one product and the
-      // next: the tensor cores run dry behind every one of them.
+    } else if (has_item && warp == MMA_WARP && most > 0) {
+      // The warp runs together on uniform values and one elected lane issues: a few
+      // instructions a product, where a branch for one lane takes about 20 and the
+      // tensor cores run dry behind them. (A warp for each tile measured slower: two
+      // tiles' products in turn finish later than one tile's, then the other's.)
+      const uint32_t lead = elect_lane();
+      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+      const uint32_t q_at = __shfl_sync(0xffffffffu, smem_u32(q_tiles), 0), ring_at = __shfl_sync(0xffffffffu, smem_u32(ring), 0);
+      const int count[2] = {__shfl_sync(0xffffffffu, blocks[0], 0), __shfl_sync(0xffffffffu, blocks[1], 0)};
+      const int all = max(count[0], count[1]);
+      const bool partial = __shfl_sync(0xffffffffu, it.keys - (most - 1) * BLK, 0) < BLK;
       constexpr uint32_t fmt = DType<T>::code == KF_BF16 ? 1u : 0u;
       constexpr uint32_t idesc_s = instr_desc_f16(fmt, 0, 0, BLK, BLK), idesc_o = instr_desc_f16(fmt, 0, 1, BLK, DH);
-      const uint64_t q_desc = smem_desc_sw128(smem_u32(q_tiles), 16, 1024);
-      const uint64_t k_desc = smem_desc_sw128(smem_u32(ring), 16, 1024), v_desc = smem_desc_sw128(smem_u32(ring), BLK * 128, 1024);
+      const uint64_t q_desc = smem_desc_sw128(q_at, 16, 1024);
+      const uint64_t k_desc = smem_desc_sw128(ring_at, 16, 1024), v_desc = smem_desc_sw128(ring_at, BLK * 128, 1024);
       int slot = 0, phase = 0;  // of the ring's next tile
       bool ok = true;
       auto wait = [&](uint32_t bar, int parity) {
-        if (!mbar_try_wait(bar, parity)) ok = mbar_wait(bar, parity, abort_flag, status, SITE_ATTN_MMA) && ok;
+        if (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity)))
+          ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, SITE_ATTN_MMA)) && ok;
         tc_fence_after();
       };
       auto wait_tile = [&]() {
@@ -245,50 +256,51 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
         for (int k = 0; k < DH / 16; ++k) {
           const uint64_t step = static_cast<uint64_t>((k / 4) * (BLK * 128 / 16) + (k % 4) * 2);
-          tc_mma_f16(tmem + t * BLK, a + step, b + step, idesc_s, k > 0);
+          tc_mma_f16_by(lead, tm + t * BLK, a + step, b + step, idesc_s, k > 0);
         }
-        tc_commit(s_full + 8 * t);  // with it all products before are done, O_t's too
+        tc_commit_by(lead, s_full + 8 * t);  // with it all products before are done, O_t's too
       };
-      auto products = [&](int t, int at, bool accumulate) {  // O_t += P_t V
+      auto products = [&](int t, int at, bool accumulate, int k0, int k1) {  // O_t += P_t V
         const uint64_t b = v_desc + static_cast<uint64_t>(at * (S::TILE / 16));
 #pragma unroll
-        for (int k = 0; k < BLK / 16; ++k)
-          tc_mma_f16_ta(tmem + 2 * BLK + t * BLK, tmem + t * BLK + 8 * k, b + static_cast<uint64_t>(k * 128), idesc_o,
-                        accumulate || k > 0);
+        for (int k = k0; k < k1; ++k)
+          tc_mma_f16_ta_by(lead, tm + 2 * BLK + t * BLK, tm + t * BLK + 8 * k, b + static_cast<uint64_t>(k * 128), idesc_o,
+                           accumulate || k > 0);
       };
       int k_at = wait_tile();
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         wait(q_bar + 8 * t, 0);
-        if (ok && blocks[t] > 0) scores(t, k_at);
+        if (ok && count[t] > 0) scores(t, k_at);
       }
-      tc_commit(empty + 8 * k_at);
-      for (int j = 0; ok && j < most; ++j) {
+      tc_commit_by(lead, empty + 8 * k_at);
+      for (int j = 0; ok && j < all; ++j) {
         const int v_at = wait_tile();
-        if (j + 1 < most) {
+        if (j + 1 < all) {
           k_at = wait_tile();
-        } else if (it.keys - j * BLK < BLK) {
-          mbar_arrive(dirty);
+        } else if (partial) {
+          if (lead) mbar_arrive(dirty);
           wait(clean, 0);
         }
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          if (j >= blocks[t]) continue;
+          if (j >= count[t]) continue;
+          wait(p_half + 8 * t, j & 1);
+          if (ok) products(t, v_at, j > 0, 0, 4);
           wait(p_full + 8 * t, j & 1);
-          if (!ok) break;
-          products(t, v_at, j > 0);
-          if (j + 1 < blocks[t]) {
-            scores(t, k_at);
+          if (ok) products(t, v_at, true, 4, 8);
+          if (j + 1 < count[t]) {
+            if (ok) scores(t, k_at);
           } else {
-            tc_commit(o_full + 8 * t);
+            tc_commit_by(lead, o_full + 8 * t);
           }
         }
-        tc_commit(empty + 8 * v_at);
-        if (j + 1 < most) tc_commit(empty + 8 * k_at);
+        tc_commit_by(lead, empty + 8 * v_at);
+        if (j + 1 < all) tc_commit_by(lead, empty + 8 * k_at);
       }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     if (has_item) {
     const int t = warp >> 2;
     const int row = (warp & 3) * 32 + lane;  // of the tile
@@ -335,7 +347,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
       }
       const float cm = m == -INFINITY ? 0.0f : m * c;
-      l += row_weights<T>(s, c, cm, s_addr, p_full + 8 * t, lane);
+      l += row_weights<T, true>(s, c, cm, s_addr, p_half + 8 * t, p_full + 8 * t, lane);
     }
     if (ok && blocks[t] > 0) {
       ok = mbar_wait(o_full + 8 * t, 0, abort_flag, status, SITE_ATTN_SOFTMAX);
@@ -345,6 +357,9 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (ok && it.rows > t * BLK) {
       const int q_row = it.row0 + i;
       T* out = static_cast<T*>(p.out) + static_cast<long long>(q_row) * p.so_t + head * p.so_h;
+      // The largest weight of a row is one or more, and a key it does not see
+      // weighs at most 2^-126: a sum between is that of no key.
+      if (l < 5.4e-20f) l = 0.0f;  // 2^-64
       const float inv = l > 0.0f ? 1.0f / l : 0.0f;
       float bad = 0.0f;  // NaN if anything in the row is not finite
 #pragma unroll 1

@@ -324,7 +324,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
       }
       const float cm = m == -INFINITY ? 0.0f : m * c;
-      l += row_weights<T>(s, c, cm, s_addr, p_full + 8 * (unit & 1), lane);
+      l += row_weights<T, false>(s, c, cm, s_addr, 0, p_full + 8 * (unit & 1), lane);
       first = walk.item_ends(at);
       if (!first) {
         walk.advance(p, at);
