@@ -280,60 +280,99 @@ __device__ __forceinline__ void redo_rows(const AttnArgs& p, bool bad, int t, in
   }
 }
 
-// Joins the partial results of CTAs [owner, last] in the order of the keys, by
-// THREADS threads that each take 8 columns of a row: the owner holds the item's
-// first blocks in its second slot, the others theirs in their first.
-template <typename T, int M, int DP, int THREADS>
+// A running (maximum, sum, 8 columns), and another one added to it.
+struct Sums8 {
+  float m = -INFINITY, l = 0.0f, o[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+
+  __device__ __forceinline__ void raise(float top) {
+    const float old = m == -INFINITY ? 0.0f : ex2_ftz(m - top);
+    l *= old;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] *= old;
+    m = top;
+  }
+  __device__ __forceinline__ void add(float pm, float pl, const float (&e)[8]) {  // pm <= m
+    const float fix = pm == -INFINITY ? 0.0f : ex2_ftz(pm - m);
+    if (fix == 0.0f) return;
+    l = fmaf(pl, fix, l);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = fmaf(e[i], fix, o[i]);
+  }
+};
+
+// Joins the partial results of CTAs [owner, last], by THREADS threads that each
+// take 8 columns of a row: the owner holds the item's first blocks in its second
+// slot, the others theirs in their first. With few rows several threads share a
+// row's CTAs and add up through `scratch` (10 floats a thread, or null). The order
+// of the sums goes by the numbers alone.
+template <typename T, int M, int DP, int THREADS, typename Barrier>
 __device__ __forceinline__ void join_partials(const AttnArgs& p, const Cursor& c, const TileRows& tile, int owner, int last,
-                                              int tid, int vector_out) {
+                                              int tid, int vector_out, float* scratch, Barrier barrier) {
   constexpr int LANES = DP / 8, PASS = THREADS / LANES;
   const int col = (tid % LANES) * 8;
+  int share = 1;  // threads to a row's CTAs
+  if (scratch != nullptr)
+    while (2 * share * tile.rows() <= PASS && share < 8) share *= 2;
+  const int pass = PASS / share, part = tid / LANES / pass;
 #pragma unroll 1
-  for (int row0 = 0; row0 < tile.rows(); row0 += PASS) {
-    const int row = row0 + tid / LANES;
+  for (int row0 = 0; row0 < tile.rows(); row0 += pass) {
+    const int row = row0 + tid / LANES % pass;
     int t, head;
     const bool mine = tile.find(row, &t, &head);
     t += c.row0;
     bool bad = false;
+    Sums8 sums;
     if (mine) {
-      float m = -INFINITY, l = 0.0f, o[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) o[i] = 0.0f;
 #pragma unroll 1
-      for (int b0 = owner; b0 <= last; b0 += 4) {
+      for (int b0 = owner + part; b0 <= last; b0 += 4 * share) {
         float pm[4], pl[4];
         float4 w[4][2];
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
+          const int b = b0 + x * share;
           pm[x] = -INFINITY;
           pl[x] = 0.0f;
           w[x][0] = w[x][1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          if (b0 + x <= last) {
-            const Partial<M, DP> part(p, b0 + x, b0 + x == owner);
-            pm[x] = __ldcg(part.top(row));
-            pl[x] = __ldcg(part.sum(row));
-            w[x][0] = __ldcg(reinterpret_cast<const float4*>(part.row(row) + col));
-            w[x][1] = __ldcg(reinterpret_cast<const float4*>(part.row(row) + col + 4));
+          if (b <= last) {
+            const Partial<M, DP> from(p, b, b == owner);
+            pm[x] = __ldcg(from.top(row));
+            pl[x] = __ldcg(from.sum(row));
+            w[x][0] = __ldcg(reinterpret_cast<const float4*>(from.row(row) + col));
+            w[x][1] = __ldcg(reinterpret_cast<const float4*>(from.row(row) + col + 4));
           }
         }
-        const float top = fmaxf(fmaxf(m, fmaxf(pm[0], pm[1])), fmaxf(pm[2], pm[3]));
-        const float old = m == -INFINITY ? 0.0f : ex2_ftz(m - top);
-        l *= old;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] *= old;
-        m = top;
+        sums.raise(fmaxf(fmaxf(sums.m, fmaxf(pm[0], pm[1])), fmaxf(pm[2], pm[3])));
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          const float fix = pm[x] == -INFINITY ? 0.0f : ex2_ftz(pm[x] - top);
-          if (fix == 0.0f) continue;
-          l = fmaf(pl[x], fix, l);
           const float e[8] = {w[x][0].x, w[x][0].y, w[x][0].z, w[x][0].w, w[x][1].x, w[x][1].y, w[x][1].z, w[x][1].w};
-#pragma unroll
-          for (int i = 0; i < 8; ++i) o[i] = fmaf(e[i], fix, o[i]);
+          sums.add(pm[x], pl[x], e);
         }
       }
-      if (col < p.dim) bad = store_8<T>(p, t, head, col, o, l, vector_out);
-      if (col == 0) store_lse(p, t, head, m, l);
+    }
+    if (share > 1) {
+      float* mine_at = scratch + 10 * (tid - LANES * pass);
+      if (part > 0) {
+        mine_at[0] = sums.m;
+        mine_at[1] = sums.l;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mine_at[2 + i] = sums.o[i];
+      }
+      barrier();
+      if (part == 0) {
+        for (int x = 1; x < share; ++x) {
+          const float* other = scratch + 10 * (tid + (x - 1) * LANES * pass);
+          float e[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) e[i] = other[2 + i];
+          sums.raise(fmaxf(sums.m, other[0]));
+          sums.add(other[0], other[1], e);
+        }
+      }
+      barrier();
+    }
+    if (mine && part == 0) {
+      if (col < p.dim) bad = store_8<T>(p, t, head, col, sums.o, sums.l, vector_out);
+      if (col == 0) store_lse(p, t, head, sums.m, sums.l);
     }
     redo_rows<T, DP / 32>(p, bad, t, head, threadIdx.x & 31);
   }

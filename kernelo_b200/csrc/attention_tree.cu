@@ -43,7 +43,8 @@ constexpr int M = 16;         // rows of a tile
 constexpr int KEYS = 64;      // of a block
 constexpr int WARPS = 4;      // of products
 constexpr int KW = KEYS / WARPS;
-constexpr int THREADS = 32 * (WARPS + 1);
+constexpr int LOAD_WARP = WARPS, FINISH_WARP = WARPS + 1;
+constexpr int THREADS = 32 * (WARPS + 2);
 constexpr int MIN_RUN = 4;    // positions of a run: fewer blocks cost more to join than to read
 constexpr int ITEM_COST = 2;  // blocks that an item's queries and results are worth
 constexpr uint64_t DRAIN_NS = 100000000ull;
@@ -57,7 +58,7 @@ struct Shape {
   static constexpr int PITCH = DP + 8;              // floats of a row of the joined result
   // ring | queries | joined result | maxima, sums | barriers | present
   static constexpr int SMEM =
-      1024 + STAGES * 2 * TILE + Q_TILE + M * PITCH * 4 + 2 * M * WARPS * 4 + 8 * (2 * STAGES + 2) + 8 * STAGES;
+      1024 + STAGES * 2 * TILE + Q_TILE + M * PITCH * 4 + 2 * M * WARPS * 4 + 8 * (2 * STAGES + 3) + 8 * STAGES;
 };
 
 __device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, bool present) {
@@ -76,6 +77,22 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t add
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(addr)
                : "memory");
+}
+
+// Where ldmatrix finds 16 x 16 elements of a tile in the swizzle of chunk_at: this
+// lane's row and half of a pair of chunks give `first` (of a tile on a 1 KB
+// boundary), and pair k of the row is one XOR and a constant away.
+template <int DP, int ROWS>
+__device__ __forceinline__ uint32_t first_pair(int row, int half) {
+  if constexpr (DP >= 64) {
+    return static_cast<uint32_t>(row * 128 + ((half ^ (row & 7)) << 4));
+  } else {
+    return static_cast<uint32_t>(row * 64 + ((half ^ ((row >> 1) & 3)) << 4));
+  }
+}
+template <int ROWS>
+__device__ __forceinline__ uint32_t pair_at(uint32_t first, int k) {
+  return (first ^ static_cast<uint32_t>((k & 3) << 5)) + static_cast<uint32_t>((k >> 2) * (ROWS * 128));
 }
 
 // Byte offset of 16-byte chunk `chunk` of row `row` in a tile, as TMA's swizzles
@@ -103,15 +120,17 @@ __global__ void __launch_bounds__(THREADS, 2)
   float* part_m = joined + M * S::PITCH;
   float* part_l = part_m + M * WARPS;
   uint64_t* bars = reinterpret_cast<uint64_t*>(part_l + M * WARPS);
-  volatile uint32_t* present = reinterpret_cast<volatile uint32_t*>(bars + 2 * STAGES + 2);  // a bit per key of each stage
+  volatile uint32_t* present = reinterpret_cast<volatile uint32_t*>(bars + 2 * STAGES + 3);  // a bit per key of each stage
   static_assert(S::TILE % 1024 == 0 && S::Q_TILE % 1024 == 0 && S::PITCH % 4 == 0 && Partial<M, DP>::FLOATS % 4 == 0,
                 "vectors of 16 bytes");
   __shared__ int last_one, abort_word;
+  __shared__ Cursor first_item;
+  __shared__ int first_is_last;
   volatile int* abort_flag = &abort_word;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t ring = smem_u32(smem), full = smem_u32(bars), empty = full + 8 * STAGES, q_full = empty + 8 * STAGES,
-                 q_empty = q_full + 8;
+                 q_empty = q_full + 8, finished = q_empty + 8;
 
   if (tid == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -120,6 +139,7 @@ __global__ void __launch_bounds__(THREADS, 2)
     }
     mbar_init(q_full, 32);
     mbar_init(q_empty, WARPS);
+    mbar_init(finished, 1);
     abort_word = 0;
     mbar_init_fence();
   }
@@ -131,8 +151,25 @@ __global__ void __launch_bounds__(THREADS, 2)
   Cursor at;
   const Run run = walk.template find<THREADS>(p, MIN_RUN, at);
   if (run.count == 0) return;
+  // The run begins inside an item and goes on behind it: the item's arrival (a
+  // fence and an atomic, a few microseconds when the memory is busy) is left to a
+  // warp of its own, and its joining, if it falls to this CTA, to the end.
+  const bool defer = at.blk > 0 && at.left > at.blocks + ITEM_COST - at.blk;
+  const int first_owner = static_cast<int>((run.first - at.blk) / run.per);
+  const int first_last = static_cast<int>((run.first - at.blk + at.blocks - 1) / run.per);
 
-  if (warp == WARPS) {
+  if (warp == FINISH_WARP) {
+    if (!defer) return;
+    if (lane == 0) first_item = at;
+    asm volatile("bar.sync 2, %0;" ::"n"(32 * (WARPS + 1)) : "memory");  // the partial result is written
+    __threadfence();
+    if (lane == 0) {
+      first_is_last = atomicAdd(static_cast<int*>(p.workspace) + first_owner, 1) == first_last - first_owner;
+      mbar_arrive(finished);
+    }
+    return;
+  }
+  if (warp == LOAD_WARP) {
     // ------------------------------------------------------------ loads
     constexpr int OPS = 2 * S::HALVES;  // boxes of one run of keys
     const int chunks = static_cast<int>(p.dim) / 8;
@@ -239,6 +276,8 @@ __global__ void __launch_bounds__(THREADS, 2)
   float m[2], l[2];
   int stage = 0, phase = 0, items = 0;
   bool fresh = true;
+  const uint32_t k_first = first_pair<DP, KEYS>(warp * KW + ((lane >> 4) << 3) + (lane & 7), (lane >> 3) & 1);
+  const uint32_t v_first = S::TILE + first_pair<DP, KEYS>(warp * KW + (((lane >> 3) & 1) << 3) + (lane & 7), lane >> 4);
   while (at.left > 0) {
     if (fresh) {
       fresh = false;
@@ -246,7 +285,7 @@ __global__ void __launch_bounds__(THREADS, 2)
       __syncwarp();
 #pragma unroll
       for (int k = 0; k < DP / 16; ++k)
-        ldmatrix_x4(qf[k], smem_u32(q_tile) + chunk_at<DP, M>((((lane >> 3) & 1) << 3) + (lane & 7), 2 * k + (lane >> 4)));
+        ldmatrix_x4(qf[k], pair_at<M>(smem_u32(q_tile) + first_pair<DP, M>((((lane >> 3) & 1) << 3) + (lane & 7), lane >> 4), k));
       __syncwarp();
       if (lane == 0) mbar_arrive(q_empty);
       ++items;
@@ -260,16 +299,23 @@ __global__ void __launch_bounds__(THREADS, 2)
     }
     mbar_wait(full + 8 * stage, phase, abort_flag, status, SITE_ATTN_SOFTMAX);
     __syncwarp();
-    const uint32_t k_tile = ring + stage * 2 * S::TILE, v_tile = k_tile + S::TILE;
-    float s[KW / 8][4];
+    const uint32_t tile_at = ring + stage * 2 * S::TILE;
+    // two sums for each half of the head: their products wait less for one another
+    float s[KW / 8][4], s2[KW / 8][4];
 #pragma unroll
-    for (int n = 0; n < KW / 8; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+    for (int n = 0; n < KW / 8; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = s2[n][0] = s2[n][1] = s2[n][2] = s2[n][3] = 0.0f;
 #pragma unroll
     for (int k = 0; k < DP / 16; ++k) {
       uint32_t b[4];
-      ldmatrix_x4(b, k_tile + chunk_at<DP, KEYS>(warp * KW + ((lane >> 4) << 3) + (lane & 7), 2 * k + ((lane >> 3) & 1)));
-      mma16816<T>(s[0], qf[k][0], qf[k][1], qf[k][2], qf[k][3], b[0], b[1]);
-      mma16816<T>(s[1], qf[k][0], qf[k][1], qf[k][2], qf[k][3], b[2], b[3]);
+      ldmatrix_x4(b, pair_at<KEYS>(tile_at + k_first, k));
+      auto& to = k % 2 ? s2 : s;
+      mma16816<T>(to[0], qf[k][0], qf[k][1], qf[k][2], qf[k][3], b[0], b[1]);
+      mma16816<T>(to[1], qf[k][0], qf[k][1], qf[k][2], qf[k][3], b[2], b[3]);
+    }
+#pragma unroll
+    for (int n = 0; n < KW / 8; ++n) {
+#pragma unroll
+      for (int x = 0; x < 4; ++x) s[n][x] += s2[n][x];
     }
     // base-2 scores, -inf where a row sees nothing
     const int key0 = at.blk * KEYS + warp * KW;
@@ -334,7 +380,7 @@ __global__ void __launch_bounds__(THREADS, 2)
 #pragma unroll
       for (int n = 0; n < DP / 16; ++n) {
         uint32_t b[4];
-        ldmatrix_x4_trans(b, v_tile + chunk_at<DP, KEYS>(warp * KW + (((lane >> 3) & 1) << 3) + (lane & 7), 2 * n + (lane >> 4)));
+        ldmatrix_x4_trans(b, pair_at<KEYS>(tile_at + v_first, n));
         mma16816<T>(o[2 * n], a0, a1, a2, a3, b[0], b[1]);
         mma16816<T>(o[2 * n + 1], a0, a1, a2, a3, b[2], b[3]);
       }
@@ -429,7 +475,9 @@ __global__ void __launch_bounds__(THREADS, 2)
       }
       redo_rows<T, DP / 32>(p, bad, t, head, lane);
     }
-    if (!whole) {
+    if (!whole && defer && item < 0) {
+      asm volatile("bar.arrive 2, %0;" ::"n"(32 * (WARPS + 1)) : "memory");
+    } else if (!whole) {
       int* counters = static_cast<int*>(p.workspace);
       const int owner = static_cast<int>((run.first + item) / run.per);
       const int last = static_cast<int>((run.first + item + at.blocks - 1) / run.per);
@@ -439,12 +487,22 @@ __global__ void __launch_bounds__(THREADS, 2)
       join();
       if (last_one) {
         __threadfence();
-        join_partials<T, M, DP, 32 * WARPS>(p, at, tile, owner, last, tid, vector_out);
+        join_partials<T, M, DP, 32 * WARPS>(p, at, tile, owner, last, tid, vector_out, DP >= 64 ? joined : nullptr, join);
         if (tid == 0) counters[owner] = 0;
       }
     }
     join();  // `joined` and the maxima may be written again
     walk.advance(p, at);
+  }
+  if (defer) {
+    mbar_wait(finished, 0, abort_flag, status, SITE_ATTN_SOFTMAX);
+    if (first_is_last) {
+      __threadfence();
+      const Cursor c = first_item;
+      join_partials<T, M, DP, 32 * WARPS>(p, c, TileRows(p, walk, c), first_owner, first_last, tid, vector_out,
+                                          DP >= 64 ? joined : nullptr, join);
+      if (tid == 0) static_cast<int*>(p.workspace)[first_owner] = 0;
+    }
   }
 }
 

@@ -383,7 +383,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         join();
         if (last_one) {
           __threadfence();
-          join_partials<T, M, DP, 32 * SOFTMAX_WARPS>(p, at, TileRows(p, walk, at), owner, last, tid, vector_out);
+          join_partials<T, M, DP, 32 * SOFTMAX_WARPS>(p, at, TileRows(p, walk, at), owner, last, tid, vector_out, nullptr, join);
           if (tid == 0) counters[owner] = 0;
         }
         join();

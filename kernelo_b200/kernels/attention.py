@@ -79,6 +79,27 @@ def _outputs(q: torch.Tensor, out: torch.Tensor | None, return_lse: bool):
     return out, lse
 
 
+def _check_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor,
+                   cu_k: torch.Tensor | None) -> torch.Tensor:
+    _check_query(q)
+    if k.ndim != 3 or v.shape != k.shape:
+        raise ValueError(f"expected k and v as (keys, kv_heads, dim), got {tuple(k.shape)} and {tuple(v.shape)}")
+    _check_operand("k", k, q)
+    _check_operand("v", v, q)
+    _check_index("cu_q", cu_q, q)
+    if cu_q.ndim != 1 or cu_q.shape[0] < 1:
+        raise ValueError(f"cu_q must have shape (requests + 1,), got {tuple(cu_q.shape)}")
+    if cu_k is None:
+        if k.shape[0] != q.shape[0]:
+            raise ValueError(f"{k.shape[0]} keys for {q.shape[0]} rows: pass cu_k")
+        cu_k = cu_q
+    elif cu_k is not cu_q:
+        _check_index("cu_k", cu_k, q)
+        if cu_k.shape != cu_q.shape:
+            raise ValueError(f"cu_q and cu_k must have one shape, got {tuple(cu_q.shape)} and {tuple(cu_k.shape)}")
+    return cu_k
+
+
 def prefill_attention(
     q: torch.Tensor,
     k: torch.Tensor,
@@ -100,27 +121,56 @@ def prefill_attention(
     rows. ``scale`` defaults to ``dim ** -0.5``. Returns the output, and with
     ``return_lse`` also the fp32 natural log-sum-exp ``(rows, heads)``.
     """
-    _check_query(q)
-    if k.ndim != 3 or v.shape != k.shape:
-        raise ValueError(f"expected k and v as (keys, kv_heads, dim), got {tuple(k.shape)} and {tuple(v.shape)}")
-    _check_heads(q, k.shape[1], k.shape[2])
-    _check_operand("k", k, q)
-    _check_operand("v", v, q)
-    _check_index("cu_q", cu_q, q)
-    if cu_q.ndim != 1 or cu_q.shape[0] < 1:
-        raise ValueError(f"cu_q must have shape (requests + 1,), got {tuple(cu_q.shape)}")
-    if cu_k is None:
-        if k.shape[0] != q.shape[0]:
-            raise ValueError(f"{k.shape[0]} keys for {q.shape[0]} rows: pass cu_k")
+    dtype, device = q.dtype, q.get_device()
+    if cu_k is None and k.shape[:1] == q.shape[:1]:
         cu_k = cu_q
-    elif cu_k is not cu_q:
-        _check_index("cu_k", cu_k, q)
-        if cu_k.shape != cu_q.shape:
-            raise ValueError(f"cu_q and cu_k must have one shape, got {tuple(cu_q.shape)} and {tuple(cu_k.shape)}")
+    # one expression for what is right, and the reasons only where it is not: a
+    # call costs the host about as long as a short prompt's kernel the GPU
+    if not (q.is_cuda and q.ndim == 3 == k.ndim and v.shape == k.shape and cu_k is not None
+            and k.dtype is dtype and v.dtype is dtype and k.get_device() == device == v.get_device()
+            and q.stride(2) == 1 == k.stride(2) and v.stride(2) == 1
+            and cu_q.dtype is torch.int32 and cu_q.get_device() == device and cu_q.ndim == 1 and cu_q.is_contiguous()
+            and (cu_k is cu_q or (cu_k.dtype is torch.int32 and cu_k.get_device() == device
+                                  and cu_k.shape == cu_q.shape and cu_k.is_contiguous()))):
+        cu_k = _check_prefill(q, k, v, cu_q, cu_k)
+    _check_heads(q, k.shape[1], k.shape[2])
+    if cu_q.shape[0] < 1:
+        raise ValueError(f"cu_q must have shape (requests + 1,), got {tuple(cu_q.shape)}")
     out, lse = _outputs(q, out, return_lse)
     if q.numel():
         native.prefill_attention(q, k, v, out, lse, cu_q, cu_k, q.shape[2] ** -0.5 if scale is None else scale, causal)
     return (out, lse) if return_lse else out
+
+
+def _check_tree(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                context_lens: torch.Tensor, cu_q: torch.Tensor | None, tree_mask: torch.Tensor | None) -> None:
+    _check_query(q)
+    if k_cache.ndim != 4 or v_cache.shape != k_cache.shape:
+        raise ValueError("expected k_cache and v_cache as (pages, kv_heads, block, dim), got "
+                         f"{tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
+    _check_operand("k_cache", k_cache, q)
+    _check_operand("v_cache", v_cache, q)
+    if block_table.ndim != 2 or block_table.dtype != torch.int32:
+        raise ValueError(f"block_table must be int32 (requests, blocks), got {block_table.dtype} "
+                         f"{tuple(block_table.shape)}")
+    if block_table.get_device() != q.get_device():
+        raise ValueError(f"block_table must be on {q.device}, got {block_table.device}")
+    if block_table.stride(1) != 1 and block_table.shape[1] > 1:
+        raise ValueError("block_table must have contiguous rows")
+    seqs = block_table.shape[0]
+    _check_index("context_lens", context_lens, q)
+    if context_lens.ndim != 1 or context_lens.shape[0] != seqs:
+        raise ValueError(f"context_lens must have shape ({seqs},), got {tuple(context_lens.shape)}")
+    if cu_q is not None:
+        _check_index("cu_q", cu_q, q)
+        if cu_q.ndim != 1 or cu_q.shape[0] != seqs + 1:
+            raise ValueError(f"cu_q must have shape ({seqs + 1},), got {tuple(cu_q.shape)}")
+    elif q.shape[0] != seqs:
+        raise ValueError(f"{q.shape[0]} rows for {seqs} requests: pass cu_q")
+    if tree_mask is not None:
+        _check_index("tree_mask", tree_mask, q, torch.int64)
+        if tree_mask.ndim != 2 or tree_mask.shape[0] != q.shape[0] or tree_mask.shape[1] < 1:
+            raise ValueError(f"tree_mask must have shape ({q.shape[0]}, words), got {tuple(tree_mask.shape)}")
 
 
 def tree_attention(
@@ -147,36 +197,19 @@ def tree_attention(
     ``(rows, words)``): bit ``b`` says whether the row sees row ``b`` of its
     request, itself included; without it the rows are a chain.
     """
-    _check_query(q)
-    if k_cache.ndim != 4 or v_cache.shape != k_cache.shape:
-        raise ValueError("expected k_cache and v_cache as (pages, kv_heads, block, dim), got "
-                         f"{tuple(k_cache.shape)} and {tuple(v_cache.shape)}")
+    dtype, device = q.dtype, q.get_device()
+    if not (q.is_cuda and q.ndim == 3 and k_cache.ndim == 4 and v_cache.shape == k_cache.shape
+            and k_cache.dtype is dtype and v_cache.dtype is dtype
+            and k_cache.get_device() == device == v_cache.get_device() == block_table.get_device()
+            and q.stride(2) == 1 == k_cache.stride(3) and v_cache.stride(3) == 1
+            and block_table.ndim == 2 and block_table.dtype is torch.int32 and block_table.stride(1) == 1
+            and context_lens.dtype is torch.int32 and context_lens.get_device() == device
+            and context_lens.shape == block_table.shape[:1] and context_lens.is_contiguous()
+            and cu_q is None and tree_mask is None and q.shape[:1] == context_lens.shape):
+        _check_tree(q, k_cache, v_cache, block_table, context_lens, cu_q, tree_mask)
     _check_heads(q, k_cache.shape[1], k_cache.shape[3])
     if k_cache.shape[2] < 1:
         raise ValueError("pages must hold at least one token")
-    _check_operand("k_cache", k_cache, q)
-    _check_operand("v_cache", v_cache, q)
-    if block_table.ndim != 2 or block_table.dtype != torch.int32:
-        raise ValueError(f"block_table must be int32 (requests, blocks), got {block_table.dtype} "
-                         f"{tuple(block_table.shape)}")
-    if block_table.get_device() != q.get_device():
-        raise ValueError(f"block_table must be on {q.device}, got {block_table.device}")
-    if block_table.stride(1) != 1 and block_table.shape[1] > 1:
-        raise ValueError("block_table must have contiguous rows")
-    seqs = block_table.shape[0]
-    _check_index("context_lens", context_lens, q)
-    if context_lens.ndim != 1 or context_lens.shape[0] != seqs:
-        raise ValueError(f"context_lens must have shape ({seqs},), got {tuple(context_lens.shape)}")
-    if cu_q is not None:
-        _check_index("cu_q", cu_q, q)
-        if cu_q.ndim != 1 or cu_q.shape[0] != seqs + 1:
-            raise ValueError(f"cu_q must have shape ({seqs + 1},), got {tuple(cu_q.shape)}")
-    elif q.shape[0] != seqs:
-        raise ValueError(f"{q.shape[0]} rows for {seqs} requests: pass cu_q")
-    if tree_mask is not None:
-        _check_index("tree_mask", tree_mask, q, torch.int64)
-        if tree_mask.ndim != 2 or tree_mask.shape[0] != q.shape[0] or tree_mask.shape[1] < 1:
-            raise ValueError(f"tree_mask must have shape ({q.shape[0]}, words), got {tuple(tree_mask.shape)}")
     out, lse = _outputs(q, out, return_lse)
     if q.numel():
         native.tree_attention(q, k_cache, v_cache, out, lse, block_table, context_lens, cu_q, tree_mask,

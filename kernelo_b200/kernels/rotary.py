@@ -71,6 +71,15 @@ def rotary_table(
 
 
 def _check(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, table: torch.Tensor) -> None:
+    device = q.get_device()
+    # one expression for what is right, and the reasons only where it is not
+    if (q.is_cuda and q.ndim == 3 == k.ndim and k.dtype is q.dtype and q.shape[0] == k.shape[0]
+            and q.shape[2] == k.shape[2] and q.stride(2) == 1 == k.stride(2) and k.get_device() == device
+            and positions.dtype is torch.int32 and positions.get_device() == device and positions.ndim == 1
+            and positions.shape[0] == q.shape[0] and positions.is_contiguous()
+            and table.dtype is torch.float32 and table.get_device() == device and table.ndim == 2
+            and table.is_contiguous() and table.shape[1] <= q.shape[2] and table.shape[1] % 2 == 0):
+        return
     if q.ndim != 3 or k.ndim != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
         raise ValueError("expected q (tokens, heads, dim) and k (tokens, kv_heads, dim), got "
                          f"{tuple(q.shape)} and {tuple(k.shape)}")
@@ -85,6 +94,22 @@ def _check(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, table: tor
     if table.ndim != 2 or table.shape[1] % 2 or table.shape[1] > q.shape[2]:
         raise ValueError(f"table must be (positions, rotary_dim) with an even rotary_dim of at most {q.shape[2]}, "
                          f"got {tuple(table.shape)}")
+
+
+def _check_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                 slots: torch.Tensor) -> None:
+    if v.shape != k.shape:
+        raise ValueError(f"v must have k's shape {tuple(k.shape)}, got {tuple(v.shape)}")
+    _check_operand("v", v, q)
+    if k_cache.ndim != 4 or k_cache.shape != v_cache.shape or k_cache.shape[1] != k.shape[1] \
+            or k_cache.shape[3] != k.shape[2] or k_cache.shape[2] < 1:
+        raise ValueError(f"expected caches (pages, {k.shape[1]}, block, {k.shape[2]}), got {tuple(k_cache.shape)} "
+                         f"and {tuple(v_cache.shape)}")
+    _check_operand("k_cache", k_cache, q)
+    _check_operand("v_cache", v_cache, q)
+    _check_index("slots", slots, q, torch.int64)
+    if slots.ndim != 1 or slots.shape[0] != q.shape[0]:
+        raise ValueError(f"slots must have shape ({q.shape[0]},), got {tuple(slots.shape)}")
 
 
 def _output(name: str, out: torch.Tensor | None, like: torch.Tensor) -> torch.Tensor:
@@ -144,18 +169,15 @@ def rotary_to_cache(
     end up in it.
     """
     _check(q, k, positions, table)
-    if v.shape != k.shape:
-        raise ValueError(f"v must have k's shape {tuple(k.shape)}, got {tuple(v.shape)}")
-    _check_operand("v", v, q)
-    if k_cache.ndim != 4 or k_cache.shape != v_cache.shape or k_cache.shape[1] != k.shape[1] \
-            or k_cache.shape[3] != k.shape[2] or k_cache.shape[2] < 1:
-        raise ValueError(f"expected caches (pages, {k.shape[1]}, block, {k.shape[2]}), got {tuple(k_cache.shape)} "
-                         f"and {tuple(v_cache.shape)}")
-    _check_operand("k_cache", k_cache, q)
-    _check_operand("v_cache", v_cache, q)
-    _check_index("slots", slots, q, torch.int64)
-    if slots.ndim != 1 or slots.shape[0] != q.shape[0]:
-        raise ValueError(f"slots must have shape ({q.shape[0]},), got {tuple(slots.shape)}")
+    dtype, device = q.dtype, q.get_device()
+    if not (v.shape == k.shape and v.dtype is dtype and v.get_device() == device and v.stride(2) == 1
+            and k_cache.ndim == 4 and v_cache.shape == k_cache.shape and k_cache.shape[1] == k.shape[1]
+            and k_cache.shape[3] == k.shape[2] and k_cache.shape[2] > 0 and k_cache.dtype is dtype
+            and v_cache.dtype is dtype and k_cache.get_device() == device == v_cache.get_device()
+            and k_cache.stride(3) == 1 == v_cache.stride(3) and slots.dtype is torch.int64
+            and slots.get_device() == device and slots.ndim == 1 and slots.shape[0] == q.shape[0]
+            and slots.is_contiguous()):
+        _check_cache(q, k, v, k_cache, v_cache, slots)
     q_out = _output("q_out", q_out, q)
     if k_out is not None:
         k_out = _output("k_out", k_out, k)
