@@ -1,8 +1,9 @@
 // Prompt attention on the 5th-generation tensor cores: causal or not, grouped
 // heads, requests of any lengths packed without padding.
 //
-// A CTA takes 256 rows of one request and head as two tiles of 128 and walks
-// the keys 128 at a time, with the softmax's running maximum and sum:
+// One CTA stays on each SM and takes items in turn: 256 rows of one request and
+// head, as two tiles of 128. It walks an item's keys 128 at a time, with the
+// softmax's running maximum and sum:
 //
 //   S = Q K^T                      tcgen05, fp32 in TMEM, 128 x 128 per tile
 //   m' = max(m, max S),  P = 2^(c S - c m'),  l = l 2^(c m - c m') + sum P
@@ -15,6 +16,8 @@
 //                    weights the tensor cores work for the other tile; the second
 //                    product starts when half of a block's weights are there.
 //   warp 10          zeroes what the last V block holds of the next request.
+//   warp 11          finds the CTA's next item while this one is computed, so that
+//                    its loads and first products start behind this one's results.
 //
 // m is raised, and O (in TMEM) rescaled, only when a row's maximum grew by more
 // than 2^8: until then the weights are at most 256, which 16 bits and the fp32 sums
@@ -38,7 +41,7 @@ namespace {
 constexpr int BLK = 128;       // rows of a tile, keys of a block
 constexpr int PAIR = 2 * BLK;  // rows of a CTA
 constexpr int SOFTMAX_WARPS = 8;
-constexpr int TMA_WARP = 8, MMA_WARP = 9, CLEAN_WARP = 10;
+constexpr int TMA_WARP = 8, MMA_WARP = 9, CLEAN_WARP = 10, PLAN_WARP = 11;
 // Three warpgroups; the last (loads, products) hands registers to the softmax:
 // 3 x 168 a thread become 2 x 208 and 88.
 constexpr int THREADS = 3 * 128;
@@ -52,16 +55,18 @@ struct Shape {
   static constexpr int HALVES = DH / 64;            // 128-byte swizzle atoms of a row
   static constexpr int TILE = BLK * DH * 2;         // bytes of a Q, K or V tile
   static constexpr int STAGES = DH == 128 ? 5 : 8;  // K and V tiles in flight
-  static constexpr int SMEM = 1024 + 2 * TILE + STAGES * TILE + 256;
+  static constexpr int SMEM = 1024 + 2 * TILE + STAGES * TILE + 320;
 };
 
 struct Item {
   int row0;       // first row of q
-  int rows;       // of the request from row0 on, at most PAIR
+  int rows;       // of the request from row0 on, at most PAIR; 0: there is no item
   int node0;      // row0's place in its request
   int first_key;  // first row of k and v
   int keys;
   int shift;      // keys - rows of the request: row i sees i + 1 + shift keys
+  int head;
+  int blocks[2];  // key blocks of each tile: those that its last row sees some of
 };
 
 // The tile pair with number `g`, counted through the requests, the last rows of
@@ -107,7 +112,7 @@ __device__ __forceinline__ int visible(const AttnArgs& p, const Item& it, int i)
 template <typename T, int DH>
 __device__ __noinline__ void redo_row(const AttnArgs& p, int t, int head, int lane) {
   float acc[DH / 32], m, l;
-  attend_row<T, DH / 32>(p, t, head, lane, acc, &m, &l);
+  attend_row<T, DH / 32, 1>(p, t, head, lane, acc, &m, &l);
   write_row<T, DH / 32>(p, t, head, lane, acc, m, l);
 }
 
@@ -123,29 +128,30 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint8_t* q_tiles = smem;
   uint8_t* ring = smem + 2 * S::TILE;
   uint64_t* bars = reinterpret_cast<uint64_t*>(ring + STAGES * S::TILE);
-  // bars: q[2] | full[STAGES] | empty[STAGES] | s_full[2] | p_half[2] | p_full[2] | o_full[2] | dirty | clean
-  __shared__ Item item;
-  __shared__ int has_item;
+  // bars: item[2] | item_free[2] | q[2] | q_free[2] | full[STAGES] | empty[STAGES] | s_full[2] | p_half[2] |
+  //       p_full[2] | o_full[2] | dirty | clean
+  __shared__ Item items[2];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word;
   volatile int* abort_flag = &abort_word;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t q_bar = smem_u32(bars), full = q_bar + 16, empty = full + 8 * STAGES, s_full = empty + 8 * STAGES,
-                 p_half = s_full + 16, p_full = p_half + 16, o_full = p_full + 16, dirty = o_full + 16, clean = dirty + 8;
-  const int heads = static_cast<int>(p.heads);
-  const int head = static_cast<int>(blockIdx.x % heads);
+  const uint32_t item_bar = smem_u32(bars), item_free = item_bar + 16, q_bar = item_free + 16, q_free = q_bar + 16,
+                 full = q_free + 16, empty = full + 8 * STAGES, s_full = empty + 8 * STAGES, p_half = s_full + 16,
+                 p_full = p_half + 16, o_full = p_full + 16, dirty = o_full + 16, clean = dirty + 8;
 
-  if (warp == 0) {
-    const bool found = find_item(p, static_cast<int>(blockIdx.x / heads), lane, &item);
-    if (lane == 0) has_item = found;
-  } else if (warp == TMA_WARP && lane == 0) {
-    for (int i = 0; i < 2 + 2 * STAGES + 2; ++i) mbar_init(q_bar + 8 * i, 1);
-    for (int t = 0; t < 2; ++t) {
-      mbar_init(p_half + 8 * t, SOFTMAX_WARPS / 2);
-      mbar_init(p_full + 8 * t, SOFTMAX_WARPS / 2);
-      mbar_init(o_full + 8 * t, 1);
+  if (warp == TMA_WARP && lane == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(item_bar + 8 * i, 1);
+      mbar_init(item_free + 8 * i, SOFTMAX_WARPS + 3);  // softmax, loads, products, cleaning
+      mbar_init(q_bar + 8 * i, 1);
+      mbar_init(q_free + 8 * i, 1);
+      mbar_init(s_full + 8 * i, 1);
+      mbar_init(p_half + 8 * i, SOFTMAX_WARPS / 2);
+      mbar_init(p_full + 8 * i, SOFTMAX_WARPS / 2);
+      mbar_init(o_full + 8 * i, 1);
     }
+    for (int i = 0; i < 2 * STAGES; ++i) mbar_init(full + 8 * i, 1);
     mbar_init(dirty, 1);
     mbar_init(clean, 1);
     abort_word = 0;
@@ -161,56 +167,102 @@ __global__ void __launch_bounds__(THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
-  const Item it = item;
-  // key blocks of each tile: those that its last row sees some of
-  int blocks[2] = {0, 0};
-  if (has_item) {
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-      if (it.rows > t * BLK) blocks[t] = (visible(p, it, min(it.rows, (t + 1) * BLK) - 1) + BLK - 1) / BLK;
-  }
-  const int most = max(blocks[0], blocks[1]);
+
+  // The n-th item of this CTA, for each role in turn; rows 0 when there are no
+  // more, or a wait gave up. All roles go through the same items in order, and
+  // every barrier below is waited for phase by phase.
+  auto next_item = [&](int n, int site) {
+    Item it;
+    const bool ok = __all_sync(0xffffffffu, mbar_wait(item_bar + 8 * (n & 1), (n >> 1) & 1, abort_flag, status, site));
+    it = items[n & 1];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(item_free + 8 * (n & 1));
+    if (!ok) it.rows = 0;
+    return it;
+  };
 
   if (warp >= SOFTMAX_WARPS) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    if (has_item && warp == TMA_WARP) {
-    if (lane == 0 && most > 0) {
-      const int kv_head = head / static_cast<int>(p.heads / p.kv_heads);
+    if (warp == PLAN_WARP) {
+      // Items: tile pairs x heads, dealt out to the CTAs in turn, forwards and
+      // backwards, so that each gets large and small ones alike.
+      const int heads = static_cast<int>(p.heads), ctas = static_cast<int>(gridDim.x), me = static_cast<int>(blockIdx.x);
+      for (int n = 0;; ++n) {
+        const long long i = static_cast<long long>(n) * ctas + (n & 1 ? ctas - 1 - me : me);
+        const bool ok = __all_sync(
+            0xffffffffu, mbar_wait(item_free + 8 * (n & 1), ((n >> 1) & 1) ^ 1, abort_flag, status, SITE_ATTN_LOAD));
+        Item* it = &items[n & 1];
+        const bool found = ok && find_item(p, static_cast<int>(i / heads), lane, it);
+        __syncwarp();
+        if (lane == 0) {
+          if (found) {
+            it->head = static_cast<int>(i % heads);
+            for (int t = 0; t < 2; ++t)
+              it->blocks[t] =
+                  it->rows > t * BLK ? (visible(p, *it, min(it->rows, (t + 1) * BLK) - 1) + BLK - 1) / BLK : 0;
+          } else {
+            it->rows = 0;
+          }
+          mbar_arrive(item_bar + 8 * (n & 1));
+        }
+        __syncwarp();
+        if (!found) break;
+      }
+    } else if (warp == TMA_WARP) {
       bool ok = true;
-      int issued = 0;
+      int issued = 0, loaded = 0;  // K and V tiles, and items with any
       auto load = [&](uint32_t dst, const CUtensorMap* map, uint32_t bar, int h, int row) {
         mbar_arrive_expect_tx(bar, S::TILE);
 #pragma unroll
         for (int x = 0; x < S::HALVES; ++x) tma_load_3d(dst + x * BLK * 128, map, bar, 64 * x, h, row);
       };
-      auto next = [&](const CUtensorMap* map, int block) {
-        const int slot = issued % STAGES;
-        if (!mbar_wait(empty + 8 * slot, ((issued / STAGES) & 1) ^ 1, abort_flag, status, SITE_ATTN_LOAD)) return false;
-        load(smem_u32(ring + slot * S::TILE), map, full + 8 * slot, kv_head, it.first_key + block * BLK);
-        ++issued;
-        return true;
-      };
-      load(smem_u32(q_tiles), &tm_q, q_bar, head, it.row0);
-      ok = next(&tm_k, 0);
-      load(smem_u32(q_tiles + S::TILE), &tm_q, q_bar + 8, head, it.row0 + BLK);
-      for (int j = 0; ok && j < most; ++j) {
-        ok = next(&tm_v, j);
-        if (ok && j + 1 < most) ok = next(&tm_k, j + 1);
+      for (int n = 0;; ++n) {
+        const Item it = next_item(n, SITE_ATTN_LOAD);
+        if (it.rows == 0) break;
+        const int most = max(it.blocks[0], it.blocks[1]);
+        if (most == 0) continue;
+        if (lane == 0) {
+          const int kv_head = it.head / static_cast<int>(p.heads / p.kv_heads);
+          auto next = [&](const CUtensorMap* map, int block) {
+            const int slot = issued % STAGES;
+            if (!mbar_wait(empty + 8 * slot, ((issued / STAGES) & 1) ^ 1, abort_flag, status, SITE_ATTN_LOAD)) return false;
+            load(smem_u32(ring + slot * S::TILE), map, full + 8 * slot, kv_head, it.first_key + block * BLK);
+            ++issued;
+            return true;
+          };
+          auto query = [&](int t) {
+            if (!mbar_wait(q_free + 8 * t, (loaded & 1) ^ 1, abort_flag, status, SITE_ATTN_LOAD)) return false;
+            load(smem_u32(q_tiles + t * S::TILE), &tm_q, q_bar + 8 * t, it.head, it.row0 + t * BLK);
+            return true;
+          };
+          ok = query(0) && next(&tm_k, 0) && query(1);
+          for (int j = 0; ok && j < most; ++j) {
+            ok = next(&tm_v, j);
+            if (ok && j + 1 < most) ok = next(&tm_k, j + 1);
+          }
+        }
+        ++loaded;
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
       }
-      if (!ok) {  // let the copies in flight land before the shared memory goes away
-        for (int t = 0; t < 2; ++t) mbar_wait(q_bar + 8 * t, 0, nullptr, status, SITE_DRAIN, DRAIN_NS);
+      if (!ok && lane == 0) {  // let the copies in flight land before the shared memory goes away
+        for (int t = 0; t < 2; ++t) mbar_wait(q_bar + 8 * t, (loaded - 1) & 1, nullptr, status, SITE_DRAIN, DRAIN_NS);
         for (int s = 0; s < STAGES && s < issued; ++s)
           mbar_wait(full + 8 * s, ((issued - 1 - s) / STAGES) & 1, nullptr, status, SITE_DRAIN, DRAIN_NS);
       }
-    }
-    } else if (has_item && warp == CLEAN_WARP) {
+    } else if (warp == CLEAN_WARP) {
       // The last block of a request: its V rows past the request's keys, when the
-      // thread of the products has seen them land
-      const int held = it.keys - (most - 1) * BLK;
-      if (most > 0 && held < BLK) {
-        const int slot = (2 * most - 1) % STAGES;  // of the ring: K V K V ...
-        mbar_wait(dirty, 0, abort_flag, status, SITE_ATTN_LOAD);
-        __syncwarp();
+      // warp of the products has seen them land
+      int tiles = 0, cleaned = 0;  // K and V tiles before the item's
+      for (int n = 0;; ++n) {
+        const Item it = next_item(n, SITE_ATTN_LOAD);
+        if (it.rows == 0) break;
+        const int most = max(it.blocks[0], it.blocks[1]);
+        if (most == 0) continue;
+        tiles += 2 * most;
+        const int held = it.keys - (most - 1) * BLK, slot = (tiles - 1) % STAGES;
+        if (held >= BLK) continue;
+        if (!__all_sync(0xffffffffu, mbar_wait(dirty, cleaned & 1, abort_flag, status, SITE_ATTN_LOAD))) break;
         for (int i = lane; i < (BLK - held) * S::HALVES * 8; i += 32) {
           const int h = i / ((BLK - held) * 8), rest = i - h * (BLK - held) * 8;
           *reinterpret_cast<uint4*>(ring + slot * S::TILE + h * BLK * 128 + held * 128 + rest * 16) =
@@ -219,23 +271,24 @@ __global__ void __launch_bounds__(THREADS, 1)
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(clean);
+        ++cleaned;
       }
-    } else if (has_item && warp == MMA_WARP && most > 0) {
-      // The warp runs together on uniform values and one elected lane issues: a few
-      // instructions a product, where a branch for one lane takes about 20 and the
-      // tensor cores run dry behind them. (A warp for each tile measured slower: two
-      // tiles' products in turn finish later than one tile's, then the other's.)
+    } else {
+      // MMA_WARP. The warp runs together on uniform values and one elected lane
+      // issues: a few instructions a product, where a branch for one lane takes
+      // about 20 and the tensor cores run dry behind them. (A warp for each tile
+      // measured slower: two tiles' products in turn finish later than one tile's,
+      // then the other's.)
       const uint32_t lead = elect_lane();
       const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
       const uint32_t q_at = __shfl_sync(0xffffffffu, smem_u32(q_tiles), 0), ring_at = __shfl_sync(0xffffffffu, smem_u32(ring), 0);
-      const int count[2] = {__shfl_sync(0xffffffffu, blocks[0], 0), __shfl_sync(0xffffffffu, blocks[1], 0)};
-      const int all = max(count[0], count[1]);
-      const bool partial = __shfl_sync(0xffffffffu, it.keys - (most - 1) * BLK, 0) < BLK;
       constexpr uint32_t fmt = DType<T>::code == KF_BF16 ? 1u : 0u;
       constexpr uint32_t idesc_s = instr_desc_f16(fmt, 0, 0, BLK, BLK), idesc_o = instr_desc_f16(fmt, 0, 1, BLK, DH);
       const uint64_t q_desc = smem_desc_sw128(q_at, 16, 1024);
       const uint64_t k_desc = smem_desc_sw128(ring_at, 16, 1024), v_desc = smem_desc_sw128(ring_at, BLK * 128, 1024);
       int slot = 0, phase = 0;  // of the ring's next tile
+      int done[2] = {0, 0};     // blocks of each tile, over all items
+      int loaded = 0, cleaned = 0;
       bool ok = true;
       auto wait = [&](uint32_t bar, int parity) {
         if (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity)))
@@ -251,7 +304,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         return at;
       };
-      auto scores = [&](int t, int at) {  // S_t = Q_t K^T
+      auto scores = [&](int t, int at, bool last) {  // S_t = Q_t K^T
         const uint64_t a = q_desc + static_cast<uint64_t>(t * S::TILE / 16), b = k_desc + static_cast<uint64_t>(at * (S::TILE / 16));
 #pragma unroll
         for (int k = 0; k < DH / 16; ++k) {
@@ -259,6 +312,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           tc_mma_f16_by(lead, tm + t * BLK, a + step, b + step, idesc_s, k > 0);
         }
         tc_commit_by(lead, s_full + 8 * t);  // with it all products before are done, O_t's too
+        if (last) tc_commit_by(lead, q_free + 8 * t);
       };
       auto products = [&](int t, int at, bool accumulate, int k0, int k1) {  // O_t += P_t V
         const uint64_t b = v_desc + static_cast<uint64_t>(at * (S::TILE / 16));
@@ -267,96 +321,122 @@ __global__ void __launch_bounds__(THREADS, 1)
           tc_mma_f16_ta_by(lead, tm + 2 * BLK + t * BLK, tm + t * BLK + 8 * k, b + static_cast<uint64_t>(k * 128), idesc_o,
                            accumulate || k > 0);
       };
-      int k_at = wait_tile();
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        wait(q_bar + 8 * t, 0);
-        if (ok && count[t] > 0) scores(t, k_at);
-      }
-      tc_commit_by(lead, empty + 8 * k_at);
-      for (int j = 0; ok && j < all; ++j) {
-        const int v_at = wait_tile();
-        if (j + 1 < all) {
-          k_at = wait_tile();
-        } else if (partial) {
-          if (lead) mbar_arrive(dirty);
-          wait(clean, 0);
+      for (int n = 0; ok; ++n) {
+        const Item it = next_item(n, SITE_ATTN_MMA);
+        if (__shfl_sync(0xffffffffu, it.rows, 0) == 0) break;
+        const int count[2] = {__shfl_sync(0xffffffffu, it.blocks[0], 0), __shfl_sync(0xffffffffu, it.blocks[1], 0)};
+        const int all = max(count[0], count[1]);
+        const bool partial = __shfl_sync(0xffffffffu, it.keys, 0) - (all - 1) * BLK < BLK;
+        if (all == 0) continue;
+        wait(q_bar, loaded & 1);
+        int k_at = wait_tile();
+        if (count[0] > 0) {
+          if (ok) scores(0, k_at, count[0] == 1);
+        } else {
+          tc_commit_by(lead, q_free);
         }
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          if (j >= count[t]) continue;
-          wait(p_half + 8 * t, j & 1);
-          if (ok) products(t, v_at, j > 0, 0, 4);
-          wait(p_full + 8 * t, j & 1);
-          if (ok) products(t, v_at, true, 4, 8);
-          if (j + 1 < count[t]) {
-            if (ok) scores(t, k_at);
-          } else {
-            tc_commit_by(lead, o_full + 8 * t);
+        wait(q_bar + 8, loaded & 1);
+        if (count[1] > 0) {
+          if (ok) scores(1, k_at, count[1] == 1);
+        } else {
+          tc_commit_by(lead, q_free + 8);
+        }
+        ++loaded;
+        tc_commit_by(lead, empty + 8 * k_at);
+        for (int j = 0; ok && j < all; ++j) {
+          const int v_at = wait_tile();
+          if (j + 1 < all) {
+            k_at = wait_tile();
+          } else if (partial) {
+            if (lead) mbar_arrive(dirty);
+            wait(clean, cleaned & 1);
+            ++cleaned;
           }
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (j >= count[t]) continue;
+            const int parity = (done[t] + j) & 1;
+            wait(p_half + 8 * t, parity);
+            if (ok) products(t, v_at, j > 0, 0, 4);
+            wait(p_full + 8 * t, parity);
+            if (ok) products(t, v_at, true, 4, 8);
+            if (j + 1 < count[t]) {
+              if (ok) scores(t, k_at, j + 2 == count[t]);
+            } else {
+              tc_commit_by(lead, o_full + 8 * t);
+            }
+          }
+          tc_commit_by(lead, empty + 8 * v_at);
+          if (j + 1 < all) tc_commit_by(lead, empty + 8 * k_at);
         }
-        tc_commit_by(lead, empty + 8 * v_at);
-        if (j + 1 < all) tc_commit_by(lead, empty + 8 * k_at);
+        done[0] += count[0];
+        done[1] += count[1];
       }
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-    if (has_item) {
     const int t = warp >> 2;
     const int row = (warp & 3) * 32 + lane;  // of the tile
     const int i = t * BLK + row;             // of the item
-    const bool valid = i < it.rows;
-    const int limit = valid ? visible(p, it, i) : 0;
     const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const uint32_t s_addr = lanes + t * BLK, o_addr = lanes + 2 * BLK + t * BLK;
     const float c = p.scale_log2;
-    float m = -INFINITY, l = 0.0f;
+    int done = 0, results = 0;  // blocks of this tile, and items with any, before this item
     bool ok = true;
-    for (int j = 0; j < blocks[t]; ++j) {
-      ok = mbar_wait(s_full + 8 * t, j & 1, abort_flag, status, SITE_ATTN_SOFTMAX);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      tc_fence_after();
-      float s[BLK];
+    for (int n = 0; ok; ++n) {
+      const Item it = next_item(n, SITE_ATTN_SOFTMAX);
+      if (it.rows == 0) break;
+      const int blocks = t == 0 ? it.blocks[0] : it.blocks[1];
+      const bool valid = i < it.rows;
+      const int limit = valid ? visible(p, it, i) : 0;
+      float m = -INFINITY, l = 0.0f;
+      for (int j = 0; j < blocks; ++j) {
+        ok = mbar_wait(s_full + 8 * t, (done + j) & 1, abort_flag, status, SITE_ATTN_SOFTMAX);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        float s[BLK];
 #pragma unroll
-      for (int x = 0; x < BLK; x += 32) tmem_ld_32(s_addr + x, reinterpret_cast<uint32_t*>(s + x));
-      tmem_ld_wait();
-      const int left = limit - j * BLK;
-      if (left < BLK) {
+        for (int x = 0; x < BLK; x += 32) tmem_ld_32(s_addr + x, reinterpret_cast<uint32_t*>(s + x));
+        tmem_ld_wait();
+        const int left = limit - j * BLK;
+        if (left < BLK) {
 #pragma unroll
-        for (int x = 0; x < BLK; ++x)
-          if (x >= left) s[x] = -INFINITY;
-      }
-      __syncwarp();
-      const float m_new = row_max(s, m);
-      if (j == 0) {
-        m = m_new;
-      } else if (__any_sync(0xffffffffu, (m_new - m) * c > RAISE_LOG2)) {
-        // S of this block came with the end of all products before it: O rests
-        const float fix = m_new > m ? ex2_ftz((m - m_new) * c) : 1.0f;
-        l *= fix;
-        m = m_new;
-#pragma unroll 1
-        for (int x = 0; x < DH; x += 32) {
-          uint32_t o[32];
-          tmem_ld_32(o_addr + x, o);
-          tmem_ld_wait();
-#pragma unroll
-          for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * fix);
-          tmem_st_32(o_addr + x, o);
+          for (int x = 0; x < BLK; ++x)
+            if (x >= left) s[x] = -INFINITY;
         }
+        __syncwarp();
+        const float m_new = row_max(s, m);
+        if (j == 0) {
+          m = m_new;
+        } else if (__any_sync(0xffffffffu, (m_new - m) * c > RAISE_LOG2)) {
+          // S of this block came with the end of all products before it: O rests
+          const float fix = m_new > m ? ex2_ftz((m - m_new) * c) : 1.0f;
+          l *= fix;
+          m = m_new;
+#pragma unroll 1
+          for (int x = 0; x < DH; x += 32) {
+            uint32_t o[32];
+            tmem_ld_32(o_addr + x, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * fix);
+            tmem_st_32(o_addr + x, o);
+          }
+        }
+        const float cm = m == -INFINITY ? 0.0f : m * c;
+        l += row_weights<T, true>(s, c, cm, s_addr, p_half + 8 * t, p_full + 8 * t, lane);
       }
-      const float cm = m == -INFINITY ? 0.0f : m * c;
-      l += row_weights<T, true>(s, c, cm, s_addr, p_half + 8 * t, p_full + 8 * t, lane);
-    }
-    if (ok && blocks[t] > 0) {
-      ok = mbar_wait(o_full + 8 * t, 0, abort_flag, status, SITE_ATTN_SOFTMAX);
-      ok = __all_sync(0xffffffffu, ok);
-      tc_fence_after();
-    }
-    if (ok && it.rows > t * BLK) {
+      done += blocks;
+      if (ok && blocks > 0) {
+        ok = mbar_wait(o_full + 8 * t, results & 1, abort_flag, status, SITE_ATTN_SOFTMAX);
+        ok = __all_sync(0xffffffffu, ok);
+        tc_fence_after();
+        ++results;
+      }
+      if (!ok || it.rows <= t * BLK) continue;
       const int q_row = it.row0 + i;
-      T* out = static_cast<T*>(p.out) + static_cast<long long>(q_row) * p.so_t + head * p.so_h;
+      T* out = static_cast<T*>(p.out) + static_cast<long long>(q_row) * p.so_t + it.head * p.so_h;
       // The largest weight of a row is one or more, and a key it does not see
       // weighs at most 2^-126: a sum between is that of no key.
       if (l < 5.4e-20f) l = 0.0f;  // 2^-64
@@ -365,7 +445,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll 1
       for (int x = 0; x < DH; x += 32) {
         uint32_t o[32];
-        if (blocks[t] > 0) {
+        if (blocks > 0) {
           tmem_ld_32(o_addr + x, o);
           tmem_ld_wait();
         } else {
@@ -397,16 +477,15 @@ __global__ void __launch_bounds__(THREADS, 1)
         __syncwarp();
       }
       if (p.lse != nullptr && valid)
-        p.lse[static_cast<long long>(q_row) * heads + head] =
+        p.lse[static_cast<long long>(q_row) * p.heads + it.head] =
             l > 0.0f ? m * c * 0.69314718055994530942f + logf(l) : -INFINITY;
       // l that is NaN (a score is) has left zeros: those rows too
       uint32_t again = __ballot_sync(0xffffffffu, valid && (!(bad == 0.0f) || !(l >= 0.0f && l < INFINITY)));
       while (again != 0) {
         const int src = __ffs(again) - 1;
         again &= again - 1;
-        redo_row<T, DH>(p, __shfl_sync(0xffffffffu, q_row, src), head, lane);
+        redo_row<T, DH>(p, __shfl_sync(0xffffffffu, q_row, src), it.head, lane);
       }
-    }
     }
   }
   tc_fence_before();
@@ -439,7 +518,8 @@ int launch_typed(const AttnArgs& a, const DeviceInfo& dev, cudaStream_t stream) 
   if (attr != cudaSuccess) return cuda_error(attr, "prefill attributes");
   if (registers < LAUNCH_REGISTERS)  // the warpgroups' shares must not exceed what the block is launched with
     return set_error(KF_ERR_UNSUPPORTED, "prompt attention: built with too few registers to split");
-  const int64_t blocks = (a.rows / PAIR + a.seqs + 1) * a.heads;
+  const int64_t most = (a.rows / PAIR + a.seqs + 1) * a.heads;  // items
+  const int64_t blocks = most < dev.sm_count ? most : dev.sm_count;
   const int vector_out = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.so_t % 8 == 0 && a.so_h % 8 == 0;
   prefill_kernel<T, DH><<<static_cast<unsigned>(blocks), THREADS, Shape<DH>::SMEM, stream>>>(q, k, v, a, vector_out,
                                                                                             dev.status);
