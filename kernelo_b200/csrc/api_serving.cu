@@ -69,7 +69,7 @@ int32_t kf_prefill_attention(const kf_prefill_args* args, void* stream) {
   a.scale_log2 = static_cast<float>(g.scale * LOG2_E);
   a.causal = g.causal != 0;
   if (attention_prefill_supported(a)) return launch_attention_prefill(a, *dev, static_cast<cudaStream_t>(stream));
-  return launch_attention_rows(a, *dev, static_cast<cudaStream_t>(stream));
+  return launch_attention_block(a, *dev, static_cast<cudaStream_t>(stream));
 }
 
 int32_t kf_tree_attention(const kf_tree_args* args, void* stream) {
@@ -107,7 +107,7 @@ int32_t kf_tree_attention(const kf_tree_args* args, void* stream) {
   a.scale_log2 = static_cast<float>(g.scale * LOG2_E);
   a.workspace = g.workspace, a.workspace_bytes = g.workspace_bytes;
   if (attention_tree_supported(a)) return launch_attention_tree(a, *dev, static_cast<cudaStream_t>(stream));
-  return launch_attention_rows(a, *dev, static_cast<cudaStream_t>(stream));
+  return launch_attention_block(a, *dev, static_cast<cudaStream_t>(stream));
 }
 
 int64_t kf_tree_attention_workspace_bytes(int32_t device, int32_t dtype, int64_t seqs, int64_t rows, int64_t heads,

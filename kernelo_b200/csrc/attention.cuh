@@ -68,15 +68,13 @@ __device__ __forceinline__ long long key_offset(const AttnArgs& p, int r, long l
   return page * s_page + (pos - col * p.block_size) * s_row;
 }
 
-// One row of attention by one warp: for lane's elements e = lane + 32 i of the
-// head, acc = sum_j p_j v_j with the running maximum m and sum l of the softmax in
-// base 2 (q is read times scale * log2(e)), KEYS at a time, so that their loads and
-// sums over the lanes overlap. Keys that the row does not see are not read, so
-// nothing in them reaches the result. `part` of `parts` takes an equal share of the
-// keys.
-template <typename T, int NE, int KEYS>
+// One row of attention by one warp, key by key: for lane's elements
+// e = lane + 32 i of the head, acc = sum_j p_j v_j with the running maximum m
+// and sum l of the softmax in base 2 (q is read times scale * log2(e)). Keys that
+// the row does not see are not read, so nothing in them reaches the result.
+template <typename T, int NE>
 __device__ __forceinline__ void attend_row(const AttnArgs& p, int t, int head, int lane, float (&acc)[NE], float* m_out,
-                                           float* l_out, int part = 0, int parts = 1) {
+                                           float* l_out) {
   const int r = request_of(p, t);
   int row0, row1;
   request_rows(p, r, &row0, &row1);
@@ -106,62 +104,31 @@ __device__ __forceinline__ void attend_row(const AttnArgs& p, int t, int head, i
     last = prefix;
   }
   const unsigned long long* mask = p.mask != nullptr ? p.mask + t * p.mask_words : nullptr;
-  const long long share = ((last + parts - 1) / parts + 3) / 4 * 4;
-  const long long stop = min(last, share * (part + 1));
-  for (long long pos0 = share * part; pos0 < stop; pos0 += KEYS) {
-    long long ko[KEYS], vo[KEYS];
-    float s[KEYS];
-#pragma unroll
-    for (int x = 0; x < KEYS; ++x) {
-      const long long pos = pos0 + x, j = pos - prefix;
-      bool seen = pos < stop;
-      if (seen && j >= 0)
-        seen = j < 64ll * p.mask_words && ((__ldg(mask + (j >> 6)) >> (j & 63)) & 1ull);
-      ko[x] = seen ? key_offset(p, r, first, pos, p.sk_p, p.sk_t) : -1;
-      vo[x] = ko[x] >= 0 ? key_offset(p, r, first, pos, p.sv_p, p.sv_t) : -1;
-      s[x] = 0.0f;
+  for (long long pos = 0; pos < last; ++pos) {
+    if (pos >= prefix) {
+      const long long j = pos - prefix;
+      if (j >= 64ll * p.mask_words || !((__ldg(mask + (j >> 6)) >> (j & 63)) & 1ull)) continue;
     }
+    const long long ko = key_offset(p, r, first, pos, p.sk_p, p.sk_t);
+    if (ko < 0) continue;
+    const long long vo = key_offset(p, r, first, pos, p.sv_p, p.sv_t);
+    float s = 0.0f;
 #pragma unroll
     for (int i = 0; i < NE; ++i) {
       const int e = lane + 32 * i;
-      if (e < D) {
-#pragma unroll
-        for (int x = 0; x < KEYS; ++x)
-          if (ko[x] >= 0) s[x] = fmaf(qf[i], to_f32(k[ko[x] + e]), s[x]);
-      }
+      if (e < D) s = fmaf(qf[i], to_f32(k[ko + e]), s);
     }
-    float top = m;
 #pragma unroll
-    for (int x = 0; x < KEYS; ++x) {
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) s[x] += __shfl_xor_sync(0xffffffffu, s[x], o);
-      if (ko[x] < 0) s[x] = -INFINITY;
-      top = s[x] > top ? s[x] : top;  // a score that is not a number stays to be seen in the weights
-    }
-    if (top == -INFINITY) {
-      // no weight so far (a score may still be none at all)
-      bool nan = false;
-#pragma unroll
-      for (int x = 0; x < KEYS; ++x) nan = nan || s[x] != s[x];
-      if (!nan) continue;
-    }
-    const float fix = m == -INFINITY ? 0.0f : ex2_ftz(m - top);
-    float w[KEYS];
-    l *= fix;
-#pragma unroll
-    for (int x = 0; x < KEYS; ++x) {
-      w[x] = s[x] == -INFINITY ? 0.0f : ex2_ftz(s[x] - top);
-      l += w[x];
-    }
-    m = top;
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (s == -INFINITY) continue;  // weight zero, also while m is still -inf
+    const float m_new = fmaxf(m, s);
+    const float fix = ex2_ftz(m - m_new), w = ex2_ftz(s - m_new);
+    m = m_new;
+    l = fmaf(l, fix, w);
 #pragma unroll
     for (int i = 0; i < NE; ++i) {
       const int e = lane + 32 * i;
-      float sum = acc[i] * fix;
-#pragma unroll
-      for (int x = 0; x < KEYS; ++x)
-        if (e < D && ko[x] >= 0 && s[x] != -INFINITY) sum = fmaf(w[x], to_f32(v[vo[x] + e]), sum);
-      acc[i] = sum;
+      acc[i] = fmaf(acc[i], fix, e < D ? w * to_f32(v[vo + e]) : 0.0f);
     }
   }
   *m_out = m;

@@ -225,7 +225,7 @@ __device__ __forceinline__ uint32_t nodes_seen(const AttnArgs& p, const Cursor& 
 template <typename T, int NE>
 __device__ __noinline__ void redo_row(const AttnArgs& p, int t, int head, int lane) {
   float acc[NE], m, l;
-  attend_row<T, NE, 1>(p, t, head, lane, acc, &m, &l);
+  attend_row<T, NE>(p, t, head, lane, acc, &m, &l);
   write_row<T, NE>(p, t, head, lane, acc, m, l);
 }
 

@@ -112,7 +112,7 @@ __device__ __forceinline__ int visible(const AttnArgs& p, const Item& it, int i)
 template <typename T, int DH>
 __device__ __noinline__ void redo_row(const AttnArgs& p, int t, int head, int lane) {
   float acc[DH / 32], m, l;
-  attend_row<T, DH / 32, 1>(p, t, head, lane, acc, &m, &l);
+  attend_row<T, DH / 32>(p, t, head, lane, acc, &m, &l);
   write_row<T, DH / 32>(p, t, head, lane, acc, m, l);
 }
 

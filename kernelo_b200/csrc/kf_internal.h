@@ -271,8 +271,9 @@ int encode_heads(CUtensorMap* map, int dtype, const void* ptr, int64_t rows, int
 // last page is filled with zeros. False where no tensor map describes the cache.
 bool encode_pages(CUtensorMap* map, const AttnArgs& args, const void* ptr, int64_t s_page, int64_t s_head, int64_t s_slot,
                   int box_rows, int width);
-// A warp or several per row and head: every type, stride and mask.
-int launch_attention_rows(const AttnArgs& args, const DeviceInfo& dev, cudaStream_t stream);
+// Tiles of 16 or 64 rows in fp32 arithmetic (attention_block.cu): every type, stride,
+// head dimension up to ATTN_MAX_DIM and mask.
+int launch_attention_block(const AttnArgs& args, const DeviceInfo& dev, cudaStream_t stream);
 // Packed prompts on tcgen05 tiles (attention_prefill.cu): fp16/bf16, heads of up
 // to 128 elements on the 16-byte grid, a positive scale.
 bool attention_prefill_supported(const AttnArgs& args);

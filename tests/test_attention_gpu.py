@@ -439,3 +439,47 @@ def test_tree_refusals(device):
         args = dict(q=q, k_cache=k, v_cache=v, block_table=table, context_lens=lens) | change
         with pytest.raises(ValueError, match=message):
             tree_attention(**args)
+
+
+# ---------------------------------------------------- tiles in fp32 arithmetic
+@pytest.mark.parametrize("block", [1, 3, 8, 24, 256])
+@pytest.mark.parametrize("count", [1, 4, 20, 70])
+@pytest.mark.parametrize("heads,kv_heads", [(5, 1), (8, 8), (32, 8)])
+def test_fp32_trees(heads, kv_heads, count, block, device):
+    """Both tile sizes; keys of a tile shared by up to 16 CTAs, and none; mask bits across blocks of 32 keys."""
+    context, nodes = (33, 0, 700, 31), (count, 1, max(1, count - 1), max(1, count // 2))
+    masks, words = random_trees(nodes, words=2)
+    check_tree(context, nodes, *cache(context, nodes, heads, kv_heads, 64, block, torch.float32, device, columns=3000 // block),
+               f"{heads}/{kv_heads} {count} {block}", masks=masks, words=words)
+
+
+@pytest.mark.parametrize("dim", [24, 96, 128, 250])
+def test_fp32_long_cache(dim, device):
+    context, nodes = (5000,), (2,)
+    args = cache(context, nodes, 4, 1, dim, 16, torch.float32, device, stale=float("nan"))
+    out, lse = check_tree(context, nodes, *args, f"dim {dim}")
+    q, k, v, table, lens = args
+    again, again_lse = tree_attention(q, k, v, table, lens, offsets(nodes, device), return_lse=True)
+    assert torch.equal(out, again) and torch.equal(lse, again_lse)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(7, 1, 128), (3, 3, 33), (4, 2, 256)])
+def test_fp32_prompts(heads, kv_heads, dim, causal, device):
+    lens_q, lens_k = (333, 1, 64, 0, 90), (400, 1, 64, 5, 700)
+    check_prompt(lens_q, lens_k, *prompt(lens_q, lens_k, heads, kv_heads, dim, torch.float32, device),
+                 f"{heads}/{kv_heads} {dim} causal={causal}", causal=causal)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_elements_off_the_grid(dtype, device):
+    """Rows that begin on odd elements, of odd lengths, and pages whose rows lie backwards in memory's order of heads."""
+    lens = (70, 41)
+    q, k, v, cu_q, cu_k = prompt(lens, lens, 4, 2, 77, dtype, device)
+    q, k, v = (torch.nn.functional.pad(t, (1, 2))[:, :, 1:78] for t in (q, k, v))
+    assert q.stride(1) == 80 and q.storage_offset() == 1
+    check_prompt(lens, lens, q, k, v, cu_q, cu_k, f"{dtype}")
+    context, nodes = (50, 7), (2, 1)
+    q, k, v, table, at = cache(context, nodes, 4, 2, 77, 16, dtype, device)
+    k, v = (torch.nn.functional.pad(t.transpose(1, 2).contiguous(), (1, 2))[..., 1:78].transpose(1, 2) for t in (k, v))
+    check_tree(context, nodes, q, k, v, table, at, f"{dtype}")
