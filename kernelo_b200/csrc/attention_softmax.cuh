@@ -31,17 +31,6 @@ __device__ __forceinline__ void tmem_st_16(uint32_t taddr, const uint32_t* r) {
       : "memory");
 }
 
-template <typename T>
-__device__ __forceinline__ uint32_t pack_pair(float a, float b) {
-  uint32_t r;
-  if constexpr (DType<T>::code == KF_BF16) {
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
-  } else {
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
-  }
-  return r;
-}
-
 // The largest of `m` and the row's scores.
 __device__ __forceinline__ float row_max(const float (&s)[128], float m) {
   float top[4] = {m, s[0], s[1], s[2]};

@@ -496,6 +496,18 @@ __device__ __forceinline__ float gelu_tanh(float x) {
   return x * (u >= 0.0f ? r : e * r);
 }
 
+// Two values rounded to 16 bits, the first in the lower half.
+template <typename T>
+__device__ __forceinline__ uint32_t pack_pair(float a, float b) {
+  uint32_t r;
+  if constexpr (DType<T>::code == KF_BF16) {
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  } else {
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+  }
+  return r;
+}
+
 // ---- packed fp32x2 arithmetic (sm_100: one instruction for two lanes)
 __device__ __forceinline__ uint64_t f2_pack(float a, float b) {
   uint64_t r;
