@@ -483,3 +483,16 @@ def test_elements_off_the_grid(dtype, device):
     q, k, v, table, at = cache(context, nodes, 4, 2, 77, 16, dtype, device)
     k, v = (torch.nn.functional.pad(t.transpose(1, 2).contiguous(), (1, 2))[..., 1:78].transpose(1, 2) for t in (k, v))
     check_tree(context, nodes, q, k, v, table, at, f"{dtype}")
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("requests", [3, 30, 31, 32, 40, 150])
+def test_many_prompts_of_all_lengths(requests, causal, device):
+    """More items than SMs, dealt out by their lengths or, for many requests, as they come; every row has to be there."""
+    rng = np.random.default_rng(requests)
+    lens_q = [int(n) for n in rng.choice([0, 1, 130, 256, 257, 600], requests)]
+    lens_q[0] = 900
+    lens_k = [n + int(m) for n, m in zip(lens_q, rng.choice([0, 0, 200], requests))]
+    kv_heads = max(1, 150 // requests)
+    check_prompt(lens_q, lens_k, *prompt(lens_q, lens_k, 2 * kv_heads, kv_heads, 32, torch.float16, device),
+                 f"{requests} {causal}", causal=causal)
