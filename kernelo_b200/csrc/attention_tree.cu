@@ -50,9 +50,10 @@ constexpr int KW = KEYS / WARPS;
 constexpr int LOAD_WARP = WARPS, FINISH_WARP = WARPS + 1;
 constexpr int THREADS = 32 * (WARPS + 2);
 constexpr int MIN_RUN = 4;  // positions of a run: fewer blocks cost more to join than to read (8: 19.0 us for 18.4, one short request)
-// Blocks that an item's queries and results are worth. 64 requests of up to 4096 keys: 118 us
-// (133 without); 16 of up to 8192, two nodes each: 70 (93); one of 131072: 114 (111).
-constexpr int ITEM_COST = 2;
+// Blocks that an item's queries and results are worth. 64 requests of up to 4096 keys: 115 us
+// (133 with none, 118 with 2, 117 with 6); 128 of up to 1000: 77 (81 with 2 and with 6); one of
+// 131072: 114 with any.
+constexpr int ITEM_COST = 3;
 constexpr uint64_t DRAIN_NS = 100000000ull;
 
 template <int DP_, int STAGES_>
