@@ -514,9 +514,6 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (!ok || it.rows <= t * BLK) continue;
       const int q_row = it.row0 + i;
       T* out = static_cast<T*>(p.out) + static_cast<long long>(q_row) * p.so_t + it.head * p.so_h;
-      // The largest weight of a row is one or more, and a key it does not see
-      // weighs at most 2^-126: a sum between is that of no key.
-      if (l < 5.4e-20f) l = 0.0f;  // 2^-64
       const float inv = l > 0.0f ? 1.0f / l : 0.0f;
       float bad = 0.0f;  // NaN if anything in the row is not finite
 #pragma unroll 1

@@ -7,8 +7,8 @@
 // for a tile of 128 x 128, as long as the tile's two products. Where two tiles
 // share an SM a quarter of the exponentials is computed on the FMA pipe instead
 // (EMULATE): x = n + f with n the nearest integer, 2^f by the degree-4 polynomial
-// of least relative error on [-1/2, 1/2] (2.6e-6, fitted by Remez exchange), and n
-// added to the exponent. One 8192-token prompt at 32/8 heads of 128 in bursts: 465 us
+// with constant term 1 of least relative error on [-1/2, 1/2] (2.9e-6 as computed),
+// and n added to the exponent. One 8192-token prompt at 32/8 heads of 128 in bursts: 465 us
 // without it, 450 with it.
 #pragma once
 
@@ -45,27 +45,28 @@ __device__ __forceinline__ float row_max(const float (&s)[128], float m) {
   return fmaxf(max3(top[0], top[1], top[2]), top[3]);
 }
 
-// 2^x of two values without the special-function unit.
+// 2^x of two values without the special-function unit; x = -127 and below (a key
+// that the row does not see) give exactly zero.
 __device__ __forceinline__ uint64_t ex2_poly2(float2 v) {
-  // -126 and below stay normal numbers: what they round to in 16 bits is nothing
-  const uint64_t x = f2_pack(fmaxf(v.x, -126.0f), fmaxf(v.y, -126.0f));
+  // n = -127, f = 0 make the polynomial 1, whose exponent field the addition clears. Down to
+  // there f is not negative, so the field does not wrap: what is below 2^-126 comes out as
+  // some number from zero to that.
+  const uint64_t x = f2_pack(fmaxf(v.x, -127.0f), fmaxf(v.y, -127.0f));
   const uint64_t magic = f2_splat(12582912.0f);  // 1.5 x 2^23: adding it leaves the nearest integer in the low bits
   const uint64_t t = f2_add(x, magic);
   const uint64_t f = f2_add(x, f2_fma(t, f2_splat(-1.0f), magic));
-  uint64_t r = f2_fma(f, f2_splat(0.009570102207362652f), f2_splat(0.05591785907745361f));
-  r = f2_fma(r, f, f2_splat(0.240247443318367f));
-  r = f2_fma(r, f, f2_splat(0.6931217908859253f));
-  r = f2_fma(r, f, f2_splat(0.9999992847442627f));
+  uint64_t r = f2_fma(f, f2_splat(0.009582852944731712f), f2_splat(0.055906426161527634f));
+  r = f2_fma(r, f, f2_splat(0.24024099111557007f));
+  r = f2_fma(r, f, f2_splat(0.6931241750717163f));
+  r = f2_fma(r, f, f2_splat(1.0f));
   const float2 tf = f2_unpack(t), rf = f2_unpack(r);
   return f2_pack(__int_as_float(__float_as_int(rf.x) + (__float_as_int(tf.x) << 23)),
                  __int_as_float(__float_as_int(rf.y) + (__float_as_int(tf.y) << 23)));
 }
 
 // P = 2^(c s - cm) of 32 keys to TMEM at `to`, 16 columns; returns the sums of the
-// unrounded weights (two of them, to be added). With EMULATE the least weight is
-// 2^-126, not zero, a masked key's too: the caller takes a row's sum of such
-// weights alone for none. (A second copy of the code without it for masked
-// blocks costs 4 %: the instructions no longer stay near.)
+// unrounded weights (two of them, to be added). A masked key, whose score is
+// -infinity, weighs exactly zero either way.
 template <typename T, bool EMULATE>
 __device__ __forceinline__ uint64_t weights_32(const float* s, uint64_t c2, uint64_t minus_cm2, uint32_t to) {
   uint64_t sum[2] = {0ull, 0ull};
