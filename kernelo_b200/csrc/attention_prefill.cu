@@ -502,6 +502,9 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
         }
         const float cm = m == -INFINITY ? 0.0f : m * c;
+        // NaN among the row's scores, or infinity: the row is NaN (`m` need not have been raised, and
+        // the polynomial takes NaN for zero)
+        if (!(m_new * c < INFINITY)) l = NAN;
         l += row_weights<T, true>(s, c, cm, s_addr, p_half + 8 * t, p_full + 8 * t, lane);
       }
       done += blocks;

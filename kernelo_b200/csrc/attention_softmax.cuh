@@ -16,9 +16,15 @@
 
 namespace kf {
 
+// Maxima that a NaN among their operands makes NaN.
+__device__ __forceinline__ float max2(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 
@@ -31,22 +37,23 @@ __device__ __forceinline__ void tmem_st_16(uint32_t taddr, const uint32_t* r) {
       : "memory");
 }
 
-// The largest of `m` and the row's scores.
+// The largest of `m` and the row's scores; NaN if one of them is.
 __device__ __forceinline__ float row_max(const float (&s)[128], float m) {
   float top[4] = {m, s[0], s[1], s[2]};
-  top[0] = fmaxf(top[0], s[3]);
+  top[0] = max2(top[0], s[3]);
 #pragma unroll
   for (int x = 4; x < 124; x += 8) {
 #pragma unroll
     for (int y = 0; y < 4; ++y) top[y] = max3(top[y], s[x + y], s[x + 4 + y]);
   }
 #pragma unroll
-  for (int y = 0; y < 4; ++y) top[y] = fmaxf(top[y], s[124 + y]);
-  return fmaxf(max3(top[0], top[1], top[2]), top[3]);
+  for (int y = 0; y < 4; ++y) top[y] = max2(top[y], s[124 + y]);
+  return max2(max3(top[0], top[1], top[2]), top[3]);
 }
 
 // 2^x of two values without the special-function unit; x = -127 and below (a key
-// that the row does not see) give exactly zero.
+// that the row does not see) give exactly zero, and so does NaN: a row that has
+// one is known by its maximum.
 __device__ __forceinline__ uint64_t ex2_poly2(float2 v) {
   // n = -127, f = 0 make the polynomial 1, whose exponent field the addition clears. Down to
   // there f is not negative, so the field does not wrap: what is below 2^-126 comes out as

@@ -39,3 +39,55 @@ def test_an_unseen_large_value_weighs_nothing(dim, dtype, device):
         large[key] = LARGE[dtype]
         out, lse = prefill_attention(q, k, large, cu, return_lse=True)
         check_rows(slice(0, key), out, lse, want, want_lse, bound, off, f"{dtype} key {key}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("causal", [True, False])
+def test_a_seen_nan_key_makes_a_row_nan(causal, dim, dtype, device):
+    lens = (300, 40)
+    q, k, v, cu, _ = prompt(lens, lens, 2, 1, dim, dtype, device)
+    want, want_lse, bound, off = ref.packed(q, k, v, lens, lens, causal=causal)
+    for key in (*range(0, 8), *range(40, 48), *range(200, 208), 299):
+        broken = k.clone()
+        broken[key, 0, 3] = torch.nan
+        out, lse = prefill_attention(q, broken, v, cu, causal=causal, return_lse=True)
+        first = key if causal else 0
+        assert out[first:300].isnan().all() and lse[first:300].isnan().all(), f"{dtype} key {key}"
+        fine = [*range(first), *range(300, 340)]
+        check_rows(fine, out, lse, want, want_lse, bound, off, f"{dtype} key {key}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_infinite_scores_of_a_prompt(dim, dtype, device):
+    """A key of +infinity in one element: NaN where the query's element is positive, no weight where it is negative."""
+    lens = (300,)
+    q, k, v, cu, _ = prompt(lens, lens, 2, 1, dim, dtype, device)
+    q[:, :, 3] = torch.where(q[:, :, 3] == 0, torch.ones_like(q[:, :, 3]), q[:, :, 3])
+    for key in (*range(0, 8), *range(200, 208)):
+        broken = k.clone()
+        broken[key, 0, 3] = torch.inf
+        out, lse = prefill_attention(q, broken, v, cu, return_lse=True)
+        at = torch.arange(300, device=device)
+        for h in range(2):
+            up = (at >= key) & (q[:, h, 3] > 0)
+            assert out[up, h].isnan().all() and not (lse[up, h] < torch.inf).any(), f"{dtype} key {key}"
+            seen = at[None, :] <= at[:, None]
+            seen[:, key] = False  # a score of -infinity
+            want, want_lse, bound, off = ref.attend(q[:, h], k[:, 0], v[:, 0], seen, dim ** -0.5)
+            check_rows(~up, out[:, h], lse[:, h], want, want_lse, bound, off, f"{dtype} key {key}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_nan_query_of_a_prompt(dtype, device):
+    lens = (300, 7)
+    q, k, v, cu, _ = prompt(lens, lens, 4, 2, 64, dtype, device)
+    want, want_lse, bound, off = ref.packed(q, k, v, lens, lens)
+    rows = torch.tensor([0, 5, 130, 299, 303], device=device)
+    q[rows, 1, 2] = torch.nan
+    out, lse = prefill_attention(q, k, v, cu, return_lse=True)
+    hit = torch.zeros(307, 4, dtype=torch.bool, device=device)
+    hit[rows, 1] = True
+    assert out[hit].isnan().all() and lse[hit].isnan().all()
+    check_rows(~hit, out, lse, want, want_lse, bound, off, f"{dtype}")
