@@ -291,9 +291,10 @@ struct Sums8 {
     for (int i = 0; i < 8; ++i) o[i] *= old;
     m = top;
   }
-  __device__ __forceinline__ void add(float pm, float pl, const float (&e)[8]) {  // pm <= m
+  // pm <= m. A part that weighs nothing is added like any other: its sums are NaN
+  // where its scores or values are (with all scores NaN its maximum is -infinity).
+  __device__ __forceinline__ void add(float pm, float pl, const float (&e)[8]) {
     const float fix = pm == -INFINITY ? 0.0f : ex2_ftz(pm - m);
-    if (fix == 0.0f) return;
     l = fmaf(pl, fix, l);
 #pragma unroll
     for (int i = 0; i < 8; ++i) o[i] = fmaf(e[i], fix, o[i]);

@@ -12,9 +12,9 @@ from __future__ import annotations
 import pytest
 import torch
 
-from kernelo_b200.kernels.attention import prefill_attention
+from kernelo_b200.kernels.attention import prefill_attention, tree_attention
 from tests import attention_reference as ref
-from tests.test_attention_gpu import DTYPES, prompt
+from tests.test_attention_gpu import DTYPES, HALF, cache, offsets, prompt, random_trees
 
 pytestmark = pytest.mark.gpu
 
@@ -91,3 +91,69 @@ def test_a_nan_query_of_a_prompt(dtype, device):
     hit[rows, 1] = True
     assert out[hit].isnan().all() and lse[hit].isnan().all()
     check_rows(~hit, out, lse, want, want_lse, bound, off, f"{dtype}")
+
+
+# ------------------------------------------------------------------ paged caches
+# (query heads, key heads, nodes): tiles of 16 rows and of 128; contexts that are cut over many CTAs and that are not
+CUTS = [((33000,), 1), ((33000,), 16), ((20000, 40, 9001), 1), ((20000, 40, 9001), 9), ((50, 3), 2)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("context,count", CUTS)
+def test_a_nan_query_over_a_cache(context, count, dtype, device):
+    """The same answer whether the row's keys lie in one CTA's share or in many."""
+    nodes = (count,) * len(context)
+    masks, words = random_trees(nodes)
+    q, k, v, table, lens = cache(context, nodes, 8, 2, 128, 32, dtype, device)
+    want, want_lse, bound, off = ref.paged(q, k, v, table, context, nodes, masks)
+    hit = torch.zeros(q.shape[:2], dtype=torch.bool, device=device)
+    for r in range(len(context)):
+        hit[r * count + count // 2, r % 8] = True
+    q[..., 3] = torch.where(hit, torch.nan, q[..., 3].float()).to(dtype)
+    out, lse = tree_attention(q, k, v, table, lens, offsets(nodes, device), words.to(device), return_lse=True)
+    assert out[hit].isnan().all() and lse[hit].isnan().all()
+    check_rows(~hit, out, lse, want, want_lse, bound, off, f"{dtype} {context} {count}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("count", [1, 16])
+def test_a_stretch_of_nan_keys_in_a_long_cache(count, dtype, device):
+    """Whole shares of the cache in which every score is NaN, and a single key; other requests are untouched."""
+    context, nodes = (33000, 500), (count, count)
+    masks, words = random_trees(nodes)
+    q, k, v, table, lens = cache(context, nodes, 8, 2, 128, 32, dtype, device)
+    want, want_lse, bound, off = ref.paged(q, k, v, table, context, nodes, masks)
+    for pages in (slice(300, 700), slice(500, 501)):
+        broken = k.clone()
+        broken[table[0, pages].long(), 1] = torch.nan  # of the second key head
+        out, lse = tree_attention(q, broken, v, table, lens, offsets(nodes, device), words.to(device), return_lse=True)
+        assert out[:count, 4:].isnan().all() and lse[:count, 4:].isnan().all()
+        hit = torch.zeros(q.shape[:2], dtype=torch.bool, device=device)
+        hit[:count, 4:] = True
+        check_rows(~hit, out, lse, want, want_lse, bound, off, f"{dtype} {pages}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("count", [1, 16])
+def test_infinite_scores_over_a_cache(count, dtype, device):
+    context, nodes = (9000, 60), (count, count)
+    q, k, v, table, lens = cache(context, nodes, 8, 2, 128, 16, dtype, device)
+    masks = [torch.ones(count, count, dtype=torch.bool).tril() for _ in nodes]
+    q[..., 3] = torch.where(q[..., 3] == 0, torch.ones_like(q[..., 3]), q[..., 3])
+    broken = k.clone()
+    for r, place in ((0, 4001), (1, 38)):
+        broken[table[r, place // 16].long(), :, place % 16, 3] = torch.inf
+    out, lse = tree_attention(q, broken, v, table, lens, offsets(nodes, device), return_lse=True)
+    up = q[..., 3] > 0
+    assert out[up].isnan().all() and not (lse[up] < torch.inf).any()
+    for r, place in ((0, 4001), (1, 38)):
+        at = torch.arange(context[r] + count, device=device)
+        page = table[r].long()[at // 16]
+        seen = torch.ones(count, context[r] + count, dtype=torch.bool, device=device)
+        seen[:, context[r]:] = masks[r].to(device)
+        seen[:, place] = False
+        rows = slice(r * count, (r + 1) * count)
+        for h in range(8):
+            want, want_lse, bound, off = ref.attend(q[rows, h], k[page, h // 4, at % 16], v[page, h // 4, at % 16], seen,
+                                                    128 ** -0.5)
+            check_rows(~up[rows, h], out[rows, h], lse[rows, h], want, want_lse, bound, off, f"{dtype} head {h}")
