@@ -180,6 +180,10 @@ KF_API int32_t kf_sm_count(int32_t device);
  * *out receives KF_OK or KF_ERR_TIMEOUT with the kernel site in the high bits. */
 KF_API int32_t kf_device_status(int32_t device, int32_t* out);
 
+/* *id receives the number of the capture that `stream` is in (calls captured into one
+ * CUDA graph share it), 0 where it is in none. */
+KF_API int32_t kf_stream_capture_id(void* stream, int64_t* id);
+
 /* ---- GEMM: C[M,N] = A[M,K] . B[K,N] --------------------------------------- *
  * Strides are in elements: A(m,k) = a[m*sa_m + k*sa_k], B(k,n) = b[k*sb_k + n*sb_n],
  * C(m,n) = c[m*sc_m + n*sc_n]. Accumulation is fp32; C has the operand dtype.

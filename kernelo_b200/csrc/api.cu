@@ -531,6 +531,16 @@ int32_t kf_device_status(int32_t device, int32_t* out) {
   return KF_OK;
 }
 
+int32_t kf_stream_capture_id(void* stream, int64_t* id) {
+  if (id == nullptr) return set_error(KF_ERR_INVALID_ARGUMENT, "null id pointer");
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long n = 0;
+  const cudaError_t err = cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &status, &n);
+  if (err != cudaSuccess) return cuda_error(err, "kf_stream_capture_id");
+  *id = status == cudaStreamCaptureStatusActive ? static_cast<int64_t>(n) : 0;
+  return KF_OK;
+}
+
 int32_t kf_gemm(int32_t dtype, const void* a, int64_t sa_m, int64_t sa_k, const void* b,
                 int64_t sb_k, int64_t sb_n, void* c, int64_t sc_m, int64_t sc_n, int64_t M,
                 int64_t N, int64_t K, const kf_gemm_config* cfg, void* workspace,

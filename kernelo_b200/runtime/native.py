@@ -56,6 +56,7 @@ EXPORTED_SYMBOLS = (
     "kf_last_error",
     "kf_sm_count",
     "kf_device_status",
+    "kf_stream_capture_id",
     "kf_gemm",
     "kf_linear_bias_act",
     "kf_gemv",
@@ -207,6 +208,7 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "kf_tree_attention": (_i32, [_packed, _vp]),
     "kf_tree_attention_workspace_bytes": (_i64, [_i32, _i32, _i64, _i64, _i64, _i64, _i64]),
     "kf_rotary": (_i32, [_packed, _vp]),
+    "kf_stream_capture_id": (_i32, [_vp, ctypes.POINTER(_i64)]),
     "kf_build_slots": (_i32, [_packed, _vp]),
 }
 
@@ -395,20 +397,39 @@ def query_gemm_config(dtype: torch.dtype, launch: GemmLaunch) -> tuple[int, int,
 class _WorkspacePool:
     """Zero-initialised workspaces, one per (device, stream), grown on demand.
 
-    Stream-K kernels leave their counters at zero when they finish, so a
-    workspace is reused without re-clearing. Calls on one stream are ordered,
+    Kernels that keep counters in a workspace leave them at zero when they
+    finish, so it is reused without re-clearing. Calls on one stream are ordered,
     so sharing within a stream is safe; different streams get different buffers.
+
+    Calls captured into a CUDA graph get a workspace of that graph's own, in the
+    graph's memory, whose counters a node of the graph clears: graphs may be
+    replayed in any order and beside one another and other calls, and a
+    workspace that grows frees nothing that a graph still uses.
     """
+
+    COUNTER_BYTES = 64 * 1024  # every layout begins with its counters; only they have to be zero
 
     def __init__(self) -> None:
         self._buffers: dict[tuple[int, int], torch.Tensor] = {}
+        # of captures that may still be going on: (capture, buffer)
+        self._captured: dict[tuple[int, int], tuple[int, torch.Tensor]] = {}
         self._lock = threading.Lock()
 
     def get(self, device: torch.device, stream: int, nbytes: int) -> torch.Tensor | None:
         if nbytes <= 0:
             return None
         key = (device.index if device.index is not None else torch.cuda.current_device(), stream)
+        capture = _capture_id(stream)
         with self._lock:
+            if capture:
+                held, buf = self._captured.get(key, (0, None))
+                if held != capture or buf.numel() < nbytes:
+                    # one that is given up here goes back to the graph's memory, for what the graph does later
+                    buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
+                    buf[:self.COUNTER_BYTES].zero_()
+                    self._captured[key] = (capture, buf)
+                return buf
+            self._captured.clear()
             buf = self._buffers.get(key)
             if buf is None or buf.numel() < nbytes:
                 size = max(nbytes, 0 if buf is None else 2 * buf.numel())
@@ -420,6 +441,16 @@ class _WorkspacePool:
         """Drop every workspace (after a device error left counters unknown)."""
         with self._lock:
             self._buffers.clear()
+            self._captured.clear()
+
+
+def _capture_id(stream: int) -> int:
+    """The capture that the device's current stream, ``stream``, is in; 0 for none."""
+    if not torch.cuda.is_current_stream_capturing():
+        return 0
+    out = ctypes.c_int64(0)
+    check(load().kf_stream_capture_id(stream, ctypes.byref(out)), "kf_stream_capture_id")
+    return out.value
 
 
 workspaces = _WorkspacePool()
