@@ -86,6 +86,8 @@ int32_t kf_tree_attention(const kf_tree_args* args, void* stream) {
       (g.seqs > 0 && g.table_cols > 0 && g.block_table == nullptr) ||
       (g.pages > 0 && (g.k_cache == nullptr || g.v_cache == nullptr)) || (g.mask_words > 0 && g.tree_mask == nullptr))
     return invalid("null pointer");
+  if ((reinterpret_cast<uintptr_t>(g.workspace) & 255u) != 0)
+    return set_error(KF_ERR_WORKSPACE, "workspace must be 256-byte aligned");
   DeviceInfo* dev = nullptr;
   rc = this_device(&dev);
   if (rc != KF_OK) return rc;

@@ -106,3 +106,20 @@ def test_rotary_table_scalings():
 def test_rotary_table_refusals(kw, message):
     with pytest.raises(ValueError, match=message):
         rotary_table(**(dict(max_positions=10, rotary_dim=16, device="cpu") | kw))
+
+
+def test_a_workspace_off_its_alignment_is_refused_on_the_host():
+    """Partial results are moved 16 bytes at a time: an address between would fault."""
+    if torch.cuda.is_available():
+        pytest.skip("the addresses are made up: only where nothing can be launched")
+    lib = native.load()
+    names = ("dtype q sq_row sq_head k_cache sk_page sk_head sk_slot v_cache sv_page sv_head sv_slot out so_row so_head lse "
+             "block_table table_stride table_cols pages block_size context cu_q tree_mask mask_words seqs rows heads "
+             "kv_heads dim scale workspace workspace_bytes").split()
+    values = dict.fromkeys(names, 0) | dict(heads=4, kv_heads=2, dim=64, scale=1.0, block_size=16, rows=1, seqs=1, pages=1,
+                                            table_cols=1, workspace_bytes=1 << 30)
+    values |= dict.fromkeys(("q", "k_cache", "v_cache", "out", "block_table", "context"), 4096)  # never read here
+    for off in (1, 8, 16, 128):
+        packed = native.TREE_ARGS.pack(*((values | dict(workspace=4096 + off))[n] for n in names))
+        assert lib.kf_tree_attention(packed, None) == native.KF_ERR_WORKSPACE
+        assert "256-byte aligned" in native.last_error()
