@@ -68,6 +68,21 @@ __device__ __forceinline__ long long key_offset(const AttnArgs& p, int r, long l
   return page * s_page + (pos - col * p.block_size) * s_row;
 }
 
+// A wait of a kernel whose rows may be computed again beside it (redo_begin).
+__device__ __forceinline__ bool attn_wait(uint32_t bar, uint32_t parity, volatile int* flag, int* status, int site) {
+  return mbar_wait<true>(bar, parity, flag, status, site);
+}
+// Around rows that a warp computes again, whose time goes by their keys: the other
+// warps' waits do not run out meanwhile. `flag` is the CTA's abort flag.
+__device__ __forceinline__ void redo_begin(volatile int* flag, int lane) {
+  if (lane == 0) atomicAdd(const_cast<int*>(flag), 2);
+  __syncwarp();
+}
+__device__ __forceinline__ void redo_end(volatile int* flag, int lane) {
+  __syncwarp();
+  if (lane == 0) atomicAdd(const_cast<int*>(flag), -2);
+}
+
 // One row of attention by one warp, key by key: for lane's elements
 // e = lane + 32 i of the head, acc = sum_j p_j v_j with the running maximum m
 // and sum l of the softmax in base 2 (q is read times scale * log2(e)). Keys that

@@ -270,13 +270,15 @@ __device__ __forceinline__ void store_lse(const AttnArgs& p, int t, int head, fl
 
 // Rows that came out non-finite, key by key: `bad` and the row of each lane.
 template <typename T, int NE>
-__device__ __forceinline__ void redo_rows(const AttnArgs& p, bool bad, int t, int head, int lane) {
+__device__ __forceinline__ void redo_rows(const AttnArgs& p, bool bad, int t, int head, int lane, volatile int* flag) {
   uint32_t again = __ballot_sync(0xffffffffu, bad);
+  if (again != 0) redo_begin(flag, lane);
   while (again != 0) {
     const int src = __ffs(again) - 1;
     const int row = __shfl_sync(0xffffffffu, t, src), h = __shfl_sync(0xffffffffu, head, src);
     redo_row<T, NE>(p, row, h, lane);
     again &= ~__ballot_sync(0xffffffffu, t == row && head == h);
+    if (again == 0) redo_end(flag, lane);
   }
 }
 
@@ -308,7 +310,7 @@ struct Sums8 {
 // of the sums goes by the numbers alone.
 template <typename T, int M, int DP, int THREADS, typename Barrier>
 __device__ __forceinline__ void join_partials(const AttnArgs& p, const Cursor& c, const TileRows& tile, int owner, int last,
-                                              int tid, int vector_out, float* scratch, Barrier barrier) {
+                                              int tid, int vector_out, float* scratch, volatile int* flag, Barrier barrier) {
   constexpr int LANES = DP / 8, PASS = THREADS / LANES;
   const int col = (tid % LANES) * 8;
   int share = 1;  // threads to a row's CTAs
@@ -375,7 +377,7 @@ __device__ __forceinline__ void join_partials(const AttnArgs& p, const Cursor& c
       if (col < p.dim) bad = store_8<T>(p, t, head, col, sums.o, sums.l, vector_out);
       if (col == 0) store_lse(p, t, head, sums.m, sums.l);
     }
-    redo_rows<T, DP / 32>(p, bad, t, head, threadIdx.x & 31);
+    redo_rows<T, DP / 32>(p, bad, t, head, threadIdx.x & 31, flag);
   }
 }
 

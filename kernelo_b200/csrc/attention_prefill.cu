@@ -242,7 +242,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   // every barrier below is waited for phase by phase.
   auto next_item = [&](int n, int site) {
     Item it;
-    const bool ok = __all_sync(0xffffffffu, mbar_wait(item_bar + 8 * (n & 1), (n >> 1) & 1, abort_flag, status, site));
+    const bool ok = __all_sync(0xffffffffu, attn_wait(item_bar + 8 * (n & 1), (n >> 1) & 1, abort_flag, status, site));
     it = items[n & 1];
     __syncwarp();
     if (lane == 0) mbar_arrive(item_free + 8 * (n & 1));
@@ -266,7 +266,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       for (int n = 0;; ++n) {
         const long long i = static_cast<long long>(n) * ctas + (n & 1 ? ctas - 1 - me : me);
         const bool ok = __all_sync(
-            0xffffffffu, mbar_wait(item_free + 8 * (n & 1), ((n >> 1) & 1) ^ 1, abort_flag, status, SITE_ATTN_LOAD));
+            0xffffffffu, attn_wait(item_free + 8 * (n & 1), ((n >> 1) & 1) ^ 1, abort_flag, status, SITE_ATTN_LOAD));
         Item* it = &items[n & 1];
         const int g = static_cast<int>(i / heads);
         const bool found = ok && (ordered ? order.find(p, g, lane, it) : find_item(p, g, lane, it));
@@ -302,13 +302,13 @@ __global__ void __launch_bounds__(THREADS, 1)
           const int kv_head = it.head / static_cast<int>(p.heads / p.kv_heads);
           auto next = [&](const CUtensorMap* map, int block) {
             const int slot = issued % STAGES;
-            if (!mbar_wait(empty + 8 * slot, ((issued / STAGES) & 1) ^ 1, abort_flag, status, SITE_ATTN_LOAD)) return false;
+            if (!attn_wait(empty + 8 * slot, ((issued / STAGES) & 1) ^ 1, abort_flag, status, SITE_ATTN_LOAD)) return false;
             load(smem_u32(ring + slot * S::TILE), map, full + 8 * slot, kv_head, it.first_key + block * BLK);
             ++issued;
             return true;
           };
           auto query = [&](int t) {
-            if (!mbar_wait(q_free + 8 * t, (loaded & 1) ^ 1, abort_flag, status, SITE_ATTN_LOAD)) return false;
+            if (!attn_wait(q_free + 8 * t, (loaded & 1) ^ 1, abort_flag, status, SITE_ATTN_LOAD)) return false;
             load(smem_u32(q_tiles + t * S::TILE), &tm_q, q_bar + 8 * t, it.head, it.row0 + t * BLK);
             return true;
           };
@@ -339,7 +339,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         tiles += 2 * most;
         const int held = it.keys - (most - 1) * BLK, slot = (tiles - 1) % STAGES;
         if (held >= BLK) continue;
-        if (!__all_sync(0xffffffffu, mbar_wait(dirty, cleaned & 1, abort_flag, status, SITE_ATTN_LOAD))) break;
+        if (!__all_sync(0xffffffffu, attn_wait(dirty, cleaned & 1, abort_flag, status, SITE_ATTN_LOAD))) break;
         for (int i = lane; i < (BLK - held) * S::HALVES * 8; i += 32) {
           const int h = i / ((BLK - held) * 8), rest = i - h * (BLK - held) * 8;
           *reinterpret_cast<uint4*>(ring + slot * S::TILE + h * BLK * 128 + held * 128 + rest * 16) =
@@ -369,7 +369,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       bool ok = true;
       auto wait = [&](uint32_t bar, int parity) {
         if (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity)))
-          ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, SITE_ATTN_MMA)) && ok;
+          ok = __all_sync(0xffffffffu, attn_wait(bar, parity, abort_flag, status, SITE_ATTN_MMA)) && ok;
         tc_fence_after();
       };
       auto wait_tile = [&]() {
@@ -468,7 +468,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       const int limit = valid ? visible(p, it, i) : 0;
       float m = -INFINITY, l = 0.0f;
       for (int j = 0; j < blocks; ++j) {
-        ok = mbar_wait(s_full + 8 * t, (done + j) & 1, abort_flag, status, SITE_ATTN_SOFTMAX);
+        ok = attn_wait(s_full + 8 * t, (done + j) & 1, abort_flag, status, SITE_ATTN_SOFTMAX);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
@@ -509,7 +509,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       done += blocks;
       if (ok && blocks > 0) {
-        ok = mbar_wait(o_full + 8 * t, results & 1, abort_flag, status, SITE_ATTN_SOFTMAX);
+        ok = attn_wait(o_full + 8 * t, results & 1, abort_flag, status, SITE_ATTN_SOFTMAX);
         ok = __all_sync(0xffffffffu, ok);
         tc_fence_after();
         ++results;
@@ -558,10 +558,12 @@ __global__ void __launch_bounds__(THREADS, 1)
             l > 0.0f ? m * c * 0.69314718055994530942f + logf(l) : -INFINITY;
       // l that is NaN (a score is) has left zeros: those rows too
       uint32_t again = __ballot_sync(0xffffffffu, valid && (!(bad == 0.0f) || !(l >= 0.0f && l < INFINITY)));
+      if (again != 0) redo_begin(abort_flag, lane);
       while (again != 0) {
         const int src = __ffs(again) - 1;
         again &= again - 1;
         redo_row<T, DH>(p, __shfl_sync(0xffffffffu, q_row, src), it.head, lane);
+        if (again == 0) redo_end(abort_flag, lane);
       }
     }
   }

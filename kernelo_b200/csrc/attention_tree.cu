@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(THREADS, 2)
     bool fresh = true;
     while (at.left > 0) {
       if (fresh) {  // the item's queries
-        mbar_wait(q_empty, (items & 1) ^ 1, abort_flag, status, SITE_ATTN_LOAD);
+        attn_wait(q_empty, (items & 1) ^ 1, abort_flag, status, SITE_ATTN_LOAD);
         __syncwarp();
         const TileRows tile(p, walk, at);
         const uint32_t dst = smem_u32(q_tile);
@@ -215,7 +215,7 @@ __global__ void __launch_bounds__(THREADS, 2)
         }
         bits[0] = __reduce_or_sync(0xffffffffu, bits[0]);
         bits[1] = __reduce_or_sync(0xffffffffu, bits[1]);
-        mbar_wait(empty + 8 * slot, phase, abort_flag, status, SITE_ATTN_LOAD);
+        attn_wait(empty + 8 * slot, phase, abort_flag, status, SITE_ATTN_LOAD);
         __syncwarp();
         if (lane == 0) {
           present[2 * slot] = bits[0];
@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(THREADS, 2)
           page[i] = page_of(p, by_page, at, pos0 + lane + 32 * i, &in_page[i]);
           bits[i] = __ballot_sync(0xffffffffu, page[i] >= 0);
         }
-        mbar_wait(empty + 8 * slot, phase, abort_flag, status, SITE_ATTN_LOAD);
+        attn_wait(empty + 8 * slot, phase, abort_flag, status, SITE_ATTN_LOAD);
         __syncwarp();
         if (lane < 2) present[2 * slot + lane] = bits[lane];
 #pragma unroll
@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(THREADS, 2)
       fresh = walk.item_ends(at);
       walk.advance(p, at);
     }
-    if (*abort_flag) {
+    if (*abort_flag & 1) {
       // a wait gave up: let the copies in flight land before the shared memory goes away
       asm volatile("cp.async.wait_all;" ::: "memory");
       for (int s = 0; s < STAGES && s < blocks; ++s)
@@ -288,7 +288,7 @@ __global__ void __launch_bounds__(THREADS, 2)
   while (at.left > 0) {
     if (fresh) {
       fresh = false;
-      mbar_wait(q_full, items & 1, abort_flag, status, SITE_ATTN_SOFTMAX);
+      attn_wait(q_full, items & 1, abort_flag, status, SITE_ATTN_SOFTMAX);
       __syncwarp();
 #pragma unroll
       for (int k = 0; k < DP / 16; ++k)
@@ -304,7 +304,7 @@ __global__ void __launch_bounds__(THREADS, 2)
 #pragma unroll
       for (int n = 0; n < DP / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
     }
-    mbar_wait(full + 8 * stage, phase, abort_flag, status, SITE_ATTN_SOFTMAX);
+    attn_wait(full + 8 * stage, phase, abort_flag, status, SITE_ATTN_SOFTMAX);
     __syncwarp();
     const uint32_t tile_at = ring + stage * 2 * S::TILE;
     // two sums for each half of the head: their products wait less for one another
@@ -480,7 +480,7 @@ __global__ void __launch_bounds__(THREADS, 2)
           }
         }
       }
-      redo_rows<T, DP / 32>(p, bad, t, head, lane);
+      redo_rows<T, DP / 32>(p, bad, t, head, lane, abort_flag);
     }
     if (!whole && defer && item < 0) {
       asm volatile("bar.arrive 2, %0;" ::"n"(32 * (WARPS + 1)) : "memory");
@@ -494,7 +494,7 @@ __global__ void __launch_bounds__(THREADS, 2)
       join();
       if (last_one) {
         __threadfence();
-        join_partials<T, M, DP, 32 * WARPS>(p, at, tile, owner, last, tid, vector_out, DP >= 64 ? joined : nullptr, join);
+        join_partials<T, M, DP, 32 * WARPS>(p, at, tile, owner, last, tid, vector_out, DP >= 64 ? joined : nullptr, abort_flag, join);
         if (tid == 0) counters[owner] = 0;
       }
     }
@@ -502,12 +502,12 @@ __global__ void __launch_bounds__(THREADS, 2)
     walk.advance(p, at);
   }
   if (defer) {
-    mbar_wait(finished, 0, abort_flag, status, SITE_ATTN_SOFTMAX);
+    attn_wait(finished, 0, abort_flag, status, SITE_ATTN_SOFTMAX);
     if (first_is_last) {
       __threadfence();
       const Cursor c = first_item;
       join_partials<T, M, DP, 32 * WARPS>(p, c, TileRows(p, walk, c), first_owner, first_last, tid, vector_out,
-                                          DP >= 64 ? joined : nullptr, join);
+                                          DP >= 64 ? joined : nullptr, abort_flag, join);
       if (tid == 0) static_cast<int*>(p.workspace)[first_owner] = 0;
     }
   }

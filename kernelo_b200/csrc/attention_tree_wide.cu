@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     const bool mine = lane * box_rows < KEYS;
     auto load = [&](const CUtensorMap* map, int page, int slot_in_page, int head) {
       const int slot = issued % STAGES;
-      mbar_wait(empty + 8 * slot, ((issued / STAGES) & 1) ^ 1, abort_flag, status, SITE_ATTN_LOAD);
+      attn_wait(empty + 8 * slot, ((issued / STAGES) & 1) ^ 1, abort_flag, status, SITE_ATTN_LOAD);
       __syncwarp();
       if (lane == 0) mbar_arrive_expect_tx(full + 8 * slot, S::TILE);
       __syncwarp();
@@ -135,7 +135,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     while (at.left > 0) {
       if (fresh) {
         const int buf = items & 1;
-        mbar_wait(q_empty + 8 * buf, ((items >> 1) & 1) ^ 1, abort_flag, status, SITE_ATTN_LOAD);
+        attn_wait(q_empty + 8 * buf, ((items >> 1) & 1) ^ 1, abort_flag, status, SITE_ATTN_LOAD);
         __syncwarp();
         if (lane == 0) {
           const TileRows tile(p, walk, at);
@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       walk.advance(p, at);
     }
     load(&tm_v, v_page, v_slot, v_head);
-    if (*abort_flag) {  // let the copies in flight land before the shared memory goes away
+    if (*abort_flag & 1) {  // let the copies in flight land before the shared memory goes away
       for (int i = 0; i < 2 && i < items; ++i)
         mbar_wait(q_full + 8 * i, ((items - 1 - i) >> 1) & 1, nullptr, status, SITE_DRAIN, DRAIN_NS);
       for (int s = 0; s < STAGES && s < issued; ++s)
@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     const uint32_t idesc_s = instr_desc_f16(fmt, 0, 0, M, KEYS), idesc_o = instr_desc_f16(fmt, 0, 1, M, DP);
     int taken = 0, items = 0, unit = 0;
     auto wait = [&](uint32_t bar, int parity) {
-      mbar_wait(bar, parity, abort_flag, status, SITE_ATTN_MMA);
+      attn_wait(bar, parity, abort_flag, status, SITE_ATTN_MMA);
       __syncwarp();
       tc_fence_after();
     };
@@ -278,11 +278,11 @@ __global__ void __launch_bounds__(THREADS, 1)
         l = 0.0f;
         real = TileRows(p, walk, at).find(row, &node, &head);
       }
-      mbar_wait(info + 8 * (unit % INFO), (unit / INFO) & 1, abort_flag, status, SITE_ATTN_SOFTMAX);
-      mbar_wait(s_full + 8 * (unit & 1), (unit >> 1) & 1, abort_flag, status, SITE_ATTN_SOFTMAX);
+      attn_wait(info + 8 * (unit % INFO), (unit / INFO) & 1, abort_flag, status, SITE_ATTN_SOFTMAX);
+      attn_wait(s_full + 8 * (unit & 1), (unit >> 1) & 1, abort_flag, status, SITE_ATTN_SOFTMAX);
       // A parity says "done" of the phase before the last one too, so no phase of
       // o_done may be skipped; S of this block was issued behind those products.
-      if (unit >= 2) mbar_wait(o_done + 8 * (unit & 1), ((unit >> 1) - 1) & 1, abort_flag, status, SITE_ATTN_SOFTMAX);
+      if (unit >= 2) attn_wait(o_done + 8 * (unit & 1), ((unit >> 1) - 1) & 1, abort_flag, status, SITE_ATTN_SOFTMAX);
       __syncwarp();
       tc_fence_after();
       float s[KEYS];
@@ -309,7 +309,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (first) {
         m = m_new;
       } else if (__any_sync(0xffffffffu, (m_new - m) * c > RAISE_LOG2)) {
-        mbar_wait(o_done + 8 * ((unit - 1) & 1), ((unit - 1) >> 1) & 1, abort_flag, status, SITE_ATTN_SOFTMAX);
+        attn_wait(o_done + 8 * ((unit - 1) & 1), ((unit - 1) >> 1) & 1, abort_flag, status, SITE_ATTN_SOFTMAX);
         __syncwarp();
         tc_fence_after();
         const float fix = m_new > m ? ex2_ftz((m - m_new) * c) : 1.0f;
@@ -334,7 +334,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
 
       // The item's last block of this run: its result, or its partial one.
-      mbar_wait(o_done + 8 * (unit & 1), (unit >> 1) & 1, abort_flag, status, SITE_ATTN_SOFTMAX);
+      attn_wait(o_done + 8 * (unit & 1), (unit >> 1) & 1, abort_flag, status, SITE_ATTN_SOFTMAX);
       __syncwarp();
       tc_fence_after();
       const int item = run.count - at.left - at.blk;
@@ -370,7 +370,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       ++items;
       if (whole) {
         if (real) store_lse(p, t, head, top2, l);
-        redo_rows<T, DP / 32>(p, bad, t, head, lane);
+        redo_rows<T, DP / 32>(p, bad, t, head, lane, abort_flag);
       } else {
         if (real) {
           __stcg(part.top(row), top2);
@@ -385,7 +385,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         join();
         if (last_one) {
           __threadfence();
-          join_partials<T, M, DP, 32 * SOFTMAX_WARPS>(p, at, TileRows(p, walk, at), owner, last, tid, vector_out, nullptr, join);
+          join_partials<T, M, DP, 32 * SOFTMAX_WARPS>(p, at, TileRows(p, walk, at), owner, last, tid, vector_out, nullptr, abort_flag, join);
           if (tid == 0) counters[owner] = 0;
         }
         join();

@@ -100,16 +100,22 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
 
 // Waits for the phase with the given parity to complete. Returns false when
 // the CTA's abort flag was raised or the time limit passed (which raises it).
+// BESIDE: the flag also counts, in steps of 2, warps of the CTA that are at work
+// which may take longer than the limit; it is counted from where there are none.
+template <bool BESIDE = false>
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag,
                                           int* status, int site,
                                           uint64_t limit_ns = KF_WAIT_LIMIT_NS) {
   if (mbar_try_wait(bar, parity)) return true;
-  const uint64_t start = global_timer_ns();
+  uint64_t start = global_timer_ns();
   for (uint32_t spin = 1;; ++spin) {
     if (mbar_try_wait(bar, parity)) return true;
     if ((spin & 7u) == 0) {
-      if (abort_flag != nullptr && *abort_flag) return false;
-      if (global_timer_ns() - start > limit_ns) {
+      const int flag = abort_flag != nullptr ? *abort_flag : 0;
+      if (BESIDE ? flag & 1 : flag) return false;
+      if (BESIDE && flag != 0) {
+        start = global_timer_ns();
+      } else if (global_timer_ns() - start > limit_ns) {
         record_status(status, KF_ERR_TIMEOUT, site);
         if (abort_flag != nullptr) *abort_flag = 1;
         return false;

@@ -13,6 +13,7 @@ import pytest
 import torch
 
 from kernelo_b200.kernels.attention import prefill_attention, tree_attention
+from kernelo_b200.runtime import native
 from tests import attention_reference as ref
 from tests.test_attention_gpu import DTYPES, HALF, cache, offsets, prompt, random_trees
 
@@ -157,3 +158,50 @@ def test_infinite_scores_over_a_cache(count, dtype, device):
             want, want_lse, bound, off = ref.attend(q[rows, h], k[page, h // 4, at % 16], v[page, h // 4, at % 16], seen,
                                                     128 ** -0.5)
             check_rows(~up[rows, h], out[rows, h], lse[rows, h], want, want_lse, bound, off, f"{dtype} head {h}")
+
+
+# ------------------------------------------------------- rows computed again
+def check_columns(got, want, bound, column, what):
+    """Every column but `column`, in which a seen value is infinite."""
+    keep = [e for e in range(got.shape[-1]) if e != column]
+    ref.check(got[..., keep], want[..., keep], bound[..., keep], what)
+    assert not got[..., column].isfinite().any(), what
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("count", [1, 16])
+def test_an_infinite_value_that_long_requests_see(count, dtype, device):
+    """All rows of a long cache are computed again, which takes its time: the waits beside it do not run out, and
+    neither the rows' other columns nor other requests lose anything."""
+    context, nodes = (131072, 300, 40), (count,) * 3
+    masks, words = random_trees(nodes)
+    q, k, v, table, lens = cache(context, nodes, 8, 2, 128, 32, dtype, device)
+    want, want_lse, bound, off = ref.paged(q, k, v, table, context, nodes, masks)
+    v[table[0, 5].long(), 0, 7, 9] = torch.inf  # of the first key head
+    native.device_status()
+    out, lse = tree_attention(q, k, v, table, lens, offsets(nodes, device), words.to(device), return_lse=True)
+    assert native.device_status() == 0
+    check_columns(out[:count, :4], want[:count, :4], bound[:count, :4], 9, f"{dtype}")
+    ref.check_lse(lse, want_lse, off, f"{dtype}")
+    ref.check(out[count:], want[count:], bound[count:], f"{dtype}")
+    ref.check(out[:count, 4:], want[:count, 4:], bound[:count, 4:], f"{dtype}")
+
+
+@pytest.mark.parametrize("dtype", HALF)
+def test_an_infinite_value_that_a_long_prompt_sees(dtype, device):
+    lens = (40000, 500)
+    q, k, v, cu, _ = prompt(lens, lens, 1, 1, 64, dtype, device)
+    v[3, 0, 9] = torch.inf
+    native.device_status()
+    out, lse = prefill_attention(q, k, v, cu, return_lse=True)
+    assert native.device_status() == 0
+    at = torch.arange(40000, device=device)
+    clean = v.clone()
+    clean[3, 0, 9] = 0.0
+    for rows in (slice(3, 130), slice(20000, 20100), slice(39900, 40000)):
+        want, want_lse, bound, off = ref.attend(q[rows, 0], k[:40000, 0], clean[:40000, 0], at[None, :] <= at[rows, None], 0.125)
+        check_columns(out[rows, 0], want, bound, 9, f"{dtype} {rows}")
+        ref.check_lse(lse[rows, 0], want_lse, off, f"{dtype} {rows}")
+    want, want_lse, bound, off = ref.packed(q[40000:], k[40000:], v[40000:], (500,), (500,))
+    ref.check(out[40000:], want, bound, f"{dtype}")
+    ref.check_lse(lse[40000:], want_lse, off, f"{dtype}")
