@@ -305,7 +305,10 @@ KF_API int32_t kf_rmsnorm_rows(int32_t dtype, const void* x, int64_t sx_row, con
  * Offsets and lengths are read on the device only, and clamped to the arrays
  * they index. A row that sees no key gets zeros and a log-sum-exp of -infinity,
  * and so do rows of q past the last offset. What a row does not see does not
- * reach it, whatever it holds (stale pages, infinities, NaN).
+ * reach it, whatever it holds (stale pages, infinities, NaN). Among the scores that
+ * it sees (q k^T in fp32, then the scale) NaN or +infinity makes a row and its
+ * log-sum-exp NaN; an infinite value makes its column infinite, or NaN where the
+ * value's weight rounds to zero.
  *
  * kf_prefill_attention: prompts of any lengths packed without padding. q and out
  * are [rows, heads, dim], k and v [keys, kv_heads, dim]; request r has the rows

@@ -224,6 +224,9 @@ __device__ __forceinline__ uint32_t nodes_seen(const AttnArgs& p, const Cursor& 
 
 template <typename T, int NE>
 __device__ __noinline__ void redo_row(const AttnArgs& p, int t, int head, int lane) {
+  // cached tokens are seen by all nodes, so only nodes can have done it
+  const RowKeys keys(p, t);
+  if (last_unseen_nonfinite<T, NE>(p, t, head, keys.prefix, keys.length, lane) < 0) return;
   float acc[NE], m, l;
   attend_row<T, NE>(p, t, head, lane, acc, &m, &l);
   write_row<T, NE>(p, t, head, lane, acc, m, l);
@@ -241,15 +244,16 @@ struct Partial {
   __device__ __forceinline__ float* sum(int r) const { return at + M * DP + M + r; }
 };
 
-// Writes 8 elements of a finished row, o / l, at column `col`; true if any is not finite.
+// Writes 8 elements of a finished row, o / l, at column `col`; true if the row has to be
+// computed again, if a key that it does not see did it.
 template <typename T>
 __device__ __forceinline__ bool store_8(const AttnArgs& p, int t, int head, int col, const float (&o)[8], float l,
                                         int vector_out) {
-  const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   float v[8], zero = 0.0f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    v[i] = l > 0.0f ? o[i] * inv : 0.0f;  // a row that sees nothing may hold anything
+    v[i] = l == 0.0f ? 0.0f : o[i] * inv;  // a row that sees nothing may hold anything
     zero = fmaf(v[i], 0.0f, zero);
   }
   T* out = static_cast<T*>(p.out) + static_cast<long long>(t) * p.so_t + head * p.so_h + col;
@@ -260,15 +264,15 @@ __device__ __forceinline__ bool store_8(const AttnArgs& p, int t, int head, int 
 #pragma unroll
     for (int i = 0; i < 8; ++i) out[i] = from_f32<T>(v[i]);
   }
-  return !(zero == 0.0f) || !(l >= 0.0f && l < INFINITY);
+  return suspect(zero == 0.0f, l);
 }
 
 __device__ __forceinline__ void store_lse(const AttnArgs& p, int t, int head, float m, float l) {
   if (p.lse != nullptr)
-    p.lse[static_cast<long long>(t) * p.heads + head] = l > 0.0f ? m * 0.69314718055994530942f + logf(l) : -INFINITY;
+    p.lse[static_cast<long long>(t) * p.heads + head] = l == 0.0f ? -INFINITY : m * 0.69314718055994530942f + logf(l);
 }
 
-// Rows that came out non-finite, key by key: `bad` and the row of each lane.
+// Rows that may have to be computed again: `bad` and the row of each lane.
 template <typename T, int NE>
 __device__ __forceinline__ void redo_rows(const AttnArgs& p, bool bad, int t, int head, int lane, volatile int* flag) {
   uint32_t again = __ballot_sync(0xffffffffu, bad);

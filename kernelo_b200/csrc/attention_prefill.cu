@@ -26,8 +26,8 @@
 //
 // Keys of the next request in a request's last block have weight zero, and
 // their V rows are zeroed in shared memory (0 x inf is NaN); a row that still
-// comes out non-finite (its own later tokens hold infinities) is recomputed key
-// by key.
+// comes out non-finite, with later tokens of its own in the block that hold
+// infinities, is computed again from the keys that it sees.
 //
 // The tensor cores bound it from below and the softmax's chain (maximum,
 // exponentials, sums, conversions, ~1800 cycles for 128 x 128 scores a warp group)
@@ -178,6 +178,10 @@ __device__ __forceinline__ int visible(const AttnArgs& p, const Item& it, int i)
   return min(it.keys, max(0, it.node0 + i + 1 + it.shift));
 }
 
+template <typename T, int DH>
+__device__ __noinline__ long long last_unseen(const AttnArgs& p, int t, int head, long long from, long long to, int lane) {
+  return last_unseen_nonfinite<T, DH / 32>(p, t, head, from, to, lane);
+}
 template <typename T, int DH>
 __device__ __noinline__ void redo_row(const AttnArgs& p, int t, int head, int lane) {
   float acc[DH / 32], m, l;
@@ -517,7 +521,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (!ok || it.rows <= t * BLK) continue;
       const int q_row = it.row0 + i;
       T* out = static_cast<T*>(p.out) + static_cast<long long>(q_row) * p.so_t + it.head * p.so_h;
-      const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
       float bad = 0.0f;  // NaN if anything in the row is not finite
 #pragma unroll 1
       for (int x = 0; x < DH; x += 32) {
@@ -533,8 +537,8 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
         for (int y = 0; y < 32; y += 2) {
           // a row that sees nothing may hold anything in O: its result is zero
-          const float a = l > 0.0f ? __uint_as_float(o[y]) * inv : 0.0f;
-          const float b = l > 0.0f ? __uint_as_float(o[y + 1]) * inv : 0.0f;
+          const float a = l == 0.0f ? 0.0f : __uint_as_float(o[y]) * inv;
+          const float b = l == 0.0f ? 0.0f : __uint_as_float(o[y + 1]) * inv;
           bad = fmaf(a, 0.0f, fmaf(b, 0.0f, bad));
           w[y / 2] = pack_pair<T>(a, b);
         }
@@ -555,15 +559,20 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       if (p.lse != nullptr && valid)
         p.lse[static_cast<long long>(q_row) * p.heads + it.head] =
-            l > 0.0f ? m * c * 0.69314718055994530942f + logf(l) : -INFINITY;
-      // l that is NaN (a score is) has left zeros: those rows too
-      uint32_t again = __ballot_sync(0xffffffffu, valid && (!(bad == 0.0f) || !(l >= 0.0f && l < INFINITY)));
-      if (again != 0) redo_begin(abort_flag, lane);
-      while (again != 0) {
+            l == 0.0f ? -INFINITY : m * c * 0.69314718055994530942f + logf(l);
+      uint32_t again = __ballot_sync(0xffffffffu, valid && suspect(bad == 0.0f, l));
+      if (again != 0) {
+        redo_begin(abort_flag, lane);
+        // the first of them sees the fewest keys, the others more of the same
         const int src = __ffs(again) - 1;
-        again &= again - 1;
-        redo_row<T, DH>(p, __shfl_sync(0xffffffffu, q_row, src), it.head, lane);
-        if (again == 0) redo_end(abort_flag, lane);
+        const long long last = last_unseen<T, DH>(p, __shfl_sync(0xffffffffu, q_row, src), it.head,
+                                                  __shfl_sync(0xffffffffu, limit, src), blocks * BLK, lane);
+        again = __ballot_sync(0xffffffffu, ((again >> lane) & 1u) && limit <= last);
+        while (again != 0) {
+          redo_row<T, DH>(p, __shfl_sync(0xffffffffu, q_row, __ffs(again) - 1), it.head, lane);
+          again &= again - 1;
+        }
+        redo_end(abort_flag, lane);
       }
     }
   }

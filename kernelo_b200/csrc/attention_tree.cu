@@ -23,7 +23,8 @@
 // with 16-byte cp.async. Pages a table does not name are read as zeros (a box
 // past the last page); V rows past the request's end are zeroed in shared memory
 // (0 x NaN is NaN); weights of keys that a row does not see are zero. A row that
-// comes out non-finite (a node it does not see holds infinities) is recomputed key by key.
+// comes out non-finite (a node it does not see holds infinities) is computed again from
+// the keys that it sees.
 //
 // With one new token and G heads to a key head, G of the 16 rows are real: the
 // products are free beside the cache's bytes, which bound the call. 64 requests of up
@@ -282,129 +283,124 @@ __global__ void __launch_bounds__(THREADS, 2)
   float o[DP / 8][4];
   float m[2], l[2];
   int stage = 0, phase = 0, items = 0;
-  bool fresh = true;
   const uint32_t k_first = first_pair<DP, KEYS>(warp * KW + ((lane >> 4) << 3) + (lane & 7), (lane >> 3) & 1);
   const uint32_t v_first = S::TILE + first_pair<DP, KEYS>(warp * KW + (((lane >> 3) & 1) << 3) + (lane & 7), lane >> 4);
-  while (at.left > 0) {
-    if (fresh) {
-      fresh = false;
-      attn_wait(q_full, items & 1, abort_flag, status, SITE_ATTN_SOFTMAX);
-      __syncwarp();
-#pragma unroll
-      for (int k = 0; k < DP / 16; ++k)
-        ldmatrix_x4(qf[k], pair_at<M>(smem_u32(q_tile) + first_pair<DP, M>((((lane >> 3) & 1) << 3) + (lane & 7), lane >> 4), k));
-      __syncwarp();
-      if (lane == 0) mbar_arrive(q_empty);
-      ++items;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        m[h] = -INFINITY;
-        l[h] = 0.0f;
-      }
-#pragma unroll
-      for (int n = 0; n < DP / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
-    }
-    attn_wait(full + 8 * stage, phase, abort_flag, status, SITE_ATTN_SOFTMAX);
+  while (at.left > 0) {  // items; what a block needs is dead between them
+    attn_wait(q_full, items & 1, abort_flag, status, SITE_ATTN_SOFTMAX);
     __syncwarp();
-    const uint32_t tile_at = ring + stage * 2 * S::TILE;
-    // two sums for each half of the head: their products wait less for one another
-    float s[KW / 8][4], s2[KW / 8][4];
 #pragma unroll
-    for (int n = 0; n < KW / 8; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = s2[n][0] = s2[n][1] = s2[n][2] = s2[n][3] = 0.0f;
+    for (int k = 0; k < DP / 16; ++k)
+      ldmatrix_x4(qf[k], pair_at<M>(smem_u32(q_tile) + first_pair<DP, M>((((lane >> 3) & 1) << 3) + (lane & 7), lane >> 4), k));
+    __syncwarp();
+    if (lane == 0) mbar_arrive(q_empty);
+    ++items;
 #pragma unroll
-    for (int k = 0; k < DP / 16; ++k) {
-      uint32_t b[4];
-      ldmatrix_x4(b, pair_at<KEYS>(tile_at + k_first, k));
-      auto& to = k % 2 ? s2 : s;
-      mma16816<T>(to[0], qf[k][0], qf[k][1], qf[k][2], qf[k][3], b[0], b[1]);
-      mma16816<T>(to[1], qf[k][0], qf[k][1], qf[k][2], qf[k][3], b[2], b[3]);
+    for (int h = 0; h < 2; ++h) {
+      m[h] = -INFINITY;
+      l[h] = 0.0f;
     }
 #pragma unroll
-    for (int n = 0; n < KW / 8; ++n) {
+    for (int n = 0; n < DP / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
+    for (;;) {
+      attn_wait(full + 8 * stage, phase, abort_flag, status, SITE_ATTN_SOFTMAX);
+      __syncwarp();
+      const uint32_t tile_at = ring + stage * 2 * S::TILE;
+      // two sums for each half of the head: their products wait less for one another
+      float s[KW / 8][4], s2[KW / 8][4];
 #pragma unroll
-      for (int x = 0; x < 4; ++x) s[n][x] += s2[n][x];
-    }
-    // base-2 scores, -inf where a row sees nothing
-    const int key0 = at.blk * KEYS + warp * KW;
-    const uint32_t mine = (present[2 * stage + warp / 2] >> (warp % 2 * KW)) & 0xffffu;  // this warp's keys, from bit 0
-    if (key0 + KW <= at.context && mine == 0xffffu) {
+      for (int n = 0; n < KW / 8; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = s2[n][0] = s2[n][1] = s2[n][2] = s2[n][3] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < DP / 16; ++k) {
+        uint32_t b[4];
+        ldmatrix_x4(b, pair_at<KEYS>(tile_at + k_first, k));
+        auto& to = k % 2 ? s2 : s;
+        mma16816<T>(to[0], qf[k][0], qf[k][1], qf[k][2], qf[k][3], b[0], b[1]);
+        mma16816<T>(to[1], qf[k][0], qf[k][1], qf[k][2], qf[k][3], b[2], b[3]);
+      }
 #pragma unroll
       for (int n = 0; n < KW / 8; ++n) {
 #pragma unroll
-        for (int x = 0; x < 4; ++x) s[n][x] *= p.scale_log2;
+        for (int x = 0; x < 4; ++x) s[n][x] += s2[n][x];
       }
-    } else {
-      const TileRows tile(p, walk, at);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        int node, head;
-        tile.find((lane >> 2) + 8 * h, &node, &head);
-        const uint32_t seen = mine & nodes_seen(p, at, node, key0 - at.context);
+      // base-2 scores, -inf where a row sees nothing
+      const int key0 = at.blk * KEYS + warp * KW;
+      const uint32_t mine = (present[2 * stage + warp / 2] >> (warp % 2 * KW)) & 0xffffu;  // this warp's keys, from bit 0
+      if (key0 + KW <= at.context && mine == 0xffffu) {
 #pragma unroll
         for (int n = 0; n < KW / 8; ++n) {
 #pragma unroll
-          for (int x = 0; x < 2; ++x)
-            s[n][2 * h + x] = (seen >> (n * 8 + 2 * (lane & 3) + x)) & 1u ? s[n][2 * h + x] * p.scale_log2 : -INFINITY;
+          for (int x = 0; x < 4; ++x) s[n][x] *= p.scale_log2;
+        }
+      } else {
+        const TileRows tile(p, walk, at);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          int node, head;
+          tile.find((lane >> 2) + 8 * h, &node, &head);
+          const uint32_t seen = mine & nodes_seen(p, at, node, key0 - at.context);
+#pragma unroll
+          for (int n = 0; n < KW / 8; ++n) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+              s[n][2 * h + x] = (seen >> (n * 8 + 2 * (lane & 3) + x)) & 1u ? s[n][2 * h + x] * p.scale_log2 : -INFINITY;
+          }
+        }
+        if (BULK && key0 + KW > at.length) {  // rows past the request's end hold anything
+          const int from = max(at.length - key0, 0);
+          for (int i = from * (DP / 8) + lane; i < KW * (DP / 8); i += 32)
+            *reinterpret_cast<uint4*>(smem + (2 * stage + 1) * S::TILE +
+                                      chunk_at<DP, KEYS>(warp * KW + i / (DP / 8), i % (DP / 8))) = make_uint4(0u, 0u, 0u, 0u);
+          fence_proxy_async_smem();  // before the next box lands here
+        }
+        __syncwarp();
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float top = m[h];
+#pragma unroll
+        for (int n = 0; n < KW / 8; ++n) top = fmaxf(top, fmaxf(s[n][2 * h], s[n][2 * h + 1]));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        if (__any_sync(0xffffffffu, top > m[h])) {
+          const float fix = top > m[h] ? ex2_ftz(m[h] - top) : 1.0f;
+          l[h] *= fix;
+#pragma unroll
+          for (int n = 0; n < DP / 8; ++n) {
+            o[n][2 * h] *= fix;
+            o[n][2 * h + 1] *= fix;
+          }
+          m[h] = top;
+        }
+        const float base = m[h] == -INFINITY ? 0.0f : m[h];
+#pragma unroll
+        for (int n = 0; n < KW / 8; ++n) {
+          s[n][2 * h] = ex2_ftz(s[n][2 * h] - base);
+          s[n][2 * h + 1] = ex2_ftz(s[n][2 * h + 1] - base);
+          l[h] += s[n][2 * h] + s[n][2 * h + 1];
         }
       }
-      if (BULK && key0 + KW > at.length) {  // rows past the request's end hold anything
-        const int from = max(at.length - key0, 0);
-        for (int i = from * (DP / 8) + lane; i < KW * (DP / 8); i += 32)
-          *reinterpret_cast<uint4*>(smem + (2 * stage + 1) * S::TILE +
-                                    chunk_at<DP, KEYS>(warp * KW + i / (DP / 8), i % (DP / 8))) = make_uint4(0u, 0u, 0u, 0u);
-        fence_proxy_async_smem();  // before the next box lands here
+      {
+        const uint32_t a0 = pack_pair<T>(s[0][0], s[0][1]), a1 = pack_pair<T>(s[0][2], s[0][3]);
+        const uint32_t a2 = pack_pair<T>(s[1][0], s[1][1]), a3 = pack_pair<T>(s[1][2], s[1][3]);
+#pragma unroll
+        for (int n = 0; n < DP / 16; ++n) {
+          uint32_t b[4];
+          ldmatrix_x4_trans(b, pair_at<KEYS>(tile_at + v_first, n));
+          mma16816<T>(o[2 * n], a0, a1, a2, a3, b[0], b[1]);
+          mma16816<T>(o[2 * n + 1], a0, a1, a2, a3, b[2], b[3]);
+        }
       }
       __syncwarp();
-    }
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float top = m[h];
-#pragma unroll
-      for (int n = 0; n < KW / 8; ++n) top = fmaxf(top, fmaxf(s[n][2 * h], s[n][2 * h + 1]));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      if (__any_sync(0xffffffffu, top > m[h])) {
-        const float fix = top > m[h] ? ex2_ftz(m[h] - top) : 1.0f;
-        l[h] *= fix;
-#pragma unroll
-        for (int n = 0; n < DP / 8; ++n) {
-          o[n][2 * h] *= fix;
-          o[n][2 * h + 1] *= fix;
-        }
-        m[h] = top;
+      if (lane == 0) mbar_arrive(empty + 8 * stage);
+      if (++stage == STAGES) {
+        stage = 0;
+        phase ^= 1;
       }
-      const float base = m[h] == -INFINITY ? 0.0f : m[h];
-#pragma unroll
-      for (int n = 0; n < KW / 8; ++n) {
-        s[n][2 * h] = ex2_ftz(s[n][2 * h] - base);
-        s[n][2 * h + 1] = ex2_ftz(s[n][2 * h + 1] - base);
-        l[h] += s[n][2 * h] + s[n][2 * h + 1];
-      }
-    }
-    {
-      const uint32_t a0 = pack_pair<T>(s[0][0], s[0][1]), a1 = pack_pair<T>(s[0][2], s[0][3]);
-      const uint32_t a2 = pack_pair<T>(s[1][0], s[1][1]), a3 = pack_pair<T>(s[1][2], s[1][3]);
-#pragma unroll
-      for (int n = 0; n < DP / 16; ++n) {
-        uint32_t b[4];
-        ldmatrix_x4_trans(b, pair_at<KEYS>(tile_at + v_first, n));
-        mma16816<T>(o[2 * n], a0, a1, a2, a3, b[0], b[1]);
-        mma16816<T>(o[2 * n + 1], a0, a1, a2, a3, b[2], b[3]);
-      }
-    }
-    __syncwarp();
-    if (lane == 0) mbar_arrive(empty + 8 * stage);
-    if (++stage == STAGES) {
-      stage = 0;
-      phase ^= 1;
-    }
-    if (!walk.item_ends(at)) {
+      if (walk.item_ends(at)) break;
       walk.advance(p, at);
-      continue;
     }
 
     // The item's last block of this run: join the warps' sums.
-    fresh = true;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);

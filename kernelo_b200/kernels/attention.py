@@ -13,7 +13,8 @@ needs once prompts have different lengths and keys live in pages.
 Lengths and offsets stay on the device: no call reads them on the host, so both
 can be captured in a CUDA graph and replayed with other lengths. A row that
 sees no key gives zeros (log-sum-exp ``-inf``), and what a row does not see
-never reaches it, whatever is stored there.
+never reaches it, whatever is stored there. A score that is NaN or +infinity
+makes the rows that see it NaN, log-sum-exp included.
 """
 
 from __future__ import annotations

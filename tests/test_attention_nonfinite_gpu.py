@@ -171,8 +171,7 @@ def check_columns(got, want, bound, column, what):
 @pytest.mark.parametrize("dtype", HALF)
 @pytest.mark.parametrize("count", [1, 16])
 def test_an_infinite_value_that_long_requests_see(count, dtype, device):
-    """All rows of a long cache are computed again, which takes its time: the waits beside it do not run out, and
-    neither the rows' other columns nor other requests lose anything."""
+    """Only the column that the rows see it in is not finite; other requests lose nothing."""
     context, nodes = (131072, 300, 40), (count,) * 3
     masks, words = random_trees(nodes)
     q, k, v, table, lens = cache(context, nodes, 8, 2, 128, 32, dtype, device)
@@ -205,3 +204,43 @@ def test_an_infinite_value_that_a_long_prompt_sees(dtype, device):
     want, want_lse, bound, off = ref.packed(q[40000:], k[40000:], v[40000:], (500,), (500,))
     ref.check(out[40000:], want, bound, f"{dtype}")
     ref.check_lse(lse[40000:], want_lse, off, f"{dtype}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("count", [2, 16])
+def test_an_infinite_value_of_one_node_over_a_long_cache(count, dtype, device):
+    """The other nodes' rows are computed again, which takes its time: the waits beside it do not run out, and
+    neither these rows nor other requests lose anything."""
+    context, nodes = (131072, 300, 40), (count,) * 3
+    masks, words = random_trees(nodes)
+    for r in range(3):
+        masks[r][:, count - 1] = torch.arange(count) == count - 1
+    q, k, v, table, lens = cache(context, nodes, 8, 2, 128, 32, dtype, device)
+    want, want_lse, bound, off = ref.paged(q, k, v, table, context, nodes, masks)
+    place = context[0] + count - 1
+    v[table[0, place // 32].long(), :, place % 32, 9] = torch.inf
+    native.device_status()
+    out, lse = tree_attention(q, k, v, table, lens, offsets(nodes, device), words.to(device), return_lse=True)
+    assert native.device_status() == 0
+    fine = [i for i in range(3 * count) if i != count - 1]
+    check_rows(fine, out, lse, want, want_lse, bound, off, f"{dtype}")
+    check_columns(out[count - 1], want[count - 1], bound[count - 1], 9, f"{dtype}")
+
+
+@pytest.mark.parametrize("dtype", HALF)
+def test_an_infinite_value_at_the_end_of_a_long_prompt(dtype, device):
+    lens = (40000, 500)
+    q, k, v, cu, _ = prompt(lens, lens, 1, 1, 64, dtype, device)
+    clean = v.clone()
+    v[39999, 0, 9] = torch.inf
+    native.device_status()
+    out, lse = prefill_attention(q, k, v, cu, return_lse=True)
+    assert native.device_status() == 0
+    at = torch.arange(40000, device=device)
+    for rows in (slice(0, 130), slice(39700, 39800), slice(39900, 39999)):
+        want, want_lse, bound, off = ref.attend(q[rows, 0], k[:40000, 0], clean[:40000, 0], at[None, :] <= at[rows, None], 0.125)
+        ref.check(out[rows, 0], want, bound, f"{dtype} {rows}")
+        ref.check_lse(lse[rows, 0], want_lse, off, f"{dtype} {rows}")
+    assert not out[39999, 0, 9].isfinite() and out[39999, 0, :9].isfinite().all()
+    want, want_lse, bound, off = ref.packed(q[40000:], k[40000:], v[40000:], (500,), (500,))
+    ref.check(out[40000:], want, bound, f"{dtype}")
