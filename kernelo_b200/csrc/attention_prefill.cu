@@ -330,6 +330,12 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int t = 0; t < 2; ++t) mbar_wait(q_bar + 8 * t, (loaded - 1) & 1, nullptr, status, SITE_DRAIN, DRAIN_NS);
         for (int s = 0; s < STAGES && s < issued; ++s)
           mbar_wait(full + 8 * s, ((issued - 1 - s) / STAGES) & 1, nullptr, status, SITE_DRAIN, DRAIN_NS);
+      } else if (lane == 0) {  // the products' last arrivals here come behind those that the results wait for
+        for (int s = 0; s < STAGES && s < issued; ++s)
+          attn_wait(empty + 8 * ((issued - 1 - s) % STAGES), ((issued - 1 - s) / STAGES) & 1, abort_flag, status,
+                    SITE_ATTN_LOAD);
+        for (int t = 0; t < 2 && loaded > 0; ++t)
+          attn_wait(q_free + 8 * t, (loaded - 1) & 1, abort_flag, status, SITE_ATTN_LOAD);
       }
     } else if (warp == CLEAN_WARP) {
       // The last block of a request: its V rows past the request's keys, when the
