@@ -301,7 +301,8 @@ KF_API int32_t kf_rmsnorm_rows(int32_t dtype, const void* x, int64_t sx_row, con
  * o = softmax(scale q k^T) v per head, query head h reading key head
  * h / (heads / kv_heads); scores, statistics and sums in fp32 (matrix products on
  * tensor cores read the weights p rounded to the operands' 16-bit type). Strides
- * in elements; the last dimension of every operand is contiguous; dim <= 256.
+ * in elements; the last dimension of every operand is contiguous; dim <= 256; out
+ * shares no element with the other operands or itself.
  * Offsets and lengths are read on the device only, and clamped to the arrays
  * they index. A row that sees no key gets zeros and a log-sum-exp of -infinity,
  * and so do rows of q past the last offset. What a row does not see does not

@@ -36,6 +36,14 @@ int check_heads(int64_t dtype, int64_t rows, int64_t seqs, int64_t heads, int64_
   return KF_OK;
 }
 
+// Rows may be computed again from q when others have been written, and every element by one
+// thread alone. (Partial overlaps are the caller's to avoid.)
+int check_output(const void* q, const void* out, int64_t rows, int64_t so_row, int64_t heads, int64_t so_head) {
+  if (out == q) return invalid("out must not be q");
+  if ((rows > 1 && so_row == 0) || (heads > 1 && so_head == 0)) return invalid("out overlaps itself: a stride of zero");
+  return KF_OK;
+}
+
 }  // namespace
 }  // namespace kf
 
@@ -54,6 +62,8 @@ int32_t kf_prefill_attention(const kf_prefill_args* args, void* stream) {
   if (g.q == nullptr || g.out == nullptr || g.cu_q == nullptr || g.cu_k == nullptr ||
       (g.keys > 0 && (g.k == nullptr || g.v == nullptr)))
     return invalid("null pointer");
+  rc = check_output(g.q, g.out, g.rows, g.so_row, g.heads, g.so_head);
+  if (rc != KF_OK) return rc;
   DeviceInfo* dev = nullptr;
   rc = this_device(&dev);
   if (rc != KF_OK) return rc;
@@ -88,6 +98,8 @@ int32_t kf_tree_attention(const kf_tree_args* args, void* stream) {
     return invalid("null pointer");
   if ((reinterpret_cast<uintptr_t>(g.workspace) & 255u) != 0)
     return set_error(KF_ERR_WORKSPACE, "workspace must be 256-byte aligned");
+  rc = check_output(g.q, g.out, g.rows, g.so_row, g.heads, g.so_head);
+  if (rc != KF_OK) return rc;
   DeviceInfo* dev = nullptr;
   rc = this_device(&dev);
   if (rc != KF_OK) return rc;

@@ -60,6 +60,46 @@ def _empty_like(t: torch.Tensor) -> torch.Tensor:
     return torch.empty(t.shape, device=t.device, dtype=t.dtype)
 
 
+def _elements(t: torch.Tensor) -> int:
+    """From the first element to the last, whatever lies between."""
+    return sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1 if t.numel() else 0
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors of one type share an element: exact for views of equal strides (the parts of one
+    projection, say), and true for others whose address ranges meet."""
+    size, delta = a.element_size(), b.data_ptr() - a.data_ptr()
+    if not a.numel() or not b.numel() or delta >= _elements(a) * size or -delta >= _elements(b) * size:
+        return False
+    dims = sorted(zip(a.stride(), b.stride(), a.shape, b.shape), reverse=True) if a.ndim == b.ndim else None
+    if dims is None or delta % size or any(s != r and (n > 1 or m > 1) for s, r, n, m in dims):
+        return True
+
+    def meet(delta, dims):  # sum of i s over the dimensions is delta for some i > -m and < n in each
+        if not dims:
+            return delta == 0
+        (s, _, n, m), rest = dims[0], dims[1:]
+        if s == 0 or n == m == 1:
+            return meet(delta, rest)
+        low, high = -sum((d[3] - 1) * d[0] for d in rest), sum((d[2] - 1) * d[0] for d in rest)
+        first, last = max(1 - m, -((high - delta) // s)), min(n - 1, (delta - low) // s)
+        return last - first > 64 or any(meet(delta - i * s, rest) for i in range(first, last + 1))
+
+    return meet(delta // size, dims)
+
+
+def _check_output(name: str, out: torch.Tensor, operands: dict[str, torch.Tensor]) -> None:
+    """An output written by many threads, beside others that still read, shares no element with itself or them."""
+    span = 0
+    for s, n in sorted((s, n) for s, n in zip(out.stride(), out.shape) if n > 1):
+        if s <= span:
+            raise ValueError(f"{name} overlaps itself: strides {out.stride()} for shape {tuple(out.shape)}")
+        span += (n - 1) * s
+    for other, t in operands.items():
+        if _overlap(out, t):
+            raise ValueError(f"{name} shares memory with {other}")
+
+
 def _check_query(q: torch.Tensor) -> None:
     if q.ndim != 3:
         raise ValueError(f"expected q as (rows, heads, dim), got shape {tuple(q.shape)}")
@@ -69,13 +109,16 @@ def _check_query(q: torch.Tensor) -> None:
         raise ValueError("q must have a contiguous last dimension. Pass q.contiguous() explicitly.")
 
 
+def _check_given(out: torch.Tensor, q: torch.Tensor, operands: dict[str, torch.Tensor]) -> None:
+    if out.shape != q.shape:
+        raise ValueError(f"out must have shape {tuple(q.shape)}, got {tuple(out.shape)}")
+    _check_operand("out", out, q)
+    _check_output("out", out, operands)
+
+
 def _outputs(q: torch.Tensor, out: torch.Tensor | None, return_lse: bool):
     if out is None:
         out = _empty_like(q)
-    else:
-        if out.shape != q.shape:
-            raise ValueError(f"out must have shape {tuple(q.shape)}, got {tuple(out.shape)}")
-        _check_operand("out", out, q)
     lse = torch.empty(q.shape[0], q.shape[1], device=q.device, dtype=torch.float32) if return_lse else None
     return out, lse
 
@@ -120,7 +163,8 @@ def prefill_attention(
     ``causal``: a request's last row sees all of its keys and each row before
     it one less, so a prompt that continues cached keys passes more keys than
     rows. ``scale`` defaults to ``dim ** -0.5``. Returns the output, and with
-    ``return_lse`` also the fp32 natural log-sum-exp ``(rows, heads)``.
+    ``return_lse`` also the fp32 natural log-sum-exp ``(rows, heads)``. ``out``
+    shares no memory with q, k or v.
     """
     dtype, device = q.dtype, q.get_device()
     if cu_k is None and k.shape[:1] == q.shape[:1]:
@@ -137,6 +181,8 @@ def prefill_attention(
     _check_heads(q, k.shape[1], k.shape[2])
     if cu_q.shape[0] < 1:
         raise ValueError(f"cu_q must have shape (requests + 1,), got {tuple(cu_q.shape)}")
+    if out is not None:
+        _check_given(out, q, {"q": q, "k": k, "v": v})
     out, lse = _outputs(q, out, return_lse)
     if q.numel():
         native.prefill_attention(q, k, v, out, lse, cu_q, cu_k, q.shape[2] ** -0.5 if scale is None else scale, causal)
@@ -196,7 +242,8 @@ def tree_attention(
     (``rotary_to_cache`` does). ``cu_q`` are the offsets of each request's rows;
     without it every request has one row (plain decoding). ``tree_mask`` (int64
     ``(rows, words)``): bit ``b`` says whether the row sees row ``b`` of its
-    request, itself included; without it the rows are a chain.
+    request, itself included; without it the rows are a chain. ``out`` shares
+    no memory with q or the cache.
     """
     dtype, device = q.dtype, q.get_device()
     if not (q.is_cuda and q.ndim == 3 and k_cache.ndim == 4 and v_cache.shape == k_cache.shape
@@ -211,6 +258,8 @@ def tree_attention(
     _check_heads(q, k_cache.shape[1], k_cache.shape[3])
     if k_cache.shape[2] < 1:
         raise ValueError("pages must hold at least one token")
+    if out is not None:
+        _check_given(out, q, {"q": q, "k_cache": k_cache, "v_cache": v_cache})
     out, lse = _outputs(q, out, return_lse)
     if q.numel():
         native.tree_attention(q, k_cache, v_cache, out, lse, block_table, context_lens, cu_q, tree_mask,

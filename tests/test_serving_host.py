@@ -10,6 +10,7 @@ from pathlib import Path
 import pytest
 import torch
 
+from kernelo_b200.kernels import attention
 from kernelo_b200.kernels.attention import prefill_attention, tree_attention
 from kernelo_b200.kernels.paged import build_slots
 from kernelo_b200.kernels.rotary import rotary, rotary_table
@@ -123,3 +124,50 @@ def test_a_workspace_off_its_alignment_is_refused_on_the_host():
         packed = native.TREE_ARGS.pack(*((values | dict(workspace=4096 + off))[n] for n in names))
         assert lib.kf_tree_attention(packed, None) == native.KF_ERR_WORKSPACE
         assert "256-byte aligned" in native.last_error()
+
+
+def test_overlaps_of_outputs_are_found():
+    """Views of one buffer, against the elements that they really hold."""
+    buf = torch.arange(4000)
+
+    def held(t):
+        return set(t.reshape(-1).tolist())
+
+    gen = torch.Generator().manual_seed(0)
+    for _ in range(3000):
+        n, m, h, g, d = (int(x) for x in torch.randint(1, 6, (5,), generator=gen))
+        strides = [int(x) for x in torch.randint(1, 40, (2,), generator=gen)]
+        a, b = (buf.as_strided((rows, heads, d), (*strides, 1), int(torch.randint(0, 300, (1,), generator=gen)))
+                for rows, heads in ((n, h), (m, g)))
+        assert attention._overlap(a, b) == attention._overlap(b, a) == bool(held(a) & held(b))
+        twice = len(held(a)) < a.numel()
+        try:
+            attention._check_output("out", a, {})
+        except ValueError:
+            continue  # it may refuse strides that interleave without meeting
+        assert not twice
+    qkv = torch.zeros(7, 12, 16)
+    q, k, v, rest = qkv[:, :4], qkv[:, 4:6], qkv[:, 6:8], qkv[:, 8:]
+    attention._check_output("out", rest, {"q": q, "k": k, "v": v})
+    attention._check_output("out", torch.zeros(4, 7, 16).transpose(0, 1), {"q": q})
+    for out, other in ((q, q), (qkv[:, 1:5], q), (qkv[:, 7:11], v), (qkv.view(12, 7, 16)[:4].transpose(0, 1), q)):
+        with pytest.raises(ValueError, match="shares memory with x"):
+            attention._check_output("out", out, {"x": other})
+    for out in (torch.zeros(1, 4, 16).expand(7, 4, 16), torch.zeros(7, 1, 16).expand(7, 4, 16)):
+        with pytest.raises(ValueError, match="overlaps itself"):
+            attention._check_output("out", out, {})
+
+
+def test_c_entries_refuse_outputs_that_overlap():
+    if torch.cuda.is_available():
+        pytest.skip("the addresses are made up: only where nothing can be launched")
+    lib = native.load()
+    names = ("dtype q sq_row sq_head k sk_row sk_head v sv_row sv_head out so_row so_head lse cu_q cu_k seqs rows "
+             "keys heads kv_heads dim scale causal").split()
+    base = dict.fromkeys(names, 0) | dict(heads=4, kv_heads=2, dim=64, scale=1.0, rows=5, seqs=1, keys=5, so_row=256,
+                                          so_head=64, q=4096, out=8192, k=4096, v=4096, cu_q=4096, cu_k=4096)
+    for change, message in ((dict(out=4096), "must not be q"), (dict(so_row=0), "overlaps itself"),
+                            (dict(so_head=0), "overlaps itself")):
+        packed = native.PREFILL_ARGS.pack(*((base | change)[n] for n in names))
+        assert lib.kf_prefill_attention(packed, None) == native.KF_ERR_INVALID_ARGUMENT
+        assert message in native.last_error()
