@@ -273,6 +273,7 @@ def check(status: int, what: str) -> None:
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_is_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
 
 
 def current_stream_handle(device: torch.device) -> int:
@@ -420,6 +421,10 @@ class _WorkspacePool:
             return None
         key = (device.index if device.index is not None else torch.cuda.current_device(), stream)
         capture = _capture_id(stream)
+        if not (capture or self._captured):  # the usual call, at the cost of a look
+            buf = self._buffers.get(key)
+            if buf is not None and buf.nbytes >= nbytes:
+                return buf
         with self._lock:
             if capture:
                 held, buf = self._captured.get(key, (0, None))
@@ -446,7 +451,7 @@ class _WorkspacePool:
 
 def _capture_id(stream: int) -> int:
     """The capture that the device's current stream, ``stream``, is in; 0 for none."""
-    if not torch.cuda.is_current_stream_capturing():
+    if not _is_capturing():
         return 0
     out = ctypes.c_int64(0)
     check(load().kf_stream_capture_id(stream, ctypes.byref(out)), "kf_stream_capture_id")
