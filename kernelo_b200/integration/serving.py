@@ -10,8 +10,8 @@ decoding steps -- one token or a tree of drafted ones per request -- extend:
     y = block.prompts(x, cache, step)         # x: all prompts' tokens, packed
     cache.advance(step)
     step = cache.plan([4, 4])                 # four drafted tokens each ..
-    y = block.tokens(x, cache, step, mask)    # ... that see their ancestors
-    cache.advance(step, kept=[3, 1])          # as many as were accepted (the rest is written over)
+    y = block.tokens(x, cache, step, mask, depths)  # ... that see their ancestors
+    cache.advance(step, kept=[[0, 1, 3], 1])  # the accepted branch, or the first so many (the rest is written over)
 """
 
 from __future__ import annotations
@@ -96,10 +96,29 @@ class PagedCache:
         return Step(new_lens, slots, context)
 
     def advance(self, step: Step, kept=None) -> None:
-        """The step's tokens are the requests' now, or the first ``kept[r]`` of them: pages of the rest go back."""
-        kept = step.new_lens if kept is None else tuple(int(k) for k in kept)
-        if len(kept) != len(self.lens) or any(not 0 <= k <= n for k, n in zip(kept, step.new_lens)):
-            raise ValueError(f"kept must be counts of at most {step.new_lens}, got {kept}")
+        """The step's tokens are the requests' now, or those that ``kept[r]`` names: pages of the rest go back.
+
+        A number keeps the first so many, which is right for a chain. Of a tree a
+        list names the accepted branch, from the root on, by its tokens' places in
+        the step: its keys and values move to the places behind the request's
+        last token, which its rotary positions (``depths``) have assumed already.
+        """
+        paths = []
+        for k in step.new_lens if kept is None else kept:
+            several = isinstance(k, (list, tuple, range)) or getattr(k, "ndim", 0)
+            paths.append([int(i) for i in k] if several else list(range(int(k))) if int(k) >= 0 else [-1])
+        if len(paths) != len(self.lens) or any(
+                p and not (0 <= p[0] and p[-1] < n and all(a < b for a, b in zip(p, p[1:])))
+                for p, n in zip(paths, step.new_lens)):
+            raise ValueError(f"kept must be counts of at most {step.new_lens}, or rising places below them, got {kept}")
+        moves = [(r, self.lens[r] + a, self.lens[r] + b) for r, p in enumerate(paths) for b, a in enumerate(p) if a != b]
+        if moves:
+            size = self.config.block_size
+            rows, source, to = torch.tensor(moves, device=self.free.device).unbind(1)
+            source_page, to_page = (self.block_table[rows, at // size].long() for at in (source, to))
+            for pages in (self.k, self.v):
+                pages[to_page, :, to % size] = pages[source_page, :, source % size]
+        kept = [len(p) for p in paths]
         before, after, keep = self._pages([0] * len(kept)), self._pages(step.new_lens), self._pages(kept)
         free = self.free[sum(after) - sum(before):]
         back = [(r, c) for r in range(len(kept)) for c in range(keep[r], after[r])]
