@@ -12,6 +12,7 @@ decoding steps -- one token or a tree of drafted ones per request -- extend:
     step = cache.plan([4, 4])                 # four drafted tokens each ..
     y = block.tokens(x, cache, step, mask, depths)  # ... that see their ancestors
     cache.advance(step, kept=[[0, 1, 3], 1])  # the accepted branch, or the first so many (the rest is written over)
+    cache.release(0)                          # finished: its pages go back, its row takes another request
 """
 
 from __future__ import annotations
@@ -54,6 +55,7 @@ class Step:
     new_lens: tuple[int, ...]
     slots: StepSlots
     context_lens: torch.Tensor  # tokens of each request before the step
+    lens: tuple[int, ...] | None = None  # the same on the host
 
 
 class PagedCache:
@@ -93,7 +95,7 @@ class PagedCache:
         context = self._device_ints(self.lens)
         slots = build_slots(context, self._device_ints(new_lens), self.block_table, self.free,
                             block_size=self.config.block_size, max_tokens=sum(new_lens))
-        return Step(new_lens, slots, context)
+        return Step(new_lens, slots, context, tuple(self.lens))
 
     def advance(self, step: Step, kept=None) -> None:
         """The step's tokens are the requests' now, or those that ``kept[r]`` names: pages of the rest go back.
@@ -103,6 +105,8 @@ class PagedCache:
         the step: its keys and values move to the places behind the request's
         last token, which its rotary positions (``depths``) have assumed already.
         """
+        if step.lens is not None and list(step.lens) != self.lens:
+            raise ValueError(f"the step was planned for requests of {list(step.lens)} tokens; they have {self.lens}")
         paths = []
         for k in step.new_lens if kept is None else kept:
             several = isinstance(k, (list, tuple, range)) or getattr(k, "ndim", 0)
@@ -127,6 +131,15 @@ class PagedCache:
             free = torch.cat([self.block_table[rows, columns], free])
         self.free = free
         self.lens = [n + k for n, k in zip(self.lens, kept)]
+
+    def release(self, request: int) -> None:
+        """A finished request's pages go back, and its row is free for another. Between steps, not during one."""
+        if not 0 <= request < len(self.lens):
+            raise ValueError(f"request must be one of {len(self.lens)}, got {request}")
+        pages = -(-self.lens[request] // self.config.block_size)
+        self.free = torch.cat([self.free, self.block_table[request, :pages]])
+        self.block_table[request] = -1
+        self.lens[request] = 0
 
 
 class ServingBlock(nn.Module):

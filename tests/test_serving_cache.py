@@ -62,6 +62,61 @@ def test_what_is_no_branch_is_refused(kept):
     assert cache.lens == [5, 8] and torch.equal(cache.k, before)
 
 
+def test_a_released_request_gives_its_pages_back():
+    cache, step = planned((5, 8, 0), (4, 0, 3))
+    cache.advance(step)
+    taken = [cache.block_table[r, :-(-n // 4)].tolist() for r, n in enumerate(cache.lens)]
+    free = cache.free.tolist()
+    cache.release(1)
+    cache.release(2)
+    assert cache.lens == [9, 0, 0] and cache.free.tolist() == free + taken[1] + taken[2]
+    assert cache.block_table[0, :3].tolist() == taken[0] and (cache.block_table[1:] == -1).all()
+    cache.release(1)  # of nothing
+    assert cache.free.shape[0] == 37
+    for request in (3, -1):
+        with pytest.raises(ValueError, match="request must be"):
+            cache.release(request)
+
+
+def test_a_step_planned_for_other_lengths_is_refused():
+    cache, step = planned((5, 8), (1, 1))
+    step = Step(step.new_lens, None, None, (5, 8))
+    cache.advance(step)
+    with pytest.raises(ValueError, match="planned"):
+        cache.advance(step)
+    cache, _ = planned((5, 8), (1, 1))
+    cache.release(0)
+    with pytest.raises(ValueError, match="planned"):
+        cache.advance(step)
+
+
+@pytest.mark.gpu
+def test_a_server_goes_on_with_the_pages_of_finished_requests(device):
+    """More requests one after another than the cache has pages for at once."""
+    block = make_block(torch.float16, device)
+    cache = PagedCache(TINY, requests=2, blocks=6, device=device)  # 48 tokens
+    gen = torch.Generator(device=device).manual_seed(3)
+    with torch.inference_mode():
+        for turn in range(5):
+            row = turn % 2
+            lens = [0, 0]
+            lens[row] = 17 + turn
+            x, step = torch.randn(17 + turn, TINY.hidden, generator=gen, device=device).half(), cache.plan(lens)
+            got = block.prompts(x, cache, step)
+            at = torch.arange(17 + turn, device=device)
+            want = plain_block(block, x, at, at[None, :] <= at[:, None])
+            assert_verified(want, got, dtype=torch.float16, context="prompt")
+            cache.advance(step)
+            y, step = torch.randn(1, TINY.hidden, generator=gen, device=device).half(), cache.plan([int(r == row) for r in range(2)])
+            got = block.tokens(y, cache, step)
+            at = torch.arange(18 + turn, device=device)
+            want = plain_block(block, torch.cat([x, y]), at, at[None, :] <= at[:, None])[-1:]
+            assert_verified(want, got, dtype=torch.float16, context="token")
+            cache.advance(step)
+            cache.release(row)
+        assert sorted(cache.free.tolist()) == list(range(6))
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
 def test_tokens_after_an_accepted_branch(dtype, device):
