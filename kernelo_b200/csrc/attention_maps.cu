@@ -50,6 +50,10 @@ bool encode_pages(CUtensorMap* map, const AttnArgs& a, const void* ptr, int64_t 
                   int box_rows, int width) {
   auto enc = encoder();
   if (enc == nullptr) return false;
+  // strides outside of what a tensor map may have are not left to the encoder to find: a head or
+  // a page that stands for several has one of zero
+  const auto fits = [](int64_t s, int64_t n) { return n <= 1 || (s > 0 && s % 8 == 0 && s < (1ll << 38)); };
+  if (!fits(s_slot, a.block_size) || !fits(s_head, a.kv_heads) || !fits(s_page, a.pages)) return false;
   const auto bytes = [](int64_t s, int64_t n) { return static_cast<cuuint64_t>(n > 1 ? 2 * s : 16); };
   const cuuint64_t dims[4] = {static_cast<cuuint64_t>(a.dim), static_cast<cuuint64_t>(a.block_size),
                               static_cast<cuuint64_t>(a.kv_heads), static_cast<cuuint64_t>(a.pages)};

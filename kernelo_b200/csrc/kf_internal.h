@@ -268,7 +268,8 @@ int encode_heads(CUtensorMap* map, int dtype, const void* ptr, int64_t rows, int
                  int64_t s_head, int box_heads, int box_rows);
 // Pages [pages, kv_heads, block_size, dim] as boxes of box_rows slots x `width`
 // elements (64, or 32 in the 64-byte swizzle); what lies past the head or past the
-// last page is filled with zeros. False where no tensor map describes the cache.
+// last page is filled with zeros. False where no tensor map describes the cache (strides of
+// zero, as of expanded tensors, among others).
 bool encode_pages(CUtensorMap* map, const AttnArgs& args, const void* ptr, int64_t s_page, int64_t s_head, int64_t s_slot,
                   int box_rows, int width);
 // Tiles of 16 or 64 rows in fp32 arithmetic (attention_block.cu): every type, stride,
