@@ -34,7 +34,7 @@
 // from above. One prompt of 8192 tokens, 32 heads to 8 of 128 elements, bf16: 449 us,
 // 1.22 PFLOP/s in a burst (75% of a plain product's rate), 511 to 525 us, 1.05 to 1.08
 // PFLOP/s, under the power cap (77%). Nine ragged prompts (53 GFLOP) 104 us, 0.51 PFLOP/s:
-// an SM has five items of two to eleven blocks, whose beginnings and ends nothing hides. 10.9 us for four prompts of up to 160.
+// an SM has five items of two to eleven blocks, whose beginnings and ends nothing hides. 11.1 us for four prompts of up to 160.
 #include <cuda.h>
 
 #include <mutex>

@@ -28,9 +28,9 @@
 //
 // With one new token and G heads to a key head, G of the 16 rows are real: the
 // products are free beside the cache's bytes, which bound the call. 64 requests of up
-// to 4096 keys, 32 heads to 8 of 128 elements, bf16: 115 us, 540 MB at 4.7 TB/s (71%
-// of a copy's rate); one of 131072 keys 112 us, 537 MB at 4.8 TB/s; one of 100 keys
-// 7.7 us. What is left: the chain of products, maxima and exponentials of a block is
+// to 4096 keys, 32 heads to 8 of 128 elements, bf16: 98 us, 540 MB at 5.5 TB/s (84%
+// of a copy's rate); one of 131072 keys 98 us, 537 MB at 5.5 TB/s; one of 100 keys
+// 9.0 us. What is left: the chain of products, maxima and exponentials of a block is
 // longer than its bytes take to come, and each item's joining is in nobody's shadow.
 #include <cuda.h>
 
@@ -50,10 +50,10 @@ constexpr int WARPS = 4;      // of products
 constexpr int KW = KEYS / WARPS;
 constexpr int LOAD_WARP = WARPS, FINISH_WARP = WARPS + 1;
 constexpr int THREADS = 32 * (WARPS + 2);
-constexpr int MIN_RUN = 4;  // positions of a run: fewer blocks cost more to join than to read (8: 19.0 us for 18.4, one short request)
-// Blocks that an item's queries and results are worth. 64 requests of up to 4096 keys: 115 us
-// (133 with none, 118 with 2, 117 with 6); 128 of up to 1000: 77 (81 with 2 and with 6); one of
-// 131072: 114 with any.
+constexpr int MIN_RUN = 4;  // positions of a run: fewer blocks cost more to join than to read (8: 14.5 us for 12.2, one request of 100 keys, calls back to back)
+// Blocks that an item's queries and results are worth. 64 requests of up to 4096 keys: 98.5 us
+// (104.6 with none, 97.4 with 2, 99.8 with 6); 128 of up to 1000: 57.9 (76.5, 59.5, 61.7); one of
+// 131072: 98 to 100 with any.
 constexpr int ITEM_COST = 3;
 constexpr uint64_t DRAIN_NS = 100000000ull;
 
@@ -569,9 +569,10 @@ bool attention_tree_supported(const AttnArgs& a) {
 }
 
 // Rows that a request has for a key head on average: above 16 the products of
-// mma.sync tiles take longer than the cache's bytes. 16 trees, 32 heads to 8, by
-// their largest number of nodes, here and on tcgen05 tiles: 2 70 us and 88, 4 72 and
-// 88, 8 107 and 88, 16 154 and 88; 64 requests of one token 118 and 149.
+// mma.sync tiles take longer than the cache's bytes. 16 trees over 8192 keys, 32 heads to 8,
+// by their nodes, here and on tcgen05 tiles: 4 99 us and 106, 5 174 and 107, 9 253 and 110,
+// 16 330 and 114; 64 requests of one token 98 and 150. (With up to 8 nodes over up to 8192
+// keys 75 and 83: trees far apart in size are taken for their mean.)
 static bool many_rows(const AttnArgs& a) {
   return ceil_div(a.rows, a.seqs > 0 ? a.seqs : 1) * (a.heads / a.kv_heads) > M;
 }

@@ -17,8 +17,8 @@
 // 128 keys of one head are 64 KB: 1.5 us of this SM's share of the HBM's rate, in
 // which the two products take 0.55 us and 128 x 128 exponentials 0.55 us, so the
 // cache's bytes bound the call; with mma.sync tiles of 64 rows the products did
-// (1.2 us per 64 keys). 16 trees of up to 16 nodes over up to 8192 keys, 32 heads to 8 of 128 elements: 86 us,
-// 276 MB at 3.2 TB/s (154 on mma.sync tiles); what is left are the latencies between
+// (1.2 us per 64 keys). 16 trees of up to 16 nodes over up to 8192 keys, 32 heads to 8 of 128 elements: 84 us,
+// 276 MB at 3.3 TB/s (102 on mma.sync tiles); what is left are the latencies between
 // a block's two products and its softmax, since 64 rows of a tile's 128 are real.
 #include <cuda.h>
 
