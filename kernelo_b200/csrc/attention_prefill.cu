@@ -20,8 +20,8 @@
 //                    its loads and first products start behind this one's results.
 //
 // m is raised, and O (in TMEM) rescaled, only when a row's maximum grew by more
-// than 2^8: until then the weights are at most 256, which 16 bits and the fp32 sums
-// hold as well. P is rounded to the operands' type for the second product; l sums
+// than 2^8: until then the weights are at most 256 (bf16: one, see WEIGHT_SHIFT), which 16
+// bits and the fp32 sums hold as well. P is rounded to the operands' type for the second product; l sums
 // the unrounded weights.
 //
 // Keys of the next request in a request's last block have weight zero, and
@@ -54,7 +54,6 @@ constexpr int TMA_WARP = 8, MMA_WARP = 9, CLEAN_WARP = 10, PLAN_WARP = 11;
 constexpr int THREADS = 3 * 128;
 constexpr int LAUNCH_REGISTERS = 168;
 constexpr uint32_t TMEM_COLS = 512;  // S0 | S1 | O0 | O1, 128 each
-constexpr float RAISE_LOG2 = 8.0f;
 constexpr uint64_t DRAIN_NS = 100000000ull;
 
 template <int DH>
@@ -511,7 +510,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             tmem_st_32(o_addr + x, o);
           }
         }
-        const float cm = m == -INFINITY ? 0.0f : m * c;
+        const float cm = m == -INFINITY ? 0.0f : fmaf(m, c, WEIGHT_SHIFT<T>);
         // NaN among the row's scores, or infinity: the row is NaN (`m` need not have been raised, and
         // the polynomial takes NaN for zero)
         if (!(m_new * c < INFINITY)) l = NAN;
@@ -565,7 +564,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
       if (p.lse != nullptr && valid)
         p.lse[static_cast<long long>(q_row) * p.heads + it.head] =
-            l == 0.0f ? -INFINITY : m * c * 0.69314718055994530942f + logf(l);
+            l == 0.0f ? -INFINITY : fmaf(m, c, WEIGHT_SHIFT<T>) * 0.69314718055994530942f + logf(l);
       uint32_t again = __ballot_sync(0xffffffffu, valid && suspect(bad == 0.0f, l));
       if (again != 0) {
         redo_begin(abort_flag, lane);

@@ -16,6 +16,15 @@
 
 namespace kf {
 
+// A row's maximum is raised, and its sums rescaled, when it grew by more than this.
+constexpr float RAISE_LOG2 = 8.0f;
+// By so much are the weights made smaller, and the row's maximum (for its sums' base) larger.
+// bf16 weights stay at one or below: a value near the end of the type's range, which is
+// fp32's, would overflow the sums times 2^8. fp16's values are far from that, and its
+// weights would lose bits.
+template <typename T>
+constexpr float WEIGHT_SHIFT = DType<T>::code == KF_BF16 ? RAISE_LOG2 : 0.0f;
+
 // Maxima that a NaN among their operands makes NaN.
 __device__ __forceinline__ float max2(float a, float b) {
   float r;

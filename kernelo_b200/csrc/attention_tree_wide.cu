@@ -40,7 +40,6 @@ constexpr int MIN_RUN = 2;
 constexpr int ITEM_COST = 2;
 constexpr int INFO = 16;  // blocks whose `present` bits are kept: more than the loads run ahead
 constexpr uint32_t TMEM_COLS = 512;  // S0 | S1 | O0 | O1, 128 each
-constexpr float RAISE_LOG2 = 8.0f;
 constexpr uint64_t DRAIN_NS = 100000000ull;
 
 template <int DP_>
@@ -325,7 +324,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           tmem_st_32(o_addr + x, o);
         }
       }
-      const float cm = m == -INFINITY ? 0.0f : m * c;
+      const float cm = m == -INFINITY ? 0.0f : fmaf(m, c, WEIGHT_SHIFT<T>);
       l += row_weights<T, false>(s, c, cm, s_addr, 0, p_full + 8 * (unit & 1), lane);
       first = walk.item_ends(at);
       if (!first) {
@@ -341,7 +340,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       const bool whole = item >= 0 && at.blk + 1 == at.blocks;
       const Partial<M, DP> part(p, blockIdx.x, item >= 0);
       const int t = at.row0 + node;
-      const float top2 = m == -INFINITY ? -INFINITY : m * c;  // base 2, as the partial results keep it
+      const float top2 = m == -INFINITY ? -INFINITY : fmaf(m, c, WEIGHT_SHIFT<T>);  // base 2, as the partial results keep it
       bool bad = false;
 #pragma unroll 1
       for (int x = 0; x < DP; x += 32) {

@@ -15,7 +15,7 @@ import torch
 from kernelo_b200.kernels.attention import prefill_attention, tree_attention
 from kernelo_b200.runtime import native
 from tests import attention_reference as ref
-from tests.test_attention_gpu import DTYPES, HALF, cache, offsets, prompt, random_trees
+from tests.test_attention_gpu import DTYPES, HALF, cache, check_prompt, check_tree, offsets, prompt, random_trees
 
 pytestmark = pytest.mark.gpu
 
@@ -244,3 +244,30 @@ def test_an_infinite_value_at_the_end_of_a_long_prompt(dtype, device):
     assert not out[39999, 0, 9].isfinite() and out[39999, 0, :9].isfinite().all()
     want, want_lse, bound, off = ref.packed(q[40000:], k[40000:], v[40000:], (500,), (500,))
     ref.check(out[40000:], want, bound, f"{dtype}")
+
+
+# --------------------------------------------------------- large values, seen
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_a_seen_large_value_of_a_prompt(dim, dtype, device):
+    """One value of the type's largest size times weights of up to one stays finite, as the result does."""
+    lens = (300,)
+    q, k, v, cu, _ = prompt(lens, lens, 2, 1, dim, dtype, device)
+    for key in (0, 5, *range(128, 136), 200, 290):
+        large = v.clone()
+        large[key] = LARGE[dtype]
+        check_prompt(lens, lens, q, k, large, cu, cu, f"{dtype} key {key}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("context,count", CUTS)
+def test_a_seen_large_value_of_a_cache(context, count, dtype, device):
+    nodes = (count,) * len(context)
+    masks, words = random_trees(nodes)
+    q, k, v, table, lens = cache(context, nodes, 8, 2, 128, 32, dtype, device)
+    for place in (0, 40, context[0] // 2, context[0]):
+        large = v.clone()
+        for r, c in enumerate(context):
+            at = min(place, c)
+            large[table[r, at // 32].long(), :, at % 32] = LARGE[dtype]
+        check_tree(context, nodes, q, k, large, table, lens, f"{dtype} {context} {count} {place}", masks=masks, words=words)
