@@ -498,8 +498,11 @@ __global__ void __launch_bounds__(THREADS, 2)
     walk.advance(p, at);
   }
   if (defer) {
-    attn_wait(finished, 0, abort_flag, status, SITE_ATTN_SOFTMAX);
-    if (first_is_last) {
+    // one thread looks: the warps take one way even where the wait gave up
+    const bool there = attn_wait(finished, 0, abort_flag, status, SITE_ATTN_SOFTMAX);
+    if (tid == 0) last_one = there && first_is_last;
+    join();
+    if (last_one) {
       __threadfence();
       const Cursor c = first_item;
       join_partials<T, M, DP, 32 * WARPS>(p, c, TileRows(p, walk, c), first_owner, first_last, tid, vector_out,
