@@ -22,11 +22,13 @@ int this_device(DeviceInfo** dev) {
 
 constexpr double LOG2_E = 1.4426950408889634;
 constexpr int64_t INT32_LIMIT = 0x7fffffffll;
+// Rows, keys and requests: steps of up to 256 beyond the last one still fit 32 bits.
+constexpr int64_t COUNT_LIMIT = 0x7fffff00ll;
 
 int check_heads(int64_t dtype, int64_t rows, int64_t seqs, int64_t heads, int64_t kv_heads, int64_t dim) {
   if (!known_dtype(dtype)) return invalid("unknown dtype code");
   if (rows < 0 || seqs < 0 || heads < 0 || kv_heads < 0 || dim < 0) return invalid("negative size");
-  if (rows > INT32_LIMIT || seqs > INT32_LIMIT) return invalid("rows and requests are counted in 32 bits");
+  if (rows > COUNT_LIMIT || seqs > COUNT_LIMIT) return invalid("rows and requests are counted in 32 bits");
   if (heads > 0 && (kv_heads == 0 || heads % kv_heads != 0))
     return invalid("query heads must be a multiple of key heads; got " + std::to_string(heads) + " and " +
                    std::to_string(kv_heads));
@@ -56,7 +58,7 @@ int32_t kf_prefill_attention(const kf_prefill_args* args, void* stream) {
   const kf_prefill_args& g = *args;
   int rc = check_heads(g.dtype, g.rows, g.seqs, g.heads, g.kv_heads, g.dim);
   if (rc != KF_OK) return rc;
-  if (g.keys < 0 || g.keys > INT32_LIMIT) return invalid("keys are counted in 32 bits");
+  if (g.keys < 0 || g.keys > COUNT_LIMIT) return invalid("keys are counted in 32 bits");
   if (!std::isfinite(g.scale)) return invalid("scale must be finite");
   if (g.rows == 0 || g.heads == 0 || g.dim == 0) return KF_OK;
   if (g.q == nullptr || g.out == nullptr || g.cu_q == nullptr || g.cu_k == nullptr ||

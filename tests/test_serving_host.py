@@ -171,3 +171,17 @@ def test_c_entries_refuse_outputs_that_overlap():
         packed = native.PREFILL_ARGS.pack(*((base | change)[n] for n in names))
         assert lib.kf_prefill_attention(packed, None) == native.KF_ERR_INVALID_ARGUMENT
         assert message in native.last_error()
+
+
+def test_counts_that_a_step_would_carry_past_32_bits_are_refused():
+    """The kernels go through requests 32, rows 256 and keys 128 at a time, in 32 bits."""
+    lib = native.load()
+    names = ("dtype q sq_row sq_head k sk_row sk_head v sv_row sv_head out so_row so_head lse cu_q cu_k seqs rows "
+             "keys heads kv_heads dim scale causal").split()
+    base = dict.fromkeys(names, 0) | dict(heads=4, kv_heads=2, dim=64, scale=1.0)
+    for name in ("rows", "keys", "seqs"):
+        packed = native.PREFILL_ARGS.pack(*((base | {name: 0x7fffff01})[n] for n in names))
+        assert lib.kf_prefill_attention(packed, None) == native.KF_ERR_INVALID_ARGUMENT, name
+        assert "32 bits" in native.last_error()
+    assert lib.kf_tree_attention_workspace_bytes(0, native.native_code(torch.bfloat16), 0x7fffff01, 1, 4, 2,
+                                                 64) == -native.KF_ERR_INVALID_ARGUMENT
