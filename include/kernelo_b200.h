@@ -410,6 +410,42 @@ typedef struct kf_rotary_args {
 } kf_rotary_args;
 KF_API int32_t kf_rotary(const kf_rotary_args* args, void* stream);
 
+/* kf_norm_rotary: kf_rotary (inverse 0) on heads that are normalised first, each
+ * head x of q and of k to weight * x / sqrt(mean(x^2) + eps), weights [dim] of the
+ * operands' type, in fp32 and rounded once; v is copied as it is. Heads of up to
+ * 256 elements. */
+typedef struct kf_norm_rotary_args {
+  kf_rotary_args rotary;
+  const void* q_weight;
+  const void* k_weight;
+  double eps;
+} kf_norm_rotary_args;
+KF_API int32_t kf_norm_rotary(const kf_norm_rotary_args* args, void* stream);
+
+/* Its gradient, without a cache (rotary.slots null): dq and dk are the gradients of
+ * the outputs; those of the inputs rotary.q and rotary.k go to rotary.q_out and
+ * rotary.k_out, those of the weights (fp32 [dim], sums over all tokens and heads in
+ * a fixed order) to q_weight_grad and k_weight_grad. The workspace
+ * (kf_norm_rotary_grad_workspace_bytes, 4-byte aligned, of any content) is written
+ * and read by this call alone. */
+typedef struct kf_norm_rotary_grad_args {
+  kf_rotary_args rotary;
+  const void* q_weight;
+  const void* k_weight;
+  double eps;
+  const void* dq;
+  int64_t sdq_row, sdq_head;
+  const void* dk;
+  int64_t sdk_row, sdk_head;
+  float* q_weight_grad;
+  float* k_weight_grad;
+  void* workspace;
+  int64_t workspace_bytes;
+} kf_norm_rotary_grad_args;
+KF_API int32_t kf_norm_rotary_grad(const kf_norm_rotary_grad_args* args, void* stream);
+KF_API int64_t kf_norm_rotary_grad_workspace_bytes(int32_t device, int64_t tokens, int64_t heads, int64_t kv_heads,
+                                                   int64_t dim);
+
 /* ---- block tables and slot maps ------------------------------------------------ *
  * One serving step's plan from request lengths. Request r holds context[r] tokens
  * in the first ceil(context[r] / block_size) pages of its row of block_table

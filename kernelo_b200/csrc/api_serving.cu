@@ -46,6 +46,55 @@ int check_output(const void* q, const void* out, int64_t rows, int64_t so_row, i
   return KF_OK;
 }
 
+// *nothing: no element to turn (the other fields are then not set).
+int rotary_args(const kf_rotary_args& g, RotaryArgs* to, bool* nothing) {
+  if (!known_dtype(g.dtype)) return invalid("unknown dtype code");
+  if (g.tokens < 0 || g.heads < 0 || g.kv_heads < 0 || g.dim < 0 || g.table_rows < 0 || g.rot < 0 || g.pages < 0)
+    return invalid("negative size");
+  if (g.rot % 2 != 0 || g.rot > g.dim)
+    return invalid("the turned part must be even and at most the head; got " + std::to_string(g.rot) + " of " +
+                   std::to_string(g.dim));
+  if (g.heads > INT32_LIMIT / 4 || g.kv_heads > INT32_LIMIT / 4 || g.dim > INT32_LIMIT / 4)
+    return invalid("heads and their elements are counted in 32 bits");
+  *nothing = g.tokens == 0 || g.dim == 0 || g.heads + g.kv_heads == 0;
+  if (*nothing) return KF_OK;
+  if ((g.heads > 0 && (g.q == nullptr || g.q_out == nullptr)) || (g.kv_heads > 0 && g.k == nullptr) ||
+      (g.rot > 0 && (g.positions == nullptr || (g.table_rows > 0 && g.table == nullptr))))
+    return invalid("null pointer");
+  const bool cached = g.slots != nullptr && g.kv_heads > 0;
+  if (g.kv_heads > 0 && g.k_out == nullptr && !cached) return invalid("k needs an output or a cache");
+  if (cached && g.block_size < 1) return invalid("block_size must be positive");
+  if (cached && (g.v == nullptr || (g.pages > 0 && (g.k_cache == nullptr || g.v_cache == nullptr))))
+    return invalid("null pointer");
+  RotaryArgs& a = *to;
+  a.dtype = static_cast<int>(g.dtype);
+  a.q = g.q, a.sq_t = g.sq_row, a.sq_h = g.sq_head;
+  a.q_out = g.q_out, a.sqo_t = g.sqo_row, a.sqo_h = g.sqo_head;
+  a.k = g.k, a.sk_t = g.sk_row, a.sk_h = g.sk_head;
+  a.k_out = g.k_out, a.sko_t = g.sko_row, a.sko_h = g.sko_head;
+  a.positions = g.positions, a.table = g.table, a.table_rows = g.table_rows, a.rot = g.rot;
+  if (cached) {
+    a.v = g.v, a.sv_t = g.sv_row, a.sv_h = g.sv_head;
+    a.k_cache = g.k_cache, a.skc_p = g.skc_page, a.skc_h = g.skc_head, a.skc_s = g.skc_slot;
+    a.v_cache = g.v_cache, a.svc_p = g.svc_page, a.svc_h = g.svc_head, a.svc_s = g.svc_slot;
+    a.pages = g.pages, a.block_size = g.block_size;
+    a.slots = g.slots;
+  }
+  a.tokens = g.tokens, a.heads = g.heads, a.kv_heads = g.kv_heads, a.dim = g.dim;
+  a.interleaved = g.interleaved != 0, a.inverse = g.inverse != 0;
+  return KF_OK;
+}
+
+int norm_args(int64_t dim, double eps, NormArgs* to) {
+  if (dim > NORM_ROTARY_MAX_DIM)
+    return set_error(KF_ERR_UNSUPPORTED, "norms of heads of at most " + std::to_string(NORM_ROTARY_MAX_DIM) +
+                                             " elements; got " + std::to_string(dim));
+  if (!(eps > 0.0) || !std::isfinite(eps)) return invalid("eps must be finite and positive");
+  to->eps = static_cast<float>(eps);
+  to->inv_dim = dim > 0 ? 1.0f / static_cast<float>(dim) : 0.0f;
+  return KF_OK;
+}
+
 }  // namespace
 }  // namespace kf
 
@@ -142,44 +191,75 @@ int64_t kf_tree_attention_workspace_bytes(int32_t device, int32_t dtype, int64_t
 
 int32_t kf_rotary(const kf_rotary_args* args, void* stream) {
   if (args == nullptr) return invalid("null arguments");
-  const kf_rotary_args& g = *args;
-  if (!known_dtype(g.dtype)) return invalid("unknown dtype code");
-  if (g.tokens < 0 || g.heads < 0 || g.kv_heads < 0 || g.dim < 0 || g.table_rows < 0 || g.rot < 0 || g.pages < 0)
-    return invalid("negative size");
-  if (g.rot % 2 != 0 || g.rot > g.dim)
-    return invalid("the turned part must be even and at most the head; got " + std::to_string(g.rot) + " of " +
-                   std::to_string(g.dim));
-  if (g.heads > INT32_LIMIT / 4 || g.kv_heads > INT32_LIMIT / 4 || g.dim > INT32_LIMIT / 4)
-    return invalid("heads and their elements are counted in 32 bits");
-  if (g.tokens == 0 || g.dim == 0 || g.heads + g.kv_heads == 0) return KF_OK;
-  if ((g.heads > 0 && (g.q == nullptr || g.q_out == nullptr)) || (g.kv_heads > 0 && g.k == nullptr) ||
-      (g.rot > 0 && (g.positions == nullptr || (g.table_rows > 0 && g.table == nullptr))))
-    return invalid("null pointer");
-  const bool cached = g.slots != nullptr && g.kv_heads > 0;
-  if (g.kv_heads > 0 && g.k_out == nullptr && !cached) return invalid("k needs an output or a cache");
-  if (cached && g.block_size < 1) return invalid("block_size must be positive");
-  if (cached && (g.v == nullptr || (g.pages > 0 && (g.k_cache == nullptr || g.v_cache == nullptr))))
-    return invalid("null pointer");
   RotaryArgs a;
-  a.dtype = static_cast<int>(g.dtype);
-  a.q = g.q, a.sq_t = g.sq_row, a.sq_h = g.sq_head;
-  a.q_out = g.q_out, a.sqo_t = g.sqo_row, a.sqo_h = g.sqo_head;
-  a.k = g.k, a.sk_t = g.sk_row, a.sk_h = g.sk_head;
-  a.k_out = g.k_out, a.sko_t = g.sko_row, a.sko_h = g.sko_head;
-  a.positions = g.positions, a.table = g.table, a.table_rows = g.table_rows, a.rot = g.rot;
-  if (cached) {
-    a.v = g.v, a.sv_t = g.sv_row, a.sv_h = g.sv_head;
-    a.k_cache = g.k_cache, a.skc_p = g.skc_page, a.skc_h = g.skc_head, a.skc_s = g.skc_slot;
-    a.v_cache = g.v_cache, a.svc_p = g.svc_page, a.svc_h = g.svc_head, a.svc_s = g.svc_slot;
-    a.pages = g.pages, a.block_size = g.block_size;
-    a.slots = g.slots;
-  }
-  a.tokens = g.tokens, a.heads = g.heads, a.kv_heads = g.kv_heads, a.dim = g.dim;
-  a.interleaved = g.interleaved != 0, a.inverse = g.inverse != 0;
+  bool nothing = false;
+  int rc = rotary_args(*args, &a, &nothing);
+  if (rc != KF_OK || nothing) return rc;
   DeviceInfo* dev = nullptr;
-  const int rc = this_device(&dev);
+  rc = this_device(&dev);
   if (rc != KF_OK) return rc;
   return launch_rotary(a, *dev, static_cast<cudaStream_t>(stream));
+}
+
+int32_t kf_norm_rotary(const kf_norm_rotary_args* args, void* stream) {
+  if (args == nullptr) return invalid("null arguments");
+  const kf_norm_rotary_args& g = *args;
+  RotaryArgs a;
+  NormArgs n;
+  bool nothing = false;
+  int rc = rotary_args(g.rotary, &a, &nothing);
+  if (rc == KF_OK) rc = norm_args(g.rotary.dim, g.eps, &n);
+  if (rc != KF_OK) return rc;
+  if (g.rotary.inverse != 0) return invalid("inverse: the gradient of norms and turn is kf_norm_rotary_grad");
+  if (nothing) return KF_OK;
+  if ((a.heads > 0 && g.q_weight == nullptr) || (a.kv_heads > 0 && g.k_weight == nullptr)) return invalid("null pointer");
+  n.q_weight = g.q_weight, n.k_weight = g.k_weight;
+  DeviceInfo* dev = nullptr;
+  rc = this_device(&dev);
+  if (rc != KF_OK) return rc;
+  return launch_norm_rotary(a, n, *dev, static_cast<cudaStream_t>(stream));
+}
+
+int32_t kf_norm_rotary_grad(const kf_norm_rotary_grad_args* args, void* stream) {
+  if (args == nullptr) return invalid("null arguments");
+  const kf_norm_rotary_grad_args& g = *args;
+  NormGradArgs a;
+  bool nothing = false;
+  int rc = rotary_args(g.rotary, &a.rotary, &nothing);
+  if (rc == KF_OK) rc = norm_args(g.rotary.dim, g.eps, &a.norm);
+  if (rc != KF_OK) return rc;
+  if (g.rotary.inverse != 0) return invalid("inverse: the gradient is of the forward turn");
+  if (g.rotary.slots != nullptr) return invalid("the gradient has no cache");
+  if (g.rotary.dim == 0) return KF_OK;
+  if (g.q_weight_grad == nullptr || g.k_weight_grad == nullptr) return invalid("null pointer");
+  if (!nothing && ((g.rotary.heads > 0 && (g.dq == nullptr || g.q_weight == nullptr)) ||
+                   (g.rotary.kv_heads > 0 && (g.dk == nullptr || g.k_weight == nullptr))))
+    return invalid("null pointer");
+  if (nothing) a.rotary.tokens = 0, a.rotary.dim = g.rotary.dim;
+  DeviceInfo* dev = nullptr;
+  rc = this_device(&dev);
+  if (rc != KF_OK) return rc;
+  const RotaryArgs& r = a.rotary;
+  if (g.workspace_bytes < norm_rotary_grad_workspace_bytes(r.tokens, r.heads, r.kv_heads, r.dim, *dev) ||
+      (g.workspace == nullptr && g.workspace_bytes > 0))
+    return set_error(KF_ERR_WORKSPACE, "workspace too small for the weights' partial sums");
+  if ((reinterpret_cast<uintptr_t>(g.workspace) & 3u) != 0)
+    return set_error(KF_ERR_WORKSPACE, "workspace must be 4-byte aligned");
+  a.norm.q_weight = g.q_weight, a.norm.k_weight = g.k_weight;
+  a.dq = g.dq, a.sdq_t = g.sdq_row, a.sdq_h = g.sdq_head;
+  a.dk = g.dk, a.sdk_t = g.sdk_row, a.sdk_h = g.sdk_head;
+  a.q_weight_grad = g.q_weight_grad, a.k_weight_grad = g.k_weight_grad;
+  a.partial = static_cast<float*>(g.workspace);
+  return launch_norm_rotary_grad(a, *dev, static_cast<cudaStream_t>(stream));
+}
+
+int64_t kf_norm_rotary_grad_workspace_bytes(int32_t device, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim) {
+  if (tokens < 0 || heads < 0 || kv_heads < 0 || dim < 0) return -invalid("negative size");
+  if (heads > INT32_LIMIT / 4 || kv_heads > INT32_LIMIT / 4) return -invalid("heads are counted in 32 bits");
+  DeviceInfo* dev = nullptr;
+  const int rc = device_info(device, &dev);
+  if (rc != KF_OK) return -rc;
+  return norm_rotary_grad_workspace_bytes(tokens, heads, kv_heads, dim, *dev);
 }
 
 int32_t kf_build_slots(const kf_slots_args* args, void* stream) {

@@ -320,6 +320,31 @@ struct RotaryArgs {
 };
 int launch_rotary(const RotaryArgs& args, const DeviceInfo& dev, cudaStream_t stream);
 
+// The same with each head of q and k normalised first (norm_rotary.cu).
+struct NormArgs {
+  const void* q_weight = nullptr;
+  const void* k_weight = nullptr;
+  float eps = 0.0f, inv_dim = 0.0f;
+};
+constexpr int NORM_ROTARY_MAX_DIM = 256;
+int launch_norm_rotary(const RotaryArgs& args, const NormArgs& norm, const DeviceInfo& dev, cudaStream_t stream);
+// Its gradient: `rotary` has the inputs q and k, and in q_out and k_out the places of their gradients; dq and dk are those
+// of the outputs. `partial` (norm_rotary_grad_workspace_bytes): sums of the weights' gradients that blocks leave.
+struct NormGradArgs {
+  RotaryArgs rotary;
+  NormArgs norm;
+  const void* dq = nullptr;
+  int64_t sdq_t = 0, sdq_h = 0;
+  const void* dk = nullptr;
+  int64_t sdk_t = 0, sdk_h = 0;
+  float* q_weight_grad = nullptr;
+  float* k_weight_grad = nullptr;
+  float* partial = nullptr;
+};
+int64_t norm_rotary_grad_workspace_bytes(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim,
+                                         const DeviceInfo& dev);
+int launch_norm_rotary_grad(const NormGradArgs& args, const DeviceInfo& dev, cudaStream_t stream);
+
 // Block tables and slot maps from request lengths (slots.cu).
 int launch_slots(const kf_slots_args& args, const DeviceInfo& dev, cudaStream_t stream);
 

@@ -6,6 +6,10 @@ the token's position: pairs ``(i, i + rot/2)``, or ``(2i, 2i + 1)`` with
 from a table that :func:`rotary_table` makes once, in 64 bits, plain or scaled
 for contexts longer than a model was trained on. The rotation is orthogonal, so
 its gradient is the turn back: ``inverse=True``.
+
+Models that normalise each head of q and k before the turn do both in one pass
+with :func:`norm_rotary` and :func:`norm_rotary_to_cache`, and have the gradient
+of both from :func:`norm_rotary_backward`.
 """
 
 from __future__ import annotations
@@ -14,10 +18,12 @@ import math
 
 import torch
 
-from kernelo_b200.kernels.attention import _check_index, _check_operand, _empty_like
+from kernelo_b200.kernels.attention import _check_index, _check_operand, _check_output, _empty_like
+from kernelo_b200.kernels.rmsnorm import DEFAULT_EPS
 from kernelo_b200.runtime import native
 
 SCALINGS = ("linear", "base", "parts")
+MAX_NORM_DIM = 256
 
 
 def rotary_table(
@@ -112,6 +118,19 @@ def _check_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: tor
         raise ValueError(f"slots must have shape ({q.shape[0]},), got {tuple(slots.shape)}")
 
 
+def _check_cached(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                  slots: torch.Tensor) -> None:
+    dtype, device = q.dtype, q.get_device()
+    if not (v.shape == k.shape and v.dtype is dtype and v.get_device() == device and v.stride(2) == 1
+            and k_cache.ndim == 4 and v_cache.shape == k_cache.shape and k_cache.shape[1] == k.shape[1]
+            and k_cache.shape[3] == k.shape[2] and k_cache.shape[2] > 0 and k_cache.dtype is dtype
+            and v_cache.dtype is dtype and k_cache.get_device() == device == v_cache.get_device()
+            and k_cache.stride(3) == 1 == v_cache.stride(3) and slots.dtype is torch.int64
+            and slots.get_device() == device and slots.ndim == 1 and slots.shape[0] == q.shape[0]
+            and slots.is_contiguous()):
+        _check_cache(q, k, v, k_cache, v_cache, slots)
+
+
 def _output(name: str, out: torch.Tensor | None, like: torch.Tensor) -> torch.Tensor:
     if out is None:
         return _empty_like(like)
@@ -169,15 +188,7 @@ def rotary_to_cache(
     end up in it.
     """
     _check(q, k, positions, table)
-    dtype, device = q.dtype, q.get_device()
-    if not (v.shape == k.shape and v.dtype is dtype and v.get_device() == device and v.stride(2) == 1
-            and k_cache.ndim == 4 and v_cache.shape == k_cache.shape and k_cache.shape[1] == k.shape[1]
-            and k_cache.shape[3] == k.shape[2] and k_cache.shape[2] > 0 and k_cache.dtype is dtype
-            and v_cache.dtype is dtype and k_cache.get_device() == device == v_cache.get_device()
-            and k_cache.stride(3) == 1 == v_cache.stride(3) and slots.dtype is torch.int64
-            and slots.get_device() == device and slots.ndim == 1 and slots.shape[0] == q.shape[0]
-            and slots.is_contiguous()):
-        _check_cache(q, k, v, k_cache, v_cache, slots)
+    _check_cached(q, k, v, k_cache, v_cache, slots)
     q_out = _output("q_out", q_out, q)
     if k_out is not None:
         k_out = _output("k_out", k_out, k)
@@ -185,3 +196,131 @@ def rotary_to_cache(
         native.rotary(q, k, q_out, k_out, positions, table, interleaved=interleaved, inverse=False, v=v,
                       k_cache=k_cache, v_cache=v_cache, slots=slots)
     return q_out
+
+
+def _check_norm(q: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, eps: float) -> None:
+    dim = q.shape[2]
+    if dim > MAX_NORM_DIM:
+        raise ValueError(f"norms take heads of at most {MAX_NORM_DIM} elements, got {dim}")
+    if not 0.0 < eps < math.inf:
+        raise ValueError(f"eps must be finite and positive, got {eps}")
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w.ndim != 1 or w.shape[0] != dim:
+            raise ValueError(f"{name} must have shape ({dim},), got {tuple(w.shape)}")
+        _check_operand(name, w, q)
+
+
+def _same_place(a: torch.Tensor, b: torch.Tensor) -> bool:
+    return a.data_ptr() == b.data_ptr() and a.shape == b.shape and a.stride() == b.stride()
+
+
+def _norm_outputs(q: torch.Tensor, k: torch.Tensor, q_out: torch.Tensor | None, k_out: torch.Tensor | None,
+                  others: dict[str, torch.Tensor]) -> None:
+    """Outputs given by the caller: q and k themselves, or memory that no operand and no other output shares."""
+    given = {name: (out, x) for name, out, x in (("q_out", q_out, q), ("k_out", k_out, k)) if out is not None}
+    for name, (out, x) in given.items():
+        if out.shape != x.shape:
+            raise ValueError(f"{name} must have shape {tuple(x.shape)}, got {tuple(out.shape)}")
+        _check_operand(name, out, x)
+        own = "q" if x is q else "k"
+        operands = {"q": q, "k": k, **others}
+        if _same_place(out, x):
+            del operands[own]
+        if name == "k_out" and q_out is not None:
+            operands["q_out"] = q_out
+        _check_output(name, out, operands)
+
+
+def norm_rotary(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    positions: torch.Tensor,
+    table: torch.Tensor,
+    q_weight: torch.Tensor,
+    k_weight: torch.Tensor,
+    *,
+    eps: float = DEFAULT_EPS,
+    interleaved: bool = False,
+    q_out: torch.Tensor | None = None,
+    k_out: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """:func:`rotary` of heads normalised first: each head ``x`` of q and k becomes
+    ``weight * x / sqrt(mean(x^2) + eps)`` before its turn.
+
+    ``q_weight`` and ``k_weight`` (``(dim,)``, of the operands' type) are shared
+    by the heads of q and those of k. Everything is computed in fp32 and rounded
+    once, so the result is nearer than that of a norm and a turn apart. ``q_out``
+    / ``k_out`` may be q and k themselves, and share no other operand's memory.
+    """
+    _check(q, k, positions, table)
+    _check_norm(q, q_weight, k_weight, eps)
+    if q_out is not None or k_out is not None:
+        _norm_outputs(q, k, q_out, k_out, {})
+    q_out = _empty_like(q) if q_out is None else q_out
+    k_out = _empty_like(k) if k_out is None else k_out
+    if q.numel() or k.numel():
+        native.norm_rotary(q, k, q_out, k_out, positions, table, q_weight, k_weight, eps, interleaved=interleaved)
+    return q_out, k_out
+
+
+def norm_rotary_to_cache(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    positions: torch.Tensor,
+    table: torch.Tensor,
+    q_weight: torch.Tensor,
+    k_weight: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    slots: torch.Tensor,
+    *,
+    eps: float = DEFAULT_EPS,
+    interleaved: bool = False,
+    q_out: torch.Tensor | None = None,
+    k_out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """:func:`rotary_to_cache` of heads normalised first, as :func:`norm_rotary` does; v is written as it is."""
+    _check(q, k, positions, table)
+    _check_cached(q, k, v, k_cache, v_cache, slots)
+    _check_norm(q, q_weight, k_weight, eps)
+    if q_out is not None or k_out is not None:
+        _norm_outputs(q, k, q_out, k_out, {"v": v, "k_cache": k_cache, "v_cache": v_cache})
+    q_out = _empty_like(q) if q_out is None else q_out
+    if q.numel() or k.numel():
+        native.norm_rotary(q, k, q_out, k_out, positions, table, q_weight, k_weight, eps, interleaved=interleaved, v=v,
+                           k_cache=k_cache, v_cache=v_cache, slots=slots)
+    return q_out
+
+
+def norm_rotary_backward(
+    dq: torch.Tensor,
+    dk: torch.Tensor,
+    q: torch.Tensor,
+    k: torch.Tensor,
+    positions: torch.Tensor,
+    table: torch.Tensor,
+    q_weight: torch.Tensor,
+    k_weight: torch.Tensor,
+    *,
+    eps: float = DEFAULT_EPS,
+    interleaved: bool = False,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Gradients of q, k, ``q_weight`` and ``k_weight``, given those of :func:`norm_rotary`'s outputs and its inputs.
+
+    The weights' gradients are fp32 sums over all tokens and heads, added in a
+    fixed order: a call on the same operands gives the same bits. A token whose
+    position the table lacks makes them NaN.
+    """
+    _check(q, k, positions, table)
+    _check_norm(q, q_weight, k_weight, eps)
+    for name, d, x in (("dq", dq, q), ("dk", dk, k)):
+        if d.shape != x.shape:
+            raise ValueError(f"{name} must have shape {tuple(x.shape)}, got {tuple(d.shape)}")
+        _check_operand(name, d, q)
+    q_grad, k_grad = _empty_like(q), _empty_like(k)
+    weight_grads = torch.empty(2, q.shape[2], device=q.device, dtype=torch.float32)
+    if q.shape[2]:
+        native.norm_rotary_grad(dq, dk, q, k, q_grad, k_grad, positions, table, q_weight, k_weight, eps, weight_grads,
+                                interleaved=interleaved)
+    return q_grad, k_grad, *weight_grads.unbind(0)

@@ -80,6 +80,9 @@ EXPORTED_SYMBOLS = (
     "kf_tree_attention_workspace_bytes",
     "kf_rotary",
     "kf_build_slots",
+    "kf_norm_rotary",
+    "kf_norm_rotary_grad",
+    "kf_norm_rotary_grad_workspace_bytes",
 )
 
 
@@ -170,6 +173,8 @@ PREFILL_ARGS = struct.Struct("22qdq")
 TREE_ARGS = struct.Struct("30qd2q")
 ROTARY_ARGS = struct.Struct("37q")
 SLOTS_ARGS = struct.Struct("14q")
+NORM_ROTARY_ARGS = struct.Struct("39qd")
+NORM_ROTARY_GRAD_ARGS = struct.Struct("39qd10q")
 
 _SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "kf_abi_version": (_i32, []),
@@ -210,6 +215,9 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "kf_rotary": (_i32, [_packed, _vp]),
     "kf_stream_capture_id": (_i32, [_vp, ctypes.POINTER(_i64)]),
     "kf_build_slots": (_i32, [_packed, _vp]),
+    "kf_norm_rotary": (_i32, [_packed, _vp]),
+    "kf_norm_rotary_grad": (_i32, [_packed, _vp]),
+    "kf_norm_rotary_grad_workspace_bytes": (_i64, [_i32, _i64, _i64, _i64, _i64]),
 }
 
 _lock = threading.Lock()
@@ -730,6 +738,15 @@ def rotary(q: torch.Tensor, k: torch.Tensor, q_out: torch.Tensor, k_out: torch.T
            slots: torch.Tensor | None = None) -> None:
     """Turn q and k by their positions' angles (and, with ``slots``, write the cache)."""
     lib = _lib or load()
+    status = lib.kf_rotary(
+        ROTARY_ARGS.pack(*_rotary_fields(q, k, q_out, k_out, positions, table, interleaved, inverse, v, k_cache, v_cache,
+                                         slots)),
+        current_stream_handle(q.device))
+    if status:
+        check(status, "kf_rotary")
+
+
+def _rotary_fields(q, k, q_out, k_out, positions, table, interleaved, inverse, v, k_cache, v_cache, slots) -> tuple:
     tokens, heads, dim = q.shape
     sq_row, sq_head, _ = q.stride()
     sqo_row, sqo_head, _ = q_out.stride()
@@ -744,17 +761,65 @@ def rotary(q: torch.Tensor, k: torch.Tensor, q_out: torch.Tensor, k_out: torch.T
         svc_page, svc_head, svc_slot, _ = v_cache.stride()
         cached = (v.data_ptr(), sv_row, sv_head, k_cache.data_ptr(), skc_page, skc_head, skc_slot, v_cache.data_ptr(),
                   svc_page, svc_head, svc_slot, k_cache.shape[0], k_cache.shape[2], slots.data_ptr())
-    status = lib.kf_rotary(
-        ROTARY_ARGS.pack(native_code(q.dtype), q.data_ptr(), sq_row, sq_head, q_out.data_ptr(), sqo_row, sqo_head,
-                         k.data_ptr(), sk_row, sk_head, 0 if k_out is None else k_out.data_ptr(), sko_row, sko_head,
-                         positions.data_ptr(), table.data_ptr(), table_rows, rot, tokens, heads, k.shape[1], dim,
-                         interleaved, inverse, *cached),
-        current_stream_handle(q.device))
-    if status:
-        check(status, "kf_rotary")
+    return (native_code(q.dtype), q.data_ptr(), sq_row, sq_head, q_out.data_ptr(), sqo_row, sqo_head, k.data_ptr(), sk_row,
+            sk_head, 0 if k_out is None else k_out.data_ptr(), sko_row, sko_head, positions.data_ptr(), table.data_ptr(),
+            table_rows, rot, tokens, heads, k.shape[1], dim, interleaved, inverse, *cached)
 
 
 _NO_CACHE = (0,) * 14
+
+
+def norm_rotary(q: torch.Tensor, k: torch.Tensor, q_out: torch.Tensor, k_out: torch.Tensor | None,
+                positions: torch.Tensor, table: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, eps: float, *,
+                interleaved: bool, v: torch.Tensor | None = None, k_cache: torch.Tensor | None = None,
+                v_cache: torch.Tensor | None = None, slots: torch.Tensor | None = None) -> None:
+    """Normalise and turn q's and k's heads (and, with ``slots``, write the cache)."""
+    lib = _lib or load()
+    _launch(lib.kf_norm_rotary,
+            NORM_ROTARY_ARGS.pack(*_rotary_fields(q, k, q_out, k_out, positions, table, interleaved, False, v, k_cache,
+                                                  v_cache, slots), q_weight.data_ptr(), k_weight.data_ptr(), eps),
+            q.device, "kf_norm_rotary")
+
+
+def _launch(entry, packed: bytes, device: torch.device, what: str) -> None:
+    """The entry on the device's current stream, with the device made the current one where it is not."""
+    if device.index == torch.cuda.current_device():
+        status = entry(packed, current_stream_handle(device))
+    else:
+        with torch.cuda.device(device):
+            status = entry(packed, current_stream_handle(device))
+    if status:
+        check(status, what)
+
+
+def norm_rotary_grad(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor, k: torch.Tensor, q_grad: torch.Tensor,
+                     k_grad: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, q_weight: torch.Tensor,
+                     k_weight: torch.Tensor, eps: float, weight_grads: torch.Tensor, *, interleaved: bool) -> None:
+    """``weight_grads``: fp32 (2, dim), q's and k's."""
+    lib = _lib or load()
+    dev = q.device
+    tokens, heads, dim = q.shape
+    kv_heads = k.shape[1]
+    key = ("norm_rotary_grad", dev.index, tokens, heads, kv_heads, dim)
+    ws_bytes = _workspace_sizes.get(key)
+    if ws_bytes is None:
+        ws_bytes = lib.kf_norm_rotary_grad_workspace_bytes(dev.index or 0, tokens, heads, kv_heads, dim)
+        if ws_bytes < 0:
+            check(int(-ws_bytes), "kf_norm_rotary_grad_workspace_bytes")
+        if len(_workspace_sizes) > 4096:
+            _workspace_sizes.clear()
+        _workspace_sizes[key] = ws_bytes
+    # plain memory of this call, not the stream's workspace, whose first words are other kernels' counters
+    partial = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    sdq_row, sdq_head, _ = dq.stride()
+    sdk_row, sdk_head, _ = dk.stride()
+    _launch(lib.kf_norm_rotary_grad,
+            NORM_ROTARY_GRAD_ARGS.pack(*_rotary_fields(q, k, q_grad, k_grad, positions, table, interleaved, False, None, None,
+                                                       None, None), q_weight.data_ptr(), k_weight.data_ptr(), eps,
+                                       dq.data_ptr(), sdq_row, sdq_head, dk.data_ptr(), sdk_row, sdk_head,
+                                       weight_grads.data_ptr(), weight_grads.data_ptr() + 4 * dim, partial.data_ptr(),
+                                       ws_bytes),
+            dev, "kf_norm_rotary_grad")
 
 
 def build_slots(context: torch.Tensor, added: torch.Tensor, block_table: torch.Tensor, free_blocks: torch.Tensor,
