@@ -471,6 +471,43 @@ typedef struct kf_slots_args {
 } kf_slots_args;
 KF_API int32_t kf_build_slots(const kf_slots_args* args, void* stream);
 
+/* ---- logits: penalties, biases, masks -------------------------------------------- *
+ * out = logits [rows, vocab] (out may be logits; otherwise no memory is shared) after,
+ * in this order and in fp32: the penalties of the row's history, its biases, its mask.
+ * tokens [rows, token_cols] (null: no history) begins with the row's token_lens[r]
+ * tokens, of which the first prompt_lens[r] (null: none) are a prompt. Every token of
+ * the history: x / repetition[r] where x is positive, else x * repetition[r]. Those
+ * that stand n > 0 times behind the prompt: x - (frequency[r] * n + presence[r]). (Null
+ * factors have no effect.) bias_tokens and bias_values [rows, bias_cols] (null: none):
+ * x + value; of several entries with one token the last counts. allowed: bit v % 32 of
+ * word v / 32 of a mask [masks, at least ceil(vocab / 32)] is 0 where token v becomes
+ * -infinity; the row's mask is allowed_rows[r] (null: r), and where that is none of the
+ * masks every token is allowed. Tokens outside the vocabulary are ignored. */
+typedef struct kf_logits_args {
+  int64_t dtype;
+  const void* logits;
+  int64_t s_row;
+  void* out;
+  int64_t so_row;
+  int64_t rows, vocab;
+  const int32_t* tokens;
+  int64_t st_row, token_cols;
+  const int32_t* token_lens;
+  const int32_t* prompt_lens;
+  const float* repetition;
+  const float* frequency;
+  const float* presence;
+  const int32_t* bias_tokens;
+  int64_t sb_row;
+  const float* bias_values;
+  int64_t sv_row;
+  int64_t bias_cols;
+  const int32_t* allowed;
+  int64_t sa_row, masks;
+  const int32_t* allowed_rows;
+} kf_logits_args;
+KF_API int32_t kf_adjust_logits(const kf_logits_args* args, void* stream);
+
 /* ---- fused linear + all-gather over NVLink ---------------------------------- *
  * kf_linear_bias_act, and every output tile is also stored into the n_peers
  * buffers y_peers[i]: device pointers (peer-mapped, e.g. symmetric memory) to

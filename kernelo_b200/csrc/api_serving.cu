@@ -24,6 +24,8 @@ constexpr double LOG2_E = 1.4426950408889634;
 constexpr int64_t INT32_LIMIT = 0x7fffffffll;
 // Rows, keys and requests: steps of up to 256 beyond the last one still fit 32 bits.
 constexpr int64_t COUNT_LIMIT = 0x7fffff00ll;
+// Tokens of a vocabulary, a history or a list of biases: a chunk or a stride of a block beyond the last one, too.
+constexpr int64_t LOGITS_LIMIT = 0x7fff0000ll;
 
 int check_heads(int64_t dtype, int64_t rows, int64_t seqs, int64_t heads, int64_t kv_heads, int64_t dim) {
   if (!known_dtype(dtype)) return invalid("unknown dtype code");
@@ -260,6 +262,24 @@ int64_t kf_norm_rotary_grad_workspace_bytes(int32_t device, int64_t tokens, int6
   const int rc = device_info(device, &dev);
   if (rc != KF_OK) return -rc;
   return norm_rotary_grad_workspace_bytes(tokens, heads, kv_heads, dim, *dev);
+}
+
+int32_t kf_adjust_logits(const kf_logits_args* args, void* stream) {
+  if (args == nullptr) return invalid("null arguments");
+  const kf_logits_args& g = *args;
+  if (!known_dtype(g.dtype)) return invalid("unknown dtype code");
+  if (g.rows < 0 || g.vocab < 0 || g.token_cols < 0 || g.bias_cols < 0 || g.masks < 0) return invalid("negative size");
+  if (g.rows > COUNT_LIMIT || g.vocab > LOGITS_LIMIT || g.token_cols > LOGITS_LIMIT || g.bias_cols > LOGITS_LIMIT)
+    return invalid("rows, tokens and biases are counted in 32 bits");
+  if (g.rows == 0 || g.vocab == 0) return KF_OK;
+  if (g.logits == nullptr || g.out == nullptr || (g.tokens != nullptr && g.token_lens == nullptr) ||
+      (g.bias_tokens != nullptr && g.bias_values == nullptr))
+    return invalid("null pointer");
+  if (g.rows > 1 && g.so_row == 0) return invalid("out overlaps itself: a stride of zero");
+  DeviceInfo* dev = nullptr;
+  const int rc = this_device(&dev);
+  if (rc != KF_OK) return rc;
+  return launch_logits(g, *dev, static_cast<cudaStream_t>(stream));
 }
 
 int32_t kf_build_slots(const kf_slots_args* args, void* stream) {

@@ -348,6 +348,9 @@ int launch_norm_rotary_grad(const NormGradArgs& args, const DeviceInfo& dev, cud
 // Block tables and slot maps from request lengths (slots.cu).
 int launch_slots(const kf_slots_args& args, const DeviceInfo& dev, cudaStream_t stream);
 
+// Penalties, biases and masks on rows of logits (logits.cu).
+int launch_logits(const kf_logits_args& args, const DeviceInfo& dev, cudaStream_t stream);
+
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 }  // namespace kf

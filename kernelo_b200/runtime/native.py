@@ -80,6 +80,7 @@ EXPORTED_SYMBOLS = (
     "kf_tree_attention_workspace_bytes",
     "kf_rotary",
     "kf_build_slots",
+    "kf_adjust_logits",
     "kf_norm_rotary",
     "kf_norm_rotary_grad",
     "kf_norm_rotary_grad_workspace_bytes",
@@ -173,6 +174,7 @@ PREFILL_ARGS = struct.Struct("22qdq")
 TREE_ARGS = struct.Struct("30qd2q")
 ROTARY_ARGS = struct.Struct("37q")
 SLOTS_ARGS = struct.Struct("14q")
+LOGITS_ARGS = struct.Struct("24q")
 NORM_ROTARY_ARGS = struct.Struct("39qd")
 NORM_ROTARY_GRAD_ARGS = struct.Struct("39qd10q")
 
@@ -215,6 +217,7 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "kf_rotary": (_i32, [_packed, _vp]),
     "kf_stream_capture_id": (_i32, [_vp, ctypes.POINTER(_i64)]),
     "kf_build_slots": (_i32, [_packed, _vp]),
+    "kf_adjust_logits": (_i32, [_packed, _vp]),
     "kf_norm_rotary": (_i32, [_packed, _vp]),
     "kf_norm_rotary_grad": (_i32, [_packed, _vp]),
     "kf_norm_rotary_grad_workspace_bytes": (_i64, [_i32, _i64, _i64, _i64, _i64]),
@@ -820,6 +823,23 @@ def norm_rotary_grad(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor, k: tor
                                        weight_grads.data_ptr(), weight_grads.data_ptr() + 4 * dim, partial.data_ptr(),
                                        ws_bytes),
             dev, "kf_norm_rotary_grad")
+
+
+def adjust_logits(logits: torch.Tensor, out: torch.Tensor, tokens: torch.Tensor | None, token_lens: torch.Tensor | None,
+                  prompt_lens: torch.Tensor | None, repetition: torch.Tensor | None, frequency: torch.Tensor | None,
+                  presence: torch.Tensor | None, bias_tokens: torch.Tensor | None, bias_values: torch.Tensor | None,
+                  allowed: torch.Tensor | None, allowed_rows: torch.Tensor | None) -> None:
+    lib = _lib or load()
+    rows, vocab = logits.shape
+    history = (0, 0, 0) if tokens is None else (tokens.data_ptr(), tokens.stride(0), tokens.shape[1])
+    biases = (0, 0, 0, 0, 0) if bias_tokens is None else (
+        bias_tokens.data_ptr(), bias_tokens.stride(0), bias_values.data_ptr(), bias_values.stride(0), bias_tokens.shape[1])
+    masks = (0, 0, 0) if allowed is None else (allowed.data_ptr(), allowed.stride(0), allowed.shape[0])
+    _launch(lib.kf_adjust_logits,
+            LOGITS_ARGS.pack(native_code(logits.dtype), logits.data_ptr(), logits.stride(0), out.data_ptr(), out.stride(0),
+                             rows, vocab, *history, _ptr(token_lens) or 0, _ptr(prompt_lens) or 0, _ptr(repetition) or 0,
+                             _ptr(frequency) or 0, _ptr(presence) or 0, *biases, *masks, _ptr(allowed_rows) or 0),
+            logits.device, "kf_adjust_logits")
 
 
 def build_slots(context: torch.Tensor, added: torch.Tensor, block_table: torch.Tensor, free_blocks: torch.Tensor,
