@@ -471,6 +471,83 @@ typedef struct kf_slots_args {
 } kf_slots_args;
 KF_API int32_t kf_build_slots(const kf_slots_args* args, void* stream);
 
+/* ---- pages that fork, end, and move ------------------------------------------------ *
+ * Requests whose rows of block_table [rows, table_cols] hold the pages of their
+ * context[r] tokens (as in kf_build_slots) may hold pages together: holders[p]
+ * (int32 [pages]) counts those that hold page p besides the first, so it is 0 for a
+ * page of one request and for a free one. Caches of one type, shape and strides
+ * [pages, heads, block_size, dim] (every layer's keys and values) change together;
+ * `caches` is a host array of their addresses. Page and request numbers that are
+ * none are skipped, never followed. */
+typedef struct kf_page_caches {
+  int64_t dtype;
+  void* const* caches;
+  int64_t n_caches;
+  int64_t s_page, s_head, s_slot;
+  int64_t pages, heads, block_size, dim;
+} kf_page_caches;
+
+/* kf_fork: row children[i] becomes a copy of the request in row parents[i]: its whole
+ * pages are held together from now on, and the tokens of its last, partial page are
+ * copied in every cache to a page of the child's own, the next one of free_blocks for
+ * each pair in order. The rest of the child's row becomes -1, its context its
+ * parent's. A pair whose child is named by two pairs, or is a parent, or whose rows
+ * are none, does nothing. counts[0]: pages taken (of the front of free_blocks; more
+ * than n_free: it ran out, and the last pairs have -1 for the partial page);
+ * counts[1]: pairs that did nothing or lack a page. */
+typedef struct kf_fork_args {
+  kf_page_caches caches;
+  int32_t* block_table;
+  int64_t table_stride, table_cols, rows;
+  int32_t* context;
+  int32_t* holders;
+  const int32_t* free_blocks;
+  int64_t n_free;
+  const int32_t* parents;
+  const int32_t* children;
+  int64_t pairs;
+  int32_t* counts;
+} kf_fork_args;
+KF_API int32_t kf_fork(const kf_fork_args* args, void* stream);
+
+/* kf_release: the requests in the rows that `requests` [count] names end: their pages
+ * have one holder less, those that nobody holds any more are listed in `freed`
+ * [count x table_cols] in the order of the list and of their columns (a page of several
+ * of them where the first has it), -1 behind the last of the n_freed[0]; their rows
+ * become -1 and their context 0. A row that is named twice ends once. `held` [count]
+ * is scratch. */
+typedef struct kf_release_args {
+  int32_t* block_table;
+  int64_t table_stride, table_cols, rows;
+  int32_t* context;
+  int32_t* holders;
+  int64_t pages, block_size;
+  const int32_t* requests;
+  int64_t count;
+  int32_t* held;
+  int32_t* freed;
+  int32_t* n_freed;
+} kf_release_args;
+KF_API int32_t kf_release(const kf_release_args* args, void* stream);
+
+/* kf_compact: the live pages, counts[0] of them, become the first ones: those behind
+ * move, in order, to the holes among the first, in every cache (whole pages), and the
+ * table and the holders follow. renamed [pages]: each page's new number, -1 for a free
+ * one; sources and targets [pages / 2]: the counts[1] moves. Moved pages keep their old
+ * contents where they were. */
+typedef struct kf_compact_args {
+  kf_page_caches caches;
+  int32_t* block_table;
+  int64_t table_stride, table_cols, rows;
+  const int32_t* context;
+  int32_t* holders;
+  int32_t* renamed;
+  int32_t* sources;
+  int32_t* targets;
+  int32_t* counts;
+} kf_compact_args;
+KF_API int32_t kf_compact(const kf_compact_args* args, void* stream);
+
 /* ---- logits: penalties, biases, masks -------------------------------------------- *
  * out = logits [rows, vocab] (out may be logits; otherwise no memory is shared) after,
  * in this order and in fp32: the penalties of the row's history, its biases, its mask.

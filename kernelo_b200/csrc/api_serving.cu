@@ -87,6 +87,44 @@ int rotary_args(const kf_rotary_args& g, RotaryArgs* to, bool* nothing) {
   return KF_OK;
 }
 
+// Rows that one call's bits take 96 KB of shared memory for; and pages that a cluster's do 1 MB for.
+constexpr int64_t TABLE_ROWS_LIMIT = 1 << 18;
+constexpr int64_t COMPACT_PAGES_LIMIT = 1 << 22;
+
+int check_table(int64_t rows, int64_t cols, const void* table, const void* context, int64_t pages, const void* holders) {
+  if (rows < 0 || cols < 0) return invalid("negative size");
+  if (rows > TABLE_ROWS_LIMIT) return invalid("block tables of at most " + std::to_string(TABLE_ROWS_LIMIT) + " rows");
+  if (cols > COUNT_LIMIT || rows * cols > (1ll << 40)) return invalid("columns are counted in 32 bits");
+  if ((rows > 0 && cols > 0 && table == nullptr) || (rows > 0 && context == nullptr) || (pages > 0 && holders == nullptr))
+    return invalid("null pointer");
+  return KF_OK;
+}
+
+int page_geometry(const kf_page_caches& c, PageGeometry* to) {
+  if (!known_dtype(c.dtype)) return invalid("unknown dtype code");
+  if (c.n_caches < 0 || c.pages < 0 || c.heads < 0 || c.dim < 0) return invalid("negative size");
+  if (c.pages > COUNT_LIMIT) return invalid("pages are counted in 32 bits");
+  if (c.block_size < 1) return invalid("block_size must be positive");
+  if (c.block_size > INT32_LIMIT || c.heads > INT32_LIMIT || c.dim > INT32_LIMIT ||
+      (c.heads > 0 && c.dim > 0 && c.block_size > INT32_LIMIT / 2 / c.heads / c.dim))
+    return invalid("a page's elements are counted in 32 bits");
+  if (c.n_caches > 0 && c.caches == nullptr) return invalid("null pointer");
+  for (int64_t i = 0; i < c.n_caches; ++i)
+    if (c.caches[i] == nullptr && c.pages * c.heads * c.dim > 0) return invalid("null pointer");
+  to->elem = c.dtype == KF_FP32 ? 4 : 2;
+  to->s_page = c.s_page, to->s_head = c.s_head, to->s_slot = c.s_slot;
+  to->pages = c.pages, to->heads = c.heads, to->block = c.block_size, to->dim = c.dim;
+  return KF_OK;
+}
+
+PageCaches page_caches(const kf_page_caches& c, int64_t first) {
+  PageCaches to{};
+  const int64_t left = c.heads > 0 && c.dim > 0 ? c.n_caches - first : 0;  // empty pages have nothing to copy
+  to.count = static_cast<int>(left < PAGE_CACHES ? left : PAGE_CACHES);
+  for (int i = 0; i < to.count; ++i) to.at[i] = c.caches[first + i];
+  return to;
+}
+
 int norm_args(int64_t dim, double eps, NormArgs* to) {
   if (dim > NORM_ROTARY_MAX_DIM)
     return set_error(KF_ERR_UNSUPPORTED, "norms of heads of at most " + std::to_string(NORM_ROTARY_MAX_DIM) +
@@ -209,8 +247,8 @@ int32_t kf_norm_rotary(const kf_norm_rotary_args* args, void* stream) {
   RotaryArgs a;
   NormArgs n;
   bool nothing = false;
-  int rc = rotary_args(g.rotary, &a, &nothing);
-  if (rc == KF_OK) rc = norm_args(g.rotary.dim, g.eps, &n);
+  int rc = norm_args(g.rotary.dim, g.eps, &n);
+  if (rc == KF_OK) rc = rotary_args(g.rotary, &a, &nothing);
   if (rc != KF_OK) return rc;
   if (g.rotary.inverse != 0) return invalid("inverse: the gradient of norms and turn is kf_norm_rotary_grad");
   if (nothing) return KF_OK;
@@ -227,8 +265,8 @@ int32_t kf_norm_rotary_grad(const kf_norm_rotary_grad_args* args, void* stream) 
   const kf_norm_rotary_grad_args& g = *args;
   NormGradArgs a;
   bool nothing = false;
-  int rc = rotary_args(g.rotary, &a.rotary, &nothing);
-  if (rc == KF_OK) rc = norm_args(g.rotary.dim, g.eps, &a.norm);
+  int rc = norm_args(g.rotary.dim, g.eps, &a.norm);
+  if (rc == KF_OK) rc = rotary_args(g.rotary, &a.rotary, &nothing);
   if (rc != KF_OK) return rc;
   if (g.rotary.inverse != 0) return invalid("inverse: the gradient is of the forward turn");
   if (g.rotary.slots != nullptr) return invalid("the gradient has no cache");
@@ -262,6 +300,77 @@ int64_t kf_norm_rotary_grad_workspace_bytes(int32_t device, int64_t tokens, int6
   const int rc = device_info(device, &dev);
   if (rc != KF_OK) return -rc;
   return norm_rotary_grad_workspace_bytes(tokens, heads, kv_heads, dim, *dev);
+}
+
+int32_t kf_fork(const kf_fork_args* args, void* stream) {
+  if (args == nullptr) return invalid("null arguments");
+  const kf_fork_args& g = *args;
+  PageGeometry geometry;
+  int rc = page_geometry(g.caches, &geometry);
+  if (rc == KF_OK) rc = check_table(g.rows, g.table_cols, g.block_table, g.context, g.caches.pages, g.holders);
+  if (rc != KF_OK) return rc;
+  if (g.pairs < 0 || g.n_free < 0) return invalid("negative size");
+  if (g.pairs > TABLE_ROWS_LIMIT || g.n_free > COUNT_LIMIT) return invalid("too many pairs or free pages");
+  if (g.counts == nullptr || (g.pairs > 0 && (g.parents == nullptr || g.children == nullptr)) ||
+      (g.n_free > 0 && g.free_blocks == nullptr))
+    return invalid("null pointer");
+  DeviceInfo* dev = nullptr;
+  rc = this_device(&dev);
+  if (rc != KF_OK) return rc;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (g.pairs == 0) {
+    const cudaError_t err = cudaMemsetAsync(g.counts, 0, 2 * sizeof(int32_t), s);
+    return err == cudaSuccess ? KF_OK : cuda_error(err, "memset(fork)");
+  }
+  kf_fork_args f = g;
+  for (int64_t first = 0; first == 0 || first < g.caches.n_caches; first += PAGE_CACHES) {
+    rc = launch_fork(page_caches(g.caches, first), geometry, f, *dev, s);
+    if (rc != KF_OK) return rc;
+    f.counts = nullptr;  // the books are kept; the other caches' pages are copied
+  }
+  return KF_OK;
+}
+
+int32_t kf_release(const kf_release_args* args, void* stream) {
+  if (args == nullptr) return invalid("null arguments");
+  const kf_release_args& g = *args;
+  if (g.pages < 0 || g.count < 0) return invalid("negative size");
+  if (g.pages > COUNT_LIMIT) return invalid("pages are counted in 32 bits");
+  int rc = check_table(g.rows, g.table_cols, g.block_table, g.context, g.pages, g.holders);
+  if (rc != KF_OK) return rc;
+  if (g.block_size < 1) return invalid("block_size must be positive");
+  if (g.count > TABLE_ROWS_LIMIT || g.count * g.table_cols >= (1 << 30))
+    return invalid("requests x columns of one call must be below 2^30");
+  if (g.n_freed == nullptr || (g.count > 0 && (g.requests == nullptr || g.held == nullptr)) ||
+      (g.count * g.table_cols > 0 && g.freed == nullptr))
+    return invalid("null pointer");
+  DeviceInfo* dev = nullptr;
+  rc = this_device(&dev);
+  if (rc != KF_OK) return rc;
+  return launch_release(g, *dev, static_cast<cudaStream_t>(stream));
+}
+
+int32_t kf_compact(const kf_compact_args* args, void* stream) {
+  if (args == nullptr) return invalid("null arguments");
+  const kf_compact_args& g = *args;
+  PageGeometry geometry;
+  int rc = page_geometry(g.caches, &geometry);
+  if (rc == KF_OK) rc = check_table(g.rows, g.table_cols, g.block_table, g.context, g.caches.pages, g.holders);
+  if (rc != KF_OK) return rc;
+  if (g.caches.pages > COMPACT_PAGES_LIMIT)
+    return set_error(KF_ERR_UNSUPPORTED, "compact takes at most " + std::to_string(COMPACT_PAGES_LIMIT) + " pages; got " +
+                                             std::to_string(g.caches.pages));
+  if (g.counts == nullptr || (g.caches.pages > 0 && g.renamed == nullptr) ||
+      (g.caches.pages > 1 && (g.sources == nullptr || g.targets == nullptr)))
+    return invalid("null pointer");
+  DeviceInfo* dev = nullptr;
+  rc = this_device(&dev);
+  if (rc != KF_OK) return rc;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  rc = launch_compact_plan(g, geometry, *dev, s);
+  for (int64_t first = 0; rc == KF_OK && first < g.caches.n_caches; first += PAGE_CACHES)
+    rc = launch_move_pages(page_caches(g.caches, first), geometry, g, *dev, s);
+  return rc;
 }
 
 int32_t kf_adjust_logits(const kf_logits_args* args, void* stream) {

@@ -348,6 +348,24 @@ int launch_norm_rotary_grad(const NormGradArgs& args, const DeviceInfo& dev, cud
 // Block tables and slot maps from request lengths (slots.cu).
 int launch_slots(const kf_slots_args& args, const DeviceInfo& dev, cudaStream_t stream);
 
+// Caches of one shape that change together, and their pages' layout (pages.cu).
+constexpr int PAGE_CACHES = 64;  // of a launch
+struct PageCaches {
+  void* at[PAGE_CACHES];
+  int count;
+};
+struct PageGeometry {
+  int elem;  // bytes of an element
+  int64_t s_page, s_head, s_slot;  // in elements
+  int64_t pages, heads, block, dim;
+};
+int launch_fork(const PageCaches& caches, const PageGeometry& g, const kf_fork_args& args, const DeviceInfo& dev,
+                cudaStream_t stream);
+int launch_release(const kf_release_args& args, const DeviceInfo& dev, cudaStream_t stream);
+int launch_compact_plan(const kf_compact_args& args, const PageGeometry& g, const DeviceInfo& dev, cudaStream_t stream);
+int launch_move_pages(const PageCaches& caches, const PageGeometry& g, const kf_compact_args& args, const DeviceInfo& dev,
+                      cudaStream_t stream);
+
 // Penalties, biases and masks on rows of logits (logits.cu).
 int launch_logits(const kf_logits_args& args, const DeviceInfo& dev, cudaStream_t stream);
 

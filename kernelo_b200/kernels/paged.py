@@ -4,10 +4,18 @@
 launch, everything that the step's other calls read: new pages into the block
 table, and the offset, position and cache slot of every added token. Nothing is
 read on the host, so it can be captured with the step.
+
+Requests may hold pages together: :func:`fork_requests` answers one prompt several
+ways with one copy of its whole pages, :func:`release_requests` gives back the
+pages that nobody holds any more, and :func:`compact_pages` moves the live pages
+of a pool to its front. All three keep ``holders`` (int32 ``(pages,)``, zeros at
+first): how many requests hold a page besides the first. They too read nothing on
+the host.
 """
 
 from __future__ import annotations
 
+from collections.abc import Sequence
 from typing import NamedTuple
 
 import torch
@@ -84,3 +92,158 @@ def build_slots(
         .split_with_sizes((max_tokens, seqs + 1, 1, 1))
     native.build_slots(context_lens, new_lens, block_table, free_blocks, block_size, cu_new, positions, slots, taken)
     return StepSlots(cu_new, positions, slots, taken, dropped)
+
+
+class Forked(NamedTuple):
+    """What :func:`fork_requests` reports."""
+
+    blocks_taken: torch.Tensor  # int32 (1,): pages taken; more than the free list has: it ran out
+    dropped: torch.Tensor  # int32 (1,): pairs that did nothing, or whose child lacks its last page
+
+
+class Released(NamedTuple):
+    """What :func:`release_requests` gives back."""
+
+    pages: torch.Tensor  # int32 (requests * blocks,): pages that nobody holds any more, -1 behind the last
+    count: torch.Tensor  # int32 (1,): how many
+
+
+class Compacted(NamedTuple):
+    """What :func:`compact_pages` has done."""
+
+    renamed: torch.Tensor  # int32 (pages,): each page's new number, -1 for a free page
+    live: torch.Tensor  # int32 (1,): live pages, which are the first ones now
+    moves: torch.Tensor  # int32 (1,): pages that have moved
+
+
+def _check_table(block_table: torch.Tensor, context_lens: torch.Tensor, holders: torch.Tensor) -> None:
+    if block_table.ndim != 2 or block_table.dtype is not torch.int32:
+        raise ValueError(f"block_table must be int32 (requests, blocks), got {block_table.dtype} "
+                         f"{tuple(block_table.shape)}")
+    if not block_table.is_cuda:
+        raise ValueError(f"block_table must be a CUDA tensor, got {block_table.device}")
+    rows, cols = block_table.shape
+    if (block_table.stride(1) != 1 and cols > 1) or (block_table.stride(0) < cols and rows > 1):
+        raise ValueError("block_table must have contiguous rows that do not overlap")
+    _check_index("context_lens", context_lens, block_table)
+    if context_lens.ndim != 1 or context_lens.shape[0] != rows:
+        raise ValueError(f"context_lens must have shape ({rows},), got {tuple(context_lens.shape)}")
+    _check_index("holders", holders, block_table)
+    if holders.ndim != 1:
+        raise ValueError(f"holders must have one dimension, got shape {tuple(holders.shape)}")
+
+
+def _check_list(name: str, t: torch.Tensor, block_table: torch.Tensor) -> None:
+    _check_index(name, t, block_table)
+    if t.ndim != 1:
+        raise ValueError(f"{name} must have one dimension, got shape {tuple(t.shape)}")
+
+
+def _check_caches(caches: Sequence[torch.Tensor], block_table: torch.Tensor, holders: torch.Tensor) -> list[torch.Tensor]:
+    caches = list(caches)
+    if not caches:
+        raise ValueError("expected at least one cache")
+    first = caches[0]
+    shape, stride, dtype, device = first.shape, first.stride(), first.dtype, block_table.get_device()
+    if len(shape) != 4 or shape[2] < 1:
+        raise ValueError(f"expected caches (pages, kv_heads, block, dim), got {tuple(shape)}")
+    if shape[0] != holders.shape[0]:
+        raise ValueError(f"holders must have shape ({shape[0]},) for caches {tuple(shape)}, got {tuple(holders.shape)}")
+    for c in caches:
+        if c.shape != shape or c.stride() != stride or c.dtype is not dtype:
+            raise ValueError(f"caches must have one type, shape and strides, got {dtype} {tuple(shape)} {stride} and "
+                             f"{c.dtype} {tuple(c.shape)} {c.stride()}")
+        if c.get_device() != device:
+            raise ValueError(f"caches must be on {block_table.device}, got {c.device}")
+    if stride[3] != 1 and shape[3] > 1:
+        raise ValueError("caches must have a contiguous last dimension")
+    if any(s == 0 and n > 1 for s, n in zip(stride, shape)):
+        raise ValueError(f"caches overlap themselves: strides {stride} for shape {tuple(shape)}")
+    return caches
+
+
+def fork_requests(
+    caches: Sequence[torch.Tensor],
+    block_table: torch.Tensor,
+    context_lens: torch.Tensor,
+    holders: torch.Tensor,
+    free_blocks: torch.Tensor,
+    parents: torch.Tensor,
+    children: torch.Tensor,
+) -> Forked:
+    """Row ``children[i]`` becomes a copy of the request in row ``parents[i]`` (int32 both).
+
+    ``caches``: every layer's keys and values ``(pages, kv_heads, block, dim)``, of
+    one type, shape and strides. A child holds its parent's whole pages together
+    with it; for the tokens of a last, partial page it gets a page of its own
+    from ``free_blocks`` (int32), one for each such pair in order, and those tokens
+    are copied in all caches. The rest of its row becomes -1, and
+    ``context_lens[child]`` its parent's length. So nobody ever writes to a page
+    held together: new tokens go behind the last one.
+
+    Children are free rows: all different, and none of them a parent. A pair
+    that breaks this, or names a row that is none, does nothing and counts as
+    dropped, as does a child whose page the free list lacks (it has -1 there).
+    The caller drops the first ``blocks_taken`` entries of its free list.
+    """
+    _check_table(block_table, context_lens, holders)
+    caches = _check_caches(caches, block_table, holders)
+    _check_list("free_blocks", free_blocks, block_table)
+    _check_list("parents", parents, block_table)
+    _check_list("children", children, block_table)
+    if parents.shape != children.shape:
+        raise ValueError(f"parents and children must have one shape, got {tuple(parents.shape)} and {tuple(children.shape)}")
+    counts = block_table.new_empty(2)
+    native.fork(caches, block_table, context_lens, holders, free_blocks, parents, children, counts)
+    return Forked(*counts.split(1))
+
+
+def release_requests(
+    block_table: torch.Tensor,
+    context_lens: torch.Tensor,
+    holders: torch.Tensor,
+    requests: torch.Tensor,
+    *,
+    block_size: int,
+) -> Released:
+    """The requests in the rows ``requests`` (int32) end: their rows become -1, their lengths 0.
+
+    Pages that other requests still hold lose a holder; the others come back in
+    the order of the list and of their columns (a page of several of these
+    requests where the first has it). A row that is named twice ends once; one
+    that is none is skipped. The caller appends the first ``count`` of ``pages``
+    to its free list.
+    """
+    _check_table(block_table, context_lens, holders)
+    _check_list("requests", requests, block_table)
+    if block_size < 1:
+        raise ValueError(f"block_size must be positive, got {block_size}")
+    n, cols = requests.shape[0], block_table.shape[1]
+    if n * cols >= 1 << 30:
+        raise ValueError(f"requests x blocks must be below 2^30, got {n} x {cols}")
+    pages, held, count = block_table.new_empty(n * cols + n + 1).split_with_sizes((n * cols, n, 1))
+    native.release(block_table, context_lens, holders, requests, block_size, held, pages, count)
+    return Released(pages, count)
+
+
+def compact_pages(
+    caches: Sequence[torch.Tensor],
+    block_table: torch.Tensor,
+    context_lens: torch.Tensor,
+    holders: torch.Tensor,
+) -> Compacted:
+    """Moves the live pages of a pool to its front, in all ``caches`` (as in :func:`fork_requests`).
+
+    Live are the pages of the tokens that the requests have. With ``live`` of them,
+    those numbered ``live`` and above go, in order, to the free places below;
+    the block table and ``holders`` follow. What the pool holds is then its first
+    ``live`` pages, and its free list ``live, live + 1, ..``. Slots and page
+    numbers taken before are stale: ``renamed`` translates them.
+    """
+    _check_table(block_table, context_lens, holders)
+    caches = _check_caches(caches, block_table, holders)
+    pages = holders.shape[0]
+    renamed, sources, targets, live, moves = block_table.new_empty(pages + 2 * (pages // 2) + 2) \
+        .split_with_sizes((pages, pages // 2, pages // 2, 1, 1))
+    native.compact(caches, block_table, context_lens, holders, renamed, sources, targets, live)
+    return Compacted(renamed, live, moves)

@@ -19,6 +19,7 @@ is missing or its recorded source hash no longer matches.
 
 from __future__ import annotations
 
+import array
 import ctypes
 import functools
 import os
@@ -81,6 +82,9 @@ EXPORTED_SYMBOLS = (
     "kf_rotary",
     "kf_build_slots",
     "kf_adjust_logits",
+    "kf_fork",
+    "kf_release",
+    "kf_compact",
     "kf_norm_rotary",
     "kf_norm_rotary_grad",
     "kf_norm_rotary_grad_workspace_bytes",
@@ -174,6 +178,9 @@ PREFILL_ARGS = struct.Struct("22qdq")
 TREE_ARGS = struct.Struct("30qd2q")
 ROTARY_ARGS = struct.Struct("37q")
 SLOTS_ARGS = struct.Struct("14q")
+FORK_ARGS = struct.Struct("22q")
+RELEASE_ARGS = struct.Struct("13q")
+COMPACT_ARGS = struct.Struct("20q")
 LOGITS_ARGS = struct.Struct("24q")
 NORM_ROTARY_ARGS = struct.Struct("39qd")
 NORM_ROTARY_GRAD_ARGS = struct.Struct("39qd10q")
@@ -217,6 +224,9 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "kf_rotary": (_i32, [_packed, _vp]),
     "kf_stream_capture_id": (_i32, [_vp, ctypes.POINTER(_i64)]),
     "kf_build_slots": (_i32, [_packed, _vp]),
+    "kf_fork": (_i32, [_packed, _vp]),
+    "kf_release": (_i32, [_packed, _vp]),
+    "kf_compact": (_i32, [_packed, _vp]),
     "kf_adjust_logits": (_i32, [_packed, _vp]),
     "kf_norm_rotary": (_i32, [_packed, _vp]),
     "kf_norm_rotary_grad": (_i32, [_packed, _vp]),
@@ -823,6 +833,52 @@ def norm_rotary_grad(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor, k: tor
                                        weight_grads.data_ptr(), weight_grads.data_ptr() + 4 * dim, partial.data_ptr(),
                                        ws_bytes),
             dev, "kf_norm_rotary_grad")
+
+
+def _page_caches(caches: list[torch.Tensor]) -> tuple[array.array, tuple]:
+    """The caches' addresses, to be held until the call returns, and the struct's fields."""
+    addresses = array.array("Q", [c.data_ptr() for c in caches])
+    first = caches[0]
+    pages, heads, block_size, dim = first.shape
+    s_page, s_head, s_slot, _ = first.stride()
+    return addresses, (native_code(first.dtype), addresses.buffer_info()[0], len(caches), s_page, s_head, s_slot, pages,
+                       heads, block_size, dim)
+
+
+def _table_fields(block_table: torch.Tensor) -> tuple[int, int, int, int]:
+    rows, cols = block_table.shape
+    return block_table.data_ptr(), block_table.stride(0), cols, rows
+
+
+def fork(caches: list[torch.Tensor], block_table: torch.Tensor, context: torch.Tensor, holders: torch.Tensor,
+         free_blocks: torch.Tensor, parents: torch.Tensor, children: torch.Tensor, counts: torch.Tensor) -> None:
+    lib = _lib or load()
+    addresses, fields = _page_caches(caches)
+    _launch(lib.kf_fork,
+            FORK_ARGS.pack(*fields, *_table_fields(block_table), context.data_ptr(), holders.data_ptr(),
+                           free_blocks.data_ptr(), free_blocks.shape[0], parents.data_ptr(), children.data_ptr(),
+                           parents.shape[0], counts.data_ptr()),
+            block_table.device, "kf_fork")
+
+
+def release(block_table: torch.Tensor, context: torch.Tensor, holders: torch.Tensor, requests: torch.Tensor,
+            block_size: int, held: torch.Tensor, freed: torch.Tensor, n_freed: torch.Tensor) -> None:
+    lib = _lib or load()
+    _launch(lib.kf_release,
+            RELEASE_ARGS.pack(*_table_fields(block_table), context.data_ptr(), holders.data_ptr(), holders.shape[0],
+                              block_size, requests.data_ptr(), requests.shape[0], held.data_ptr(), freed.data_ptr(),
+                              n_freed.data_ptr()),
+            block_table.device, "kf_release")
+
+
+def compact(caches: list[torch.Tensor], block_table: torch.Tensor, context: torch.Tensor, holders: torch.Tensor,
+            renamed: torch.Tensor, sources: torch.Tensor, targets: torch.Tensor, counts: torch.Tensor) -> None:
+    lib = _lib or load()
+    addresses, fields = _page_caches(caches)
+    _launch(lib.kf_compact,
+            COMPACT_ARGS.pack(*fields, *_table_fields(block_table), context.data_ptr(), holders.data_ptr(),
+                              renamed.data_ptr(), sources.data_ptr(), targets.data_ptr(), counts.data_ptr()),
+            block_table.device, "kf_compact")
 
 
 def adjust_logits(logits: torch.Tensor, out: torch.Tensor, tokens: torch.Tensor | None, token_lens: torch.Tensor | None,
