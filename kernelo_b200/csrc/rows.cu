@@ -192,24 +192,23 @@ __global__ void __launch_bounds__(max_threads_for<NV>()) rows_kernel(const RowsP
       if (has_head) m_thr = fmaxf(m_thr, xh);
       if (has_tail) m_thr = fmaxf(m_thr, xt);
       float s = 0.0f;
-      if (m_thr != -INFINITY) {
-        const float mb = m_thr * kRowLog2e;
+      // a thread whose elements are all -inf has exponentials of 0, not of -inf + inf
+      const float mb = m_thr == -INFINITY ? 0.0f : m_thr * kRowLog2e;
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-          if (g + j * G < nvec) {
-            float f[VE];
-            vec_floats(raw[j], f);
+      for (int j = 0; j < NV; ++j) {
+        if (g + j * G < nvec) {
+          float f[VE];
+          vec_floats(raw[j], f);
 #pragma unroll
-            for (int e = 0; e < VE; ++e) {
-              const float t = ex2_ftz(fmaf(f[e], kRowLog2e, -mb));
-              if constexpr (KEEP_EV) ev[j * VE + e] = t;
-              s += t;
-            }
+          for (int e = 0; e < VE; ++e) {
+            const float t = ex2_ftz(fmaf(f[e], kRowLog2e, -mb));
+            if constexpr (KEEP_EV) ev[j * VE + e] = t;
+            s += t;
           }
         }
-        if (has_head) s += (eh = ex2_ftz(fmaf(xh, kRowLog2e, -mb)));
-        if (has_tail) s += (et = ex2_ftz(fmaf(xt, kRowLog2e, -mb)));
       }
+      if (has_head) s += (eh = ex2_ftz(fmaf(xh, kRowLog2e, -mb)));
+      if (has_tail) s += (et = ex2_ftz(fmaf(xt, kRowLog2e, -mb)));
       part = warp_max_sum(m_thr, s);
     } else {
       float ss = 0.0f;
@@ -262,7 +261,7 @@ __global__ void __launch_bounds__(max_threads_for<NV>()) rows_kernel(const RowsP
       // exp(x - M) / S = exp(x - m_thr) * (exp(m_thr - M) / S)
       const float factor =
           m_thr == -INFINITY ? 0.0f : ex2_ftz((m_thr - tot.x) * kRowLog2e) / tot.y;
-      const float mb = m_thr * kRowLog2e;
+      const float mb = m_thr == -INFINITY ? 0.0f : m_thr * kRowLog2e;
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         const int v = g + j * G;

@@ -246,24 +246,23 @@ __global__ void __launch_bounds__(STREAM_THREADS, stream_min_blocks<NV>())
       if (has_head) m_thr = fmaxf(m_thr, xh);
       if (has_tail) m_thr = fmaxf(m_thr, xt);
       float s = 0.0f;
-      if (m_thr != -INFINITY) {
-        const float mb = m_thr * kRowLog2e;
+      // a thread whose elements are all -inf has exponentials of 0, not of -inf + inf
+      const float mb = m_thr == -INFINITY ? 0.0f : m_thr * kRowLog2e;
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-          if (tg + j * TG < nvec) {
-            float f[VE];
-            to_floats<T>(raw[j], f);
+      for (int j = 0; j < NV; ++j) {
+        if (tg + j * TG < nvec) {
+          float f[VE];
+          to_floats<T>(raw[j], f);
 #pragma unroll
-            for (int k = 0; k < VE; ++k) {
-              const float t = ex2_ftz(fmaf(f[k], kRowLog2e, -mb));
-              if constexpr (KEEP_EV) ev[j * VE + k] = t;
-              s += t;
-            }
+          for (int k = 0; k < VE; ++k) {
+            const float t = ex2_ftz(fmaf(f[k], kRowLog2e, -mb));
+            if constexpr (KEEP_EV) ev[j * VE + k] = t;
+            s += t;
           }
         }
-        if (has_head) s += (eh = ex2_ftz(fmaf(xh, kRowLog2e, -mb)));
-        if (has_tail) s += (et = ex2_ftz(fmaf(xt, kRowLog2e, -mb)));
       }
+      if (has_head) s += (eh = ex2_ftz(fmaf(xh, kRowLog2e, -mb)));
+      if (has_tail) s += (et = ex2_ftz(fmaf(xt, kRowLog2e, -mb)));
       part = warp_max_sum(m_thr, s);
     } else {
       float ss = 0.0f;
@@ -301,7 +300,7 @@ __global__ void __launch_bounds__(STREAM_THREADS, stream_min_blocks<NV>())
       // exp(x - M) / S = exp(x - m_thr) * (exp(m_thr - M) / S)
       const float factor =
           m_thr == -INFINITY ? 0.0f : ex2_ftz((m_thr - part.x) * kRowLog2e) / part.y;
-      const float mb = m_thr * kRowLog2e;
+      const float mb = m_thr == -INFINITY ? 0.0f : m_thr * kRowLog2e;
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         const int v = tg + j * TG;
