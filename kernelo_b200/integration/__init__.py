@@ -5,7 +5,7 @@ on the native kernels alone."""
 
 from __future__ import annotations
 
-from kernelo_b200.integration.serving import PagedCache, ServingBlock, ServingConfig
+from kernelo_b200.integration.serving import PagedCache, ServingBlock, ServingConfig, ServingHead
 from kernelo_b200.integration.transformer import (
     BACKEND_KERNELFORGE,
     BACKEND_TORCH,
@@ -17,4 +17,4 @@ from kernelo_b200.integration.transformer import (
 )
 
 __all__ = ["BACKENDS", "BACKEND_KERNELFORGE", "BACKEND_TORCH", "BlockConfig", "PagedCache", "ServingBlock",
-           "ServingConfig", "TransformerBlock", "amdahl_breakdown", "benchmark_block"]
+           "ServingConfig", "ServingHead", "TransformerBlock", "amdahl_breakdown", "benchmark_block"]
