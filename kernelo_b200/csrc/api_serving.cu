@@ -24,8 +24,9 @@ constexpr double LOG2_E = 1.4426950408889634;
 constexpr int64_t INT32_LIMIT = 0x7fffffffll;
 // Rows, keys and requests: steps of up to 256 beyond the last one still fit 32 bits.
 constexpr int64_t COUNT_LIMIT = 0x7fffff00ll;
-// Tokens of a vocabulary, a history or a list of biases: a chunk or a stride of a block beyond the last one, too.
+// Tokens of a vocabulary: a chunk beyond the last one, too. (Occurrences in a history are counted in 30 bits.)
 constexpr int64_t LOGITS_LIMIT = 0x7fff0000ll;
+constexpr int64_t LOGITS_BIASES = 16384;  // 32 of each thread of a block
 
 int check_heads(int64_t dtype, int64_t rows, int64_t seqs, int64_t heads, int64_t kv_heads, int64_t dim) {
   if (!known_dtype(dtype)) return invalid("unknown dtype code");
@@ -378,8 +379,11 @@ int32_t kf_adjust_logits(const kf_logits_args* args, void* stream) {
   const kf_logits_args& g = *args;
   if (!known_dtype(g.dtype)) return invalid("unknown dtype code");
   if (g.rows < 0 || g.vocab < 0 || g.token_cols < 0 || g.bias_cols < 0 || g.masks < 0) return invalid("negative size");
-  if (g.rows > COUNT_LIMIT || g.vocab > LOGITS_LIMIT || g.token_cols > LOGITS_LIMIT || g.bias_cols > LOGITS_LIMIT)
+  if (g.rows > COUNT_LIMIT || g.vocab > LOGITS_LIMIT || g.token_cols >= (1 << 30))
     return invalid("rows, tokens and biases are counted in 32 bits");
+  if (g.bias_cols > LOGITS_BIASES)
+    return set_error(KF_ERR_UNSUPPORTED, "at most " + std::to_string(LOGITS_BIASES) + " biases a row; got " +
+                                             std::to_string(g.bias_cols));
   if (g.rows == 0 || g.vocab == 0) return KF_OK;
   if (g.logits == nullptr || g.out == nullptr || (g.tokens != nullptr && g.token_lens == nullptr) ||
       (g.bias_tokens != nullptr && g.bias_values == nullptr))
