@@ -514,8 +514,9 @@ KF_API int32_t kf_fork(const kf_fork_args* args, void* stream);
  * have one holder less, those that nobody holds any more are listed in `freed`
  * [count x table_cols] in the order of the list and of their columns (a page of several
  * of them where the first has it), -1 behind the last of the n_freed[0]; their rows
- * become -1 and their context 0. A row that is named twice ends once. `held` [count]
- * is scratch. */
+ * become -1 and their context 0. A row that is named twice ends once. `scratch`,
+ * of any content: 9 words for each 256 columns, or part of them, of each request,
+ * 16-byte aligned. One call takes 200,000 such parts at most. */
 typedef struct kf_release_args {
   int32_t* block_table;
   int64_t table_stride, table_cols, rows;
@@ -524,7 +525,7 @@ typedef struct kf_release_args {
   int64_t pages, block_size;
   const int32_t* requests;
   int64_t count;
-  int32_t* held;
+  int32_t* scratch;
   int32_t* freed;
   int32_t* n_freed;
 } kf_release_args;

@@ -342,9 +342,12 @@ int32_t kf_release(const kf_release_args* args, void* stream) {
   if (g.block_size < 1) return invalid("block_size must be positive");
   if (g.count > TABLE_ROWS_LIMIT || g.count * g.table_cols >= (1 << 30))
     return invalid("requests x columns of one call must be below 2^30");
-  if (g.n_freed == nullptr || (g.count > 0 && (g.requests == nullptr || g.held == nullptr)) ||
+  if (g.n_freed == nullptr || (g.count > 0 && (g.requests == nullptr || (g.table_cols > 0 && g.scratch == nullptr))) ||
       (g.count * g.table_cols > 0 && g.freed == nullptr))
     return invalid("null pointer");
+  if ((reinterpret_cast<uintptr_t>(g.scratch) & 15u) != 0) return set_error(KF_ERR_WORKSPACE, "scratch must be 16-byte aligned");
+  if (g.count * ceil_div(g.table_cols, 256) > 200000)
+    return set_error(KF_ERR_UNSUPPORTED, "requests x columns / 256 of one call: at most 200000");
   DeviceInfo* dev = nullptr;
   rc = this_device(&dev);
   if (rc != KF_OK) return rc;

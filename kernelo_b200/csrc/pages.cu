@@ -32,6 +32,8 @@ constexpr int PLAN_THREADS = 1024;
 constexpr int PLAN_WARPS = PLAN_THREADS / 32;
 constexpr int PLAN_CLUSTER = 8;
 
+constexpr int TILE_WORDS = 8, TILE = 32 * TILE_WORDS;  // columns that a warp takes at a time
+
 // Where a run of a page's elements lies, in vectors: `outer` runs (of heads, or of heads and slots).
 struct CacheShape {
   long long s_page, s_head, s_slot;  // in vectors
@@ -174,109 +176,158 @@ struct ReleaseArgs {
   int* holders;
   long long pages, block;
   const int* requests;
-  int count;     // of requests
-  int* held;     // [count]: pages of each; -1 for one that is skipped
-  int* freed;    // [count x cols]
-  int* n_freed;  // one word
+  int count;        // of requests
+  int tiles;        // of a row
+  uint32_t* votes;  // [count x tiles][TILE_WORDS]: entries whose page goes back
+  int* held;        // [count x tiles]: pages of the tile's request, -1 where it is skipped
+  int* freed;       // [count x cols]
+  int* n_freed;     // one word
 };
 
 // A free page's count says which of its places in the rows is the first: below every count that is one.
 constexpr int MARK = -(1 << 30);
 
+// Entries (request, column) go by tiles of a row, dealt out to the warps in turn (rows end early, and a run of them for
+// each warp would leave most warps with nothing). The four phases, 0 to 3, are one launch of a cluster for few
+// entries (PHASE -1), and otherwise a launch each over the whole GPU: an entry costs five scattered accesses, and
+// a cluster's 8 SMs take 98 us for the 192 longest of 256 requests of up to 2048 pages.
+template <int PHASE>
 __global__ void __launch_bounds__(PLAN_THREADS) release_kernel(const __grid_constant__ ReleaseArgs a) {
   __shared__ int scratch[PLAN_WARPS];
-  __shared__ int cta_total;
+  extern __shared__ int places[];  // of the tiles that this CTA's warps have: where the first of their pages goes
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int rank = static_cast<int>(cluster_ctarank()), ctas = gridDim.x;
+  const int rank = static_cast<int>(blockIdx.x), ctas = static_cast<int>(gridDim.x);
   const int warps = ctas * PLAN_WARPS, my_warp = rank * PLAN_WARPS + warp;
-  const int cols = static_cast<int>(a.cols), entries = a.count * cols;  // below 2^30
-  // Requests are checked a warp each: a row that an earlier one names is skipped.
-  for (int i = my_warp; i < a.count; i += warps) {
-    const int row = __ldg(a.requests + i);
-    bool skip = row < 0 || row >= a.rows;
-    for (int j = lane; j < i; j += 32) skip |= __ldg(a.requests + j) == row;
-    skip = __any_sync(0xffffffffu, skip);
-    if (lane == 0) a.held[i] = skip ? -1 : pages_of(a.context[row], a.block, a.cols);
+  const int cols = static_cast<int>(a.cols), entries = a.count * cols, tiles = a.count * a.tiles;  // below 2^30
+  if constexpr (PHASE >= 0) {
+    griddep_launch_dependents();
+    griddep_wait();
   }
-  cluster_sync_all();
-  // Entries (request, column) in order, a run of them to each warp.
-  const int each = ((entries + warps - 1) / warps + 31) & ~31;
-  const int lo = min(static_cast<long long>(my_warp) * each, static_cast<long long>(entries));
-  const int hi = min(static_cast<long long>(lo) + each, static_cast<long long>(entries));
-  constexpr int BATCH = 4;
-  const auto page_at = [&](int e) -> int {  // -1 where there is none
-    if (e >= hi) return -1;
-    const int i = e / cols, col = e - i * cols;
-    if (col >= a.held[i]) return -1;
-    const int page = a.table[__ldg(a.requests + i) * a.table_stride + col];
-    return page < a.pages ? page : -1;
-  };
-  for (int e0 = lo + lane; e0 < hi; e0 += 32 * BATCH) {
-    int page[BATCH];
-#pragma unroll
-    for (int k = 0; k < BATCH; ++k) page[k] = page_at(e0 + 32 * k);
-#pragma unroll
-    for (int k = 0; k < BATCH; ++k)
-      if (page[k] >= 0) atomicSub(a.holders + page[k], 1);
-  }
-  cluster_sync_all();
-  for (int e0 = lo + lane; e0 < hi; e0 += 32 * BATCH) {
-    int page[BATCH], left[BATCH];
-#pragma unroll
-    for (int k = 0; k < BATCH; ++k) page[k] = page_at(e0 + 32 * k);
-#pragma unroll
-    for (int k = 0; k < BATCH; ++k) left[k] = page[k] >= 0 ? __ldcg(a.holders + page[k]) : 0;
-#pragma unroll
-    for (int k = 0; k < BATCH; ++k)
-      if (left[k] < 0) atomicMin(a.holders + page[k], MARK - (entries - (e0 + 32 * k)));
-  }
-  cluster_sync_all();
-  int total = 0;  // of this warp
-  for (int e0 = lo + lane; e0 - lane < hi; e0 += 32 * BATCH) {
-    int page[BATCH], left[BATCH];
-#pragma unroll
-    for (int k = 0; k < BATCH; ++k) page[k] = page_at(e0 + 32 * k);
-#pragma unroll
-    for (int k = 0; k < BATCH; ++k) left[k] = page[k] >= 0 ? __ldcg(a.holders + page[k]) : 0;
-#pragma unroll
-    for (int k = 0; k < BATCH; ++k)
-      total += __popc(__ballot_sync(0xffffffffu, page[k] >= 0 && left[k] == MARK - (entries - (e0 + 32 * k))));
-  }
-  if (lane == 0) scratch[warp] = total;
-  __syncthreads();
-  int place = 0, all = 0;
-  for (int w = 0; w < PLAN_WARPS; ++w) {
-    place += w < warp ? scratch[w] : 0;
-    all += scratch[w];
-  }
-  if (tid == 0) cta_total = all;
-  cluster_sync_all();
-  all = 0;
-  for (int r = 0; r < ctas; ++r) {
-    int theirs;
-    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(theirs) : "r"(mapa_shared(smem_u32(&cta_total), r)) : "memory");
-    place += r < rank ? theirs : 0;
-    all += theirs;
-  }
-  for (int e0 = lo; e0 < hi; e0 += 32) {
-    const int e = e0 + lane, page = page_at(e);
-    const bool first = page >= 0 && __ldcg(a.holders + page) == MARK - (entries - e);
-    const unsigned vote = __ballot_sync(0xffffffffu, first);
-    if (first) {
-      a.freed[place + __popc(vote & ((1u << lane) - 1))] = page;
-      a.holders[page] = 0;
+  // f(tile, its number among this CTA's, request, row, first column, pages from there on) for tiles that are not skipped.
+  const auto each_tile = [&](const auto& f) {
+    for (int t = my_warp, n = warp; t < tiles; t += warps, n += PLAN_WARPS) {
+      const int i = t / a.tiles, col = (t - i * a.tiles) * TILE, held = a.held[t];
+      if (held >= 0) f(t, n, i, __ldg(a.requests + i), col, held - col);
     }
-    place += __popc(vote);
-    if (e >= hi) continue;
-    if (e >= all) a.freed[e] = -1;
-    const int i = e / cols, col = e - i * cols;
-    if (a.held[i] < 0) continue;
-    const int row = __ldg(a.requests + i);
-    a.table[row * a.table_stride + col] = -1;
-    if (col == 0) a.context[row] = 0;
+  };
+  // A lane's pages of a tile, -1 where there is none.
+  const auto load_pages = [&](int row, int col, int left, int (&page)[TILE_WORDS]) {
+    const int* const at = a.table + row * a.table_stride + col;
+#pragma unroll
+    for (int k = 0; k < TILE_WORDS; ++k) {
+      page[k] = lane + 32 * k < left ? at[lane + 32 * k] : -1;
+      if (page[k] >= a.pages) page[k] = -1;
+    }
+  };
+  if constexpr (PHASE <= 0) {
+    // Skipped are requests whose row is none, or named by an earlier one too.
+    for (int t = my_warp; t < tiles; t += warps) {
+      const int i = t / a.tiles, row = __ldg(a.requests + i);
+      bool skip = row < 0 || row >= a.rows;
+      for (int j = lane; j < i; j += 32) skip |= __ldg(a.requests + j) == row;
+      skip = __any_sync(0xffffffffu, skip);
+      if (lane == 0) a.held[t] = skip ? -1 : pages_of(a.context[row], a.block, a.cols);
+    }
+    __syncwarp();
+    each_tile([&](int, int, int, int row, int col, int left) {
+      if (left <= 0) return;
+      int page[TILE_WORDS];
+      load_pages(row, col, left, page);
+#pragma unroll
+      for (int k = 0; k < TILE_WORDS; ++k)
+        if (page[k] >= 0) atomicSub(a.holders + page[k], 1);
+    });
   }
-  if (rank == 0 && tid == 0) *a.n_freed = all;
-  cluster_sync_all();  // nobody leaves while its total may still be read
+  if constexpr (PHASE < 0) cluster_sync_all();
+  if constexpr (PHASE < 0 || PHASE == 1) {
+    each_tile([&](int, int, int i, int row, int col, int left) {
+      if (left <= 0) return;
+      int page[TILE_WORDS], holds[TILE_WORDS];
+      load_pages(row, col, left, page);
+#pragma unroll
+      for (int k = 0; k < TILE_WORDS; ++k) holds[k] = page[k] >= 0 ? __ldcg(a.holders + page[k]) : 0;
+#pragma unroll
+      for (int k = 0; k < TILE_WORDS; ++k)
+        if (holds[k] < 0) atomicMin(a.holders + page[k], MARK - (entries - (i * cols + col + lane + 32 * k)));
+    });
+  }
+  if constexpr (PHASE < 0) cluster_sync_all();
+  if constexpr (PHASE < 0 || PHASE == 2) {
+    for (int t = my_warp; t < tiles; t += warps) {
+      const int i = t / a.tiles, col = (t - i * a.tiles) * TILE, left = a.held[t] - col;
+      uint32_t mine = 0;
+      if (left > 0) {
+        int page[TILE_WORDS], holds[TILE_WORDS];
+        load_pages(__ldg(a.requests + i), col, left, page);
+#pragma unroll
+        for (int k = 0; k < TILE_WORDS; ++k) holds[k] = page[k] >= 0 ? __ldcg(a.holders + page[k]) : 0;
+#pragma unroll
+        for (int k = 0; k < TILE_WORDS; ++k) {
+          const uint32_t vote = __ballot_sync(
+              0xffffffffu, page[k] >= 0 && holds[k] == MARK - (entries - (i * cols + col + lane + 32 * k)));
+          if (lane == k) mine = vote;
+        }
+      }
+      if (lane < TILE_WORDS) a.votes[t * TILE_WORDS + lane] = mine;
+    }
+  }
+  if constexpr (PHASE < 0) cluster_sync_all();
+  if constexpr (PHASE < 0 || PHASE == 3) {
+    // Each CTA counts all tiles' votes itself, a run of tiles to each thread, and keeps the places of its own tiles.
+    const int run = (tiles + PLAN_THREADS - 1) / PLAN_THREADS;
+    const int t0 = min(tid * run, tiles), t1 = min(t0 + run, tiles);
+    const auto votes_of = [&](int t) {
+      int n = 0;
+#pragma unroll
+      for (int k = 0; k < TILE_WORDS; k += 4) {
+        const uint4 v = __ldcg(reinterpret_cast<const uint4*>(a.votes + t * TILE_WORDS + k));
+        n += __popc(v.x) + __popc(v.y) + __popc(v.z) + __popc(v.w);
+      }
+      return n;
+    };
+    int mine = 0;
+    for (int t = t0; t < t1; ++t) mine += votes_of(t);
+    int in = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, in, o);
+      if (lane >= o) in += up;
+    }
+    if (lane == 31) scratch[warp] = in;
+    __syncthreads();
+    int place = in - mine, all = 0;
+    for (int w = 0; w < PLAN_WARPS; ++w) {
+      place += w < warp ? scratch[w] : 0;
+      all += scratch[w];
+    }
+    for (int t = t0; t < t1; ++t) {
+      if (t % warps / PLAN_WARPS == rank) places[t / warps * PLAN_WARPS + t % PLAN_WARPS] = place;
+      place += votes_of(t);
+    }
+    __syncthreads();
+    each_tile([&](int t, int n, int, int row, int col, int) {
+      int* const at = a.table + row * a.table_stride + col;
+      const uint32_t votes = lane < TILE_WORDS ? __ldcg(a.votes + t * TILE_WORDS + lane) : 0;
+      int to = places[n];
+#pragma unroll
+      for (int k = 0; k < TILE_WORDS; ++k) {
+        const uint32_t vote = __shfl_sync(0xffffffffu, votes, k);
+        if ((vote >> lane & 1u) != 0) {
+          const int page = at[lane + 32 * k];
+          a.freed[to + __popc(vote & ((1u << lane) - 1))] = page;
+          a.holders[page] = 0;
+        }
+        to += __popc(vote);
+        if (col + lane + 32 * k < cols) at[lane + 32 * k] = -1;
+      }
+    });
+    for (int e = all + rank * PLAN_THREADS + tid; e < entries; e += ctas * PLAN_THREADS) a.freed[e] = -1;
+    if (rank == 0 && tid == 0) *a.n_freed = all;
+    for (int i = rank * PLAN_THREADS + tid; i < a.count; i += ctas * PLAN_THREADS) {
+      const int row = __ldg(a.requests + i);
+      if (row >= 0 && row < a.rows) a.context[row] = 0;
+    }
+  }
 }
 
 // ---------------------------------------------------------------- compact
@@ -480,7 +531,8 @@ int launched(const char* what) {
 }
 
 template <typename Kernel, typename... Args>
-int launch_cluster(Kernel kernel, int ctas, int smem, cudaStream_t stream, const char* what, const Args&... args) {
+int launch_plan(Kernel kernel, int ctas, int smem, const cudaLaunchAttribute* attribute, cudaStream_t stream, const char* what,
+                const Args&... args) {
   if (smem > 48 * 1024) {
     const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (err != cudaSuccess) return cuda_error(err, what);
@@ -490,14 +542,30 @@ int launch_cluster(Kernel kernel, int ctas, int smem, cudaStream_t stream, const
   config.blockDim = dim3(PLAN_THREADS);
   config.dynamicSmemBytes = static_cast<size_t>(smem);
   config.stream = stream;
+  cudaLaunchAttribute copy{};
+  if (attribute != nullptr) copy = *attribute;
+  config.attrs = &copy;
+  config.numAttrs = attribute != nullptr ? 1 : 0;
+  const cudaError_t err = cudaLaunchKernelEx(&config, kernel, args...);
+  return err == cudaSuccess ? KF_OK : cuda_error(err, what);
+}
+
+template <typename Kernel, typename... Args>
+int launch_cluster(Kernel kernel, int ctas, int smem, cudaStream_t stream, const char* what, const Args&... args) {
   cudaLaunchAttribute cluster{};
   cluster.id = cudaLaunchAttributeClusterDimension;
   cluster.val.clusterDim.x = static_cast<unsigned>(ctas);
   cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
-  config.attrs = &cluster;
-  config.numAttrs = 1;
-  const cudaError_t err = cudaLaunchKernelEx(&config, kernel, args...);
-  return err == cudaSuccess ? KF_OK : cuda_error(err, what);
+  return launch_plan(kernel, ctas, smem, &cluster, stream, what, args...);
+}
+
+// A launch behind another of this call starts while that one ends, and waits for it where it needs its results.
+template <typename Kernel, typename... Args>
+int launch_behind(Kernel kernel, int ctas, int smem, cudaStream_t stream, const char* what, const Args&... args) {
+  cudaLaunchAttribute behind{};
+  behind.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  behind.val.programmaticStreamSerializationAllowed = 1;
+  return launch_plan(kernel, ctas, smem, &behind, stream, what, args...);
 }
 
 // One CTA where it does the work in a few rounds: its barriers are cheaper than a cluster's.
@@ -531,9 +599,23 @@ int launch_fork(const PageCaches& all, const PageGeometry& g, const kf_fork_args
 }
 
 int launch_release(const kf_release_args& r, const DeviceInfo& dev, cudaStream_t stream) {
-  const ReleaseArgs a{r.block_table, r.table_stride, r.table_cols, r.rows,   r.context, r.holders,  r.pages,
-                      r.block_size,  r.requests,     static_cast<int>(r.count), r.held, r.freed, r.n_freed};
-  return launch_cluster(release_kernel, plan_ctas(r.count * r.table_cols), 0, stream, "launch(release)", a);
+  const int64_t parts = ceil_div(r.table_cols, TILE), tiles = r.count * parts;
+  const ReleaseArgs a{r.block_table, r.table_stride, r.table_cols, r.rows, r.context, r.holders, r.pages, r.block_size,
+                      r.requests, static_cast<int>(r.count), static_cast<int>(parts),
+                      reinterpret_cast<uint32_t*>(r.scratch), r.scratch + tiles * TILE_WORDS, r.freed, r.n_freed};
+  const auto smem = [&](int ctas) { return static_cast<int>(ceil_div(tiles, ctas * PLAN_WARPS) * PLAN_WARPS * 4); };
+  // A cluster takes about 9 us and 5 more for each 16384 pages, the four launches 13 us.
+  if (tiles * TILE <= 32768) {
+    const int ctas = plan_ctas(tiles * TILE);
+    return launch_cluster(release_kernel<-1>, ctas, smem(ctas), stream, "launch(release)", a);
+  }
+  const int64_t want = ceil_div(tiles, PLAN_WARPS);
+  const int ctas = static_cast<int>(want < dev.sm_count ? want : dev.sm_count);
+  int rc = launch_plan(release_kernel<0>, ctas, 0, nullptr, stream, "launch(release)", a);
+  if (rc == KF_OK) rc = launch_behind(release_kernel<1>, ctas, 0, stream, "launch(release marks)", a);
+  if (rc == KF_OK) rc = launch_behind(release_kernel<2>, ctas, 0, stream, "launch(release votes)", a);
+  if (rc == KF_OK) rc = launch_behind(release_kernel<3>, ctas, smem(ctas), stream, "launch(release list)", a);
+  return rc;
 }
 
 int launch_compact_plan(const kf_compact_args& c, const PageGeometry& g, const DeviceInfo& dev, cudaStream_t stream) {

@@ -219,10 +219,11 @@ def release_requests(
     if block_size < 1:
         raise ValueError(f"block_size must be positive, got {block_size}")
     n, cols = requests.shape[0], block_table.shape[1]
-    if n * cols >= 1 << 30:
-        raise ValueError(f"requests x blocks must be below 2^30, got {n} x {cols}")
-    pages, held, count = block_table.new_empty(n * cols + n + 1).split_with_sizes((n * cols, n, 1))
-    native.release(block_table, context_lens, holders, requests, block_size, held, pages, count)
+    parts = n * -(-cols // 256)
+    if parts > 200_000 or n * cols >= 1 << 30:
+        raise ValueError(f"requests of one call must have 200000 parts of 256 blocks at most, got {n} x {cols}")
+    scratch, pages, count = block_table.new_empty(9 * parts + n * cols + 1).split_with_sizes((9 * parts, n * cols, 1))
+    native.release(block_table, context_lens, holders, requests, block_size, scratch, pages, count)
     return Released(pages, count)
 
 

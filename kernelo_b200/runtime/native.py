@@ -862,11 +862,11 @@ def fork(caches: list[torch.Tensor], block_table: torch.Tensor, context: torch.T
 
 
 def release(block_table: torch.Tensor, context: torch.Tensor, holders: torch.Tensor, requests: torch.Tensor,
-            block_size: int, held: torch.Tensor, freed: torch.Tensor, n_freed: torch.Tensor) -> None:
+            block_size: int, scratch: torch.Tensor, freed: torch.Tensor, n_freed: torch.Tensor) -> None:
     lib = _lib or load()
     _launch(lib.kf_release,
             RELEASE_ARGS.pack(*_table_fields(block_table), context.data_ptr(), holders.data_ptr(), holders.shape[0],
-                              block_size, requests.data_ptr(), requests.shape[0], held.data_ptr(), freed.data_ptr(),
+                              block_size, requests.data_ptr(), requests.shape[0], scratch.data_ptr(), freed.data_ptr(),
                               n_freed.data_ptr()),
             block_table.device, "kf_release")
 
