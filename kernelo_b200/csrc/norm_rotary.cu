@@ -12,12 +12,14 @@
 // A head is held by a power of two of lanes, each with the two vectors of a unit
 // (rotary.cuh), so that the sums are shuffles among them and nothing is read twice.
 //
-// Bound by bytes. Forward: a group of lanes takes several heads of a token with one load
-// of its angles, two heads' loads in flight. Backward: the blocks that are resident at once
-// share the tokens, those of q and those of k apart, so that a thread sums its own
-// columns of dw in registers over all of its heads and tokens; a block adds its
-// groups in shared memory, and a second small launch the blocks, each in a
-// fixed order: no atomics, the same bits from call to call.
+// Forward: bound by bytes. A group of lanes takes several heads of a token with one load of its angles, two heads'
+// loads in flight. 8192 tokens of 32 query and 8 key heads of 128 bf16 with the cache written: 49 us, 4.5 TB/s (69% of
+// a copy's rate; the turn alone, without norms, 42); 64 tokens 4.7 us.
+// Backward: rows (token, head) are dealt out in runs, those of q and of k apart, so that a thread sums its own
+// columns of dw in registers over its rows, its next rows on their way to shared memory meanwhile; a
+// block adds its groups, and a second small launch the blocks, each in a fixed order: no atomics, the
+// same bits from call to call. 4096 tokens: 44 us (2.9 TB/s) and 3 for the sums; bound by the instructions of a row (some
+// 400 a warp, with 16 warps resident to an SM) and by its latencies.
 #include <cuda.h>
 
 #include "kf_common.cuh"
@@ -28,26 +30,24 @@ namespace kf {
 namespace {
 
 constexpr int NORM_THREADS = 128;
-constexpr int BATCH = 2;       // heads whose loads are in flight together
 constexpr int HEADS_EACH = 6;  // heads that a group takes with one load of its angles
+constexpr int BATCH = 2;       // of them, whose loads are in flight together
+constexpr int FWD_BLOCKS = 7;  // of an SM, for 72 registers: 8192 tokens 49.3 us; 6 blocks 51.0, 8 65.3 (spills)
 
-// Lanes of a head, units in it (and turned ones), heads side by side, tokens of a block.
+// Lanes of a head, units in it (and turned ones); forward: heads side by side, tokens of a block, rounds through the heads.
 struct NormPlan {
-  int width, units, turned, lanes, tokens;
+  int width, units, turned, lanes, tokens, rounds;
 };
 
 // Units that a lane holds where heads of up to NORM_ROTARY_MAX_DIM elements have no wider vectors.
 template <int VE>
 constexpr int UNITS_EACH = VE >= 4 ? 1 : NORM_ROTARY_MAX_DIM / 2 / VE / 32;
 
-// The lanes of this thread's head.
-__device__ __forceinline__ unsigned group_mask(int width) {
-  const int thread = threadIdx.x + blockDim.x * (threadIdx.y + blockDim.y * threadIdx.z);
-  const unsigned lanes = width == 32 ? 0xffffffffu : (1u << width) - 1;
-  return lanes << (thread & 31 & ~(width - 1));
-}
-__device__ __forceinline__ float group_sum(float v, int width, unsigned mask) {
-  for (int o = width >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(mask, v, o);
+// Sum over the lanes of each head of a warp. All lanes of the warp take part, those without a head too: with shuffles
+// among the lanes of one head alone the warp's heads may run one after another (4096 tokens of 64 heads of 80: 57 us
+// where this takes 51).
+__device__ __forceinline__ float group_sum(float v, int width) {
+  for (int o = width >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 
@@ -59,11 +59,6 @@ __device__ __forceinline__ bool too_far(float sum) {
   return sizeof(T) == 4 || DType<T>::code == KF_BF16 ? !(sum < __int_as_float(0x7f800000)) : false;
 }
 
-template <typename T, int VE>
-struct HeadWeight {
-  Vec<T, VE> first[UNITS_EACH<VE>], second[UNITS_EACH<VE>];
-};
-
 // One thread's part of a head: its units' elements and angles.
 template <typename T, int VE>
 struct Lane {
@@ -73,26 +68,20 @@ struct Lane {
   bool active[U];
   float c[U][VE], s[U][VE];
 
-  __device__ __forceinline__ void init(const RotaryArgs& p, const NormPlan& plan) {
+  __device__ __forceinline__ void init(const RotaryArgs& p, const NormPlan& plan, int lane) {
 #pragma unroll
     for (int j = 0; j < U; ++j) {
-      const int unit = threadIdx.x + j * plan.width;
+      const int unit = lane + j * plan.width;
       active[j] = unit < plan.units;
       u[j] = unit_of<VE>(unit, plan.turned, static_cast<int>(p.rot), static_cast<int>(p.dim), p.interleaved);
     }
   }
-  template <bool BACK = false>
   __device__ __forceinline__ void angles(const RotaryArgs& p, long long t) {
     if (p.rot == 0) return;
     const int pos = __ldg(p.positions + t);
 #pragma unroll
     for (int j = 0; j < U; ++j) {
-      if (!active[j] || !u[j].turned) continue;
-      load_angles<VE>(p, pos, u[j].pairs, c[j], s[j]);
-      if constexpr (BACK) {
-#pragma unroll
-        for (int i = 0; i < VE; ++i) s[j][i] = -s[j][i];
-      }
+      if (active[j] && u[j].turned) load_angles<VE>(p, pos, u[j].pairs, c[j], s[j]);
     }
   }
   // Vectors that a head does not have are zeros.
@@ -113,8 +102,8 @@ struct Lane {
     }
   }
   // x, y: the head's vectors, left as its outputs.
-  __device__ __forceinline__ void forward(V (&x)[U], V (&y)[U], const HeadWeight<T, VE>& w, float eps, float inv_dim,
-                                          int width, unsigned mask, int interleaved) const {
+  __device__ __forceinline__ void forward(V (&x)[U], V (&y)[U], const V (&wx)[U], const V (&wy)[U], float eps, float inv_dim,
+                                          int width, int interleaved) const {
     float a[U][VE], b[U][VE], sum = 0.0f;
 #pragma unroll
     for (int j = 0; j < U; ++j) {
@@ -123,24 +112,25 @@ struct Lane {
 #pragma unroll
       for (int i = 0; i < VE; ++i) sum = fmaf(a[j][i], a[j][i], fmaf(b[j][i], b[j][i], sum));
     }
-    sum = group_sum(sum, width, mask);
-    if (too_far<T>(sum)) {
+    sum = group_sum(sum, width);
+    if (__any_sync(0xffffffffu, too_far<T>(sum))) {
+      const float less = too_far<T>(sum) ? FAR : 1.0f;
       sum = 0.0f;
 #pragma unroll
       for (int j = 0; j < U; ++j)
 #pragma unroll
         for (int i = 0; i < VE; ++i) {
-          a[j][i] *= FAR, b[j][i] *= FAR;
+          a[j][i] *= less, b[j][i] *= less;
           sum = fmaf(a[j][i], a[j][i], fmaf(b[j][i], b[j][i], sum));
         }
-      sum = group_sum(sum, width, mask);
+      sum = group_sum(sum, width);
     }
     const float r = rsqrtf(fmaf(sum, inv_dim, eps));
 #pragma unroll
     for (int j = 0; j < U; ++j) {
       float wa[VE], wb[VE];
-      widen<T, VE>(w.first[j], wa);
-      widen<T, VE>(w.second[j], wb);
+      widen<T, VE>(wx[j], wa);
+      widen<T, VE>(wy[j], wb);
 #pragma unroll
       for (int i = 0; i < VE; ++i) {
         a[j][i] = a[j][i] * r * wa[i];
@@ -154,73 +144,89 @@ struct Lane {
 };
 
 template <typename T, int VE>
-__global__ void __launch_bounds__(NORM_THREADS, VE == 8 ? 5 : 4)
+__global__ void __launch_bounds__(NORM_THREADS, FWD_BLOCKS)
     norm_rotary_kernel(const __grid_constant__ RotaryArgs p, const NormArgs n, const NormPlan plan) {
   using L = Lane<T, VE>;
   constexpr int U = L::U;
-  const long long t = static_cast<long long>(blockIdx.x) * plan.tokens + threadIdx.z;
-  if (t >= p.tokens) return;  // a head's lanes have one token: they leave together
-  const unsigned mask = group_mask(plan.width);
-  const int width = plan.width;
+  const int width = plan.width, lanes = plan.lanes, group = threadIdx.x / width;
+  const long long t = static_cast<long long>(blockIdx.x) * plan.tokens + group / lanes;
+  const bool has_token = t < p.tokens && group / lanes < plan.tokens;
   L me;
-  me.init(p, plan);
-  me.angles(p, t);
-  HeadWeight<T, VE> w;
-  const float eps = n.eps, inv_dim = n.inv_dim;
-  const int hq = static_cast<int>(p.heads), hk = static_cast<int>(p.kv_heads), lanes = plan.lanes;
-  int h = threadIdx.y;
-  if (h < hq) {
-    me.load(static_cast<const T*>(n.q_weight), w.first, w.second);
-    const T* q = static_cast<const T*>(p.q) + t * p.sq_t;
-    T* q_out = static_cast<T*>(p.q_out) + t * p.sqo_t;
-    for (; h < hq; h += BATCH * lanes) {
-      typename L::V x[BATCH][U], y[BATCH][U];
+  me.init(p, plan, threadIdx.x % width);
+  const Place at = has_token ? place_of(p, t) : Place{-1, 0};
+  // Heads of q, then of k, then of v: as far as they go anywhere.
+  const int hq = static_cast<int>(p.heads), hk = static_cast<int>(p.kv_heads);
+  const int normed = !has_token ? 0 : hq + (p.k_out != nullptr || at.page >= 0 ? hk : 0);
+  const int all = normed + (at.page >= 0 ? hk : 0);
+  const T* const q = static_cast<const T*>(p.q) + t * p.sq_t;
+  const T* const k = static_cast<const T*>(p.k) + t * p.sk_t;
+  const T* const v = static_cast<const T*>(p.v) + t * p.sv_t;
+  if (has_token) me.angles(p, t);
+  // (the same rounds for all groups of a warp)
+  for (int round = 0; round < plan.rounds; ++round) {
+    const int h0 = group % lanes + round * BATCH * lanes;
+    typename L::V x[BATCH][U], y[BATCH][U];
 #pragma unroll
-      for (int i = 0; i < BATCH; ++i)
-        if (h + i * lanes < hq) me.load(q + (h + i * lanes) * p.sq_h, x[i], y[i]);
+    for (int i = 0; i < BATCH; ++i) {
+      const int h = h0 + i * lanes;
+      if (h < all) me.load(h < hq ? q + h * p.sq_h : h < normed ? k + (h - hq) * p.sk_h : v + (h - normed) * p.sv_h, x[i], y[i]);
+    }
 #pragma unroll
-      for (int i = 0; i < BATCH; ++i) {
-        if (h + i * lanes < hq) {
-          me.forward(x[i], y[i], w, eps, inv_dim, width, mask, p.interleaved);
-          me.store(q_out + (h + i * lanes) * p.sqo_h, x[i], y[i]);
+    for (int i = 0; i < BATCH; ++i) {
+      const int h = h0 + i * lanes;
+      if (__any_sync(0xffffffffu, h < normed)) {
+        typename L::V wx[U], wy[U], ox[U], oy[U];  // weights from L1: all heads have them in common
+        me.load(static_cast<const T*>(h < hq ? n.q_weight : n.k_weight), wx, wy);
+#pragma unroll
+        for (int j = 0; j < U; ++j) ox[j] = x[i][j], oy[j] = y[i][j];
+        me.forward(ox, oy, wx, wy, n.eps, n.inv_dim, width, p.interleaved);
+        if (h < normed) {
+#pragma unroll
+          for (int j = 0; j < U; ++j) x[i][j] = ox[j], y[i][j] = oy[j];
         }
       }
+      if (h < min(hq, normed)) {
+        me.store(static_cast<T*>(p.q_out) + t * p.sqo_t + h * p.sqo_h, x[i], y[i]);
+      } else if (h < normed) {
+        const int g = h - hq;
+        if (p.k_out != nullptr) me.store(static_cast<T*>(p.k_out) + t * p.sko_t + g * p.sko_h, x[i], y[i]);
+        if (at.page >= 0) me.store(static_cast<T*>(p.k_cache) + at.page * p.skc_p + g * p.skc_h + at.slot * p.skc_s, x[i], y[i]);
+      } else if (h < all) {
+        me.store(static_cast<T*>(p.v_cache) + at.page * p.svc_p + (h - normed) * p.svc_h + at.slot * p.svc_s, x[i], y[i]);
+      }
     }
-    // on with the heads of k where this group's stride left q
-    while (h - lanes >= hq) h -= lanes;
-  }
-  const Place at = place_of(p, t);
-  if (at.page < 0 && p.k_out == nullptr) return;
-  if (h < hq + hk) me.load(static_cast<const T*>(n.k_weight), w.first, w.second);
-  for (; h < hq + hk; h += lanes) {
-    const int g = h - hq;
-    typename L::V x[U], y[U];
-    me.load(static_cast<const T*>(p.k) + t * p.sk_t + g * p.sk_h, x, y);
-    me.forward(x, y, w, eps, inv_dim, width, mask, p.interleaved);
-    if (p.k_out != nullptr) me.store(static_cast<T*>(p.k_out) + t * p.sko_t + g * p.sko_h, x, y);
-    if (at.page >= 0)
-      me.store(static_cast<T*>(p.k_cache) + at.page * p.skc_p + g * p.skc_h + at.slot * p.skc_s, x, y);
-  }
-  if (at.page < 0) return;
-  for (; h < hq + 2 * hk; h += lanes) {
-    const int g = h - hq - hk;
-    typename L::V x[U], y[U];
-    me.load(static_cast<const T*>(p.v) + t * p.sv_t + g * p.sv_h, x, y);
-    me.store(static_cast<T*>(p.v_cache) + at.page * p.svc_p + g * p.svc_h + at.slot * p.svc_s, x, y);
   }
 }
 
 // ---------------------------------------------------------------- gradient
-// Blocks of q first, then those of k. `partial` gets a row of dim sums from each.
+// Rows (token, head) of q or of k in order, a run of them to each group of lanes. A thread's vectors of the next rows
+// are on their way to its own places in shared memory (nobody else reads them: no barriers) while it computes.
+constexpr int STAGES = 4;
+// Blocks of an SM, and how many times as many the rows are dealt out to: those that run beside slower ones then end
+// earlier. 4096 tokens of 40 heads of 128 bf16: 43.8 us; 1 wave 50.4, 4 waves 50.5; 3 blocks 44.4.
+constexpr int GRAD_BLOCKS = 4, GRAD_WAVES = 2;
+
+__device__ __forceinline__ void copy_async(uint32_t to, const void* from, int bytes) {
+  if (bytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+  else if (bytes == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to), "l"(from) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
+}
+
+// `partial` gets a row of dim sums from each block, q's first. Blocks of the two kinds are mixed: those of k change
+// token oftener, and a few SMs that had only those would end last.
 template <typename T, int VE>
-__global__ void __launch_bounds__(NORM_THREADS, 4)
+__global__ void __launch_bounds__(NORM_THREADS, GRAD_BLOCKS)
     norm_rotary_grad_kernel(const __grid_constant__ NormGradArgs a, const NormPlan plan, int q_blocks, int k_blocks) {
   using L = Lane<T, VE>;
+  using V = typename L::V;
   constexpr int U = L::U;
-  __shared__ float sums[2 * VE * U * NORM_THREADS];
+  griddep_launch_dependents();  // the sums' blocks wait for this grid's end
+  __shared__ __align__(16) V ring[STAGES][4][U][NORM_THREADS];
+  static_assert(sizeof(ring) >= 2 * VE * U * NORM_THREADS * sizeof(float), "the sums lie in the ring when it is done");
   const RotaryArgs& p = a.rotary;  // q and k: the inputs; q_out and k_out: their gradients
-  const bool of_q = static_cast<int>(blockIdx.x) < q_blocks;
-  const int block = of_q ? blockIdx.x : blockIdx.x - q_blocks, blocks = of_q ? q_blocks : k_blocks;
+  const int n_k = static_cast<int>(static_cast<long long>(blockIdx.x) * k_blocks / (q_blocks + k_blocks));  // in front
+  const bool of_q = static_cast<int>(static_cast<long long>(blockIdx.x + 1) * k_blocks / (q_blocks + k_blocks)) == n_k;
+  const int block = of_q ? blockIdx.x - n_k : n_k, blocks = of_q ? q_blocks : k_blocks;
   const T* const x_all = static_cast<const T*>(of_q ? p.q : p.k);
   const T* const d_all = static_cast<const T*>(of_q ? a.dq : a.dk);
   T* const out_all = static_cast<T*>(of_q ? p.q_out : p.k_out);
@@ -228,95 +234,150 @@ __global__ void __launch_bounds__(NORM_THREADS, 4)
   const long long sd_t = of_q ? a.sdq_t : a.sdk_t, sd_h = of_q ? a.sdq_h : a.sdk_h;
   const long long so_t = of_q ? p.sqo_t : p.sko_t, so_h = of_q ? p.sqo_h : p.sko_h;
   const int heads = static_cast<int>(of_q ? p.heads : p.kv_heads);
-  const unsigned mask = group_mask(plan.width);
-  // groups of lanes: heads side by side x tokens
-  const int width = plan.width, group = threadIdx.y, groups = blockDim.y;
-  const int lanes = min(heads, groups), tokens = groups / lanes, lane = group % lanes, token = group / lanes;
+  const int width = plan.width, groups = NORM_THREADS / width, thread = threadIdx.x, group = thread / width;
   L me;
-  me.init(p, plan);
-  HeadWeight<T, VE> w;
-  me.load(static_cast<const T*>(of_q ? a.norm.q_weight : a.norm.k_weight), w.first, w.second);
-  float wsum_a[U][VE] = {}, wsum_b[U][VE] = {};
-  for (long long t = static_cast<long long>(block) * tokens + token; t < p.tokens && token < tokens;
-       t += static_cast<long long>(blocks) * tokens) {
-    me.template angles<true>(p, t);
-    for (int h = lane; h < heads; h += lanes) {
-      typename L::V x[U], y[U], dx[U], dy[U];
-      me.load(x_all + t * sx_t + h * sx_h, x, y);
-      me.load(d_all + t * sd_t + h * sd_h, dx, dy);
-      float xa[U][VE], xb[U][VE], ga[U][VE], gb[U][VE], square = 0.0f, along = 0.0f;
+  me.init(p, plan, thread % width);
+  using F = Floats<VE>;
+  F wa[U], wb[U];
+  {
+    V wx[U], wy[U];
+    me.load(static_cast<const T*>(of_q ? a.norm.q_weight : a.norm.k_weight), wx, wy);
 #pragma unroll
-      for (int j = 0; j < U; ++j) {
-        widen<T, VE>(x[j], xa[j]);
-        widen<T, VE>(y[j], xb[j]);
-        widen<T, VE>(dx[j], ga[j]);
-        widen<T, VE>(dy[j], gb[j]);
-        if (me.u[j].turned) turn<VE>(ga[j], gb[j], me.c[j], me.s[j], p.interleaved);
-        float wa[VE], wb[VE];
-        widen<T, VE>(w.first[j], wa);
-        widen<T, VE>(w.second[j], wb);
-#pragma unroll
-        for (int i = 0; i < VE; ++i) {
-          square = fmaf(xa[j][i], xa[j][i], fmaf(xb[j][i], xb[j][i], square));
-          along = fmaf(ga[j][i] * wa[i], xa[j][i], fmaf(gb[j][i] * wb[i], xb[j][i], along));
-        }
-      }
-      square = group_sum(square, width, mask);
-      along = group_sum(along, width, mask);
-      float scale = 1.0f;
-      if (too_far<T>(square)) {
-        scale = FAR, square = along = 0.0f;
-#pragma unroll
-        for (int j = 0; j < U; ++j) {
-          float wa[VE], wb[VE];
-          widen<T, VE>(w.first[j], wa);
-          widen<T, VE>(w.second[j], wb);
-#pragma unroll
-          for (int i = 0; i < VE; ++i) {
-            xa[j][i] *= FAR, xb[j][i] *= FAR;
-            square = fmaf(xa[j][i], xa[j][i], fmaf(xb[j][i], xb[j][i], square));
-            along = fmaf(ga[j][i] * wa[i], xa[j][i], fmaf(gb[j][i] * wb[i], xb[j][i], along));
-          }
-        }
-        square = group_sum(square, width, mask);
-        along = group_sum(along, width, mask);
-      }
-      const float r = rsqrtf(fmaf(square, a.norm.inv_dim, a.norm.eps));
-      const float r_true = r * scale;                         // 1 / s
-      const float back = along * r * a.norm.inv_dim * r_true;  // mean(g w u) / s
-#pragma unroll
-      for (int j = 0; j < U; ++j) {
-        float wa[VE], wb[VE];
-        widen<T, VE>(w.first[j], wa);
-        widen<T, VE>(w.second[j], wb);
-#pragma unroll
-        for (int i = 0; i < VE; ++i) {
-          const float ua = xa[j][i] * r, ub = xb[j][i] * r;
-          wsum_a[j][i] = fmaf(ga[j][i], ua, wsum_a[j][i]);
-          wsum_b[j][i] = fmaf(gb[j][i], ub, wsum_b[j][i]);
-          xa[j][i] = fmaf(ga[j][i] * wa[i], r_true, -(ua * back));
-          xb[j][i] = fmaf(gb[j][i] * wb[i], r_true, -(ub * back));
-        }
-        narrow<T, VE>(xa[j], x[j]);
-        narrow<T, VE>(xb[j], y[j]);
-      }
-      me.store(out_all + t * so_t + h * so_h, x, y);
-    }
+    for (int j = 0; j < U; ++j) wa[j] = floats<T, VE>(wx[j]), wb[j] = floats<T, VE>(wy[j]);
   }
+  // This group's run of rows, and the next one to fetch. (The rounds are the same for all groups of a warp.)
+  const long long rows = p.tokens * heads, runs = static_cast<long long>(blocks) * groups;
+  const long long run = static_cast<long long>(block) * groups + group;
+  const long long first = rows / runs * run + min(rows % runs, run);
+  const int mine = static_cast<int>(rows / runs + (run < rows % runs ? 1 : 0));
+  const int rounds = static_cast<int>((rows + runs - 1) / runs);
+  long long t = first / heads, t_next = t;
+  int h = static_cast<int>(first - t * heads), h_next = h;
+  const auto fetch = [&](int stage) {
+    const T* const x = x_all + t_next * sx_t + h_next * sx_h;
+    const T* const d = d_all + t_next * sd_t + h_next * sd_h;
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const auto piece = [&](int which, const T* from) {
+        V* const to = &ring[stage][which][j][thread];
+        if constexpr (sizeof(V) >= 4) copy_async(smem_u32(to), from, sizeof(V));
+        else *to = *reinterpret_cast<const V*>(from);
+      };
+      if (!me.active[j]) continue;
+      piece(0, x + me.u[j].e0);
+      piece(2, d + me.u[j].e0);
+      if (!me.u[j].second) continue;
+      piece(1, x + me.u[j].e1);
+      piece(3, d + me.u[j].e1);
+    }
+    if (++h_next == heads) h_next = 0, ++t_next;
+  };
+  // places that no row fills are zeros, and those of a group that has no row left are as an earlier row left them
+#pragma unroll
+  for (int s = 0; s < STAGES; ++s)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < U; ++j) ring[s][i][j][thread] = V{};
+#pragma unroll
+  for (int s = 0; s < STAGES - 1; ++s) {
+    if (s < mine) fetch(s);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  F sum_a[U], sum_b[U];
+#pragma unroll
+  for (int j = 0; j < U; ++j)
+#pragma unroll
+    for (int i = 0; i < F::N; ++i) sum_a[j].e[i] = sum_b[j].e[i] = p_splat<VE>(0.0f);
+  long long angles_of = -1;
+  for (int r = 0; r < rounds; ++r) {
+    const bool here = r < mine;  // not in the last round, it may be: zeros then
+    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+    if (here && t != angles_of) {
+      me.angles(p, t);
+#pragma unroll
+      for (int j = 0; j < U; ++j)
+#pragma unroll
+        for (int i = 0; i < VE; ++i) me.s[j][i] = -me.s[j][i];  // the turn back
+      angles_of = t;
+    }
+    const int stage = r % STAGES;
+    F xa[U], xb[U], ga[U], gb[U];
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      xa[j] = floats<T, VE>(ring[stage][0][j][thread]), xb[j] = floats<T, VE>(ring[stage][1][j][thread]);
+      V gx = ring[stage][2][j][thread], gy = ring[stage][3][j][thread];
+      if (!here) gx = gy = V{};
+      ga[j] = floats<T, VE>(gx), gb[j] = floats<T, VE>(gy);
+    }
+    // into the places that were read in the last round
+    if (r + STAGES - 1 < mine) fetch((r + STAGES - 1) % STAGES);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    // This lane's sums of x^2 and of g w x.
+    const auto sums_of = [&](float& square, float& along) {
+      auto xx = p_splat<VE>(0.0f), gwx = p_splat<VE>(0.0f);
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+#pragma unroll
+        for (int i = 0; i < F::N; ++i) {
+          xx = p_fma(xa[j].e[i], xa[j].e[i], p_fma(xb[j].e[i], xb[j].e[i], xx));
+          gwx = p_fma(p_mul(ga[j].e[i], wa[j].e[i]), xa[j].e[i], p_fma(p_mul(gb[j].e[i], wb[j].e[i]), xb[j].e[i], gwx));
+        }
+      }
+      square = group_sum(p_sum(xx), width);
+      along = group_sum(p_sum(gwx), width);
+    };
+#pragma unroll
+    for (int j = 0; j < U; ++j)
+      if (here && me.u[j].turned) turn<VE>(ga[j], gb[j], me.c[j], me.s[j], p.interleaved);
+    float square, along, scale = 1.0f;
+    sums_of(square, along);
+    if (__any_sync(0xffffffffu, too_far<T>(square))) {
+      if (too_far<T>(square)) scale = FAR;
+      const auto less = p_splat<VE>(scale);
+#pragma unroll
+      for (int j = 0; j < U; ++j)
+#pragma unroll
+        for (int i = 0; i < F::N; ++i) xa[j].e[i] = p_mul(xa[j].e[i], less), xb[j].e[i] = p_mul(xb[j].e[i], less);
+      sums_of(square, along);
+    }
+    const float inv = rsqrtf(fmaf(square, a.norm.inv_dim, a.norm.eps));
+    const float inv_true = inv * scale;                            // 1 / s
+    const float back = along * inv * a.norm.inv_dim * inv_true;  // mean(g w u) / s
+    const auto inv2 = p_splat<VE>(inv), true2 = p_splat<VE>(inv_true), back2 = p_splat<VE>(-back);
+    V x[U], y[U];
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+#pragma unroll
+      for (int i = 0; i < F::N; ++i) {
+        const auto ua = p_mul(xa[j].e[i], inv2), ub = p_mul(xb[j].e[i], inv2);
+        sum_a[j].e[i] = p_fma(ga[j].e[i], ua, sum_a[j].e[i]);
+        sum_b[j].e[i] = p_fma(gb[j].e[i], ub, sum_b[j].e[i]);
+        xa[j].e[i] = p_fma(p_mul(ga[j].e[i], wa[j].e[i]), true2, p_mul(ua, back2));
+        xb[j].e[i] = p_fma(p_mul(gb[j].e[i], wb[j].e[i]), true2, p_mul(ub, back2));
+      }
+      narrow<T, VE>(xa[j], x[j]);
+      narrow<T, VE>(xb[j], y[j]);
+    }
+    if (here) me.store(out_all + t * so_t + h * so_h, x, y);
+    if (++h == heads) h = 0, ++t;
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncthreads();
   // The block's groups of lanes, one after another.
+  float* const sums = reinterpret_cast<float*>(ring);
   const int row = 2 * VE * U * width;  // of a group: [unit of the lane][lane][first and second vector]
 #pragma unroll
   for (int j = 0; j < U; ++j)
 #pragma unroll
-    for (int i = 0; i < VE; ++i) {
-      float* const at = sums + group * row + (j * width + threadIdx.x) * 2 * VE;
-      at[i] = wsum_a[j][i];
-      at[VE + i] = wsum_b[j][i];
+    for (int i = 0; i < F::N; ++i) {
+      auto* const at = reinterpret_cast<typename F::E*>(sums + group * row + (j * width + thread % width) * 2 * VE);
+      at[i] = sum_a[j].e[i];
+      at[F::N + i] = sum_b[j].e[i];
     }
   __syncthreads();
-  float* const partial = a.partial + static_cast<long long>(blockIdx.x) * p.dim;
-  const int thread = threadIdx.x + width * group, threads = width * groups;
-  for (int e = thread; e < row; e += threads) {
+  float* const partial = a.partial + static_cast<long long>(of_q ? block : q_blocks + block) * p.dim;
+  for (int e = thread; e < row; e += width * groups) {
     const Unit u = unit_of<VE>(e / (2 * VE), plan.turned, static_cast<int>(p.rot), static_cast<int>(p.dim), p.interleaved);
     const int in = e % (2 * VE);
     if (e / (2 * VE) >= plan.units || (in >= VE && !u.second)) continue;
@@ -331,6 +392,7 @@ constexpr int SUM_ROWS = 32;
 __global__ void __launch_bounds__(32 * SUM_ROWS)
     norm_weight_sum_kernel(const float* __restrict__ partial, int q_blocks, int k_blocks, int dim, float* q_grad, float* k_grad) {
   __shared__ float sums[SUM_ROWS][33];
+  griddep_wait();
   const int half = gridDim.x / 2;
   const bool of_q = static_cast<int>(blockIdx.x) < half;
   const int column = (of_q ? blockIdx.x : blockIdx.x - half) * 32 + threadIdx.x;
@@ -386,11 +448,10 @@ int launch_typed(const RotaryArgs& a, const NormArgs& n, const DeviceInfo& dev, 
   const int64_t most = NORM_THREADS / plan.width, lanes = few ? all : ceil_div(all, HEADS_EACH);
   plan.lanes = static_cast<int>(lanes < most ? lanes : most);
   plan.tokens = NORM_THREADS / (plan.width * plan.lanes);
-  if (plan.tokens > 64) plan.tokens = 64;  // the limit of a block's third extent
+  plan.rounds = static_cast<int>(ceil_div(all, BATCH * plan.lanes));
   const int64_t blocks = ceil_div(a.tokens, plan.tokens);
   if (blocks > 0x7fffffffll) return set_error(KF_ERR_UNSUPPORTED, "norm_rotary: tokens beyond the grid");
-  norm_rotary_kernel<T, VE><<<static_cast<unsigned>(blocks), dim3(plan.width, plan.lanes, plan.tokens), 0, stream>>>(
-      a, n, plan);
+  norm_rotary_kernel<T, VE><<<static_cast<unsigned>(blocks), NORM_THREADS, 0, stream>>>(a, n, plan);
   const cudaError_t err = cudaGetLastError();
   return err == cudaSuccess ? KF_OK : cuda_error(err, "launch(norm_rotary)");
 }
@@ -401,31 +462,33 @@ int pick(const RotaryArgs& a, const NormArgs& n, const DeviceInfo& dev, cudaStre
                    [&](auto ve) { return launch_typed<T, decltype(ve)::value>(a, n, dev, stream); });
 }
 
-// Blocks of the gradient: as many as are resident at once, shared out by heads; from the sizes alone.
+// Blocks of the gradient, shared out by heads; fewer where each of their groups would have less than ROWS_EACH rows.
+constexpr int ROWS_EACH = 4;
 struct GradBlocks {
   int q, k;
 };
-GradBlocks grad_blocks(int64_t tokens, int64_t heads, int64_t kv_heads, int sm_count) {
-  const int64_t resident = 4ll * sm_count;
+GradBlocks grad_blocks(int64_t tokens, int64_t heads, int64_t kv_heads, int groups, int sm_count) {
+  const int64_t resident = static_cast<int64_t>(GRAD_BLOCKS) * GRAD_WAVES * sm_count;
   auto share = [&](int64_t mine) -> int {
-    if (mine == 0 || tokens == 0) return 0;
-    const int64_t n = ceil_div(resident * mine, heads + kv_heads);
-    return static_cast<int>(n < tokens ? n : tokens);
+    const int64_t n = ceil_div(resident * mine, heads + kv_heads > 0 ? heads + kv_heads : 1);
+    const int64_t most = ceil_div(tokens * mine, ROWS_EACH * groups);
+    return static_cast<int>(n < most ? n : most);
   };
   return {share(heads), share(kv_heads)};
 }
 
 template <typename T, int VE>
-int launch_grad_typed(const NormGradArgs& a, const GradBlocks& blocks, cudaStream_t stream) {
+int launch_grad_typed(const NormGradArgs& a, const DeviceInfo& dev, GradBlocks* used, cudaStream_t stream) {
   const NormPlan plan = head_plan<VE>(a.rotary);
-  norm_rotary_grad_kernel<T, VE><<<static_cast<unsigned>(blocks.q + blocks.k), dim3(plan.width, NORM_THREADS / plan.width), 0,
-                                   stream>>>(a, plan, blocks.q, blocks.k);
+  const RotaryArgs& r = a.rotary;
+  const GradBlocks blocks = *used = grad_blocks(r.tokens, r.heads, r.kv_heads, NORM_THREADS / plan.width, dev.sm_count);
+  norm_rotary_grad_kernel<T, VE><<<static_cast<unsigned>(blocks.q + blocks.k), NORM_THREADS, 0, stream>>>(a, plan, blocks.q, blocks.k);
   const cudaError_t err = cudaGetLastError();
   return err == cudaSuccess ? KF_OK : cuda_error(err, "launch(norm_rotary gradient)");
 }
 
 template <typename T>
-int pick_grad(const NormGradArgs& a, const GradBlocks& blocks, cudaStream_t stream) {
+int pick_grad(const NormGradArgs& a, const DeviceInfo& dev, GradBlocks* used, cudaStream_t stream) {
   const int elem = static_cast<int>(sizeof(T));
   return widest<T>(
       [&](auto ve) {
@@ -433,7 +496,7 @@ int pick_grad(const NormGradArgs& a, const GradBlocks& blocks, cudaStream_t stre
         return whole<T, VE>(a.rotary, a.norm) && on_grid(a.dq, VE, elem, {a.sdq_t, a.sdq_h}) &&
                on_grid(a.dk, VE, elem, {a.sdk_t, a.sdk_h});
       },
-      [&](auto ve) { return launch_grad_typed<T, decltype(ve)::value>(a, blocks, stream); });
+      [&](auto ve) { return launch_grad_typed<T, decltype(ve)::value>(a, dev, used, stream); });
 }
 
 }  // namespace
@@ -448,27 +511,34 @@ int launch_norm_rotary(const RotaryArgs& a, const NormArgs& n, const DeviceInfo&
 
 int64_t norm_rotary_grad_workspace_bytes(int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim,
                                          const DeviceInfo& dev) {
-  const GradBlocks blocks = grad_blocks(tokens, heads, kv_heads, dev.sm_count);
+  const GradBlocks blocks = grad_blocks(tokens, heads, kv_heads, NORM_THREADS / 32, dev.sm_count);  // the most that are used
   return static_cast<int64_t>(blocks.q + blocks.k) * dim * 4;
 }
 
 int launch_norm_rotary_grad(const NormGradArgs& a, const DeviceInfo& dev, cudaStream_t stream) {
   const RotaryArgs& r = a.rotary;
-  const GradBlocks blocks = grad_blocks(r.tokens, r.heads, r.kv_heads, dev.sm_count);
-  if (blocks.q + blocks.k > 0) {
+  GradBlocks blocks{0, 0};
+  if (r.tokens > 0 && r.heads + r.kv_heads > 0) {
     int rc;
     switch (r.dtype) {
-      case KF_FP16: rc = pick_grad<__half>(a, blocks, stream); break;
-      case KF_BF16: rc = pick_grad<__nv_bfloat16>(a, blocks, stream); break;
-      default: rc = pick_grad<float>(a, blocks, stream); break;
+      case KF_FP16: rc = pick_grad<__half>(a, dev, &blocks, stream); break;
+      case KF_BF16: rc = pick_grad<__nv_bfloat16>(a, dev, &blocks, stream); break;
+      default: rc = pick_grad<float>(a, dev, &blocks, stream); break;
     }
     if (rc != KF_OK) return rc;
   }
   const unsigned columns = static_cast<unsigned>(ceil_div(r.dim, 32));
-  norm_weight_sum_kernel<<<2 * columns, dim3(32, SUM_ROWS), 0, stream>>>(a.partial, blocks.q, blocks.k,
-                                                                       static_cast<int>(r.dim), a.q_weight_grad,
-                                                                       a.k_weight_grad);
-  const cudaError_t err = cudaGetLastError();
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(2 * columns);
+  config.blockDim = dim3(32, SUM_ROWS);
+  config.stream = stream;
+  cudaLaunchAttribute behind{};
+  behind.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  behind.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &behind;
+  config.numAttrs = blocks.q + blocks.k > 0 ? 1 : 0;
+  const cudaError_t err = cudaLaunchKernelEx(&config, norm_weight_sum_kernel, static_cast<const float*>(a.partial), blocks.q,
+                                             blocks.k, static_cast<int>(r.dim), a.q_weight_grad, a.k_weight_grad);
   return err == cudaSuccess ? KF_OK : cuda_error(err, "launch(norm weight sums)");
 }
 

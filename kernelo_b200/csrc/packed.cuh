@@ -44,5 +44,59 @@ __device__ __forceinline__ void narrow(const float (&f)[VE], Vec<T, VE>& x) {
   }
 }
 
+
+// VE elements in fp32, two to a register pair, for the packed arithmetic that does two in one instruction (kf_common.cuh).
+template <int VE>
+struct Floats {
+  static constexpr int N = VE == 1 ? 1 : VE / 2;
+  using E = std::conditional_t<VE == 1, float, uint64_t>;
+  E e[N];
+};
+__device__ __forceinline__ float p_mul(float a, float b) { return a * b; }
+__device__ __forceinline__ uint64_t p_mul(uint64_t a, uint64_t b) { return f2_mul(a, b); }
+__device__ __forceinline__ float p_fma(float a, float b, float c) { return fmaf(a, b, c); }
+__device__ __forceinline__ uint64_t p_fma(uint64_t a, uint64_t b, uint64_t c) { return f2_fma(a, b, c); }
+__device__ __forceinline__ float p_neg(float a) { return -a; }
+__device__ __forceinline__ uint64_t p_neg(uint64_t a) { return a ^ 0x8000000080000000ull; }
+__device__ __forceinline__ float p_sum(float a) { return a; }
+__device__ __forceinline__ float p_sum(uint64_t a) {
+  const float2 f = f2_unpack(a);
+  return f.x + f.y;
+}
+template <int VE>
+__device__ __forceinline__ typename Floats<VE>::E p_splat(float a) {
+  if constexpr (VE == 1) return a;
+  else return f2_splat(a);
+}
+template <int VE>
+__device__ __forceinline__ typename Floats<VE>::E p_at(const float (&f)[VE], int i) {
+  if constexpr (VE == 1) return f[0];
+  else return f2_pack(f[2 * i], f[2 * i + 1]);
+}
+
+template <typename T, int VE>
+__device__ __forceinline__ Floats<VE> floats(const Vec<T, VE>& x) {
+  float f[VE];
+  widen<T, VE>(x, f);
+  Floats<VE> to;
+#pragma unroll
+  for (int i = 0; i < Floats<VE>::N; ++i) to.e[i] = p_at<VE>(f, i);
+  return to;
+}
+template <typename T, int VE>
+__device__ __forceinline__ void narrow(const Floats<VE>& x, Vec<T, VE>& to) {
+  float f[VE];
+#pragma unroll
+  for (int i = 0; i < Floats<VE>::N; ++i) {
+    if constexpr (VE == 1) {
+      f[0] = x.e[0];
+    } else {
+      const float2 two = f2_unpack(x.e[i]);
+      f[2 * i] = two.x, f[2 * i + 1] = two.y;
+    }
+  }
+  narrow<T, VE>(f, to);
+}
+
 }  // namespace
 }  // namespace kf

@@ -40,6 +40,24 @@ __device__ __forceinline__ void turn(float (&a)[VE], float (&b)[VE], const float
     }
   }
 }
+template <int VE>
+__device__ __forceinline__ void turn(Floats<VE>& a, Floats<VE>& b, const float (&c)[VE], const float (&s)[VE], int interleaved) {
+#pragma unroll
+  for (int i = 0; i < Floats<VE>::N; ++i) {
+    if constexpr (VE > 1) {
+      if (interleaved) {  // a pair's two elements lie side by side
+        const float2 x = f2_unpack(a.e[i]), y = f2_unpack(b.e[i]);
+        const float cx = c[i], sx = s[i], cy = c[VE / 2 + i], sy = s[VE / 2 + i];
+        a.e[i] = f2_pack(fmaf(x.x, cx, -(x.y * sx)), fmaf(x.x, sx, x.y * cx));
+        b.e[i] = f2_pack(fmaf(y.x, cy, -(y.y * sy)), fmaf(y.x, sy, y.y * cy));
+        continue;
+      }
+    }
+    const auto cs = p_at<VE>(c, i), sn = p_at<VE>(s, i), x = a.e[i];
+    a.e[i] = p_fma(x, cs, p_neg(p_mul(b.e[i], sn)));
+    b.e[i] = p_fma(x, sn, p_mul(b.e[i], cs));
+  }
+}
 template <typename T, int VE>
 __device__ __forceinline__ void turn(Vec<T, VE>& x, Vec<T, VE>& y, const float (&c)[VE], const float (&s)[VE],
                                      int interleaved) {

@@ -11,7 +11,7 @@ from __future__ import annotations
 
 import torch
 
-from kernelo_b200.kernels.attention import _check_output
+from kernelo_b200.kernels.attention import _check_output, _empty_like
 from kernelo_b200.runtime import native
 
 
@@ -34,6 +34,73 @@ def _check_logits(logits: torch.Tensor) -> None:
         raise ValueError(f"logits must be a CUDA tensor, got {logits.device}")
     if logits.stride(1) != 1 and logits.shape[1] > 1:
         raise ValueError("logits must have contiguous rows. Pass logits.contiguous() explicitly.")
+
+
+def _ints(t: torch.Tensor | None, device: int, shape: tuple, dtype: torch.dtype = torch.int32) -> bool:
+    """Whether an optional operand of one dimension is right."""
+    return t is None or (t.dtype is dtype and t.get_device() == device and t.shape == shape and t.is_contiguous())
+
+
+def _history(tokens, token_lens, prompt_lens, repetition, frequency, presence, device: int, row: tuple) -> bool:
+    if tokens is None:
+        return token_lens is None and prompt_lens is None and repetition is None and frequency is None and presence is None
+    return (token_lens is not None and tokens.dtype is torch.int32 and tokens.get_device() == device and tokens.ndim == 2
+            and tokens.shape[0] == row[0] and tokens.stride(1) == 1 and _ints(token_lens, device, row)
+            and _ints(prompt_lens, device, row) and _ints(repetition, device, row, torch.float32)
+            and _ints(frequency, device, row, torch.float32) and _ints(presence, device, row, torch.float32))
+
+
+def _lists(tokens, values, device: int, rows: int) -> bool:
+    if tokens is None or values is None:
+        return tokens is values
+    return (tokens.dtype is torch.int32 and values.dtype is torch.float32 and tokens.get_device() == device
+            and values.get_device() == device and tokens.ndim == 2 and tokens.shape == values.shape
+            and tokens.shape[0] == rows and tokens.stride(1) == 1 == values.stride(1))
+
+
+def _masks(allowed, allowed_rows, device: int, row: tuple, vocab: int) -> bool:
+    if allowed is None:
+        return allowed_rows is None
+    return (allowed.dtype is torch.int32 and allowed.get_device() == device and allowed.ndim == 2 and allowed.stride(1) == 1
+            and allowed.shape[1] * 32 >= vocab and (allowed_rows is not None or allowed.shape[0] == row[0])
+            and _ints(allowed_rows, device, row))
+
+
+def _check_all(logits, tokens, token_lens, prompt_lens, repetition, frequency, presence, bias_tokens, bias_values, allowed,
+               allowed_rows) -> None:
+    _check_logits(logits)
+    rows, vocab = logits.shape
+    if (tokens is None) != (token_lens is None):
+        raise ValueError("tokens and token_lens go together")
+    if tokens is not None:
+        _check_rows("tokens", tokens, logits, torch.int32, 2, rows)
+        _check_rows("token_lens", token_lens, logits, torch.int32, 1, rows)
+        if prompt_lens is not None:
+            _check_rows("prompt_lens", prompt_lens, logits, torch.int32, 1, rows)
+        if repetition is not None:
+            _check_rows("repetition", repetition, logits, torch.float32, 1, rows)
+        if frequency is not None:
+            _check_rows("frequency", frequency, logits, torch.float32, 1, rows)
+        if presence is not None:
+            _check_rows("presence", presence, logits, torch.float32, 1, rows)
+    elif not (prompt_lens is None and repetition is None and frequency is None and presence is None):
+        raise ValueError("penalties need tokens and token_lens")
+    if (bias_tokens is None) != (bias_values is None):
+        raise ValueError("bias_tokens and bias_values go together")
+    if bias_tokens is not None:
+        _check_rows("bias_tokens", bias_tokens, logits, torch.int32, 2, rows)
+        _check_rows("bias_values", bias_values, logits, torch.float32, 2, rows)
+        if bias_tokens.shape != bias_values.shape:
+            raise ValueError(f"bias_tokens and bias_values must have one shape, got {tuple(bias_tokens.shape)} and "
+                             f"{tuple(bias_values.shape)}")
+    if allowed is not None:
+        _check_rows("allowed", allowed, logits, torch.int32, 2, rows if allowed_rows is None else None)
+        if allowed.shape[1] * 32 < vocab:
+            raise ValueError(f"allowed has {allowed.shape[1]} words for {vocab} tokens")
+        if allowed_rows is not None:
+            _check_rows("allowed_rows", allowed_rows, logits, torch.int32, 1, rows)
+    elif allowed_rows is not None:
+        raise ValueError("allowed_rows needs allowed")
 
 
 def adjust_logits(
@@ -71,41 +138,16 @@ def adjust_logits(
     be ``logits`` itself, and shares no memory with it otherwise. A row whose mask
     allows nothing is all ``-inf``.
     """
-    _check_logits(logits)
-    rows, vocab = logits.shape
-    if (tokens is None) != (token_lens is None):
-        raise ValueError("tokens and token_lens go together")
-    if tokens is not None:
-        _check_rows("tokens", tokens, logits, torch.int32, 2, rows)
-        _check_rows("token_lens", token_lens, logits, torch.int32, 1, rows)
-        if prompt_lens is not None:
-            _check_rows("prompt_lens", prompt_lens, logits, torch.int32, 1, rows)
-        if repetition is not None:
-            _check_rows("repetition", repetition, logits, torch.float32, 1, rows)
-        if frequency is not None:
-            _check_rows("frequency", frequency, logits, torch.float32, 1, rows)
-        if presence is not None:
-            _check_rows("presence", presence, logits, torch.float32, 1, rows)
-    elif not (prompt_lens is None and repetition is None and frequency is None and presence is None):
-        raise ValueError("penalties need tokens and token_lens")
-    if (bias_tokens is None) != (bias_values is None):
-        raise ValueError("bias_tokens and bias_values go together")
-    if bias_tokens is not None:
-        _check_rows("bias_tokens", bias_tokens, logits, torch.int32, 2, rows)
-        _check_rows("bias_values", bias_values, logits, torch.float32, 2, rows)
-        if bias_tokens.shape != bias_values.shape:
-            raise ValueError(f"bias_tokens and bias_values must have one shape, got {tuple(bias_tokens.shape)} and "
-                             f"{tuple(bias_values.shape)}")
-    if allowed is not None:
-        _check_rows("allowed", allowed, logits, torch.int32, 2, rows if allowed_rows is None else None)
-        if allowed.shape[1] * 32 < vocab:
-            raise ValueError(f"allowed has {allowed.shape[1]} words for {vocab} tokens")
-        if allowed_rows is not None:
-            _check_rows("allowed_rows", allowed_rows, logits, torch.int32, 1, rows)
-    elif allowed_rows is not None:
-        raise ValueError("allowed_rows needs allowed")
+    rows, vocab = logits.shape if logits.ndim == 2 else (0, 0)
+    # one expression for what is right, and the reasons only where it is not
+    device, row = logits.get_device(), (rows,)
+    if not (logits.ndim == 2 and logits.is_cuda and logits.stride(1) == 1 and _history(
+            tokens, token_lens, prompt_lens, repetition, frequency, presence, device, row)
+            and _lists(bias_tokens, bias_values, device, rows) and _masks(allowed, allowed_rows, device, row, vocab)):
+        _check_all(logits, tokens, token_lens, prompt_lens, repetition, frequency, presence, bias_tokens, bias_values, allowed,
+                   allowed_rows)
     if out is None:
-        out = torch.empty((rows, vocab), device=logits.device, dtype=logits.dtype)
+        out = _empty_like(logits)
     else:
         if out.shape != logits.shape or out.dtype is not logits.dtype or out.get_device() != logits.get_device():
             raise ValueError(f"out must be {logits.dtype} {tuple(logits.shape)} on {logits.device}, got {out.dtype} "

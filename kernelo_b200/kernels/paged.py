@@ -123,6 +123,12 @@ def _check_table(block_table: torch.Tensor, context_lens: torch.Tensor, holders:
     if not block_table.is_cuda:
         raise ValueError(f"block_table must be a CUDA tensor, got {block_table.device}")
     rows, cols = block_table.shape
+    device = block_table.get_device()
+    # one expression for what is right, and the reasons only where it is not
+    if (block_table.is_contiguous() and context_lens.dtype is torch.int32 and context_lens.get_device() == device
+            and context_lens.shape == (rows,) and context_lens.is_contiguous() and holders.dtype is torch.int32
+            and holders.get_device() == device and holders.ndim == 1 and holders.is_contiguous()):
+        return
     if (block_table.stride(1) != 1 and cols > 1) or (block_table.stride(0) < cols and rows > 1):
         raise ValueError("block_table must have contiguous rows that do not overlap")
     _check_index("context_lens", context_lens, block_table)
@@ -149,12 +155,16 @@ def _check_caches(caches: Sequence[torch.Tensor], block_table: torch.Tensor, hol
         raise ValueError(f"expected caches (pages, kv_heads, block, dim), got {tuple(shape)}")
     if shape[0] != holders.shape[0]:
         raise ValueError(f"holders must have shape ({shape[0]},) for caches {tuple(shape)}, got {tuple(holders.shape)}")
-    for c in caches:
-        if c.shape != shape or c.stride() != stride or c.dtype is not dtype:
-            raise ValueError(f"caches must have one type, shape and strides, got {dtype} {tuple(shape)} {stride} and "
-                             f"{c.dtype} {tuple(c.shape)} {c.stride()}")
-        if c.get_device() != device:
-            raise ValueError(f"caches must be on {block_table.device}, got {c.device}")
+    n = len(caches)
+    # all at once (a model has a cache for each layer's keys and values), and one by one where something is wrong
+    if not ([c.shape for c in caches].count(shape) == n == [c.stride() for c in caches].count(stride)
+            and [c.dtype for c in caches].count(dtype) == n == [c.get_device() for c in caches].count(device)):
+        for c in caches:
+            if c.shape != shape or c.stride() != stride or c.dtype is not dtype:
+                raise ValueError(f"caches must have one type, shape and strides, got {dtype} {tuple(shape)} {stride} and "
+                                 f"{c.dtype} {tuple(c.shape)} {c.stride()}")
+            if c.get_device() != device:
+                raise ValueError(f"caches must be on {block_table.device}, got {c.device}")
     if stride[3] != 1 and shape[3] > 1:
         raise ValueError("caches must have a contiguous last dimension")
     if any(s == 0 and n > 1 for s, n in zip(stride, shape)):

@@ -199,14 +199,19 @@ def rotary_to_cache(
 
 
 def _check_norm(q: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, eps: float) -> None:
-    dim = q.shape[2]
-    if dim > MAX_NORM_DIM:
-        raise ValueError(f"norms take heads of at most {MAX_NORM_DIM} elements, got {dim}")
+    shape, dtype, device = q.shape[2:], q.dtype, q.get_device()
+    # one expression for what is right, and the reasons only where it is not
+    if (q_weight.shape == shape == k_weight.shape and q_weight.dtype is dtype and k_weight.dtype is dtype
+            and q_weight.get_device() == device == k_weight.get_device() and q_weight.is_contiguous()
+            and k_weight.is_contiguous() and shape[0] <= MAX_NORM_DIM and 0.0 < eps < math.inf):
+        return
+    if shape[0] > MAX_NORM_DIM:
+        raise ValueError(f"norms take heads of at most {MAX_NORM_DIM} elements, got {shape[0]}")
     if not 0.0 < eps < math.inf:
         raise ValueError(f"eps must be finite and positive, got {eps}")
     for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w.ndim != 1 or w.shape[0] != dim:
-            raise ValueError(f"{name} must have shape ({dim},), got {tuple(w.shape)}")
+        if w.shape != shape:
+            raise ValueError(f"{name} must have shape ({shape[0]},), got {tuple(w.shape)}")
         _check_operand(name, w, q)
 
 
@@ -314,13 +319,16 @@ def norm_rotary_backward(
     """
     _check(q, k, positions, table)
     _check_norm(q, q_weight, k_weight, eps)
-    for name, d, x in (("dq", dq, q), ("dk", dk, k)):
-        if d.shape != x.shape:
-            raise ValueError(f"{name} must have shape {tuple(x.shape)}, got {tuple(d.shape)}")
-        _check_operand(name, d, q)
-    q_grad, k_grad = _empty_like(q), _empty_like(k)
-    weight_grads = torch.empty(2, q.shape[2], device=q.device, dtype=torch.float32)
-    if q.shape[2]:
+    dtype, device = q.dtype, q.get_device()
+    if not (dq.shape == q.shape and dk.shape == k.shape and dq.dtype is dtype and dk.dtype is dtype
+            and dq.get_device() == device == dk.get_device() and dq.stride(2) == 1 == dk.stride(2)):
+        for name, d, x in (("dq", dq, q), ("dk", dk, k)):
+            if d.shape != x.shape:
+                raise ValueError(f"{name} must have shape {tuple(x.shape)}, got {tuple(d.shape)}")
+            _check_operand(name, d, q)
+    q_grad, k_grad, dim = _empty_like(q), _empty_like(k), q.shape[2]
+    weight_grads = table.new_empty(2, dim)
+    if dim:
         native.norm_rotary_grad(dq, dk, q, k, q_grad, k_grad, positions, table, q_weight, k_weight, eps, weight_grads,
                                 interleaved=interleaved)
     return q_grad, k_grad, *weight_grads.unbind(0)

@@ -294,6 +294,7 @@ def check(status: int, what: str) -> None:
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 _is_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
 
 
@@ -796,8 +797,9 @@ def norm_rotary(q: torch.Tensor, k: torch.Tensor, q_out: torch.Tensor, k_out: to
 
 def _launch(entry, packed: bytes, device: torch.device, what: str) -> None:
     """The entry on the device's current stream, with the device made the current one where it is not."""
-    if device.index == torch.cuda.current_device():
-        status = entry(packed, current_stream_handle(device))
+    index = device.index
+    if _raw_stream is not None and index == _current_device():
+        status = entry(packed, _raw_stream(index))
     else:
         with torch.cuda.device(device):
             status = entry(packed, current_stream_handle(device))
@@ -823,7 +825,7 @@ def norm_rotary_grad(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor, k: tor
             _workspace_sizes.clear()
         _workspace_sizes[key] = ws_bytes
     # plain memory of this call, not the stream's workspace, whose first words are other kernels' counters
-    partial = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    partial = table.new_empty(ws_bytes // 4)
     sdq_row, sdq_head, _ = dq.stride()
     sdk_row, sdk_head, _ = dk.stride()
     _launch(lib.kf_norm_rotary_grad,
