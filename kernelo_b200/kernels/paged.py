@@ -203,9 +203,9 @@ def fork_requests(
     _check_list("children", children, block_table)
     if parents.shape != children.shape:
         raise ValueError(f"parents and children must have one shape, got {tuple(parents.shape)} and {tuple(children.shape)}")
-    counts = block_table.new_empty(2)
+    counts = block_table.new_empty((2, 1))
     native.fork(caches, block_table, context_lens, holders, free_blocks, parents, children, counts)
-    return Forked(*counts.split(1))
+    return Forked(*counts.unbind(0))
 
 
 def release_requests(

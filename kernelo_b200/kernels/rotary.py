@@ -77,14 +77,14 @@ def rotary_table(
 
 
 def _check(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, table: torch.Tensor) -> None:
-    device = q.get_device()
+    device, shape, k_shape, turned = q.get_device(), q.shape, k.shape, table.shape
     # one expression for what is right, and the reasons only where it is not
-    if (q.is_cuda and q.ndim == 3 == k.ndim and k.dtype is q.dtype and q.shape[0] == k.shape[0]
-            and q.shape[2] == k.shape[2] and q.stride(2) == 1 == k.stride(2) and k.get_device() == device
+    if (q.is_cuda and len(shape) == 3 == len(k_shape) and k.dtype is q.dtype and shape[0] == k_shape[0]
+            and shape[2] == k_shape[2] and q.stride()[2] == 1 == k.stride()[2] and k.get_device() == device
             and positions.dtype is torch.int32 and positions.get_device() == device and positions.ndim == 1
-            and positions.shape[0] == q.shape[0] and positions.is_contiguous()
-            and table.dtype is torch.float32 and table.get_device() == device and table.ndim == 2
-            and table.is_contiguous() and table.shape[1] <= q.shape[2] and table.shape[1] % 2 == 0):
+            and positions.shape[0] == shape[0] and positions.is_contiguous()
+            and table.dtype is torch.float32 and table.get_device() == device and len(turned) == 2
+            and table.is_contiguous() and turned[1] <= shape[2] and turned[1] % 2 == 0):
         return
     if q.ndim != 3 or k.ndim != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
         raise ValueError("expected q (tokens, heads, dim) and k (tokens, kv_heads, dim), got "
@@ -120,13 +120,13 @@ def _check_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: tor
 
 def _check_cached(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                   slots: torch.Tensor) -> None:
-    dtype, device = q.dtype, q.get_device()
-    if not (v.shape == k.shape and v.dtype is dtype and v.get_device() == device and v.stride(2) == 1
-            and k_cache.ndim == 4 and v_cache.shape == k_cache.shape and k_cache.shape[1] == k.shape[1]
-            and k_cache.shape[3] == k.shape[2] and k_cache.shape[2] > 0 and k_cache.dtype is dtype
-            and v_cache.dtype is dtype and k_cache.get_device() == device == v_cache.get_device()
-            and k_cache.stride(3) == 1 == v_cache.stride(3) and slots.dtype is torch.int64
-            and slots.get_device() == device and slots.ndim == 1 and slots.shape[0] == q.shape[0]
+    dtype, device, k_shape, pages = q.dtype, q.get_device(), k.shape, k_cache.shape
+    if not (v.shape == k_shape and v.dtype is dtype and v.get_device() == device and v.stride()[2] == 1
+            and len(pages) == 4 and v_cache.shape == pages and pages[1] == k_shape[1] and pages[3] == k_shape[2]
+            and pages[2] > 0 and k_cache.dtype is dtype and v_cache.dtype is dtype
+            and k_cache.get_device() == device == v_cache.get_device()
+            and k_cache.stride()[3] == 1 == v_cache.stride()[3] and slots.dtype is torch.int64
+            and slots.get_device() == device and slots.ndim == 1 and slots.shape[0] == k_shape[0]
             and slots.is_contiguous()):
         _check_cache(q, k, v, k_cache, v_cache, slots)
 
