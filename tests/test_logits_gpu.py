@@ -155,6 +155,18 @@ def test_what_lies_outside_is_ignored(device):
     check(adjust_logits(**a), a)
 
 
+@pytest.mark.parametrize("biases", [1, 2, 31, 32, 33, 512, 513, 1500])
+def test_lists_of_biases_with_tokens_listed_twice(biases, device):
+    a = make(6, 9001, torch.bfloat16, device, masks=6, biases=biases)
+    gen = torch.Generator().manual_seed(5)
+    few = torch.randint(-1, 9001, (max(1, biases // 3),), generator=gen, dtype=torch.int32)
+    a["bias_tokens"] = few[torch.randint(0, few.numel(), (6, biases), generator=gen)].to(device)
+    a["tokens"][:, ::2] = a["bias_tokens"][:, :1].clamp(min=0)
+    check(adjust_logits(**a), a)
+    view = a["logits"].clone()
+    assert torch.equal(adjust_logits(**(a | {"logits": view}), out=view), adjust_logits(**a))
+
+
 def test_a_token_listed_many_times(device):
     """Counts do not depend on an order, and of several biases the last one counts."""
     a = make(4, 9000, torch.float32, device, history=20000, biases=700)
