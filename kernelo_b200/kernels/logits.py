@@ -14,6 +14,8 @@ import torch
 from kernelo_b200.kernels.attention import _check_output, _empty_like
 from kernelo_b200.runtime import native
 
+MAX_BIASES = 16384
+
 
 def _check_rows(name: str, t: torch.Tensor, logits: torch.Tensor, dtype: torch.dtype, ndim: int, rows: int | None) -> None:
     if t.dtype is not dtype:
@@ -55,7 +57,7 @@ def _lists(tokens, values, device: int, rows: int) -> bool:
         return tokens is values
     return (tokens.dtype is torch.int32 and values.dtype is torch.float32 and tokens.get_device() == device
             and values.get_device() == device and tokens.ndim == 2 and tokens.shape == values.shape
-            and tokens.shape[0] == rows and tokens.stride(1) == 1 == values.stride(1))
+            and tokens.shape[0] == rows and tokens.shape[1] <= MAX_BIASES and tokens.stride(1) == 1 == values.stride(1))
 
 
 def _masks(allowed, allowed_rows, device: int, row: tuple, vocab: int) -> bool:
@@ -93,6 +95,8 @@ def _check_all(logits, tokens, token_lens, prompt_lens, repetition, frequency, p
         if bias_tokens.shape != bias_values.shape:
             raise ValueError(f"bias_tokens and bias_values must have one shape, got {tuple(bias_tokens.shape)} and "
                              f"{tuple(bias_values.shape)}")
+        if bias_tokens.shape[1] > MAX_BIASES:
+            raise ValueError(f"a row may have {MAX_BIASES} biases at most, got {bias_tokens.shape[1]}")
     if allowed is not None:
         _check_rows("allowed", allowed, logits, torch.int32, 2, rows if allowed_rows is None else None)
         if allowed.shape[1] * 32 < vocab:
@@ -126,7 +130,7 @@ def adjust_logits(
       divides the positive logits of all tokens of the history and multiplies the
       others. A token that stands ``n`` times behind the prompt loses
       ``frequency[r] * n + presence[r]`` (fp32 ``(rows,)``).
-    * ``bias_values[r, i]`` (fp32 ``(rows, biases)``) is added to the logit of token
+    * ``bias_values[r, i]`` (fp32 ``(rows, biases)``, 16384 at most) is added to the logit of token
       ``bias_tokens[r, i]`` (int32, negative: none). A token that is listed twice
       gets the last value.
     * ``allowed`` (int32 ``(masks, words)``): where bit ``v % 32`` of word ``v //

@@ -10,7 +10,7 @@ ways with one copy of its whole pages, :func:`release_requests` gives back the
 pages that nobody holds any more, and :func:`compact_pages` moves the live pages
 of a pool to its front. All three keep ``holders`` (int32 ``(pages,)``, zeros at
 first): how many requests hold a page besides the first. They too read nothing on
-the host.
+the host. Calls on one pool follow one another: on one stream, or ordered by events.
 """
 
 from __future__ import annotations
@@ -92,6 +92,9 @@ def build_slots(
         .split_with_sizes((max_tokens, seqs + 1, 1, 1))
     native.build_slots(context_lens, new_lens, block_table, free_blocks, block_size, cu_new, positions, slots, taken)
     return StepSlots(cu_new, positions, slots, taken, dropped)
+
+
+MAX_COMPACT_PAGES = 1 << 22
 
 
 class Forked(NamedTuple):
@@ -254,6 +257,8 @@ def compact_pages(
     _check_table(block_table, context_lens, holders)
     caches = _check_caches(caches, block_table, holders)
     pages = holders.shape[0]
+    if pages > MAX_COMPACT_PAGES:
+        raise ValueError(f"compact_pages takes pools of at most {MAX_COMPACT_PAGES} pages, got {pages}")
     renamed, sources, targets, live, moves = block_table.new_empty(pages + 2 * (pages // 2) + 2) \
         .split_with_sizes((pages, pages // 2, pages // 2, 1, 1))
     native.compact(caches, block_table, context_lens, holders, renamed, sources, targets, live)

@@ -155,7 +155,7 @@ def test_what_lies_outside_is_ignored(device):
     check(adjust_logits(**a), a)
 
 
-@pytest.mark.parametrize("biases", [1, 2, 31, 32, 33, 512, 513, 1500])
+@pytest.mark.parametrize("biases", [1, 2, 31, 32, 33, 512, 513, 1500, 16384])
 def test_lists_of_biases_with_tokens_listed_twice(biases, device):
     a = make(6, 9001, torch.bfloat16, device, masks=6, biases=biases)
     gen = torch.Generator().manual_seed(5)
@@ -268,6 +268,9 @@ def test_refusals(device):
                             (dict(out=logits.t().contiguous().t()), "contiguous rows")):
         with pytest.raises(ValueError, match=message):
             adjust_logits(**(a | change))
+    long = {"bias_tokens": torch.zeros(4, 16385, dtype=torch.int32, device=device), "bias_values": torch.zeros(4, 16385, device=device)}
+    with pytest.raises(ValueError, match="16384 biases"):
+        adjust_logits(**(a | long))
     buf = torch.zeros(8, 100, device=device, dtype=torch.float16)
     with pytest.raises(ValueError, match="shares memory with logits"):
         adjust_logits(buf[:4], out=buf[1:5])

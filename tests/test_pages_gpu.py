@@ -351,6 +351,48 @@ def test_captured_and_replayed_with_other_requests(device):
             assert torch.equal(a, b)
 
 
+def test_many_released_captured_and_replayed(device):
+    """Enough entries for a launch of each phase: a graph of them, replayed beside eager calls on another stream."""
+    rng = random.Random(3)
+    lens = [rng.randint(0, 2000) for _ in range(300)]
+    share = [(r // 5 * 5, r, rng.randint(0, min(lens[r], lens[r // 5 * 5]) // 16)) for r in range(300) if r % 5]
+    pool = Pool(lens, device, blocks=40000, cols=130, heads=1, dim=2, caches=1, share=share)
+    ended = pool.ints(rng.sample(range(300), 290))
+    state = (pool.d_table, pool.d_lens, pool.d_holders)
+    start = [x.clone() for x in state]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        release_requests(*state, ended, block_size=16)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = release_requests(*state, ended, block_size=16)
+    for seed in range(3):
+        ended.copy_(pool.ints(random.Random(seed).sample(range(300), 290)))
+        for to, x in zip(state, start):
+            to.copy_(x)
+        graph.replay()
+        graph.replay()  # of requests that have ended: nothing
+        assert captured.count.item() == 0
+        for to, x in zip(state, start):
+            to.copy_(x)
+        graph.replay()
+        torch.cuda.synchronize()
+        seen = [x.clone() for x in (*captured, *state)]
+        for to, x in zip(state, start):
+            to.copy_(x)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            eager = release_requests(*state, ended, block_size=16)
+        side.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(seen, (*eager, *state)))
+    for to, x in zip(state, start):
+        to.copy_(x)
+    pool.release(ended.tolist())
+    pool.check()
+
+
 def test_refusals(device):
     pool = Pool([40, 33, 0, 0], device)
     table, lens, holders, free = pool.d_table, pool.d_lens, pool.d_holders, pool.d_free
