@@ -32,12 +32,6 @@ constexpr int LOGITS_THREADS = 512;
 constexpr uint32_t IN_PROMPT = 0x80000000u, BIASED = 0x40000000u, TIMES = 0x3fffffffu;
 constexpr int IDS_EACH = 4;  // tokens of the history that a thread holds at a time
 
-template <typename Word>
-__device__ __forceinline__ Word bits_as(uint32_t u) {
-  if constexpr (sizeof(Word) == 4 && std::is_same_v<Word, float>) return __uint_as_float(u);
-  else return u;
-}
-
 // The vector with the elements whose bit of `off` is set at -infinity.
 template <typename T, int VE>
 __device__ __forceinline__ void mask_out(Vec<T, VE>& x, uint32_t off) {
@@ -51,20 +45,6 @@ __device__ __forceinline__ void mask_out(Vec<T, VE>& x, uint32_t off) {
       if ((off >> i & 1u) != 0) x.w[i] = from_f32<T>(__int_as_float(0xff800000));
     }
   }
-}
-
-// A vector that nobody reads again.
-template <typename V>
-__device__ __forceinline__ V load_once(const void* from) {
-  V x;
-  if constexpr (sizeof(V) == 16) {
-    const uint4 u = __ldcs(static_cast<const uint4*>(from));
-    x.w[0] = bits_as<typename V::Word>(u.x), x.w[1] = bits_as<typename V::Word>(u.y);
-    x.w[2] = bits_as<typename V::Word>(u.z), x.w[3] = bits_as<typename V::Word>(u.w);
-  } else {
-    x = *static_cast<const V*>(from);
-  }
-  return x;
 }
 
 // The elements of a vector that lie in a row of `vocab`, its first being element v.

@@ -13,8 +13,9 @@
 // (rotary.cuh), so that the sums are shuffles among them and nothing is read twice.
 //
 // Forward: bound by bytes. A group of lanes takes several heads of a token with one load of its angles, two heads'
-// loads in flight. 8192 tokens of 32 query and 8 key heads of 128 bf16 with the cache written: 49 us, 4.5 TB/s (69% of
-// a copy's rate; the turn alone, without norms, 42); 64 tokens 4.7 us.
+// loads in flight. 8192 tokens of 32 query and 8 key heads of 128 bf16 with the cache written: 47 us, 4.7 TB/s (72% of
+// a copy's rate; the turn alone, without norms, 42); 64 tokens 4.7 us. Operands and outputs pass through the cache as the
+// first to leave it, weights and angles stay (with plain accesses 49 us, and 28 instead of 25 for 2048 tokens in fp32).
 // Backward: rows (token, head) are dealt out in runs, those of q and of k apart, so that a thread sums its own
 // columns of dw in registers over its rows, its next rows on their way to shared memory meanwhile; a
 // block adds its groups, and a second small launch the blocks, each in a fixed order: no atomics, the
@@ -32,7 +33,7 @@ namespace {
 constexpr int NORM_THREADS = 128;
 constexpr int HEADS_EACH = 6;  // heads that a group takes with one load of its angles
 constexpr int BATCH = 2;       // of them, whose loads are in flight together
-constexpr int FWD_BLOCKS = 7;  // of an SM, for 72 registers: 8192 tokens 49.3 us; 6 blocks 51.0, 8 65.3 (spills)
+constexpr int FWD_BLOCKS = 7;  // of an SM, for 72 registers (with plain accesses 49.3 us; 6 blocks 51.0, 8 65.3: spills)
 
 // Lanes of a head, units in it (and turned ones); forward: heads side by side, tokens of a block, rounds through the heads.
 struct NormPlan {
@@ -85,20 +86,22 @@ struct Lane {
     }
   }
   // Vectors that a head does not have are zeros.
+  template <bool COMMON = false>  // weights
   __device__ __forceinline__ void load(const T* head, V (&x)[U], V (&y)[U]) const {
 #pragma unroll
     for (int j = 0; j < U; ++j) {
-      if (active[j]) x[j] = *reinterpret_cast<const V*>(head + u[j].e0);
+      const T *const at = head + u[j].e0, *const second = head + u[j].e1;
+      if (active[j]) x[j] = COMMON ? load_common<V>(at) : load_once<V>(at);
       else x[j] = V{};
-      if (active[j] && u[j].second) y[j] = *reinterpret_cast<const V*>(head + u[j].e1);
+      if (active[j] && u[j].second) y[j] = COMMON ? load_common<V>(second) : load_once<V>(second);
       else y[j] = V{};
     }
   }
   __device__ __forceinline__ void store(T* head, const V (&x)[U], const V (&y)[U]) const {
 #pragma unroll
     for (int j = 0; j < U; ++j) {
-      if (active[j]) *reinterpret_cast<V*>(head + u[j].e0) = x[j];
-      if (active[j] && u[j].second) *reinterpret_cast<V*>(head + u[j].e1) = y[j];
+      if (active[j]) store_once(head + u[j].e0, x[j]);
+      if (active[j] && u[j].second) store_once(head + u[j].e1, y[j]);
     }
   }
   // x, y: the head's vectors, left as its outputs.
@@ -176,7 +179,7 @@ __global__ void __launch_bounds__(NORM_THREADS, FWD_BLOCKS)
       const int h = h0 + i * lanes;
       if (__any_sync(0xffffffffu, h < normed)) {
         typename L::V wx[U], wy[U], ox[U], oy[U];  // weights from L1: all heads have them in common
-        me.load(static_cast<const T*>(h < hq ? n.q_weight : n.k_weight), wx, wy);
+        me.template load<true>(static_cast<const T*>(h < hq ? n.q_weight : n.k_weight), wx, wy);
 #pragma unroll
         for (int j = 0; j < U; ++j) ox[j] = x[i][j], oy[j] = y[i][j];
         me.forward(ox, oy, wx, wy, n.eps, n.inv_dim, width, p.interleaved);
@@ -241,7 +244,7 @@ __global__ void __launch_bounds__(NORM_THREADS, GRAD_BLOCKS)
   F wa[U], wb[U];
   {
     V wx[U], wy[U];
-    me.load(static_cast<const T*>(of_q ? a.norm.q_weight : a.norm.k_weight), wx, wy);
+    me.template load<true>(static_cast<const T*>(of_q ? a.norm.q_weight : a.norm.k_weight), wx, wy);
 #pragma unroll
     for (int j = 0; j < U; ++j) wa[j] = floats<T, VE>(wx[j]), wb[j] = floats<T, VE>(wy[j]);
   }

@@ -45,6 +45,41 @@ __device__ __forceinline__ void narrow(const float (&f)[VE], Vec<T, VE>& x) {
 }
 
 
+// A vector that this kernel does not read again, and one that it does not read: the first to leave the cache.
+template <typename V>
+__device__ __forceinline__ V load_once(const void* from) {
+  V x;
+  if constexpr (sizeof(V) == 16) {
+    const uint4 u = __ldcs(static_cast<const uint4*>(from));
+    memcpy(&x, &u, 16);
+  } else {
+    x = *static_cast<const V*>(from);
+  }
+  return x;
+}
+// One that many threads read and nobody writes.
+template <typename V>
+__device__ __forceinline__ V load_common(const void* from) {
+  V x;
+  if constexpr (sizeof(V) == 16) {
+    const uint4 u = __ldg(static_cast<const uint4*>(from));
+    memcpy(&x, &u, 16);
+  } else {
+    x = *static_cast<const V*>(from);
+  }
+  return x;
+}
+template <typename V>
+__device__ __forceinline__ void store_once(void* to, const V& x) {
+  if constexpr (sizeof(V) == 16) {
+    uint4 u;
+    memcpy(&u, &x, 16);
+    __stcs(static_cast<uint4*>(to), u);
+  } else {
+    *static_cast<V*>(to) = x;
+  }
+}
+
 // VE elements in fp32, two to a register pair, for the packed arithmetic that does two in one instruction (kf_common.cuh).
 template <int VE>
 struct Floats {
