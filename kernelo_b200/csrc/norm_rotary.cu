@@ -19,8 +19,8 @@
 // Backward: rows (token, head) are dealt out in runs, those of q and of k apart, so that a thread sums its own
 // columns of dw in registers over its rows, its next rows on their way to shared memory meanwhile; a
 // block adds its groups, and a second small launch the blocks, each in a fixed order: no atomics, the
-// same bits from call to call. 4096 tokens: 44 us (2.9 TB/s) and 3 for the sums; bound by the instructions of a row (some
-// 400 a warp, with 16 warps resident to an SM) and by its latencies.
+// same bits from call to call. 4096 tokens: 45 us (2.8 TB/s) with the sums; bound by the instructions of a row (some 400
+// a warp, with 16 warps resident to an SM) and by its latencies.
 #include <cuda.h>
 
 #include "kf_common.cuh"

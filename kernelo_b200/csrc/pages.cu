@@ -204,10 +204,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) release_kernel(const __grid_cons
   const int rank = static_cast<int>(blockIdx.x), ctas = static_cast<int>(gridDim.x);
   const int warps = ctas * PLAN_WARPS, my_warp = rank * PLAN_WARPS + warp;
   const int cols = static_cast<int>(a.cols), entries = a.count * cols, tiles = a.count * a.tiles;  // below 2^30
-  if constexpr (PHASE >= 0) {
-    griddep_launch_dependents();
-    griddep_wait();
-  }
+  if constexpr (PHASE >= 0 && PHASE < 3) griddep_launch_dependents();  // the next phase's blocks wait for this one's end
+  if constexpr (PHASE > 0) griddep_wait();
   // f(tile, its number among this CTA's, request, row, first column, pages from there on) for tiles that are not skipped.
   const auto each_tile = [&](const auto& f) {
     for (int t = my_warp, n = warp; t < tiles; t += warps, n += PLAN_WARPS) {
