@@ -52,12 +52,12 @@ __device__ __forceinline__ float group_sum(float v, int width) {
   return v;
 }
 
-// Elements whose squares' sum is beyond fp32 (never fp16's) are taken by this power of two less: u does not change, and
-// eps is nothing beside them.
+// Heads whose mean square with eps is beyond fp32 (never fp16's) are taken by this power of two less, and eps by its
+// square: u does not change. (The mean is then 2^-20 at least, so a usual eps is nothing only once it is scaled as well.)
 constexpr float FAR = 0x1p-70f;
 template <typename T>
-__device__ __forceinline__ bool too_far(float sum) {
-  return sizeof(T) == 4 || DType<T>::code == KF_BF16 ? !(sum < __int_as_float(0x7f800000)) : false;
+__device__ __forceinline__ bool too_far(float mean) {
+  return sizeof(T) == 4 || DType<T>::code == KF_BF16 ? !(mean < __int_as_float(0x7f800000)) : false;
 }
 
 // One thread's part of a head: its units' elements and angles.
@@ -115,9 +115,10 @@ struct Lane {
 #pragma unroll
       for (int i = 0; i < VE; ++i) sum = fmaf(a[j][i], a[j][i], fmaf(b[j][i], b[j][i], sum));
     }
-    sum = group_sum(sum, width);
-    if (__any_sync(0xffffffffu, too_far<T>(sum))) {
-      const float less = too_far<T>(sum) ? FAR : 1.0f;
+    float mean = fmaf(group_sum(sum, width), inv_dim, eps);
+    if (__any_sync(0xffffffffu, too_far<T>(mean))) {
+      const bool far = too_far<T>(mean);
+      const float less = far ? FAR : 1.0f;
       sum = 0.0f;
 #pragma unroll
       for (int j = 0; j < U; ++j)
@@ -126,9 +127,9 @@ struct Lane {
           a[j][i] *= less, b[j][i] *= less;
           sum = fmaf(a[j][i], a[j][i], fmaf(b[j][i], b[j][i], sum));
         }
-      sum = group_sum(sum, width);
+      mean = fmaf(group_sum(sum, width), inv_dim, eps * less * less);
     }
-    const float r = rsqrtf(fmaf(sum, inv_dim, eps));
+    const float r = rsqrtf(mean);
 #pragma unroll
     for (int j = 0; j < U; ++j) {
       float wa[VE], wb[VE];
@@ -335,16 +336,18 @@ __global__ void __launch_bounds__(NORM_THREADS, GRAD_BLOCKS)
       if (here && me.u[j].turned) turn<VE>(ga[j], gb[j], me.c[j], me.s[j], p.interleaved);
     float square, along, scale = 1.0f;
     sums_of(square, along);
-    if (__any_sync(0xffffffffu, too_far<T>(square))) {
-      if (too_far<T>(square)) scale = FAR;
+    float mean = fmaf(square, a.norm.inv_dim, a.norm.eps);
+    if (__any_sync(0xffffffffu, too_far<T>(mean))) {
+      if (too_far<T>(mean)) scale = FAR;
       const auto less = p_splat<VE>(scale);
 #pragma unroll
       for (int j = 0; j < U; ++j)
 #pragma unroll
         for (int i = 0; i < F::N; ++i) xa[j].e[i] = p_mul(xa[j].e[i], less), xb[j].e[i] = p_mul(xb[j].e[i], less);
       sums_of(square, along);
+      mean = fmaf(square, a.norm.inv_dim, a.norm.eps * scale * scale);
     }
-    const float inv = rsqrtf(fmaf(square, a.norm.inv_dim, a.norm.eps));
+    const float inv = rsqrtf(mean);
     const float inv_true = inv * scale;                            // 1 / s
     const float back = along * inv * a.norm.inv_dim * inv_true;  // mean(g w u) / s
     const auto inv2 = p_splat<VE>(inv), true2 = p_splat<VE>(inv_true), back2 = p_splat<VE>(-back);
