@@ -254,7 +254,9 @@ int32_t kf_norm_rotary(const kf_norm_rotary_args* args, void* stream) {
   if (g.rotary.inverse != 0) return invalid("inverse: the gradient of norms and turn is kf_norm_rotary_grad");
   if (nothing) return KF_OK;
   if ((a.heads > 0 && g.q_weight == nullptr) || (a.kv_heads > 0 && g.k_weight == nullptr)) return invalid("null pointer");
-  n.q_weight = g.q_weight, n.k_weight = g.k_weight;
+  // Lanes of a warp beside its last head read a weight too, which may be of the kind that has no heads.
+  n.q_weight = a.heads > 0 ? g.q_weight : g.k_weight;
+  n.k_weight = a.kv_heads > 0 ? g.k_weight : g.q_weight;
   DeviceInfo* dev = nullptr;
   rc = this_device(&dev);
   if (rc != KF_OK) return rc;
