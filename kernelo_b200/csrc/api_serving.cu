@@ -2,6 +2,7 @@
 // attention over a paged cache, rotary positions with the cache write, and
 // block tables with slot maps. Argument checks here, kernels in their own files.
 #include <cmath>
+#include <limits>
 #include <string>
 
 #include "kf_common.cuh"
@@ -130,7 +131,9 @@ int norm_args(int64_t dim, double eps, NormArgs* to) {
   if (dim > NORM_ROTARY_MAX_DIM)
     return set_error(KF_ERR_UNSUPPORTED, "norms of heads of at most " + std::to_string(NORM_ROTARY_MAX_DIM) +
                                              " elements; got " + std::to_string(dim));
-  if (!(eps > 0.0) || !std::isfinite(eps)) return invalid("eps must be finite and positive");
+  // Below the normal range squares as small as eps would lose their bits, and one rounded to zero makes NaN of zeros.
+  if (!(eps >= std::numeric_limits<float>::min() && eps <= std::numeric_limits<float>::max()))
+    return invalid("eps must be positive and in fp32's normal range");
   to->eps = static_cast<float>(eps);
   to->inv_dim = dim > 0 ? 1.0f / static_cast<float>(dim) : 0.0f;
   return KF_OK;

@@ -24,6 +24,7 @@ from kernelo_b200.runtime import native
 
 SCALINGS = ("linear", "base", "parts")
 MAX_NORM_DIM = 256
+_EPS_RANGE = torch.finfo(torch.float32).tiny, torch.finfo(torch.float32).max
 
 
 def rotary_table(
@@ -203,12 +204,12 @@ def _check_norm(q: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
     # one expression for what is right, and the reasons only where it is not
     if (q_weight.shape == shape == k_weight.shape and q_weight.dtype is dtype and k_weight.dtype is dtype
             and q_weight.get_device() == device == k_weight.get_device() and q_weight.is_contiguous()
-            and k_weight.is_contiguous() and shape[0] <= MAX_NORM_DIM and 0.0 < eps < math.inf):
+            and k_weight.is_contiguous() and shape[0] <= MAX_NORM_DIM and _EPS_RANGE[0] <= eps <= _EPS_RANGE[1]):
         return
     if shape[0] > MAX_NORM_DIM:
         raise ValueError(f"norms take heads of at most {MAX_NORM_DIM} elements, got {shape[0]}")
-    if not 0.0 < eps < math.inf:
-        raise ValueError(f"eps must be finite and positive, got {eps}")
+    if not _EPS_RANGE[0] <= eps <= _EPS_RANGE[1]:
+        raise ValueError(f"eps must be positive and in fp32's normal range, got {eps}")
     for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
         if w.shape != shape:
             raise ValueError(f"{name} must have shape ({shape[0]},), got {tuple(w.shape)}")
@@ -253,9 +254,10 @@ def norm_rotary(
     ``weight * x / sqrt(mean(x^2) + eps)`` before its turn.
 
     ``q_weight`` and ``k_weight`` (``(dim,)``, of the operands' type) are shared
-    by the heads of q and those of k. Everything is computed in fp32 and rounded
-    once, so the result is nearer than that of a norm and a turn apart. ``q_out``
-    / ``k_out`` may be q and k themselves, and share no other operand's memory.
+    by the heads of q and those of k; ``eps`` is positive and in fp32's normal
+    range. Everything is computed in fp32 and rounded once, so the result is
+    nearer than that of a norm and a turn apart. ``q_out`` / ``k_out`` may be q and
+    k themselves, and share no other operand's memory.
     """
     _check(q, k, positions, table)
     _check_norm(q, q_weight, k_weight, eps)

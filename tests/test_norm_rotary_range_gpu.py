@@ -51,3 +51,27 @@ def test_heads_whose_squares_just_leave_fp32(dim, eps, dtype, device):
     gq, gk, gqw, gkw = norm_rotary_backward(dq, dk, q, k, positions, table, qw, kw, eps=eps)
     check_gradient(gq, gqw, dq, q, qw, positions, table, False, eps)
     check_gradient(gk, gkw, dk, k, kw, positions, table, False, eps)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+def test_heads_of_zeros_and_of_the_least_eps(dtype, device):
+    """Squares beside the least normal eps are off by 2^-150 each, a rounding of their mean with it."""
+    eps, dim = 2.0 ** -126, 64
+    gen = torch.Generator().manual_seed(0)
+    q, k, dq, dk = (torch.randn(9, n, dim, generator=gen) for n in (3, 2, 3, 2))
+    q[:, 1] *= 2.0 ** -63  # (zeros in fp16)
+    q[:, 2], k[:, 1] = 0.0, 0.0
+    q, k, dq, dk = (x.to(dtype).to(device) for x in (q, k, dq, dk))
+    if dtype == torch.float16:  # the gradient of a head of zeros is 2^63 times as large as what goes in
+        dq, dk = dq.clone(), dk.clone()
+        dq[:, 1:], dk[:, 1] = 0.0, 0.0
+    w = torch.ones(dim, dtype=dtype, device=device)
+    table = rotary_table(9, dim, device=device)
+    positions = torch.arange(9, dtype=torch.int32, device=device)
+    y, z = norm_rotary(q, k, positions, table, w, w, eps=eps)
+    check(y, q, w, positions, table, False, eps)
+    check(z, k, w, positions, table, False, eps)
+    assert not y[:, 2].any() and not z[:, 1].any()
+    gq, gk, gqw, gkw = norm_rotary_backward(dq, dk, q, k, positions, table, w, w, eps=eps)
+    check_gradient(gq, gqw, dq, q, w, positions, table, False, eps)
+    check_gradient(gk, gkw, dk, k, w, positions, table, False, eps)
