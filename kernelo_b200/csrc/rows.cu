@@ -260,7 +260,7 @@ __global__ void __launch_bounds__(max_threads_for<NV>()) rows_kernel(const RowsP
     if constexpr (OP == OP_SOFTMAX) {
       // exp(x - M) / S = exp(x - m_thr) * (exp(m_thr - M) / S)
       const float factor =
-          m_thr == -INFINITY ? 0.0f : ex2_ftz((m_thr - tot.x) * kRowLog2e) / tot.y;
+          m_thr == -INFINITY ? masked_factor(tot.y) : ex2_ftz((m_thr - tot.x) * kRowLog2e) / tot.y;
       const float mb = m_thr == -INFINITY ? 0.0f : m_thr * kRowLog2e;
 #pragma unroll
       for (int j = 0; j < NV; ++j) {

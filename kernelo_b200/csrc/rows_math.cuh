@@ -205,17 +205,20 @@ __device__ __forceinline__ uint4 scale_gamma_vec(uint4 x, uint4 g, float scale) 
 }
 
 // (max, sum of exp) over the 32 lanes of a warp: the maximum first, then each
-// lane's sum rescaled to it by exp(m_lane - M). A lane with no elements has
-// m = -inf and s = 0.
+// lane's sum rescaled to it by exp(m_lane - M). A lane with no elements, or with
+// none but -inf, has m = -inf and s = 0 -- or s = NaN, where a NaN is all that it has besides.
 __device__ __forceinline__ float2 warp_max_sum(float m, float s) {
   float M = m;
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
-  float t = m == -INFINITY ? 0.0f : s * ex2_ftz((m - M) * kRowLog2e);
+  float t = m == -INFINITY ? s : s * ex2_ftz((m - M) * kRowLog2e);
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) t += __shfl_xor_sync(0xffffffffu, t, off);
   return make_float2(M, t);
 }
+
+// What a thread without anything but -inf multiplies its exponentials, zeros, by: zero, or NaN where the row's sum is NaN.
+__device__ __forceinline__ float masked_factor(float row_sum) { return 0.0f * row_sum; }
 
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll

@@ -299,7 +299,7 @@ __global__ void __launch_bounds__(STREAM_THREADS, stream_min_blocks<NV>())
     if constexpr (OP == OP_SOFTMAX) {
       // exp(x - M) / S = exp(x - m_thr) * (exp(m_thr - M) / S)
       const float factor =
-          m_thr == -INFINITY ? 0.0f : ex2_ftz((m_thr - part.x) * kRowLog2e) / part.y;
+          m_thr == -INFINITY ? masked_factor(part.y) : ex2_ftz((m_thr - part.x) * kRowLog2e) / part.y;
       const float mb = m_thr == -INFINITY ? 0.0f : m_thr * kRowLog2e;
 #pragma unroll
       for (int j = 0; j < NV; ++j) {

@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(WARP_ROW_WARPS * 32) rows_warp_kernel(const Wa
         }
       }
       const float2 tot = warp_max_sum(m, s);  // a lane without elements has m = -inf and s = 0
-      const float factor = m == -INFINITY ? 0.0f : ex2_ftz((m - tot.x) * kRowLog2e) * __frcp_rn(tot.y);
+      const float factor = m == -INFINITY ? masked_factor(tot.y) : ex2_ftz((m - tot.x) * kRowLog2e) * __frcp_rn(tot.y);
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         if (lane + 32 * j < p.nvec) {

@@ -3,7 +3,8 @@
 ``y_i = exp(x_i - max x) / sum_j exp(x_j - max x)`` with fp32 arithmetic and one
 rounding to the input dtype. The row maximum is subtracted for the reason the
 reference gives: fp16 ``exp`` overflows above x ~ 11. Elements of -inf (what a
-mask left out) get zero, and a row of nothing else is all zeros. Both native kernels read
+mask left out) get zero, and a row of nothing else is all zeros; a row with a
+NaN or with +inf is all NaN. Both native kernels read
 each row once into registers, reduce the (max, sum of exp) pair in a single
 pass with the online rescaling rule, and write the row once. Rows of 2 to
 32 KB go to the register kernel (one CTA per row, about eight 16-byte vectors
