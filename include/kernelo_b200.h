@@ -413,7 +413,9 @@ KF_API int32_t kf_rotary(const kf_rotary_args* args, void* stream);
 /* kf_norm_rotary: kf_rotary (inverse 0) on heads that are normalised first, each
  * head x of q and of k to weight * x / sqrt(mean(x^2) + eps), weights [dim] of the
  * operands' type, in fp32 and rounded once; v is copied as it is. Heads of up to
- * 256 elements. The weight of a kind without heads may be null. */
+ * 256 elements. The weight of a kind without heads may be null. q_out may be q, and
+ * k_out k; outputs, the caches among them, share no memory with an operand or with
+ * each other otherwise. */
 typedef struct kf_norm_rotary_args {
   kf_rotary_args rotary;
   const void* q_weight;

@@ -7,6 +7,7 @@
 
 #include "kf_common.cuh"
 #include "kf_internal.h"
+#include "overlap.h"
 
 namespace kf {
 namespace {
@@ -86,6 +87,43 @@ int rotary_args(const kf_rotary_args& g, RotaryArgs* to, bool* nothing) {
   }
   a.tokens = g.tokens, a.heads = g.heads, a.kv_heads = g.kv_heads, a.dim = g.dim;
   a.interleaved = g.interleaved != 0, a.inverse = g.inverse != 0;
+  return KF_OK;
+}
+
+int shared(const Region& out, const Region& other) {
+  return invalid(std::string(out.name) + " shares memory with " + other.name);
+}
+int self_shared(const Region& out) { return invalid(std::string(out.name) + " overlaps itself"); }
+
+// Outputs are written while other heads' operands are still read: each has its own memory, or (q_out, k_out) its input's.
+int check_norm_memory(const RotaryArgs& a, const NormArgs& n) {
+  const int elem = a.dtype == KF_FP32 ? 4 : 2;
+  const auto heads = [&](const char* name, const void* at, int64_t h, int64_t s_t, int64_t s_h) {
+    return Region(name, h > 0 ? at : nullptr, elem, {{a.tokens, s_t}, {h, s_h}, {a.dim, 1}});
+  };
+  const auto cache = [&](const char* name, const void* at, int64_t s_p, int64_t s_h, int64_t s_s) {
+    return Region(name, a.slots != nullptr ? at : nullptr, elem,
+                  {{a.pages, s_p}, {a.kv_heads, s_h}, {a.block_size, s_s}, {a.dim, 1}});
+  };
+  const Region in[] = {heads("q", a.q, a.heads, a.sq_t, a.sq_h),
+                       heads("k", a.k, a.kv_heads, a.sk_t, a.sk_h),
+                       heads("v", a.v, a.kv_heads, a.sv_t, a.sv_h),
+                       Region("q_weight", a.heads > 0 ? n.q_weight : nullptr, elem, {{a.dim, 1}}),
+                       Region("k_weight", a.kv_heads > 0 ? n.k_weight : nullptr, elem, {{a.dim, 1}}),
+                       Region("positions", a.rot > 0 ? a.positions : nullptr, 4, {{a.tokens, 1}}),
+                       Region("table", a.table, 4, {{a.table_rows, a.rot}, {a.rot, 1}}),
+                       Region("slots", a.slots, 8, {{a.tokens, 1}})};
+  const Region out[] = {heads("q_out", a.q_out, a.heads, a.sqo_t, a.sqo_h),
+                        heads("k_out", a.k_out, a.kv_heads, a.sko_t, a.sko_h),
+                        cache("k_cache", a.k_cache, a.skc_p, a.skc_h, a.skc_s),
+                        cache("v_cache", a.v_cache, a.svc_p, a.svc_h, a.svc_s)};
+  for (int i = 0; i < 4; ++i) {
+    if (out[i].overlaps_itself()) return self_shared(out[i]);
+    for (int j = 0; j < 8; ++j)
+      if (overlap(out[i], in[j]) && !(i < 2 && i == j && out[i].same_place(in[j]))) return shared(out[i], in[j]);
+    for (int j = 0; j < i; ++j)
+      if (overlap(out[i], out[j])) return shared(out[i], out[j]);
+  }
   return KF_OK;
 }
 
@@ -260,6 +298,8 @@ int32_t kf_norm_rotary(const kf_norm_rotary_args* args, void* stream) {
   // Lanes of a warp beside its last head read a weight too, which may be of the kind that has no heads.
   n.q_weight = a.heads > 0 ? g.q_weight : g.k_weight;
   n.k_weight = a.kv_heads > 0 ? g.k_weight : g.q_weight;
+  rc = check_norm_memory(a, n);
+  if (rc != KF_OK) return rc;
   DeviceInfo* dev = nullptr;
   rc = this_device(&dev);
   if (rc != KF_OK) return rc;

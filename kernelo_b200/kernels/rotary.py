@@ -287,7 +287,9 @@ def norm_rotary_to_cache(
     q_out: torch.Tensor | None = None,
     k_out: torch.Tensor | None = None,
 ) -> torch.Tensor:
-    """:func:`rotary_to_cache` of heads normalised first, as :func:`norm_rotary` does; v is written as it is."""
+    """:func:`rotary_to_cache` of heads normalised first, as :func:`norm_rotary` does; v is written as it is.
+
+    The caches share no memory with an operand or with each other (keys and values may lie in turn in one buffer)."""
     _check(q, k, positions, table)
     _check_cached(q, k, v, k_cache, v_cache, slots)
     _check_norm(q, q_weight, k_weight, eps)

@@ -1,11 +1,12 @@
-"""The C entry of head norms with heads of one kind alone and no weight for the other, beside the Python call that has both."""
+"""The entries of head norms and logits: heads of one kind alone and no weight for the other, and outputs that lie among
+other memory."""
 
 from __future__ import annotations
 
 import pytest
 import torch
 
-from kernelo_b200.kernels.rotary import norm_rotary, rotary_table
+from kernelo_b200.kernels.rotary import norm_rotary, norm_rotary_to_cache, rotary_table
 from kernelo_b200.runtime import native
 from tests.test_norm_rotary_gpu import inputs
 from tests.test_serving_step_host import packed
@@ -30,3 +31,32 @@ def test_heads_of_one_kind_without_the_other_weight(tokens, heads, dtype, device
         args = packed("kf_norm_rotary_args", **common, **fields)
         assert native.load().kf_norm_rotary(args, native.current_stream_handle(device)) == native.KF_OK, native.last_error()
         assert torch.equal(out, want)
+
+
+def test_outputs_among_other_memory(device):
+    """A projection of one key head turned in place, keys and values of each page side by side, and what is refused of them."""
+    tokens, dim = 33, 64
+    qkv = torch.randn(tokens, 6, dim, device=device).half()
+    w = torch.randn(3, dim, device=device).half()
+    table = rotary_table(100, dim, device=device)
+    positions = torch.arange(tokens, dtype=torch.int32, device=device)
+    slots = torch.randperm(48, device=device)[:tokens]
+    pages = torch.zeros(3, 2, 1, 16, dim, device=device, dtype=torch.float16)
+    q, k, v = qkv[:, :4], qkv[:, 4:5], qkv[:, 5:]
+    want_q, want_k = norm_rotary(q, k, positions, table, w[0], w[1])
+    value = v.clone()
+    operands = (positions, table, w[0], w[1], pages[:, 0], pages[:, 1], slots)
+    for bad, name in ((dict(k_out=v), "k_out shares memory with v"),
+                      (dict(k_out=pages.view(-1, 1, dim)[:tokens]), "k_out shares memory with k_cache")):
+        with pytest.raises(ValueError, match=name):
+            norm_rotary_to_cache(q, k, v, *operands, **bad)
+    flat = torch.zeros(tokens * dim + dim, device=device, dtype=torch.float16)
+    with pytest.raises(ValueError, match="k_out shares memory with k_weight"):
+        norm_rotary_to_cache(q, k, v, positions, table, w[0], flat[tokens * dim - dim:tokens * dim], *operands[4:],
+                             k_out=flat[:tokens * dim].view(tokens, 1, dim))
+    with pytest.raises(ValueError, match="v_cache shares memory with k_cache"):
+        norm_rotary_to_cache(q, k, v, *operands[:4], pages[:, 0], pages[:, 0], slots)
+    assert torch.equal(qkv[:, 5:], value) and not pages.any()
+    assert norm_rotary_to_cache(q, k, v, *operands, q_out=q, k_out=k) is q
+    assert torch.equal(q, want_q) and torch.equal(k, want_k)
+    assert torch.equal(pages[slots // 16, 0, :, slots % 16], want_k) and torch.equal(pages[slots // 16, 1, :, slots % 16], value)
