@@ -552,7 +552,7 @@ typedef struct kf_compact_args {
 KF_API int32_t kf_compact(const kf_compact_args* args, void* stream);
 
 /* ---- logits: penalties, biases, masks -------------------------------------------- *
- * out = logits [rows, vocab] (out may be logits; otherwise no memory is shared) after,
+ * out = logits [rows, vocab] (out may be logits; it shares no operand's memory otherwise) after,
  * in this order and in fp32: the penalties of the row's history, its biases, its mask.
  * tokens [rows, token_cols] (null: no history) begins with the row's token_lens[r]
  * tokens, of which the first prompt_lens[r] (null: none) are a prompt. Every token of

@@ -127,6 +127,28 @@ int check_norm_memory(const RotaryArgs& a, const NormArgs& n) {
   return KF_OK;
 }
 
+// A row's chunks read the row's lists while others write theirs.
+int check_logits_memory(const kf_logits_args& g) {
+  const int elem = g.dtype == KF_FP32 ? 4 : 2;
+  const Region out("out", g.out, elem, {{g.rows, g.so_row}, {g.vocab, 1}});
+  const Region logits("logits", g.logits, elem, {{g.rows, g.s_row}, {g.vocab, 1}});
+  if (out.overlaps_itself()) return self_shared(out);
+  if (overlap(out, logits) && !out.same_place(logits)) return shared(out, logits);
+  const void* const tokens = g.tokens;  // without them nothing of a history is read
+  const auto each = [&](const char* name, const void* at) { return Region(name, tokens != nullptr ? at : nullptr, 4, {{g.rows, 1}}); };
+  const void* const biases = g.bias_tokens;
+  const Region in[] = {Region("tokens", tokens, 4, {{g.rows, g.st_row}, {g.token_cols, 1}}),
+                       each("token_lens", g.token_lens), each("prompt_lens", g.prompt_lens), each("repetition", g.repetition),
+                       each("frequency", g.frequency), each("presence", g.presence),
+                       Region("bias_tokens", biases, 4, {{g.rows, g.sb_row}, {g.bias_cols, 1}}),
+                       Region("bias_values", biases != nullptr ? g.bias_values : nullptr, 4, {{g.rows, g.sv_row}, {g.bias_cols, 1}}),
+                       Region("allowed", g.allowed, 4, {{g.masks, g.sa_row}, {ceil_div(g.vocab, 32), 1}}),
+                       Region("allowed_rows", g.allowed != nullptr ? g.allowed_rows : nullptr, 4, {{g.rows, 1}})};
+  for (const Region& other : in)
+    if (overlap(out, other)) return shared(out, other);
+  return KF_OK;
+}
+
 // Rows that one call's bits take 96 KB of shared memory for; and pages that a cluster's do 1 MB for.
 constexpr int64_t TABLE_ROWS_LIMIT = 1 << 18;
 constexpr int64_t COMPACT_PAGES_LIMIT = 1 << 22;
@@ -436,9 +458,10 @@ int32_t kf_adjust_logits(const kf_logits_args* args, void* stream) {
   if (g.logits == nullptr || g.out == nullptr || (g.tokens != nullptr && g.token_lens == nullptr) ||
       (g.bias_tokens != nullptr && g.bias_values == nullptr))
     return invalid("null pointer");
-  if (g.rows > 1 && g.so_row == 0) return invalid("out overlaps itself: a stride of zero");
+  int rc = check_logits_memory(g);
+  if (rc != KF_OK) return rc;
   DeviceInfo* dev = nullptr;
-  const int rc = this_device(&dev);
+  rc = this_device(&dev);
   if (rc != KF_OK) return rc;
   return launch_logits(g, *dev, static_cast<cudaStream_t>(stream));
 }

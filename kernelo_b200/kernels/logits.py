@@ -139,7 +139,7 @@ def adjust_logits(
       the masks, every token is allowed.
 
     Token ids outside the vocabulary are ignored, also in a history. ``out`` may
-    be ``logits`` itself, and shares no memory with it otherwise. A row whose mask
+    be ``logits`` itself, and shares no operand's memory otherwise. A row whose mask
     allows nothing is all ``-inf``.
     """
     rows, vocab = logits.shape if logits.ndim == 2 else (0, 0)

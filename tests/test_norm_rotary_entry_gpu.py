@@ -6,6 +6,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+from kernelo_b200.kernels.logits import adjust_logits
 from kernelo_b200.kernels.rotary import norm_rotary, norm_rotary_to_cache, rotary_table
 from kernelo_b200.runtime import native
 from tests.test_norm_rotary_gpu import inputs
@@ -60,3 +61,16 @@ def test_outputs_among_other_memory(device):
     assert norm_rotary_to_cache(q, k, v, *operands, q_out=q, k_out=k) is q
     assert torch.equal(q, want_q) and torch.equal(k, want_k)
     assert torch.equal(pages[slots // 16, 0, :, slots % 16], want_k) and torch.equal(pages[slots // 16, 1, :, slots % 16], value)
+
+
+def test_logits_among_other_memory(device):
+    """Biases behind the logits in one buffer, and an output that would take them."""
+    buf = torch.randn(5, 640, device=device)
+    tokens = torch.randint(0, 600, (5, 40), device=device, dtype=torch.int32)
+    before = buf.clone()
+    want = adjust_logits(buf[:, :600].clone(), bias_tokens=tokens, bias_values=buf[:, 600:].clone())
+    with pytest.raises(ValueError, match="out shares memory with bias_values"):
+        adjust_logits(torch.zeros(5, 601, device=device), bias_tokens=tokens, bias_values=buf[:, 600:], out=buf[:, :601])
+    assert torch.equal(buf, before)
+    got = adjust_logits(buf[:, :600], bias_tokens=tokens, bias_values=buf[:, 600:], out=buf[:, :600])
+    assert torch.equal(got, want) and torch.equal(buf[:, 600:], before[:, 600:])

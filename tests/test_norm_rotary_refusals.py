@@ -39,6 +39,10 @@ HEADS = dict(dtype=native.native_code(torch.bfloat16), tokens=10, heads=4, kv_he
              k_out=OUT + 0x100000, sko_row=64, sko_head=64, positions=0x8000, table=0x20000, q_weight=0x3000, k_weight=0x4000)
 CACHED = dict(v=Q + 640, sv_row=448, sv_head=64, k_cache=CACHE, skc_page=2048, skc_head=1024, skc_slot=64, v_cache=CACHE + 2048,
               svc_page=2048, svc_head=1024, svc_slot=64, pages=7, block_size=16, slots=0x6000)  # a page's keys, then its values
+LOGITS = dict(dtype=native.native_code(torch.float32), logits=Q, s_row=1000, out=OUT, so_row=1040, rows=6, vocab=1000, tokens=K, st_row=20,
+              token_cols=20, token_lens=0x3000, repetition=0x3100, frequency=0x3200, presence=0x3300, prompt_lens=0x3400,
+              bias_tokens=V, sb_row=8, bias_values=0x9000, sv_row=8, bias_cols=8, allowed=0xa000, sa_row=32, masks=3,
+              allowed_rows=0x3500)
 
 
 @no_device
@@ -65,6 +69,21 @@ def test_outputs_that_share_memory_are_refused(change, message):
 
 
 @no_device
+@pytest.mark.parametrize("change,message", [
+    (dict(out=Q + 4), "out shares memory with logits"), (dict(out=Q), "out shares memory with logits"),
+    (dict(so_row=999), "out overlaps itself"),
+    (dict(out=K + 476), "out shares memory with tokens"), (dict(out=0x3000 + 20), "out shares memory with token_lens"),
+    (dict(token_lens=OUT + 3998, prompt_lens=0), "out shares memory with token_lens"),
+    (dict(prompt_lens=OUT + 500), "prompt_lens"), (dict(repetition=OUT + 500), "repetition"),
+    (dict(frequency=OUT + 500), "frequency"), (dict(presence=OUT + 500), "presence"), (dict(bias_tokens=OUT + 500), "bias_tokens"),
+    (dict(bias_values=OUT + 4000, sv_row=1040, bias_cols=41), "bias_values"), (dict(allowed=OUT + 500), "with allowed"),
+    (dict(allowed_rows=OUT + 500), "allowed_rows"),
+])
+def test_logits_that_share_memory_are_refused(change, message):
+    refused(native.load().kf_adjust_logits, "kf_logits_args", native.KF_ERR_INVALID_ARGUMENT, message, **(LOGITS | change))
+
+
+@no_device
 def test_outputs_of_their_own_pass_the_checks():
     in_place = dict(q_out=Q, sqo_row=448, k_out=Q + 512, sko_row=448)
     for change in ({}, in_place, CACHED, CACHED | in_place, CACHED | dict(k_out=0), CACHED | dict(v_cache=CACHE + 0x100000),
@@ -72,3 +91,7 @@ def test_outputs_of_their_own_pass_the_checks():
                    dict(kv_heads=0, k=0, k_out=0x3000), dict(rot=0, table=OUT, positions=OUT)):
         args = packed("kf_norm_rotary_args", **(HEADS | change))
         assert native.load().kf_norm_rotary(args, None) not in (native.KF_OK, native.KF_ERR_INVALID_ARGUMENT), change
+    for change in (dict(out=Q, so_row=1000), {}, dict(bias_values=OUT + 4000, sv_row=1040, bias_cols=40), dict(rows=1, out=Q),
+                   dict(tokens=0, token_lens=OUT), dict(allowed=0, allowed_rows=OUT), dict(bias_tokens=0, bias_values=OUT)):
+        args = packed("kf_logits_args", **(LOGITS | change))
+        assert native.load().kf_adjust_logits(args, None) not in (native.KF_OK, native.KF_ERR_INVALID_ARGUMENT), change
