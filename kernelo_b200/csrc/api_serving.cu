@@ -174,6 +174,9 @@ int page_geometry(const kf_page_caches& c, PageGeometry* to) {
   for (int64_t i = 0; i < c.n_caches; ++i)
     if (c.caches[i] == nullptr && c.pages * c.heads * c.dim > 0) return invalid("null pointer");
   to->elem = c.dtype == KF_FP32 ? 4 : 2;
+  if (c.n_caches > 0 && Region("a cache", c.caches[0], to->elem, {{c.pages, c.s_page}, {c.heads, c.s_head},
+                               {c.block_size, c.s_slot}, {c.dim, 1}}).overlaps_itself())
+    return invalid("caches overlap themselves");
   to->s_page = c.s_page, to->s_head = c.s_head, to->s_slot = c.s_slot;
   to->pages = c.pages, to->heads = c.heads, to->block = c.block_size, to->dim = c.dim;
   return KF_OK;
