@@ -66,7 +66,7 @@ class Step:
     slots: StepSlots
     context_lens: torch.Tensor  # tokens of each request before the step
     lens: tuple[int, ...] | None = None  # the same on the host
-    moved: int | None = None  # how often the cache's pages had moved then
+    moved: int | None = None  # how often the cache's pages had moved or been forked then
 
 
 class PagedCache:
@@ -115,9 +115,9 @@ class PagedCache:
         return Step(new_lens, slots, context, tuple(self.lens), self._moved)
 
     def check_step(self, step: Step) -> None:
-        """Refuses a step that was planned before the pages moved: its slots are others' now."""
+        """Refuses a step that was planned before pages moved or requests forked: its slots may be others' now."""
         if step.moved is not None and step.moved != self._moved:
-            raise ValueError("the step was planned before the cache's pages moved")
+            raise ValueError("the step was planned before the cache's pages moved or its requests forked")
 
     def advance(self, step: Step, kept=None) -> None:
         """The step's tokens are the requests' now, or those that ``kept[r]`` names: pages of the rest go back.
@@ -163,7 +163,8 @@ class PagedCache:
     def fork(self, parents: Sequence[int], children: Sequence[int]) -> None:
         """Request ``children[i]``, which has no tokens yet, goes on from where request ``parents[i]`` is.
 
-        Their whole pages are held together; a last, partial one is copied. Between steps, not during one.
+        Their whole pages are held together; a last, partial one is copied. Between steps: one that was planned before is
+        refused afterwards.
         """
         parents, children = [int(p) for p in parents], [int(c) for c in children]
         self._check_requests(parents + children)
@@ -175,8 +176,11 @@ class PagedCache:
         taken = sum(self.lens[p] % size > 0 for p in parents)
         if taken > self.free.shape[0]:
             raise ValueError(f"the cache has {taken - self.free.shape[0]} pages too few for these forks")
+        if not parents:
+            return
         fork_requests([self.k, self.v], self.block_table, self._device_ints(self.lens), self.holders, self.free,
                       self._device_ints(parents), self._device_ints(children))
+        self._moved += 1
         self.free = self.free[taken:]
         for p, c in zip(parents, children):
             held = self._together[p]
