@@ -192,12 +192,15 @@ class PagedCache:
 
     def release(self, request: int | Sequence[int]) -> None:
         """Finished requests' pages go back, unless others hold them too, and their rows are free for others. Between
-        steps, not during one."""
+        steps, not during one; a request without tokens stays as it is."""
         try:
             requests = [operator.index(request)]
         except TypeError:
             requests = list(dict.fromkeys(int(r) for r in request))
         self._check_requests(requests)
+        requests = [r for r in requests if self.lens[r]]  # others hold nothing; a step may have planned pages in their rows
+        if not requests:
+            return
         size, back = self.config.block_size, 0
         for r in requests:
             back += -(-self.lens[r] // size) - len(self._together[r])

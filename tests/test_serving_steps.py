@@ -54,3 +54,34 @@ def test_a_fork_that_is_refused_leaves_a_step_as_it_was():
         cache.fork([0], [1])
     cache.advance(step)
     assert cache.lens == [7, 4, 0]
+
+
+@pytest.mark.parametrize("released", [1, [1], [1, 2], []])
+def test_a_release_of_requests_without_tokens_leaves_a_step_as_it_was(released):
+    cache, step = planned((6, 0, 0), (3, 5, 0))
+    table, free = cache.block_table.clone(), cache.free.tolist()
+    cache.release(released)
+    assert torch.equal(cache.block_table, table) and cache.free.tolist() == free
+    cache.advance(step)
+    assert cache.lens == [9, 5, 0] and cache.free.tolist() == list(range(5, 20))
+    assert cache.block_table[0, :3].tolist() == [0, 1, 2] and cache.block_table[1, :2].tolist() == [3, 4]
+
+
+@pytest.mark.gpu
+def test_requests_without_tokens_released_and_forked_beside_a_step(device):
+    cache = PagedCache(SMALL, requests=4, blocks=20, device=device)
+    cache.advance(cache.plan([6, 0, 0, 0]))
+    step = cache.plan([1, 5, 0, 0])
+    cache.release([1, 2])
+    cache.advance(step)
+    held = [cache.block_table[r, :2].tolist() for r in range(2)]
+    assert cache.lens == [7, 5, 0, 0] and sorted([*held[0], *held[1], *cache.free.tolist()]) == list(range(20))
+    step = cache.plan([1, 1, 3, 0])
+    cache.fork([0], [3])
+    with pytest.raises(ValueError, match="planned before"):
+        cache.advance(step)
+    cache.advance(cache.plan([1, 1, 3, 1]))
+    assert cache.lens == [8, 6, 3, 8]
+    held = [p for r in range(4) for p in cache.block_table[r, :-(-cache.lens[r] // 4)].tolist()]
+    assert len(held) == 2 + 2 + 1 + 2 and held.count(held[0]) == 2
+    assert sorted([*set(held), *cache.free.tolist()]) == list(range(20))
