@@ -36,7 +36,7 @@ from kernelo_b200.kernels.logits import adjust_logits
 from kernelo_b200.kernels.matmul import matmul
 from kernelo_b200.kernels.paged import StepSlots, build_slots, compact_pages, fork_requests, release_requests
 from kernelo_b200.kernels.rmsnorm import rmsnorm
-from kernelo_b200.kernels.rotary import norm_rotary_to_cache, rotary_table, rotary_to_cache
+from kernelo_b200.kernels.rotary import MAX_NORM_DIM, norm_rotary_to_cache, rotary_table, rotary_to_cache
 from kernelo_b200.kernels.softmax import softmax
 
 
@@ -56,6 +56,8 @@ class ServingConfig(BlockConfig):
             raise ValueError(f"{self.heads} heads are not a multiple of {self.kv_heads} key heads")
         if self.block_size < 1:
             raise ValueError(f"block_size must be positive, got {self.block_size}")
+        if self.qk_norm and self.head_dim > MAX_NORM_DIM:
+            raise ValueError(f"qk_norm takes heads of at most {MAX_NORM_DIM} elements, got {self.head_dim}")
 
 
 @dataclass(frozen=True)
