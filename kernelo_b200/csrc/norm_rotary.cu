@@ -15,12 +15,14 @@
 // Forward: bound by bytes. A group of lanes takes several heads of a token with one load of its angles, two heads'
 // loads in flight. 8192 tokens of 32 query and 8 key heads of 128 bf16 with the cache written: 47 us, 4.7 TB/s (72% of
 // a copy's rate; the turn alone, without norms, 42); 64 tokens 4.7 us. Operands and outputs pass through the cache as the
-// first to leave it, weights and angles stay (with plain accesses 49 us, and 28 instead of 25 for 2048 tokens in fp32).
+// first to leave it, weights and angles stay: alone 44.4 us where plain stores take 47.5, and what follows loses nothing
+// (with the prompt's attention 468 us either way, four prompts of 512 38.3 and 38.7, a step of 64 59 to 61).
 // Backward: rows (token, head) are dealt out in runs, those of q and of k apart, so that a thread sums its own
 // columns of dw in registers over its rows, its next rows on their way to shared memory meanwhile; a
 // block adds its groups, and a second small launch the blocks, each in a fixed order: no atomics, the
-// same bits from call to call. 4096 tokens: 45 us (2.8 TB/s) with the sums; bound by the instructions of a row (some 400
-// a warp, with 16 warps resident to an SM) and by its latencies.
+// same bits from call to call. 4096 tokens: 43-45 us (2.9 TB/s) with the sums: some 12 us for a block's begin and end (first
+// angles and rows, sums, the second launch) and 7.5 for each 1024 tokens (4.2 TB/s; 16384 tokens 136 us). The latencies of
+// a row's chain, with 16 warps resident to an SM, bound that part; issue slots are half used.
 #include <cuda.h>
 
 #include "kf_common.cuh"
@@ -207,7 +209,7 @@ __global__ void __launch_bounds__(NORM_THREADS, FWD_BLOCKS)
 // are on their way to its own places in shared memory (nobody else reads them: no barriers) while it computes.
 constexpr int STAGES = 4;
 // Blocks of an SM, and how many times as many the rows are dealt out to: those that run beside slower ones then end
-// earlier. 4096 tokens of 40 heads of 128 bf16: 43.8 us; 1 wave 50.4, 4 waves 50.5; 3 blocks 44.4.
+// earlier. 4096 tokens of 40 heads of 128 bf16, in one comparison: 43.8 us; 1 wave 50.4, 4 waves 50.5; 3 blocks 44.4.
 constexpr int GRAD_BLOCKS = 4, GRAD_WAVES = 2;
 
 __device__ __forceinline__ void copy_async(uint32_t to, const void* from, int bytes) {

@@ -15,13 +15,13 @@
 //   the i-th hole among them: a plan and the table's new numbers by one
 //   cluster, then the copies by the whole GPU.
 //
-// Plans go in phases between barriers of one cluster: their work is a few dependent
-// accesses per page, and a launch for each phase would cost more. Copies are bound by
-// their bytes. Every number read from a table or a list is checked before it is used.
+// Plans go in phases of a few dependent accesses per page, between the barriers of one
+// CTA or cluster; releases of many go in a launch a phase over the whole GPU. Copies are bound
+// by their bytes. Every number read from a table or a list is checked before it is used.
 //
 // On the GPU: 16 requests of up to 2048 tokens forked 4 ways in 32 caches 14.7 us (36 MB, 5.5 at a copy's rate: the books
-// before the copies are a chain of dependent loads), one in 2 caches 5.0; one request of 256 pages released 10.3 us, 192
-// of up to 2048 pages some 40; 1300 of 2600 pages of 16 caches moved in 158 us (1.03 GB, a copy's rate) behind a
+// before the copies are a chain of dependent loads), one in 2 caches 5.0; one request of 256 pages released 9.2 us, of
+// 2048 13.5, 16 of 2048 31 to 34, 192 of 2048 34 to 36; 1300 of 2600 pages of 16 caches moved in 158 us (1.03 GB, a copy's rate) behind a
 // plan of 13.
 #include <cuda.h>
 
@@ -195,7 +195,7 @@ constexpr int MARK = -(1 << 30);
 // Entries (request, column) go by tiles of a row, dealt out to the warps in turn (rows end early, and a run of them for
 // each warp would leave most warps with nothing). The four phases, 0 to 3, are one launch of a cluster for few
 // entries (PHASE -1), and otherwise a launch each over the whole GPU: an entry costs five scattered accesses, and
-// a cluster's 8 SMs take 98 us for the 192 longest of 256 requests of up to 2048 pages.
+// a cluster's 8 SMs take 98 us for 192 of 256 requests of up to 2048 pages, the launches 34.
 template <int PHASE>
 __global__ void __launch_bounds__(PLAN_THREADS) release_kernel(const __grid_constant__ ReleaseArgs a) {
   __shared__ int scratch[PLAN_WARPS];
@@ -607,7 +607,8 @@ int launch_release(const kf_release_args& r, const DeviceInfo& dev, cudaStream_t
                       r.requests, static_cast<int>(r.count), static_cast<int>(parts),
                       reinterpret_cast<uint32_t*>(r.scratch), r.scratch + tiles * TILE_WORDS, r.freed, r.n_freed};
   const auto smem = [&](int ctas) { return static_cast<int>(ceil_div(tiles, ctas * PLAN_WARPS) * PLAN_WARPS * 4); };
-  // A cluster takes about 9 us and 5 more for each 16384 pages, the four launches 13 us.
+  // One CTA takes 9 us and 4 more by 2048 pages; a cluster 28 to 32 us for 8192 pages and 31 to 34 for 32768, where the
+  // four launches take 33 to 34, and 34 to 36 for 393216.
   if (tiles * TILE <= 32768) {
     const int ctas = plan_ctas(tiles * TILE);
     return launch_cluster(release_kernel<-1>, ctas, smem(ctas), stream, "launch(release)", a);

@@ -126,7 +126,7 @@ def adjust_logits(
 
     * ``tokens`` (int32 ``(rows, columns)``) begins with each row's history of
       ``token_lens[r]`` (int32) tokens; the first ``prompt_lens[r]`` of them (none
-      by default) are its prompt. ``repetition`` (fp32 ``(rows,)``, positive)
+      by default) are its prompt. ``repetition`` (fp32 ``(rows,)``, positive normal numbers)
       divides the positive logits of all tokens of the history and multiplies the
       others. A token that stands ``n`` times behind the prompt loses
       ``frequency[r] * n + presence[r]`` (fp32 ``(rows,)``).
