@@ -35,7 +35,7 @@ struct Region {
     for (int i = 0; i < dims; ++i) span += static_cast<Wide>(axes[i].n - 1) * axes[i].stride;
     return first() + span * elem;
   }
-  // Whether two of its indexes name one element, as far as its strides, taken in order, can rule it out.
+  // Whether two of its indexes may name one element: false only where each stride passes all that the shorter ones span.
   bool overlaps_itself() const {
     if (at == nullptr) return false;
     Axis up[MOST];

@@ -21,8 +21,8 @@
 //
 // On the GPU: 16 requests of up to 2048 tokens forked 4 ways in 32 caches 14.7 us (36 MB, 5.5 at a copy's rate: the books
 // before the copies are a chain of dependent loads), one in 2 caches 5.0; one request of 256 pages released 9.2 us, of
-// 2048 13.5, 16 of 2048 31 to 34, 192 of 2048 34 to 36; 1300 of 2600 pages of 16 caches moved in 158 us (1.03 GB, a copy's rate) behind a
-// plan of 13.
+// 2048 13.5, 16 of 2048 31 to 34, 192 of 2048 34 to 36; 1300 of 2600 pages of 16 caches moved in 158 us (1.03 GB, a copy's
+// rate) behind a plan of 13.
 #include <cuda.h>
 
 #include "kf_common.cuh"
